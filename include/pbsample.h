@@ -32,6 +32,9 @@
  *   - one step of the REPL's decode loop for many sequences
  *     (src/model_repl.rs:928-1150): pb_decode_step, pb_lmhead_decode_step,
  *     with the host helpers pb_decode_draw and pb_decode_settle;
+ *   - scores and losses of logits rows, with their gradients: pb_token_logprobs,
+ *     pb_token_logprobs_grad, pb_top_logits, pb_distill_loss, pb_policy_loss,
+ *     pb_preference_loss;
  *   - host PRNG helpers: pb_sampling_state_new, pb_next_24, pb_fill_random_24.
  */
 #ifndef PBSAMPLE_H
@@ -431,6 +434,140 @@ uint32_t pb_segments_for_rows(uint32_t rows);
  * single-workgroup and the multi-slice paths on the same rows (a forced plan
  * also turns off the small batches' tile selection). */
 void pb_context_set_segments(pb_context *ctx, uint32_t segments);
+
+/* ---- scores and losses of logits rows (no counterpart in the reference) ----
+ *
+ * What is done with logits rows beside sampling from them: the
+ * log-probabilities of their tokens, a teacher's top logits, and the losses a
+ * policy is trained with on such rows, each with its gradient.
+ *
+ *   d_logits   rows x ld elements of `dtype` (pb_dtype), ld >= vocab; vocab is
+ *              any size from 1 to PB_SCORE_MAX_VOCAB, rows up to
+ *              PB_SCORE_MAX_ROWS; aligned to an element.  Not modified, unless
+ *              a call's gradient goes in its place (below).
+ *   temperature  T, 0.01 to 100: y = x / T, and q = softmax(y) over the row.
+ *
+ * A logit of -inf (or one whose y / ln 2 is below binary32's range) weighs
+ * nothing.  A row whose token is PB_NO_TOKEN, or whose weight is 0, is
+ * skipped: its logits are not read, its outputs are 0, its gradient row is 0.
+ * A row error gives NaN outputs, a NaN gradient row and, when d_err is given,
+ * a record with `position` = the row: PB_TOKEN_ID (an id >= vocab; needed =
+ * vocab, available = the id), PB_NONFINITE_OUTPUT (a NaN or +inf logit, or a y
+ * / ln 2 above binary32's range: detail holds the first such index; or a row
+ * in which nothing weighs anything, index 0; available = the logit's bits as
+ * binary32).
+ *
+ * Sums and statistics are held in 32 bits over a few hundred terms and in 64
+ * bits above that; a row's scalars are worked out in 64 bits and rounded once.
+ * The order of every sum depends on the sizes and the alignment alone, so
+ * results repeat bit for bit.
+ *
+ * Gradients have the logits' type (rounded to nearest even) and may go in
+ * place of the logits (d_grad = d_logits and grad_ld = ld); any other overlap
+ * of the two is refused with PB_STATE.  Columns from vocab on are not written.
+ * A weight is the row's upstream gradient: gradients are multiplied by it,
+ * losses are not.  NULL weights are 1.
+ *
+ * All pointers are device pointers; calls enqueue on `stream`, never allocate
+ * and never wait, and need a context reserved with pb_context_reserve_scores
+ * for at least `rows` rows and `vocab` ids (else PB_CAPACITY).  Calls on one
+ * context share its workspace: the rule on threads and streams above holds.
+ * Returns PB_OK when the work was enqueued, else a status with *err filled
+ * (err may be NULL) and nothing enqueued. */
+enum pb_dtype { PB_F32 = 0, PB_F16 = 1, PB_BF16 = 2 };
+#define PB_SCORE_MAX_ROWS 1048576u
+#define PB_SCORE_MAX_VOCAB 4194304u
+#define PB_TOP_LOGITS_MAX 128u /* largest k of pb_top_logits and pb_distill_loss */
+
+/* Sizes the context's workspace for the calls below on up to `rows` rows of up
+ * to `vocab` ids (as pb_context_reserve: a set-up call; it never shrinks the
+ * workspace, and one it outgrows stays allocated until pb_context_destroy). */
+uint32_t pb_context_reserve_scores(pb_context *ctx, uint32_t rows, size_t vocab,
+                                   pb_inference_error *err);
+
+/* Per row: d_logprob = ln q[token], d_lse (optional) = ln sum exp(y),
+ * d_entropy (optional) = -sum q ln q.  d_token: one id per row. */
+uint32_t pb_token_logprobs(pb_context *ctx, const void *d_logits, uint32_t dtype, size_t vocab,
+                           size_t ld, uint32_t rows, double temperature, const uint32_t *d_token,
+                           float *d_logprob, float *d_lse, float *d_entropy,
+                           pb_inference_error *d_err, void *stream, pb_inference_error *err);
+
+/* The gradient of sum(grad_logprob * logprob + grad_entropy * entropy) by the
+ * logits, with d_lse and d_entropy as pb_token_logprobs left them for the same
+ * logits, tokens and temperature.  Either of d_grad_logprob and d_grad_entropy
+ * may be NULL (0); d_entropy is needed with d_grad_entropy.  A row whose token
+ * is bad, or whose d_lse is NaN, gets a NaN gradient row. */
+uint32_t pb_token_logprobs_grad(pb_context *ctx, const void *d_logits, uint32_t dtype,
+                                size_t vocab, size_t ld, uint32_t rows, double temperature,
+                                const uint32_t *d_token, const float *d_lse,
+                                const float *d_entropy, const float *d_grad_logprob,
+                                const float *d_grad_entropy, void *d_grad, size_t grad_ld,
+                                void *stream, pb_inference_error *err);
+
+/* The k largest logits of each row, largest first and the lowest id first
+ * among equal ones (-0 equals 0): d_token rows x k ids, d_value rows x k raw
+ * logits as binary32; d_lse (optional) as pb_token_logprobs.  k <= vocab and
+ * k <= PB_TOP_LOGITS_MAX.  -inf logits are taken last, like any other value.
+ * No row is skipped; a row error gives PB_NO_TOKEN ids. */
+uint32_t pb_top_logits(pb_context *ctx, const void *d_logits, uint32_t dtype, size_t vocab,
+                       size_t ld, uint32_t rows, uint32_t k, double temperature, uint32_t *d_token,
+                       float *d_value, float *d_lse, pb_inference_error *d_err, void *stream,
+                       pb_inference_error *err);
+
+/* Distillation from a teacher's top logits: d_teacher_id and d_teacher_logit
+ * (rows x k, k <= PB_TOP_LOGITS_MAX) as pb_top_logits records them, in any
+ * order; an id of PB_NO_TOKEN is padding, and its logit is not looked at.
+ * Without d_teacher_lse the teacher is p = softmax(logit / T) over its listed
+ * ids; with it (the teacher's log-sum-exp at T) p = exp(logit / T - lse), and
+ * what is left of 1 is one bucket of all other ids, compared with the
+ * student's mass off the list (no such bucket where the student has no mass
+ * there).  d_loss per row = sum p (ln p - ln q); p = 0 counts 0.  A row with
+ * nothing listed, or with no listed logit above -inf, has loss and gradient 0.
+ * Row errors: as above, and PB_TOKEN_ID for an id >= vocab or one listed twice,
+ * PB_NONFINITE_INPUT for a listed logit that is NaN or +inf, or a lse that is
+ * not finite (detail: the place in the list, k for the lse).  d_weight as
+ * above; d_lse (optional) the student's; d_grad optional. */
+uint32_t pb_distill_loss(pb_context *ctx, const void *d_logits, uint32_t dtype, size_t vocab,
+                         size_t ld, uint32_t rows, double temperature, uint32_t k,
+                         const uint32_t *d_teacher_id, const float *d_teacher_logit,
+                         const float *d_teacher_lse, const float *d_weight, float *d_loss,
+                         float *d_lse, void *d_grad, size_t grad_ld, pb_inference_error *d_err,
+                         void *stream, pb_inference_error *err);
+
+/* Clipped policy loss with a KL term: lp = ln q[token], r = exp(lp - old),
+ * d_loss = -min(r A, min(max(r, 1 - clip_low), 1 + clip_high) A) + kl_coef kl,
+ * with d = ref - lp and kl = exp(d) - d - 1 (0 without d_ref_logprob, which
+ * kl_coef != 0 needs).  The clipped branch has no gradient; where both are
+ * equal, the unclipped one counts.  d_logprob, d_kl and d_grad optional.
+ * 0 <= clip_low <= 1, clip_high >= 0, kl_coef finite. */
+uint32_t pb_policy_loss(pb_context *ctx, const void *d_logits, uint32_t dtype, size_t vocab,
+                        size_t ld, uint32_t rows, double temperature, const uint32_t *d_token,
+                        const float *d_old_logprob, const float *d_advantage,
+                        const float *d_ref_logprob, const float *d_weight, double clip_low,
+                        double clip_high, double kl_coef, float *d_loss, float *d_logprob,
+                        float *d_kl, void *d_grad, size_t grad_ld, pb_inference_error *d_err,
+                        void *stream, pb_inference_error *err);
+
+/* Preference loss over `pairs` pairs of sequences: sequence s is the rows
+ * d_seq_start[s] .. d_seq_start[s + 1] - 1 (2 x pairs + 1 offsets, not
+ * decreasing, at most `rows`), 2i the chosen and 2i + 1 the rejected one of
+ * pair i.  l_s = sum of ln q[token] over its rows, h = beta ((l_chosen -
+ * ref_chosen) - (l_rejected - ref_rejected)), d_loss[i] = -(1 - e) ln sigma(h)
+ * - e ln sigma(-h) with e = label_smoothing (0 to 1).  d_ref_logprob (NULL: 0)
+ * and d_logprob (optional, l_s) have 2 x pairs entries, d_weight `pairs`: a
+ * pair of weight 0 has loss, log-probabilities and gradient 0.  Rows before the
+ * first and behind the last sequence are not read, and their gradient rows are
+ * left as they are.  d_err (optional): one record per pair, the first of its
+ * rows that failed (the whole pair is then NaN); PB_CAPACITY (needed = rows,
+ * available = the offset) for offsets that decrease or pass `rows`, whose pair
+ * gets a NaN loss and no gradient. */
+uint32_t pb_preference_loss(pb_context *ctx, const void *d_logits, uint32_t dtype, size_t vocab,
+                            size_t ld, uint32_t rows, double temperature, const uint32_t *d_token,
+                            const uint32_t *d_seq_start, uint32_t pairs,
+                            const float *d_ref_logprob, const float *d_weight, double beta,
+                            double label_smoothing, float *d_loss, float *d_logprob, void *d_grad,
+                            size_t grad_ld, pb_inference_error *d_err, void *stream,
+                            pb_inference_error *err);
 
 /* ---- device arithmetic probes (verification hooks, no reference
  * counterpart): evaluate, on the GPU, the exact binary32 routines the sampler

@@ -12,50 +12,16 @@
 #include <mutex>
 #include <vector>
 
+#include "pb_host.h"
 #include "pb_internal.h"
 #include "pbsample.h"
 
-namespace {
+using pb::clear_error;
+using pb::device_error;
+using pb::DeviceGuard;
+using pb::set_error;
 
 constexpr size_t kRowBytes = (size_t)PB_VOCAB * 4;
-
-void set_error(pb_inference_error* e, uint32_t status, uint32_t domain, uint64_t needed,
-               uint64_t available, uint32_t kind, uint32_t sub) {
-  if (!e) return;
-  e->status = status;
-  e->domain = domain;
-  e->layer = PB_NO_LAYER;
-  e->position = 0;
-  e->tensor_id = PB_NO_TENSOR;
-  e->reserved = 0;
-  e->needed = needed;
-  e->available = available;
-  e->detail = ((uint64_t)kind << 32) | sub;
-}
-
-void clear_error(pb_inference_error* e) {
-  if (e) memset(e, 0, sizeof *e);
-}
-
-uint32_t device_error(pb_inference_error* e, hipError_t code) {
-  set_error(e, PB_DEVICE, PB_DOMAIN_NONE, 0, (uint64_t)code, PB_FIELD_NONE, 0);
-  return PB_DEVICE;
-}
-
-// Restores the caller's current device on scope exit.
-struct DeviceGuard {
-  int saved = -1;
-  explicit DeviceGuard(int device) {
-    if (hipGetDevice(&saved) != hipSuccess) saved = -1;
-    if (device >= 0 && device != saved) (void)hipSetDevice(device);
-  }
-  ~DeviceGuard() {
-    int now = -1;
-    if (saved >= 0 && hipGetDevice(&now) == hipSuccess && now != saved) (void)hipSetDevice(saved);
-  }
-};
-
-}  // namespace
 
 struct pb_context {
   int device = 0;
@@ -68,6 +34,9 @@ struct pb_context {
 
   void* d_lm = nullptr;  // fused LM head workspace
   size_t lm_bytes = 0;
+
+  void* d_scores = nullptr;  // workspace of the row scores and losses
+  size_t scores_bytes = 0;
   // Workspaces that pb_context_reserve outgrew.  A HIP graph captured before
   // the growth still launches kernels on them, so they stay allocated until
   // pb_context_destroy.
@@ -248,7 +217,7 @@ static void release(pb_context* ctx) {
   DeviceGuard guard(ctx->device);
   if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
   free_staging(ctx);
-  void* dev[] = {ctx->d_work, ctx->d_lm, ctx->d_seen};
+  void* dev[] = {ctx->d_work, ctx->d_lm, ctx->d_scores, ctx->d_seen};
   for (void* p : dev)
     if (p) (void)hipFree(p);
   for (void* p : ctx->retired) (void)hipFree(p);
@@ -563,6 +532,17 @@ static uint32_t enqueue_sample(pb_context* ctx, const uint32_t* d_logits, size_t
 namespace pb {
 
 int context_device(const pb_context* ctx) { return ctx->device; }
+
+ScoresAccess scores_access(pb_context* ctx) {
+  std::unique_lock<std::mutex> lock(ctx->mu);
+  return ScoresAccess{std::move(lock), ctx->device, ctx->d_scores, ctx->scores_bytes};
+}
+
+hipError_t scores_reserve(pb_context* ctx, size_t bytes) {
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  DeviceGuard guard(ctx->device);
+  return grow_device(&ctx->d_scores, &ctx->scores_bytes, bytes, &ctx->retired);
+}
 
 uint32_t enqueue_sample_with_workspace(pb_context* ctx, void* work, size_t work_bytes,
                                        const uint32_t* d_logits, size_t vocab, size_t ld,

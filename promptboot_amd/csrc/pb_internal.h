@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "pbsample.h"
 
 namespace pb {
@@ -136,6 +138,18 @@ hipError_t launch_probe(int which, const uint32_t* in, uint32_t* out, size_t n,
 hipError_t launch_wave_selftest(uint32_t* out, hipStream_t stream);
 hipError_t launch_read_probe(const uint32_t* in, size_t n_words, uint32_t* out, uint32_t blocks,
                              bool grid_stride, hipStream_t stream);
+
+// The context's workspace of the row scores, with the context's lock held as
+// long as the object lives (pb_api.cpp).
+struct ScoresAccess {
+  std::unique_lock<std::mutex> lock;
+  int device;
+  void* work;
+  size_t bytes;
+};
+ScoresAccess scores_access(pb_context* ctx);
+// Grows that workspace to `bytes`; takes the lock itself.
+hipError_t scores_reserve(pb_context* ctx, size_t bytes);
 
 // The context's device (pb_api.cpp).
 int context_device(const pb_context* ctx);

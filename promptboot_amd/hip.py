@@ -91,6 +91,12 @@ def set_device(device: int) -> None:
     _ok("hipSetDevice", runtime().hipSetDevice(device))
 
 
+def current_device() -> int:
+    n = _int(0)
+    _ok("hipGetDevice", runtime().hipGetDevice(ctypes.byref(n)))
+    return n.value
+
+
 def synchronize() -> None:
     _ok("hipDeviceSynchronize", runtime().hipDeviceSynchronize())
 

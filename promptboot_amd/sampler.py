@@ -63,6 +63,7 @@ END_OF_TEXT = 151_643
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libpbsample.so"
 
 u32, u64, size_t, vp = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_size_t, ctypes.c_void_p
+f64 = ctypes.c_double
 
 
 class _State(ctypes.Structure):
@@ -144,6 +145,25 @@ EXPORTS = {
     "pb_lmhead_q8_decode_step": (
         u32, [vp, vp, size_t, size_t, size_t, vp, u32, vp, size_t, vp, vp, vp, vp, vp, vp, vp,
               vp, vp, ctypes.POINTER(_Error)]),
+    "pb_context_reserve_scores": (u32, [vp, u32, size_t, ctypes.POINTER(_Error)]),
+    "pb_token_logprobs": (
+        u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, vp, vp, vp, vp,
+              ctypes.POINTER(_Error)]),
+    "pb_token_logprobs_grad": (
+        u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, vp, vp, vp, vp, size_t, vp,
+              ctypes.POINTER(_Error)]),
+    "pb_top_logits": (
+        u32, [vp, vp, u32, size_t, size_t, u32, u32, f64, vp, vp, vp, vp, vp,
+              ctypes.POINTER(_Error)]),
+    "pb_distill_loss": (
+        u32, [vp, vp, u32, size_t, size_t, u32, f64, u32, vp, vp, vp, vp, vp, vp, vp, size_t, vp,
+              vp, ctypes.POINTER(_Error)]),
+    "pb_policy_loss": (
+        u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, vp, vp, vp, f64, f64, f64, vp, vp,
+              vp, vp, size_t, vp, vp, ctypes.POINTER(_Error)]),
+    "pb_preference_loss": (
+        u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, u32, vp, vp, f64, f64, vp, vp, vp,
+              size_t, vp, vp, ctypes.POINTER(_Error)]),
     "pb_decode_draw": (None, [vp, vp, u32, vp, vp]),
     "pb_decode_settle": (u32, [vp, vp, vp, vp, u32]),
     "pb_version": (ctypes.c_char_p, []),
@@ -347,6 +367,7 @@ class BatchSampler:
         st = lib().pb_context_create(device, ctypes.byref(self._ctx))
         if st != OK:
             raise InferenceError(_Error(status=st))
+        self.device = device if device >= 0 else hip.current_device()
         self.segments = 0
         self._rows = 0          # rows reserved under the current slice plan
         self._lm = (0, 0)       # (rows, cols) reserved for the LM head
