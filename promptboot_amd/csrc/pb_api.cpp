@@ -37,6 +37,8 @@ struct pb_context {
 
   void* d_scores = nullptr;  // workspace of the row scores and losses
   size_t scores_bytes = 0;
+  void* d_ticket = nullptr;  // its tickets: a word per row, 0 between calls
+  size_t ticket_bytes = 0;
   // Workspaces that pb_context_reserve outgrew.  A HIP graph captured before
   // the growth still launches kernels on them, so they stay allocated until
   // pb_context_destroy.
@@ -217,7 +219,7 @@ static void release(pb_context* ctx) {
   DeviceGuard guard(ctx->device);
   if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
   free_staging(ctx);
-  void* dev[] = {ctx->d_work, ctx->d_lm, ctx->d_scores, ctx->d_seen};
+  void* dev[] = {ctx->d_work, ctx->d_lm, ctx->d_scores, ctx->d_ticket, ctx->d_seen};
   for (void* p : dev)
     if (p) (void)hipFree(p);
   for (void* p : ctx->retired) (void)hipFree(p);
@@ -535,13 +537,29 @@ int context_device(const pb_context* ctx) { return ctx->device; }
 
 ScoresAccess scores_access(pb_context* ctx) {
   std::unique_lock<std::mutex> lock(ctx->mu);
-  return ScoresAccess{std::move(lock), ctx->device, ctx->d_scores, ctx->scores_bytes};
+  return ScoresAccess{std::move(lock), ctx->device, ctx->d_scores, ctx->scores_bytes,
+                      static_cast<uint32_t*>(ctx->d_ticket), (uint32_t)(ctx->ticket_bytes / 4)};
 }
 
-hipError_t scores_reserve(pb_context* ctx, size_t bytes) {
+hipError_t scores_reserve(pb_context* ctx, uint32_t rows, size_t bytes) {
   std::lock_guard<std::mutex> lock(ctx->mu);
   DeviceGuard guard(ctx->device);
-  return grow_device(&ctx->d_scores, &ctx->scores_bytes, bytes, &ctx->retired);
+  hipError_t e = grow_device(&ctx->d_scores, &ctx->scores_bytes, bytes, &ctx->retired);
+  if (e != hipSuccess || (size_t)rows * 4 <= ctx->ticket_bytes) return e;
+  // the new tickets are 0 before any call can use them
+  void* fresh = nullptr;
+  size_t have = 0;
+  if ((e = grow_device(&fresh, &have, (size_t)rows * 4, &ctx->retired)) != hipSuccess) return e;
+  e = hipMemsetAsync(fresh, 0, have, ctx->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+  if (e != hipSuccess) {
+    (void)hipFree(fresh);
+    return e;
+  }
+  if (ctx->d_ticket) ctx->retired.push_back(ctx->d_ticket);
+  ctx->d_ticket = fresh;
+  ctx->ticket_bytes = have;
+  return hipSuccess;
 }
 
 uint32_t enqueue_sample_with_workspace(pb_context* ctx, void* work, size_t work_bytes,

@@ -146,10 +146,12 @@ struct ScoresAccess {
   int device;
   void* work;
   size_t bytes;
+  uint32_t* ticket;  // one word per row, 0 between calls
+  uint32_t rows;     // words of `ticket`
 };
 ScoresAccess scores_access(pb_context* ctx);
-// Grows that workspace to `bytes`; takes the lock itself.
-hipError_t scores_reserve(pb_context* ctx, size_t bytes);
+// Grows that workspace to `bytes` and the tickets to `rows`; takes the lock itself.
+hipError_t scores_reserve(pb_context* ctx, uint32_t rows, size_t bytes);
 
 // The context's device (pb_api.cpp).
 int context_device(const pb_context* ctx);

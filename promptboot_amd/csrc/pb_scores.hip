@@ -23,6 +23,8 @@ namespace {
 
 constexpr double kLn2 = 0.693147180559945309417232121458;
 constexpr uint32_t kStatsThreads = 512;
+constexpr uint32_t kStatsUnroll = 4;
+constexpr bool kStreamLoads = false;
 constexpr uint32_t kGradThreads = 256;
 constexpr uint32_t kSelectThreads = 512;
 constexpr float kTooBig = 3.0e38f;  // |u| past this has left binary32's range
@@ -97,6 +99,13 @@ __device__ __forceinline__ uint4 load_chunk(const typename E::Raw* p) {
   const Words4 v = *reinterpret_cast<const Loose4*>(p);
   return make_uint4(v.x, v.y, v.z, v.w);
 }
+// The same for data that is not needed again.
+template <typename E>
+__device__ __forceinline__ uint4 stream_chunk(const typename E::Raw* p) {
+  const Words4 v = kStreamLoads ? __builtin_nontemporal_load(reinterpret_cast<const Loose4*>(p))
+                                : *reinterpret_cast<const Loose4*>(p);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
 template <typename E>
 __device__ __forceinline__ void store_chunk(typename E::Raw* p, const uint4& v) {
   *reinterpret_cast<Loose4*>(p) = Words4{v.x, v.y, v.z, v.w};
@@ -130,14 +139,6 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1)
     v = v + __builtin_bit_cast(double, shfl_xor64(__builtin_bit_cast(uint64_t, v), m));
-  return v;
-}
-__device__ __forceinline__ double wave_max_f64(double v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    const double o = __builtin_bit_cast(double, shfl_xor64(__builtin_bit_cast(uint64_t, v), m));
-    v = o > v ? o : v;
-  }
   return v;
 }
 
@@ -206,8 +207,8 @@ __device__ __forceinline__ void unpack(const uint4& v, uint32_t marks, float (&x
 // A thread's sums over its chunks of [lo, hi), chunk i of thread t being
 // element lo + (i kStatsThreads + t) kPer.  The shift is the thread's first
 // chunk's largest u: nothing then underflows that weighs, and where a later u
-// passes it by over 2^127, or the first chunk is masked out, the sum shows it
-// (infinite, or too small) and the thread goes over its chunks again with their
+// passes it by over 100, or the first chunk is masked out, the sum shows it
+// (too large, or too small) and the thread goes over its chunks again with their
 // true maximum.  So the pass does no comparison per element.
 template <typename E, bool kEntropy, bool kTail>
 struct PartScan {
@@ -221,16 +222,16 @@ struct PartScan {
     constexpr uint32_t kPer = E::kPer;
     const uint32_t whole = (hi - lo) / kPer;
     uint32_t i = threadIdx.x;
-    for (; i + 3 * kStatsThreads < whole; i += 4 * kStatsThreads) {
-      uint4 v[4];
+    for (; i + (kStatsUnroll - 1) * kStatsThreads < whole; i += kStatsUnroll * kStatsThreads) {
+      uint4 v[kStatsUnroll];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        v[q] = load_chunk<E>(row + lo + (size_t)(i + q * kStatsThreads) * kPer);
+      for (uint32_t q = 0; q < kStatsUnroll; ++q)
+        v[q] = stream_chunk<E>(row + lo + (size_t)(i + q * kStatsThreads) * kPer);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) chunk(v[q], (i + q * kStatsThreads) * kPer, fn);
+      for (uint32_t q = 0; q < kStatsUnroll; ++q) chunk(v[q], (i + q * kStatsThreads) * kPer, fn);
     }
     for (; i < whole; i += kStatsThreads)
-      chunk(load_chunk<E>(row + lo + (size_t)i * kPer), i * kPer, fn);
+      chunk(stream_chunk<E>(row + lo + (size_t)i * kPer), i * kPer, fn);
     const uint32_t rest = (hi - lo) - whole * kPer;
     if (rest != 0 && i == whole) {
       float x[E::kPer];
@@ -268,7 +269,7 @@ struct PartScan {
       add_chunk<E, kEntropy>(s, x, c);
     });
     *bad = kNone;
-    if (first || (s.sum >= 0x1p-60f && s.sum <= 3.4e38f)) return s;
+    if (first || (s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) return s;
     // again, with the largest u of all
     float top = -__builtin_inff();
     uint32_t at_bad = kNone;
@@ -292,45 +293,49 @@ struct PartScan {
   }
 };
 
-// The workgroup's sums, valid in thread 0.
+// A row's sums (or a part's): sum 2^(u - shift), its moment, the first bad element.
+struct RowSum {
+  double shift, sum, moment;
+  uint32_t bad;
+};
+
+// One RowSum per lane into one, the same in every lane.  The factors between
+// parts come from the 32-bit exp2: the part that holds the largest u has 1.
+__device__ __forceinline__ RowSum wave_join(float shift, double sum, double moment, uint32_t bad) {
+  const bool live = sum > 0.0;
+  const float top = wave_max_f32(live ? shift : -__builtin_inff());
+  const float off = live ? shift - top : 0.0f;
+  const double f = live ? (double)exp2_hw(off) : 0.0;
+  RowSum r;
+  r.sum = wave_sum_f64(f * sum);
+  r.moment = wave_sum_f64(f * (moment + (double)off * sum));
+  r.bad = wave_min_word(bad);
+  r.shift = r.sum > 0.0 ? (double)top : 0.0;
+  return r;
+}
+
+// The workgroup's sums, valid in every lane of wave 0; one barrier.
 struct BlockSum {
   float shift[16];
+  uint32_t bad[16];
   double sum[16];
   double moment[16];
-  uint32_t bad[16];
 };
 template <uint32_t kThreads>
-__device__ __forceinline__ RowPart block_sum(const Acc& s, uint32_t bad, BlockSum& l) {
+__device__ __forceinline__ RowSum block_sum(const Acc& s, uint32_t bad, BlockSum& l) {
   const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
-  const float top = wave_max_f32(s.sum > 0.0f ? s.shift : -__builtin_inff());
-  const float off = s.shift - top;
-  const double f = s.sum > 0.0f ? (double)exp2_hw(off) : 0.0;
-  const double sum = wave_sum_f64(f * (double)s.sum);
-  const double moment =
-      wave_sum_f64(f == 0.0 ? 0.0 : f * ((double)s.moment + (double)off * (double)s.sum));
-  const uint32_t b = wave_min_word(bad);
+  const RowSum w = wave_join(s.shift, (double)s.sum, (double)s.moment, bad);
   if (lane == 0) {
-    l.shift[wave] = top;
-    l.sum[wave] = sum;
-    l.moment[wave] = moment;
-    l.bad[wave] = b;
+    l.shift[wave] = (float)w.shift;
+    l.sum[wave] = w.sum;
+    l.moment[wave] = w.moment;
+    l.bad[wave] = w.bad;
   }
   __syncthreads();
-  RowPart out{0.0f, kNone, 0.0, 0.0};
-  if (threadIdx.x == 0) {
-    float best = l.shift[0];
-    for (uint32_t w = 1; w < kThreads / 64; ++w) best = fmaxf(best, l.shift[w]);
-    for (uint32_t w = 0; w < kThreads / 64; ++w) {
-      out.bad = l.bad[w] < out.bad ? l.bad[w] : out.bad;
-      if (!(l.sum[w] > 0.0)) continue;
-      const double d = (double)l.shift[w] - (double)best;
-      const double g = exp2(d);
-      out.sum += g * l.sum[w];
-      out.moment += g * (l.moment[w] + d * l.sum[w]);
-    }
-    out.shift = out.sum > 0.0 ? best : 0.0f;
-  }
-  return out;
+  if (wave != 0) return w;
+  const bool on = lane < kThreads / 64;
+  return wave_join(on ? l.shift[lane] : 0.0f, on ? l.sum[lane] : 0.0, on ? l.moment[lane] : 0.0,
+                   on ? l.bad[lane] : kNone);
 }
 
 // Marks the teacher's ids that lie in [lo, hi); every thread, then a barrier.
@@ -345,43 +350,7 @@ __device__ __forceinline__ void mark_ids(const ScoreParams& p, uint32_t row, uin
   __syncthreads();
 }
 
-template <typename E, bool kEntropy, bool kTail>
-__global__ __launch_bounds__(kStatsThreads) void stats_kernel(const ScoreParams p) {
-  __shared__ BlockSum l;
-  extern __shared__ uint32_t marks[];
-  const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
-  if (row_unread(p, row)) return;
-  const uint32_t lo = split * p.span;
-  const uint32_t hi = p.vocab - lo < p.span ? p.vocab : lo + p.span;
-  if (kTail) mark_ids(p, row, lo, hi, marks);
-  const PartScan<E, kEntropy, kTail> scan{row_ptr<E>(p, row), marks, lo, hi, p.c};
-  uint32_t bad;
-  const Acc s = scan.run(&bad);
-  const RowPart out = block_sum<kStatsThreads>(s, bad, l);
-  if (threadIdx.x == 0) p.part[(size_t)row * p.splits + split] = out;
-}
-
-// ---- a row's scalars, one wave a row ----
-
-struct RowSum {
-  double shift, sum, moment;  // sum 2^(u - shift)
-  uint32_t bad;
-};
-
-__device__ __forceinline__ RowSum join_parts(const ScoreParams& p, uint32_t row, uint32_t lane) {
-  RowPart v{0.0f, kNone, 0.0, 0.0};
-  if (lane < p.splits) v = p.part[(size_t)row * p.splits + lane];
-  const bool live = v.sum > 0.0;
-  RowSum r;
-  const float top = wave_max_f32(live ? v.shift : -__builtin_inff());
-  r.bad = wave_min_word(v.bad);
-  const double d = live ? (double)v.shift - (double)top : 0.0;
-  const double f = live ? exp2(d) : 0.0;
-  r.sum = wave_sum_f64(f * v.sum);
-  r.moment = wave_sum_f64(f * (v.moment + d * v.sum));
-  r.shift = r.sum > 0.0 ? (double)top : 0.0;
-  return r;
-}
+// ---- a row's scalars, by one wave ----
 
 __device__ __forceinline__ void write_error(pb_inference_error* at, uint32_t status,
                                             uint32_t position, uint64_t needed,
@@ -402,12 +371,6 @@ __device__ __forceinline__ void write_error(pb_inference_error* at, uint32_t sta
 __device__ __forceinline__ void no_error(pb_inference_error* at) {
   if (at == nullptr) return;
   *at = pb_inference_error{0, 0, 0, 0, 0, 0, 0, 0, 0};
-}
-
-// The binary32 bits of a logit, for an error record.
-template <typename E>
-__device__ __forceinline__ uint32_t logit_bits(const ScoreParams& p, uint32_t row, uint32_t id) {
-  return b_of(E::one(row_ptr<E>(p, row)[id]));
 }
 
 __device__ __forceinline__ float nan32() { return f_of(0x7fc00000u); }
@@ -440,12 +403,9 @@ __device__ __forceinline__ RowCoef token_coef(double log2_sum, double slope, dou
   return r;
 }
 
-// ln q[token] in 64 bits.
-template <typename E>
-__device__ __forceinline__ double token_logprob(const ScoreParams& p, uint32_t row, uint32_t token,
-                                                double log2_sum) {
-  const double u = (double)E::one(row_ptr<E>(p, row)[token]) * (double)p.c;
-  return kLn2 * (u - log2_sum);
+// ln q[token] in 64 bits; x the token's logit.
+__device__ __forceinline__ double token_logprob(const ScoreParams& p, float x, double log2_sum) {
+  return kLn2 * ((double)x * (double)p.c - log2_sum);
 }
 
 // Reports what is wrong with a row that was read; true if anything is.
@@ -454,26 +414,48 @@ __device__ __forceinline__ bool row_failed(const ScoreParams& p, uint32_t row, u
                                            double sum, pb_inference_error* at) {
   if (bad == kNone && sum > 0.0) return false;
   const uint32_t index = bad == kNone ? 0u : bad;
-  write_error(at, PB_NONFINITE_OUTPUT, row, 0, logit_bits<E>(p, row, index), PB_FIELD_FINITE,
-              index);
+  write_error(at, PB_NONFINITE_OUTPUT, row, 0, b_of(E::one(row_ptr<E>(p, row)[index])),
+              PB_FIELD_FINITE, index);
   return true;
 }
 
+// What a row with one token needs beside its sums, requested before them.
+struct TokenRow {
+  uint32_t token;
+  float x;       // the token's logit
+  float weight;
+  float old_logprob, advantage, ref_logprob;
+};
 template <typename E>
-__device__ void finish_policy(const ScoreParams& p, uint32_t row, const RowSum& r, uint32_t lane) {
-  if (lane != 0) return;
-  const uint32_t token = p.token[row];
-  const float w = p.weight ? p.weight[row] : 1.0f;
+__device__ __forceinline__ TokenRow token_row(const ScoreParams& p, uint32_t row) {
+  TokenRow t{p.token[row], 0.0f, 1.0f, 0.0f, 0.0f, 0.0f};
+  if (t.token < p.vocab) t.x = E::one(row_ptr<E>(p, row)[t.token]);
+  if (p.mode == kModePolicy) {
+    if (p.weight != nullptr) t.weight = p.weight[row];
+    t.old_logprob = p.old_logprob[row];
+    t.advantage = p.advantage[row];
+    if (p.ref_logprob != nullptr) t.ref_logprob = p.ref_logprob[row];
+  }
+  return t;
+}
+
+// The finish_ functions write a row's outputs and return what its gradient
+// needs; lane 0's result counts.
+
+template <typename E>
+__device__ __forceinline__ RowCoef finish_policy(const ScoreParams& p, uint32_t row,
+                                                 const RowSum& r, const TokenRow& t) {
   pb_inference_error* at = p.err ? p.err + row : nullptr;
   float loss = 0.0f, logprob = 0.0f, kl_out = 0.0f;
   RowCoef coef{};
   coef.state = kRowZero;
-  if (token == PB_NO_TOKEN || w == 0.0f) {
+  if (lane_id() != 0) return coef;
+  if (t.token == PB_NO_TOKEN || t.weight == 0.0f) {
     no_error(at);
   } else {
-    bool failed = token >= p.vocab;
+    bool failed = t.token >= p.vocab;
     if (failed)
-      write_error(at, PB_TOKEN_ID, row, p.vocab, token, PB_FIELD_TOKEN, 0);
+      write_error(at, PB_TOKEN_ID, row, p.vocab, t.token, PB_FIELD_TOKEN, 0);
     else
       failed = row_failed<E>(p, row, r.bad, r.sum, at);
     if (failed) {
@@ -482,8 +464,8 @@ __device__ void finish_policy(const ScoreParams& p, uint32_t row, const RowSum& 
     } else {
       no_error(at);
       const double log2_sum = r.shift + log2(r.sum);
-      const double lp = token_logprob<E>(p, row, token, log2_sum);
-      const double ratio = exp(lp - (double)p.old_logprob[row]), adv = (double)p.advantage[row];
+      const double lp = token_logprob(p, t.x, log2_sum);
+      const double ratio = exp(lp - (double)t.old_logprob), adv = (double)t.advantage;
       const double low = 1.0 - p.clip_low, high = 1.0 + p.clip_high;
       const double kept = ratio < low ? low : ratio > high ? high : ratio;
       const double open = ratio * adv, shut = kept * adv;
@@ -492,7 +474,7 @@ __device__ void finish_policy(const ScoreParams& p, uint32_t row, const RowSum& 
       if (open != open) l = slope = open;
       double kl = 0.0;
       if (p.ref_logprob != nullptr) {
-        const double gap = (double)p.ref_logprob[row] - lp;
+        const double gap = (double)t.ref_logprob - lp;
         const double rise = expm1(gap);
         kl = rise - gap;
         if (p.kl_coef != 0.0) {
@@ -503,38 +485,37 @@ __device__ void finish_policy(const ScoreParams& p, uint32_t row, const RowSum& 
       loss = (float)l;
       logprob = (float)lp;
       kl_out = (float)kl;
-      coef = token_coef(log2_sum, slope * (double)w * p.inv_t, lp, token);
+      coef = token_coef(log2_sum, slope * (double)t.weight * p.inv_t, lp, t.token);
     }
   }
   p.loss[row] = loss;
   if (p.logprob) p.logprob[row] = logprob;
   if (p.kl) p.kl[row] = kl_out;
-  if (p.grad) p.coef[row] = coef;
+  return coef;
 }
 
 template <typename E>
-__device__ void finish_logprobs(const ScoreParams& p, uint32_t row, const RowSum& r,
-                                uint32_t lane) {
-  if (lane != 0) return;
-  const uint32_t token = p.token[row];
+__device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t row,
+                                                const RowSum& r, const TokenRow& t) {
+  if (lane_id() != 0) return;
   pb_inference_error* at = p.err ? p.err + row : nullptr;
   float logprob = 0.0f, lse = 0.0f, entropy = 0.0f;
-  if (token == PB_NO_TOKEN) {
+  if (t.token == PB_NO_TOKEN) {
     no_error(at);
   } else {
-    bool failed = token >= p.vocab;
+    bool failed = t.token >= p.vocab;
     if (failed)
-      write_error(at, PB_TOKEN_ID, row, p.vocab, token, PB_FIELD_TOKEN, 0);
+      write_error(at, PB_TOKEN_ID, row, p.vocab, t.token, PB_FIELD_TOKEN, 0);
     else
       failed = row_failed<E>(p, row, r.bad, r.sum, at);
     if (failed) {
       logprob = lse = entropy = nan32();
     } else {
       no_error(at);
-      const double log2_sum = r.shift + log2(r.sum);
-      logprob = (float)token_logprob<E>(p, row, token, log2_sum);
+      const double log2_own = log2(r.sum), log2_sum = r.shift + log2_own;
+      logprob = (float)token_logprob(p, t.x, log2_sum);
       lse = (float)(kLn2 * log2_sum);
-      entropy = (float)(kLn2 * (log2(r.sum) - r.moment / r.sum));
+      entropy = (float)(kLn2 * (log2_own - r.moment / r.sum));
     }
   }
   p.logprob[row] = logprob;
@@ -542,170 +523,311 @@ __device__ void finish_logprobs(const ScoreParams& p, uint32_t row, const RowSum
   if (p.entropy) p.entropy[row] = entropy;
 }
 
+// The preference loss' rows: ln q[token] and log2_sum for the pair's pass, or
+// what is wrong with the row.
 template <typename E>
-__device__ void finish_distill(const ScoreParams& p, uint32_t row, RowSum r, uint32_t lane) {
+__device__ __forceinline__ void finish_pair_row(const ScoreParams& p, uint32_t row,
+                                                const RowSum& r, const TokenRow& t) {
+  if (lane_id() != 0) return;
+  RowCoef coef{};
+  coef.state = kRowUntouched;
+  coef.token = r.bad;
+  coef.mass = r.sum;
+  if (r.bad == kNone && r.sum > 0.0) {
+    coef.log2_sum = r.shift + log2(r.sum);
+    coef.norm = token_logprob(p, t.x, coef.log2_sum);
+  }
+  p.coef[row] = coef;
+}
+
+// What the teacher's list says, the same in every lane: its log-sum-exp, its
+// mass sum p, sum p ln p, sum p u, and the student's weight of the listed ids,
+// sum 2^(u - top_u).
+struct ListSum {
+  double norm, mass, plogp, pu, listed, top_u;
+  uint32_t bad_id, bad_logit, bad_x;
+  uint32_t any;
+};
+
+// A row's list, two entries a lane (i = lane, lane + 64); kNone past its end.
+struct ListLanes {
+  uint32_t id[2];
+  float logit[2];
+  float lse;
+};
+__device__ __forceinline__ ListLanes load_list(const ScoreParams& p, uint32_t row, uint32_t lane) {
+  ListLanes l;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t i = lane + 64u * h;
+    const size_t at = (size_t)row * p.k + i;
+    l.id[h] = i < p.k ? p.teacher_id[at] : kNone;
+    l.logit[h] = i < p.k ? p.teacher_logit[at] : 0.0f;
+  }
+  l.lse = p.teacher_lse != nullptr ? p.teacher_lse[row] : 0.0f;
+  return l;
+}
+
+// The part of the sums that needs no student; pr: the lane's p.
+__device__ __forceinline__ ListSum sum_teacher(const ScoreParams& p, const ListLanes& l,
+                                               uint32_t lane, double (&pr)[2]) {
+  uint32_t seen[2] = {0, 0};  // entries of the same id, the entry itself included
+#pragma unroll
+  for (uint32_t j = 0; j < 64; ++j) {
+    const uint32_t a = bcast32(l.id[0], j);
+    seen[0] += a == l.id[0] ? 1u : 0u;
+    seen[1] += a == l.id[1] ? 1u : 0u;
+  }
+  if (p.k > 64) {
+#pragma unroll
+    for (uint32_t j = 0; j < 64; ++j) {
+      const uint32_t a = bcast32(l.id[1], j);
+      seen[0] += a == l.id[0] ? 1u : 0u;
+      seen[1] += a == l.id[1] ? 1u : 0u;
+    }
+  }
+  ListSum s{};
+  s.bad_id = s.bad_logit = s.bad_x = kNone;
+  float top_t = -__builtin_inff();
+  bool on[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t i = lane + 64u * h;
+    on[h] = l.id[h] != kNone;
+    if (on[h] && (l.id[h] >= p.vocab || seen[h] > 1u)) {
+      s.bad_id = i < s.bad_id ? i : s.bad_id;
+      on[h] = false;
+    }
+    if (on[h] && !(l.logit[h] < __builtin_inff())) s.bad_logit = i < s.bad_logit ? i : s.bad_logit;
+    if (on[h]) top_t = fmaxf(top_t, l.logit[h]);
+  }
+  s.bad_id = wave_min_word(s.bad_id);
+  s.bad_logit = wave_min_word(s.bad_logit);
+  if (p.teacher_lse != nullptr && !__builtin_isfinite(l.lse))
+    s.bad_logit = p.k < s.bad_logit ? p.k : s.bad_logit;
+  top_t = wave_max_f32(top_t);
+  s.any = top_t > -__builtin_inff();
+  pr[0] = pr[1] = 0.0;
+  if (!s.any) return s;
+  if (p.teacher_lse != nullptr) {
+    s.norm = (double)l.lse;
+  } else {
+    double sum = 0.0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      sum += on[h] ? exp(((double)l.logit[h] - (double)top_t) * p.inv_t) : 0.0;
+    s.norm = (double)top_t * p.inv_t + log(wave_sum_f64(sum));
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const double lp = (double)l.logit[h] * p.inv_t - s.norm;
+    pr[h] = on[h] ? exp(lp) : 0.0;
+    s.mass += pr[h];
+    if (pr[h] > 0.0) s.plogp += pr[h] * lp;
+  }
+  s.mass = wave_sum_f64(s.mass);
+  s.plogp = wave_sum_f64(s.plogp);
+  return s;
+}
+
+// The part that needs the student's logits x of the listed ids.
+__device__ __forceinline__ void sum_student(const ScoreParams& p, const uint32_t (&id)[2],
+                                            const float (&x)[2], const double (&pr)[2],
+                                            ListSum& s) {
+  float top_x = -__builtin_inff();
+  double pu = 0.0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (id[h] >= p.vocab) continue;
+    if (!(x[h] * p.c < kTooBig)) s.bad_x = id[h] < s.bad_x ? id[h] : s.bad_x;
+    top_x = fmaxf(top_x, x[h]);
+    if (pr[h] > 0.0) pu += pr[h] * ((double)x[h] * (double)p.c);
+  }
+  s.pu = wave_sum_f64(pu);
+  s.bad_x = wave_min_word(s.bad_x);
+  top_x = wave_max_f32(top_x);
+  s.top_u = top_x * p.c > -kTooBig ? (double)top_x * (double)p.c : -__builtin_inf();
+  if (p.teacher_lse == nullptr || !(s.top_u > -__builtin_inf())) return;
+  double listed = 0.0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (id[h] < p.vocab) listed += exp2((double)x[h] * (double)p.c - s.top_u);
+  s.listed = wave_sum_f64(listed);
+}
+
+// A listed id's gradient.
+__device__ __forceinline__ float listed_grad(const ScoreParams& p, const RowCoef& r, float x,
+                                             float logit) {
+  const double q = exp2((double)x * (double)p.c - r.log2_sum);
+  const double t = exp((double)logit * p.inv_t - r.norm);
+  return (float)(r.weight * (r.mass * q - t));
+}
+
+template <typename E>
+__device__ __forceinline__ RowCoef finish_distill(const ScoreParams& p, uint32_t row,
+                                                  const RowSum& r, const ListSum& s) {
   pb_inference_error* at = p.err ? p.err + row : nullptr;
   const float w = p.weight ? p.weight[row] : 1.0f;
   RowCoef coef{};
   coef.state = kRowZero;
+  if (lane_id() != 0) return coef;
   float loss = 0.0f, lse = 0.0f;
   if (w == 0.0f) {
-    if (lane == 0) no_error(at);
+    no_error(at);
   } else {
     const bool rest_bucket = p.teacher_lse != nullptr;
-    const uint32_t* ids = p.teacher_id + (size_t)row * p.k;
-    const float* logits = p.teacher_logit + (size_t)row * p.k;
-    // two list entries a lane
-    uint32_t id[2];
-    double t[2], u[2], pr[2];
-    uint32_t bad_id = kNone, bad_logit = kNone, bad_x = kNone;
-    double top_t = -__builtin_inf(), top_u = r.sum > 0.0 ? r.shift : -__builtin_inf();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t i = lane + 64u * h;
-      id[h] = i < p.k ? ids[i] : kNone;
-      t[h] = u[h] = -__builtin_inf();
-      if (id[h] == kNone) continue;
-      bool bad = id[h] >= p.vocab;
-      for (uint32_t j = 0; j < p.k; ++j) bad |= j != i && ids[j] == id[h];
-      if (bad) {
-        bad_id = i < bad_id ? i : bad_id;
-        continue;
-      }
-      const float tf = logits[i];
-      if (!(tf < __builtin_inff())) bad_logit = i < bad_logit ? i : bad_logit;
-      t[h] = (double)tf * p.inv_t;
-      const float x = E::one(row_ptr<E>(p, row)[id[h]]);
-      if (!(x * p.c < kTooBig)) bad_x = id[h] < bad_x ? id[h] : bad_x;
-      u[h] = (double)x * (double)p.c;
-      top_t = t[h] > top_t ? t[h] : top_t;
-      top_u = u[h] > top_u ? u[h] : top_u;
-    }
-    bad_id = wave_min_word(bad_id);
-    bad_logit = wave_min_word(bad_logit);
-    bad_x = wave_min_word(bad_x);
-    if (rest_bucket && !__builtin_isfinite(p.teacher_lse[row]))
-      bad_logit = p.k < bad_logit ? p.k : bad_logit;
-    top_t = wave_max_f64(top_t);
-    top_u = wave_max_f64(top_u);
     // the student's sum over the listed ids joins the rest's
     double rest = r.sum, whole = r.sum, shift = r.shift;
-    if (rest_bucket && top_u > -__builtin_inf()) {
-      const double f = r.sum > 0.0 ? exp2(r.shift - top_u) : 0.0;
-      double listed = 0.0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) listed += u[h] > -__builtin_inf() ? exp2(u[h] - top_u) : 0.0;
-      rest = f * r.sum;
-      whole = rest + wave_sum_f64(listed);
-      shift = top_u;
+    if (rest_bucket && s.top_u > -__builtin_inf()) {
+      shift = r.sum > 0.0 && r.shift > s.top_u ? r.shift : s.top_u;
+      rest = r.sum > 0.0 ? r.sum * exp2(r.shift - shift) : 0.0;
+      whole = rest + s.listed * exp2(s.top_u - shift);
     }
-    const uint32_t bad = bad_x < r.bad ? bad_x : r.bad;
-    bool failed = false;
-    if (bad_id != kNone) {
-      failed = true;
-      if (lane == 0)
-        write_error(at, PB_TOKEN_ID, row, p.vocab, ids[bad_id], PB_FIELD_TOKEN, bad_id);
-    } else if (bad_logit != kNone) {
-      failed = true;
-      if (lane == 0)
-        write_error(at, PB_NONFINITE_INPUT, row, 0,
-                    b_of(bad_logit == p.k ? p.teacher_lse[row] : logits[bad_logit]),
-                    PB_FIELD_FINITE, bad_logit);
-    } else if (bad != kNone || !(whole > 0.0)) {
-      failed = true;
-      if (lane == 0) row_failed<E>(p, row, bad, whole, at);
-    }
+    const uint32_t bad = s.bad_x < r.bad ? s.bad_x : r.bad;
+    bool failed = true;
+    if (s.bad_id != kNone)
+      write_error(at, PB_TOKEN_ID, row, p.vocab, p.teacher_id[(size_t)row * p.k + s.bad_id],
+                  PB_FIELD_TOKEN, s.bad_id);
+    else if (s.bad_logit != kNone)
+      write_error(at, PB_NONFINITE_INPUT, row, 0,
+                  b_of(s.bad_logit == p.k ? p.teacher_lse[row]
+                                          : p.teacher_logit[(size_t)row * p.k + s.bad_logit]),
+                  PB_FIELD_FINITE, s.bad_logit);
+    else
+      failed = row_failed<E>(p, row, bad, whole, at);
     if (failed) {
       loss = lse = nan32();
       coef.state = kRowNan;
     } else {
-      if (lane == 0) no_error(at);
+      no_error(at);
       const double log2_sum = shift + log2(whole);
       lse = (float)(kLn2 * log2_sum);
-      const bool any = top_t > -__builtin_inf();
-      double norm = 0.0, mass = 0.0, l = 0.0;
-      if (rest_bucket) {
-        norm = (double)p.teacher_lse[row];
-      } else if (any) {
-        double sum = 0.0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) sum += id[h] != kNone ? exp(t[h] - top_t) : 0.0;
-        norm = top_t + log(wave_sum_f64(sum));
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        pr[h] = any && id[h] != kNone ? exp(t[h] - norm) : 0.0;
-        mass += pr[h];
-        if (pr[h] > 0.0) l += pr[h] * ((t[h] - norm) - kLn2 * (u[h] - log2_sum));
-      }
-      mass = wave_sum_f64(mass);
-      l = wave_sum_f64(l);
-      double off = mass;  // what q is multiplied by off the list
-      if (rest_bucket && any) {
-        const double left = mass < 1.0 ? 1.0 - mass : 0.0;
-        if (left > 0.0 && rest > 0.0) {
-          l += left * (log(left) - log(rest / whole));
-          mass += left;
-          off = mass - left * (whole / rest);
+      if (s.any) {
+        double l = s.plogp - kLn2 * (s.pu - s.mass * log2_sum), mass = s.mass;
+        double off = mass;  // what q is multiplied by off the list
+        if (rest_bucket) {
+          const double left = mass < 1.0 ? 1.0 - mass : 0.0;
+          if (left > 0.0 && rest > 0.0) {
+            l += left * log(left * whole / rest);
+            mass += left;
+            off = mass - left * (whole / rest);
+          }
         }
-      }
-      if (any) {
         loss = (float)l;
         const double weight = (double)w * p.inv_t;
         coef.state = weight == weight ? kRowNormal : kRowNan;
         set_factors(coef, log2_sum, weight * off, 0.0);
-        coef.norm = norm;
+        coef.norm = s.norm;
         coef.mass = mass;
         coef.weight = weight;
         coef.token = kNone;
       }
     }
   }
-  if (lane == 0) {
-    p.loss[row] = loss;
-    if (p.lse) p.lse[row] = lse;
-    if (p.grad) p.coef[row] = coef;
+  p.loss[row] = loss;
+  if (p.lse) p.lse[row] = lse;
+  return coef;
+}
+
+// A row's scalars from its sums; wave 0, every lane.
+template <typename E>
+__device__ __forceinline__ void finish_row(const ScoreParams& p, uint32_t row, const RowSum& r) {
+  const uint32_t lane = lane_id();
+  if (p.mode == kModeDistill) {
+    ListSum s{};
+    if (!row_unread(p, row)) {
+      const ListLanes l = load_list(p, row, lane);
+      float x[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        x[h] = l.id[h] < p.vocab ? E::one(row_ptr<E>(p, row)[l.id[h]]) : 0.0f;
+      double pr[2];
+      s = sum_teacher(p, l, lane, pr);
+      sum_student(p, l.id, x, pr, s);
+    }
+    const RowCoef c = finish_distill<E>(p, row, r, s);
+    if (lane == 0 && p.grad) p.coef[row] = c;
+    return;
+  }
+  const TokenRow t = token_row<E>(p, row);
+  if (p.mode == kModePolicy) {
+    const RowCoef c = finish_policy<E>(p, row, r, t);
+    if (lane == 0 && p.grad) p.coef[row] = c;
+  } else if (p.mode == kModePreference) {
+    finish_pair_row<E>(p, row, r, t);
+  } else {
+    finish_logprobs<E>(p, row, r, t);
   }
 }
 
-template <typename E>
-__global__ __launch_bounds__(256) void finish_kernel(const ScoreParams p) {
-  const uint32_t row = blockIdx.x * 4u + (threadIdx.x >> 6), lane = lane_id();
-  if (row >= p.rows) return;
-  RowSum r{0.0, 0.0, 0.0, kNone};
-  if (!row_unread(p, row)) r = join_parts(p, row, lane);
-  if (p.mode == kModePolicy)
-    finish_policy<E>(p, row, r, lane);
-  else if (p.mode == kModeDistill)
-    finish_distill<E>(p, row, r, lane);
-  else
-    finish_logprobs<E>(p, row, r, lane);
+// Parts of a row pass between workgroups of one launch, which may run on XCDs
+// with an L2 each: every word goes and comes at the device's scope, past those
+// caches, and a part's words are acknowledged (vmcnt 0) before its ticket is
+// taken.  A device-wide fence instead writes back and drops the whole L2: the
+// 70 rows x 13 parts of 50,257 ids took 21.9 us with it.
+__device__ __forceinline__ void publish_part(RowPart* at, const RowSum& r) {
+  uint64_t* w = reinterpret_cast<uint64_t*>(at);
+  const uint64_t head = (uint64_t)b_of((float)r.shift) | ((uint64_t)r.bad << 32);
+  __hip_atomic_store(w, head, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store(w + 1, __builtin_bit_cast(uint64_t, r.sum), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store(w + 2, __builtin_bit_cast(uint64_t, r.moment), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ RowPart collect_part(const RowPart* at) {
+  const uint64_t* w = reinterpret_cast<const uint64_t*>(at);
+  const uint64_t head = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t sum = __hip_atomic_load(w + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t moment = __hip_atomic_load(w + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return RowPart{f_of((uint32_t)head), (uint32_t)(head >> 32), __builtin_bit_cast(double, sum),
+                 __builtin_bit_cast(double, moment)};
+}
+// Publishes this part of a row; true in the wave whose part was the last.
+__device__ __forceinline__ bool last_part(const ScoreParams& p, uint32_t row, uint32_t split,
+                                          const RowSum& r) {
+  uint32_t before = 0;
+  if (lane_id() == 0) {
+    publish_part(p.part + (size_t)row * p.splits + split, r);
+    before = __hip_atomic_fetch_add(&p.ticket[row], 1u, __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (bcast32(before, 0) != p.splits - 1u) return false;
+  if (lane_id() == 0) p.ticket[row] = 0;
+  return true;
+}
+
+// The statistics pass.  A row's parts leave their sums in the workspace, and
+// the workgroup that comes last (by the row's ticket, which it sets back to 0)
+// joins them and works out the row's scalars, so that they need no launch of
+// their own.
+template <typename E, bool kEntropy, bool kTail>
+__global__ __launch_bounds__(kStatsThreads) void stats_kernel(const ScoreParams p) {
+  __shared__ BlockSum l;
+  extern __shared__ uint32_t marks[];
+  const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
+  if (row_unread(p, row)) {
+    if (split == 0 && threadIdx.x < 64) finish_row<E>(p, row, RowSum{0.0, 0.0, 0.0, kNone});
+    return;
+  }
+  const uint32_t lo = split * p.span;
+  const uint32_t hi = p.vocab - lo < p.span ? p.vocab : lo + p.span;
+  if (kTail) mark_ids(p, row, lo, hi, marks);
+  const PartScan<E, kEntropy, kTail> scan{row_ptr<E>(p, row), marks, lo, hi, p.c};
+  uint32_t bad;
+  const Acc s = scan.run(&bad);
+  RowSum r = block_sum<kStatsThreads>(s, bad, l);
+  if (threadIdx.x >= 64) return;
+  if (p.splits > 1) {
+    if (!last_part(p, row, split, r)) return;
+    RowPart v{0.0f, kNone, 0.0, 0.0};
+    if (lane_id() < p.splits) v = collect_part(p.part + (size_t)row * p.splits + lane_id());
+    r = wave_join(v.shift, v.sum, v.moment, v.bad);
+  }
+  finish_row<E>(p, row, r);
 }
 
 // ---- preference loss: one workgroup a pair ----
-
-__global__ __launch_bounds__(256) void clear_coef_kernel(const ScoreParams p) {
-  const uint32_t row = blockIdx.x * 256u + threadIdx.x;
-  if (row < p.rows) p.coef[row].state = kRowUntouched;
-}
-
-// A row's log2 sum by one thread.
-__device__ __forceinline__ double join_parts_serial(const ScoreParams& p, uint32_t row,
-                                                    uint32_t* bad, double* sum) {
-  const RowPart* v = p.part + (size_t)row * p.splits;
-  float top = -__builtin_inff();
-  for (uint32_t i = 0; i < p.splits; ++i)
-    if (v[i].sum > 0.0) top = fmaxf(top, v[i].shift);
-  double s = 0.0;
-  uint32_t b = kNone;
-  for (uint32_t i = 0; i < p.splits; ++i) {
-    b = v[i].bad < b ? v[i].bad : b;
-    if (v[i].sum > 0.0) s += v[i].sum * exp2((double)v[i].shift - (double)top);
-  }
-  *bad = b;
-  *sum = s;
-  return (double)top + log2(s);
-}
 
 template <typename E>
 __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
@@ -732,16 +854,11 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
     for (uint32_t row = a + threadIdx.x; row < e; row += 256u) {
       const uint32_t token = p.token[row];
       if (token == PB_NO_TOKEN) continue;
-      double lp = 0.0, sum = 0.0;
-      uint32_t bad = kNone;
-      bool wrong = token >= p.vocab;
-      if (!wrong) {
-        const double log2_sum = join_parts_serial(p, row, &bad, &sum);
-        wrong = bad != kNone || !(sum > 0.0);
-        if (!wrong) lp = token_logprob<E>(p, row, token, log2_sum);
-      }
-      if (wrong) failed = row < failed ? row : failed;
-      mine[row < b ? 0 : 1] += lp;
+      const RowCoef& v = p.coef[row];
+      if (token >= p.vocab || v.token != kNone || !(v.mass > 0.0))
+        failed = row < failed ? row : failed;
+      else
+        mine[row < b ? 0 : 1] += v.norm;
     }
   }
   const double c = wave_sum_f64(mine[0]), d = wave_sum_f64(mine[1]);
@@ -766,10 +883,7 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
       if (token >= p.vocab) {
         write_error(at, PB_TOKEN_ID, first, p.vocab, token, PB_FIELD_TOKEN, 0);
       } else {
-        uint32_t bad = kNone;
-        double sum = 0.0;
-        (void)join_parts_serial(p, first, &bad, &sum);
-        row_failed<E>(p, first, bad, sum, at);
+        row_failed<E>(p, first, p.coef[first].token, p.coef[first].mass, at);
       }
       loss = slope = l[0] = l[1] = (double)nan32();
     } else {
@@ -804,11 +918,8 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
     if (slope != slope) {
       coef.state = kRowNan;
     } else if (token != PB_NO_TOKEN && w != 0.0f) {
-      uint32_t bad;
-      double sum;
-      const double log2_sum = join_parts_serial(p, row, &bad, &sum);
-      coef = token_coef(log2_sum, row < b ? slope : -slope,
-                        token_logprob<E>(p, row, token, log2_sum), token);
+      const RowCoef& v = p.coef[row];
+      coef = token_coef(v.log2_sum, row < b ? slope : -slope, v.norm, token);
     }
     p.coef[row] = coef;
   }
@@ -833,7 +944,7 @@ __global__ __launch_bounds__(256) void logprobs_coef_kernel(const ScoreParams p)
       r.state = kRowNormal;
       // g (delta - q) - ge q (ln q + H)
       set_factors(r, log2_sum, (-g - ge * h) * p.inv_t, -ge * p.inv_t);
-      const double lp = token_logprob<E>(p, row, token, log2_sum), q = exp(lp);
+      const double lp = token_logprob(p, E::one(row_ptr<E>(p, row)[token]), log2_sum), q = exp(lp);
       r.token = token;
       r.patch = (float)((g * -expm1(lp) - (q > 0.0 ? ge * q * (lp + h) : 0.0)) * p.inv_t);
     }
@@ -851,6 +962,22 @@ __device__ __forceinline__ float grad_of(float x, float c, const RowCoef& r) {
   return e * fmaf(fmaxf(a, -1000.0f), r.beta, r.alpha);
 }
 
+// A gradient row's elements lo .. hi - 1 (out: its first) of a row that has none, or that failed.
+template <typename E, uint32_t kThreads>
+__device__ __forceinline__ void fill_row(typename E::Raw* out, uint32_t lo, uint32_t hi,
+                                         uint32_t state) {
+  constexpr uint32_t kPer = E::kPer;
+  const float f = state == kRowZero ? 0.0f : nan32();
+  float fill[kPer];
+#pragma unroll
+  for (uint32_t e = 0; e < kPer; ++e) fill[e] = f;
+  const uint4 v = E::pack(fill);
+  const uint32_t whole = (hi - lo) / kPer;
+  for (uint32_t i = threadIdx.x; i < whole; i += kThreads)
+    store_chunk<E>(out + lo + (size_t)i * kPer, v);
+  for (uint32_t j = lo + whole * kPer + threadIdx.x; j < hi; j += kThreads) out[j] = E::raw(f);
+}
+
 template <typename E, bool kBeta>
 __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p) {
   using Raw = typename E::Raw;
@@ -864,14 +991,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
   Raw* out = static_cast<Raw*>(p.grad) + (size_t)row * p.grad_ld + lo;
   const uint32_t n = hi - lo, whole = n / kPer;
   if (r.state != kRowNormal) {
-    const float f = r.state == kRowZero ? 0.0f : nan32();
-    float fill[kPer];
-#pragma unroll
-    for (uint32_t e = 0; e < kPer; ++e) fill[e] = f;
-    const uint4 v = E::pack(fill);
-    for (uint32_t i = threadIdx.x; i < whole; i += kGradThreads)
-      store_chunk<E>(out + (size_t)i * kPer, v);
-    for (uint32_t j = whole * kPer + threadIdx.x; j < n; j += kGradThreads) out[j] = E::raw(f);
+    fill_row<E, kGradThreads>(out, 0, n, r.state);
     return;
   }
   // The listed ids' gradients come from scalars in 64 bits; their logits are
@@ -884,10 +1004,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
       const uint32_t id = p.teacher_id[entry];
       if (id >= lo && id < hi) {
         at = id - lo;
-        const double u = (double)E::one(in[at]) * (double)p.c;
-        const double q = exp2(u - r.log2_sum);
-        const double t = exp((double)p.teacher_logit[entry] * p.inv_t - r.norm);
-        patch = (float)(r.weight * (r.mass * q - t));
+        patch = listed_grad(p, r, E::one(in[at]), p.teacher_logit[entry]);
       }
     }
     __syncthreads();
@@ -906,6 +1023,258 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
     out[j] = E::raw(grad_of<E, kBeta>(E::one(in[j]), p.c, r));
   __syncthreads();  // the patches come after the stores they replace
   if (at != kNone) out[at] = E::raw(patch);
+}
+
+// ---- a row's loss and gradient in one launch ----
+// One workgroup takes a whole row and keeps its first kHeld chunks a thread in
+// registers between the statistics and the gradient: a row of 163,840 16-bit
+// logits is read from memory once.  What lies beyond (32-bit rows over 81,920
+// ids) is read again.  The row's special elements (its token, or the teacher's
+// list) hang in a chain on the thread that holds them, which leaves their logits
+// for the row's scalars and writes their gradients, so that no store waits for
+// another.
+
+constexpr uint32_t kHeld = 20;
+
+struct FusedShared {
+  BlockSum sums;
+  ListSum list;
+  RowCoef coef;
+  double pr[PB_TOP_LOGITS_MAX];
+  uint32_t id[PB_TOP_LOGITS_MAX];
+  uint32_t next[PB_TOP_LOGITS_MAX];
+  float x[PB_TOP_LOGITS_MAX];
+  float logit[PB_TOP_LOGITS_MAX];
+};
+
+template <typename E, uint32_t kThreads, bool kTail>
+struct FusedRow {
+  static constexpr uint32_t kPer = E::kPer;
+  using Raw = typename E::Raw;
+  const ScoreParams& p;
+  FusedShared& l;
+  const Raw* in;
+  uint32_t whole, first_entry;
+  uint64_t mine;  // bit c: the thread's chunk c holds a special element
+
+  // Takes the special elements out of chunk c (i = its index in the row).
+  __device__ __forceinline__ void leave(float (&x)[E::kPer], uint32_t i) const {
+    for (uint32_t e = first_entry; e != kNone; e = l.next[e]) {
+      const uint32_t j = l.id[e] - i * kPer;
+#pragma unroll
+      for (uint32_t q = 0; q < kPer; ++q)
+        if (q == j) {
+          l.x[e] = x[q];
+          if (kTail) x[q] = -__builtin_inff();
+        }
+    }
+  }
+  // Puts their gradients in.
+  __device__ __forceinline__ void patch(float (&g)[E::kPer], uint32_t i, const RowCoef& r) const {
+    for (uint32_t e = first_entry; e != kNone; e = l.next[e]) {
+      const uint32_t j = l.id[e] - i * kPer;
+      if (j >= kPer) continue;
+      const float f = p.mode == kModeDistill ? listed_grad(p, r, l.x[e], l.logit[e]) : r.patch;
+#pragma unroll
+      for (uint32_t q = 0; q < kPer; ++q)
+        if (q == j) g[q] = f;
+    }
+  }
+  __device__ __forceinline__ bool special(uint32_t c) const { return (mine >> c) & 1u; }
+
+  // The partial chunk behind the whole ones, by the thread whose turn it is.
+  __device__ __forceinline__ uint32_t rest() const { return p.vocab - whole * kPer; }
+  __device__ __forceinline__ bool has_rest() const {
+    return rest() != 0 && threadIdx.x == whole % kThreads;
+  }
+  __device__ __forceinline__ void load_rest(float (&x)[E::kPer]) const {
+#pragma unroll
+    for (uint32_t q = 0; q < kPer; ++q)
+      x[q] = q < rest() ? E::one(in[(size_t)whole * kPer + q]) : -__builtin_inff();
+  }
+
+  // fn(x, i) for every chunk of the thread, the special elements left out.
+  template <typename Fn>
+  __device__ __forceinline__ void each(const uint4 (&v)[kHeld], Fn fn) const {
+    float x[E::kPer];
+#pragma unroll
+    for (uint32_t c = 0; c < kHeld; ++c) {
+      const uint32_t i = c * kThreads + threadIdx.x;
+      if (i < whole) {
+        unpack<E, false>(v[c], 0, x);
+        if (special(c)) leave(x, i);
+        fn(x, i);
+      }
+    }
+    for (uint32_t c = kHeld, i = kHeld * kThreads + threadIdx.x; i < whole; ++c, i += kThreads) {
+      unpack<E, false>(load_chunk<E>(in + (size_t)i * kPer), 0, x);
+      if (special(c)) leave(x, i);
+      fn(x, i);
+    }
+    if (has_rest()) {
+      load_rest(x);
+      leave(x, whole);
+      fn(x, whole);
+    }
+  }
+
+  __device__ __forceinline__ Acc sums(const uint4 (&v)[kHeld], uint32_t* bad) const {
+    const float c = p.c;
+    Acc s;
+    bool first = true;
+    each(v, [&](const float (&x)[E::kPer], uint32_t) {
+      if (first) {
+        first = false;
+        float m = x[0];
+#pragma unroll
+        for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
+        const float u = m * c;
+        s.shift = u > -kTooBig ? u : 0.0f;
+      }
+      add_chunk<E, false>(s, x, c);
+    });
+    *bad = kNone;
+    if (first || (s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) return s;
+    return sums_again(v, bad);
+  }
+
+  // PartScan's second scan.
+  __device__ __forceinline__ Acc sums_again(const uint4 (&v)[kHeld], uint32_t* bad) const {
+    const float c = p.c;
+    float top = -__builtin_inff();
+    uint32_t at_bad = kNone;
+    each(v, [&](const float (&x)[E::kPer], uint32_t i) {
+#pragma unroll
+      for (int e = 0; e < E::kPer; ++e) {
+        const float u = x[e] * c;
+        if (!(u < kTooBig) && at_bad == kNone) at_bad = i * kPer + e;
+        top = fmaxf(top, u);
+      }
+    });
+    Acc s;
+    *bad = at_bad;
+    if (at_bad != kNone || !(top > -kTooBig)) return s;
+    s.shift = top;
+    each(v, [&](const float (&x)[E::kPer], uint32_t) { add_chunk<E, false>(s, x, c); });
+    return s;
+  }
+};
+
+template <typename E, uint32_t kThreads, bool kTail>
+__global__ __launch_bounds__(kThreads) void fused_kernel(const ScoreParams p) {
+  using Raw = typename E::Raw;
+  constexpr uint32_t kPer = E::kPer;
+  __shared__ FusedShared l;
+  __shared__ uint32_t head[kThreads];
+  const uint32_t row = blockIdx.x, lane = lane_id(), wave = threadIdx.x >> 6;
+  const bool distill = p.mode == kModeDistill;
+  const Raw* in = row_ptr<E>(p, row);
+  Raw* out = static_cast<Raw*>(p.grad) + (size_t)row * p.grad_ld;
+  const uint32_t whole = p.vocab / kPer;
+  if (row_unread(p, row)) {
+    if (wave == 0) {
+      const RowSum none{0.0, 0.0, 0.0, kNone};
+      const RowCoef c = distill ? finish_distill<E>(p, row, none, ListSum{})
+                                : finish_policy<E>(p, row, none, token_row<E>(p, row));
+      if (lane == 0) l.coef.state = c.state;
+    }
+    __syncthreads();
+    fill_row<E, kThreads>(out, 0, p.vocab, l.coef.state);
+    return;
+  }
+  // the list or the token first: its loads come back before the row's
+  ListLanes list{};
+  TokenRow token{};
+  if (wave == 0) {
+    if (distill) {
+      list = load_list(p, row, lane);
+    } else {
+      token = token_row<E>(p, row);
+      list.id[0] = lane == 0 ? token.token : kNone;
+      list.id[1] = kNone;
+    }
+  }
+  uint4 v[kHeld];
+#pragma unroll
+  for (uint32_t c = 0; c < kHeld; ++c) {
+    const uint32_t i = c * kThreads + threadIdx.x;
+    if (i < whole) v[c] = stream_chunk<E>(in + (size_t)i * kPer);
+  }
+  head[threadIdx.x] = kNone;
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t e = lane + 64u * h;
+      l.id[e] = list.id[h];
+      l.logit[e] = list.logit[h];
+      l.x[e] = 0.0f;
+      if (list.id[h] < p.vocab)
+        l.next[e] = atomicExch(&head[list.id[h] / kPer % kThreads], e);
+    }
+  }
+  __syncthreads();
+  FusedRow<E, kThreads, kTail> f{p, l, in, whole, head[threadIdx.x], 0};
+  for (uint32_t e = f.first_entry; e != kNone; e = l.next[e])
+    f.mine |= 1ull << (l.id[e] / kPer / kThreads);
+  if (wave == 0 && distill) {
+    double pr[2];
+    const ListSum s = sum_teacher(p, list, lane, pr);
+    l.pr[lane] = pr[0];
+    l.pr[lane + 64] = pr[1];
+    if (lane == 0) l.list = s;
+  }
+  uint32_t bad;
+  const Acc s = f.sums(v, &bad);
+  const RowSum r = block_sum<kThreads>(s, bad, l.sums);
+  if (wave == 0) {
+    RowCoef c;
+    if (distill) {
+      ListSum sums = l.list;
+      const uint32_t id[2] = {l.id[lane], l.id[lane + 64]};
+      const float x[2] = {l.x[lane], l.x[lane + 64]};
+      const double pr[2] = {l.pr[lane], l.pr[lane + 64]};
+      sum_student(p, id, x, pr, sums);
+      c = finish_distill<E>(p, row, r, sums);
+    } else {
+      c = finish_policy<E>(p, row, r, token);
+    }
+    if (lane == 0) l.coef = c;
+  }
+  __syncthreads();
+  const RowCoef k = l.coef;
+  if (k.state != kRowNormal) {
+    fill_row<E, kThreads>(out, 0, p.vocab, k.state);
+    return;
+  }
+  float g[kPer];
+#pragma unroll
+  for (uint32_t c = 0; c < kHeld; ++c) {
+    const uint32_t i = c * kThreads + threadIdx.x;
+    if (i < whole) {
+#pragma unroll
+      for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(E::get(v[c], e), p.c, k);
+      if (f.special(c)) f.patch(g, i, k);
+      store_chunk<E>(out + (size_t)i * kPer, E::pack(g));
+    }
+  }
+  for (uint32_t c = kHeld, i = kHeld * kThreads + threadIdx.x; i < whole; ++c, i += kThreads) {
+    const uint4 w = load_chunk<E>(in + (size_t)i * kPer);
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(E::get(w, e), p.c, k);
+    if (f.special(c)) f.patch(g, i, k);
+    store_chunk<E>(out + (size_t)i * kPer, E::pack(g));
+  }
+  if (f.has_rest()) {
+    float x[kPer];
+    f.load_rest(x);
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(x[e], p.c, k);
+    f.patch(g, whole, k);
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; ++e)
+      if (e < f.rest()) out[(size_t)whole * kPer + e] = E::raw(g[e]);
+  }
 }
 
 // ---- top logits ----
@@ -932,8 +1301,9 @@ __global__ __launch_bounds__(kStatsThreads) void top_tiles_kernel(const ScorePar
     for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
     atomicMax(&words[at >> p.tile_shift], ord_of(b_of(m)));
   });
-  const RowPart out = block_sum<kStatsThreads>(s, bad, l);
-  if (threadIdx.x == 0) p.part[(size_t)row * p.splits + split] = out;
+  const RowSum r = block_sum<kStatsThreads>(s, bad, l);
+  if (threadIdx.x == 0)
+    p.part[(size_t)row * p.splits + split] = RowPart{(float)r.shift, r.bad, r.sum, r.moment};
   const uint32_t all = (p.vocab + (1u << p.tile_shift) - 1u) >> p.tile_shift;
   uint32_t* to = p.tiles + (size_t)row * all + (lo >> p.tile_shift);
   for (uint32_t i = threadIdx.x; i < tiles; i += kStatsThreads) to[i] = words[i];
@@ -1062,7 +1432,9 @@ __global__ __launch_bounds__(kSelectThreads) void top_select_kernel(const ScoreP
   for (uint32_t i = threadIdx.x; i < tiles; i += kSelectThreads)
     l.words[i] = p.tiles[(size_t)row * tiles + i];
   if (threadIdx.x < 64) {
-    const RowSum r = join_parts(p, row, threadIdx.x);
+    RowPart v{0.0f, kNone, 0.0, 0.0};
+    if (threadIdx.x < p.splits) v = p.part[(size_t)row * p.splits + threadIdx.x];
+    const RowSum r = wave_join(v.shift, v.sum, v.moment, v.bad);
     if (threadIdx.x == 0) {
       pb_inference_error* at = p.err ? p.err + row : nullptr;
       failed = row_failed<E>(p, row, r.bad, r.sum, at);
@@ -1086,6 +1458,8 @@ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 
 // Workgroups that a pass over few rows is cut into.
 constexpr uint32_t kTargetGroups = 1024;
+// Rows from which a loss and its gradient take one launch, a workgroup a row.
+constexpr uint32_t kFusedRows = 256;
 
 uint32_t tile_shift_of(uint32_t vocab) {
   uint32_t shift = 6;
@@ -1117,7 +1491,15 @@ ScoresLayout scores_layout(uint32_t rows, uint32_t vocab) {
 }  // namespace
 
 void plan_scores(uint32_t dtype, ScoreParams* p) {
-  (void)dtype;
+  p->fused = 0;
+  if (p->grad != nullptr && (p->mode == kModeDistill || p->mode == kModePolicy)) {
+    const uint32_t chunks = ceil_div(p->vocab, dtype == PB_F32 ? 4u : 8u);
+    const uint32_t threads = chunks <= 64 * kHeld    ? 64
+                             : chunks <= 256 * kHeld ? 256
+                             : chunks <= 512 * kHeld ? 512
+                                                     : 1024;
+    if (chunks <= 64u * threads && p->rows >= kFusedRows) p->fused = threads;
+  }
   p->tile_shift = tile_shift_of(p->vocab);
   const uint32_t tile = 1u << p->tile_shift;
   if (p->rows == 0) return;
@@ -1163,7 +1545,6 @@ struct Launch {
       launch_stats<E, true, false>(p, s);
     else
       launch_stats<E, false, false>(p, s);
-    finish_kernel<E><<<ceil_div(p.rows, 4), 256, 0, s>>>(p);
   }
   static void grad(const ScoreParams& p, bool beta, hipStream_t s) {
     const uint32_t groups = p.rows * p.grad_splits;
@@ -1180,12 +1561,24 @@ struct Launch {
     top_tiles_kernel<E><<<p.rows * p.splits, kStatsThreads, 0, s>>>(p);
     top_select_kernel<E><<<p.rows, kSelectThreads, 0, s>>>(p);
   }
+  template <uint32_t kThreads>
+  static void fused(const ScoreParams& p, hipStream_t s) {
+    if (p.teacher_lse)
+      fused_kernel<E, kThreads, true><<<p.rows, kThreads, 0, s>>>(p);
+    else
+      fused_kernel<E, kThreads, false><<<p.rows, kThreads, 0, s>>>(p);
+  }
   static void row_loss(const ScoreParams& p, hipStream_t s) {
+    switch (p.fused) {
+      case 64: return fused<64>(p, s);
+      case 256: return fused<256>(p, s);
+      case 512: return fused<512>(p, s);
+      case 1024: return fused<1024>(p, s);
+    }
     if (p.teacher_lse)
       launch_stats<E, false, true>(p, s);
     else
       launch_stats<E, false, false>(p, s);
-    finish_kernel<E><<<ceil_div(p.rows, 4), 256, 0, s>>>(p);
     if (p.grad) grad(p, false, s);
   }
   static void preference(const ScoreParams& p, hipStream_t s) {
@@ -1194,7 +1587,6 @@ struct Launch {
       return;
     }
     launch_stats<E, false, false>(p, s);
-    if (p.grad) clear_coef_kernel<<<ceil_div(p.rows, 256), 256, 0, s>>>(p);
     pair_kernel<E><<<p.pairs, 256, 0, s>>>(p);
     if (p.grad) grad(p, false, s);
   }

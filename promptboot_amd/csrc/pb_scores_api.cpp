@@ -102,8 +102,13 @@ uint32_t enqueue(pb_context* ctx, ScoreParams& p, uint32_t dtype, Launch launch,
     set_error(err, PB_CAPACITY, PB_DOMAIN_NONE, need, work.bytes, PB_FIELD_BYTES, 6);
     return PB_CAPACITY;
   }
+  if (p.rows > work.rows) {
+    set_error(err, PB_CAPACITY, PB_DOMAIN_NONE, p.rows, work.rows, PB_FIELD_BYTES, 6);
+    return PB_CAPACITY;
+  }
   pb::plan_scores(dtype, &p);
   pb::place_scores(work.work, &p);
+  p.ticket = work.ticket;
   DeviceGuard guard(work.device);
   const hipError_t e = launch(p, dtype, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? PB_OK : device_error(err, e);
@@ -128,7 +133,7 @@ uint32_t pb_context_reserve_scores(pb_context* ctx, uint32_t rows, size_t vocab,
     set_error(err, PB_STATE, PB_DOMAIN_NONE, 1, 0, PB_FIELD_NONE, 0);
     return PB_STATE;
   }
-  const hipError_t e = pb::scores_reserve(ctx, pb::scores_workspace_bytes(rows, vocab));
+  const hipError_t e = pb::scores_reserve(ctx, rows, pb::scores_workspace_bytes(rows, vocab));
   return e == hipSuccess ? PB_OK : device_error(err, e);
 }
 

@@ -193,10 +193,10 @@ def test_distill_loss(scorer, rows, vocab, k, dtype, tail):
     near(loss, want["loss"], ref.scalar_tolerance(want["loss"], 2 * tol), "loss")
     near_grad(full[:, :vocab], want["grad"], distill_scale(x, ids, logit, T, lse, w), x, T, 2 * tol)
     assert (full[:, vocab:] == 5.0).all()
-    # without a gradient the outputs are the same
+    # without a gradient the loss is the same up to the order of its sums: the same bound holds
     again = out(rows)
     scorer.distill_loss(x, ids.int(), logit, teacher_lse=lse, weight=w, loss=again, temperature=T)
-    assert torch.equal(again, loss)
+    near(again, want["loss"], ref.scalar_tolerance(want["loss"], 2 * tol), "loss alone")
 
 
 @pytest.mark.parametrize("tail", [False, True])
