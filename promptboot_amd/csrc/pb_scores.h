@@ -37,11 +37,23 @@ struct RowCoef {
   uint32_t state;
   uint32_t token;
   float patch;
-  double log2_sum;  // log2 sum 2^(x c) over the whole row
-  double norm;      // the teacher's log-sum-exp
-  double mass;      // the teacher's mass, its rest bucket included
-  double weight;    // weight / T
+  double inv;     // 1 / sum 2^(x c - shift) over the whole row
+  double norm;    // the teacher's log-sum-exp
+  double mass;    // the teacher's mass, its rest bucket included
+  double weight;  // weight / T
 };
+// The same room between the preference loss' statistics and its pairs' pass: a
+// row's sums, what is wrong with it (bad as in RowPart) and ln q[token].  A row
+// that no pair takes stays untouched.
+struct PairRow {
+  float shift;
+  uint32_t bad;
+  uint32_t unused;
+  uint32_t state;  // kRowUntouched, where RowCoef has it
+  double sum;
+  double logprob;
+};
+static_assert(offsetof(PairRow, state) == offsetof(RowCoef, state), "a row's state has one place");
 
 struct ScoreParams {
   const void* logits;

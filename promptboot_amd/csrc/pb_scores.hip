@@ -93,7 +93,7 @@ struct F16 {
 
 // Rows start at any element: 16-byte accesses that are aligned to an element only.
 typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
-typedef Words4 Loose4 __attribute__((aligned(2)));
+typedef Words4 Loose4 __attribute__((aligned(2), may_alias));
 template <typename E>
 __device__ __forceinline__ uint4 load_chunk(const typename E::Raw* p) {
   const Words4 v = *reinterpret_cast<const Loose4*>(p);
@@ -144,17 +144,28 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 
 // ---- rows ----
 
+// A per-row word by a scalar load (the same row in every lane; nothing in the
+// launch writes it): counted apart from the rows' loads.
+__device__ __forceinline__ uint32_t uniform_word(const uint32_t* at) {
+  return *(const __attribute__((address_space(4))) uint32_t*)at;
+}
+__device__ __forceinline__ float uniform_float(const float* at) {
+  return f_of(uniform_word(reinterpret_cast<const uint32_t*>(at)));
+}
+
 // Whether the statistics pass leaves a row out: it is masked, or its id is bad
 // (which the finishing pass reports).
 __device__ __forceinline__ bool row_unread(const ScoreParams& p, uint32_t row) {
   if (p.mode == kModeTop) return false;
-  if (p.mode == kModeDistill) return p.weight != nullptr && p.weight[row] == 0.0f;
+  if (p.mode == kModeDistill)
+    return p.weight != nullptr && uniform_float(p.weight + row) == 0.0f;
   if (p.mode == kModePreference) {
-    const uint32_t end = p.seq_start[2 * p.pairs];
-    if (row < p.seq_start[0] || row >= end) return true;
+    if (row < uniform_word(p.seq_start) || row >= uniform_word(p.seq_start + 2 * p.pairs))
+      return true;
   }
-  if (p.mode == kModePolicy && p.weight != nullptr && p.weight[row] == 0.0f) return true;
-  return p.token[row] >= p.vocab;
+  if (p.mode == kModePolicy && p.weight != nullptr && uniform_float(p.weight + row) == 0.0f)
+    return true;
+  return uniform_word(p.token + row) >= p.vocab;
 }
 
 template <typename E>
@@ -375,48 +386,34 @@ __device__ __forceinline__ void no_error(pb_inference_error* at) {
 
 __device__ __forceinline__ float nan32() { return f_of(0x7fc00000u); }
 
-// alpha, beta and shift of a row whose gradient is q (A + B ln q) for most
-// elements: the shift is log2_sum's nearest binary32, and what that rounding
-// leaves out goes into the factors.
-__device__ __forceinline__ void set_factors(RowCoef& r, double log2_sum, double a, double b) {
-  const float shift = (float)log2_sum;
-  const double d = (double)shift - log2_sum;
-  const double f = exp2(d);
-  r.shift = shift;
-  r.alpha = (float)(f * (a + b * kLn2 * d));
-  r.beta = (float)(f * b * kLn2);
-  r.log2_sum = log2_sum;
-}
-
-// Gradient w / T (delta - q) slope of a row with one token; lp = ln q[token].
-__device__ __forceinline__ RowCoef token_coef(double log2_sum, double slope, double lp,
+// Gradient slope (delta - q) of a row with one token; shift and sum its sums,
+// lp = ln q[token].
+__device__ __forceinline__ RowCoef token_coef(float shift, double sum, double slope, double lp,
                                               uint32_t token) {
   RowCoef r{};
-  if (slope == 0.0) {
-    r.state = kRowZero;
-    return r;
-  }
-  r.state = slope == slope ? kRowNormal : kRowNan;
-  set_factors(r, log2_sum, -slope, 0.0);
+  r.state = slope == 0.0 ? kRowZero : slope == slope ? kRowNormal : kRowNan;
+  r.shift = shift;
+  r.alpha = (float)(-slope / sum);
   r.token = token;
   r.patch = (float)(slope * -expm1(lp));
   return r;
 }
 
 // ln q[token] in 64 bits; x the token's logit.
-__device__ __forceinline__ double token_logprob(const ScoreParams& p, float x, double log2_sum) {
-  return kLn2 * ((double)x * (double)p.c - log2_sum);
+__device__ __forceinline__ double token_logprob(const ScoreParams& p, float x, const RowSum& r) {
+  return kLn2 * (((double)x * (double)p.c - r.shift) - log2(r.sum));
 }
 
-// Reports what is wrong with a row that was read; true if anything is.
+// Whether a row that was read has failed, and the record of it.
+__device__ __forceinline__ bool bad_row(uint32_t bad, double sum) {
+  return bad != kNone || !(sum > 0.0);
+}
 template <typename E>
-__device__ __forceinline__ bool row_failed(const ScoreParams& p, uint32_t row, uint32_t bad,
-                                           double sum, pb_inference_error* at) {
-  if (bad == kNone && sum > 0.0) return false;
+__device__ __forceinline__ void report_row(const ScoreParams& p, uint32_t row, uint32_t bad,
+                                           pb_inference_error* at) {
   const uint32_t index = bad == kNone ? 0u : bad;
   write_error(at, PB_NONFINITE_OUTPUT, row, 0, b_of(E::one(row_ptr<E>(p, row)[index])),
               PB_FIELD_FINITE, index);
-  return true;
 }
 
 // What a row with one token needs beside its sums, requested before them.
@@ -426,72 +423,82 @@ struct TokenRow {
   float weight;
   float old_logprob, advantage, ref_logprob;
 };
-template <typename E>
 __device__ __forceinline__ TokenRow token_row(const ScoreParams& p, uint32_t row) {
-  TokenRow t{p.token[row], 0.0f, 1.0f, 0.0f, 0.0f, 0.0f};
-  if (t.token < p.vocab) t.x = E::one(row_ptr<E>(p, row)[t.token]);
+  TokenRow t{uniform_word(p.token + row), 0.0f, 1.0f, 0.0f, 0.0f, 0.0f};
   if (p.mode == kModePolicy) {
-    if (p.weight != nullptr) t.weight = p.weight[row];
-    t.old_logprob = p.old_logprob[row];
-    t.advantage = p.advantage[row];
-    if (p.ref_logprob != nullptr) t.ref_logprob = p.ref_logprob[row];
+    if (p.weight != nullptr) t.weight = uniform_float(p.weight + row);
+    t.old_logprob = uniform_float(p.old_logprob + row);
+    t.advantage = uniform_float(p.advantage + row);
+    if (p.ref_logprob != nullptr) t.ref_logprob = uniform_float(p.ref_logprob + row);
   }
   return t;
 }
 
-// The finish_ functions write a row's outputs and return what its gradient
-// needs; lane 0's result counts.
+// A row's scalars are worked out in two steps: what its gradient needs, and then
+// the outputs, which no other wave waits for.
 
+// One wave; the three exponentials are one call over three lanes.  Lane 0's
+// result counts.
+struct PolicyRow {
+  RowCoef coef;
+  double loss, logprob, kl;
+};
 template <typename E>
-__device__ __forceinline__ RowCoef finish_policy(const ScoreParams& p, uint32_t row,
-                                                 const RowSum& r, const TokenRow& t) {
+__device__ __forceinline__ PolicyRow policy_row(const ScoreParams& p, uint32_t row,
+                                                const RowSum& r, const TokenRow& t) {
+  PolicyRow o{};
+  o.coef.state = kRowZero;
   pb_inference_error* at = p.err ? p.err + row : nullptr;
-  float loss = 0.0f, logprob = 0.0f, kl_out = 0.0f;
-  RowCoef coef{};
-  coef.state = kRowZero;
-  if (lane_id() != 0) return coef;
   if (t.token == PB_NO_TOKEN || t.weight == 0.0f) {
-    no_error(at);
+    if (lane_id() == 0) no_error(at);
+    return o;
+  }
+  bool failed = t.token >= p.vocab;
+  if (failed) {
+    if (lane_id() == 0) write_error(at, PB_TOKEN_ID, row, p.vocab, t.token, PB_FIELD_TOKEN, 0);
   } else {
-    bool failed = t.token >= p.vocab;
-    if (failed)
-      write_error(at, PB_TOKEN_ID, row, p.vocab, t.token, PB_FIELD_TOKEN, 0);
-    else
-      failed = row_failed<E>(p, row, r.bad, r.sum, at);
-    if (failed) {
-      loss = logprob = kl_out = nan32();
-      coef.state = kRowNan;
-    } else {
-      no_error(at);
-      const double log2_sum = r.shift + log2(r.sum);
-      const double lp = token_logprob(p, t.x, log2_sum);
-      const double ratio = exp(lp - (double)t.old_logprob), adv = (double)t.advantage;
-      const double low = 1.0 - p.clip_low, high = 1.0 + p.clip_high;
-      const double kept = ratio < low ? low : ratio > high ? high : ratio;
-      const double open = ratio * adv, shut = kept * adv;
-      double l = open <= shut ? -open : -shut;
-      double slope = open <= shut ? -open : 0.0;
-      if (open != open) l = slope = open;
-      double kl = 0.0;
-      if (p.ref_logprob != nullptr) {
-        const double gap = (double)t.ref_logprob - lp;
-        const double rise = expm1(gap);
-        kl = rise - gap;
-        if (p.kl_coef != 0.0) {
-          l += p.kl_coef * kl;
-          slope -= p.kl_coef * rise;
-        }
-      }
-      loss = (float)l;
-      logprob = (float)lp;
-      kl_out = (float)kl;
-      coef = token_coef(log2_sum, slope * (double)t.weight * p.inv_t, lp, t.token);
+    failed = bad_row(r.bad, r.sum);
+    if (failed && lane_id() == 0) report_row<E>(p, row, r.bad, at);
+  }
+  if (failed) {
+    o.loss = o.logprob = o.kl = (double)nan32();
+    o.coef.state = kRowNan;
+    return o;
+  }
+  if (lane_id() == 0) no_error(at);
+  const double lp = token_logprob(p, t.x, r), gap = (double)t.ref_logprob - lp;
+  const uint32_t lane = lane_id();
+  const double rise = expm1(lane == 0 ? lp - (double)t.old_logprob : lane == 1 ? gap : lp);
+  const double ratio = 1.0 + bcast_f64(rise, 0), away = bcast_f64(rise, 1);
+  const double adv = (double)t.advantage;
+  const double low = 1.0 - p.clip_low, high = 1.0 + p.clip_high;
+  const double kept = ratio < low ? low : ratio > high ? high : ratio;
+  const double open = ratio * adv, shut = kept * adv;
+  double slope = open <= shut ? -open : 0.0;
+  o.logprob = lp;
+  o.loss = open <= shut ? -open : -shut;
+  if (open != open) o.loss = slope = open;
+  if (p.ref_logprob != nullptr) {
+    o.kl = away - gap;
+    if (p.kl_coef != 0.0) {
+      o.loss += p.kl_coef * o.kl;
+      slope -= p.kl_coef * away;
     }
   }
-  p.loss[row] = loss;
-  if (p.logprob) p.logprob[row] = logprob;
-  if (p.kl) p.kl[row] = kl_out;
-  return coef;
+  slope = slope * (double)t.weight * p.inv_t;
+  o.coef.state = slope == 0.0 ? kRowZero : slope == slope ? kRowNormal : kRowNan;
+  o.coef.shift = (float)r.shift;
+  o.coef.alpha = (float)(-slope / r.sum);
+  o.coef.token = t.token;
+  o.coef.patch = (float)(slope * -bcast_f64(rise, 2));
+  return o;
+}
+__device__ __forceinline__ void write_policy(const ScoreParams& p, uint32_t row,
+                                             const PolicyRow& o) {
+  if (lane_id() != 0) return;
+  p.loss[row] = (float)o.loss;
+  if (p.logprob) p.logprob[row] = (float)o.logprob;
+  if (p.kl) p.kl[row] = (float)o.kl;
 }
 
 template <typename E>
@@ -504,17 +511,19 @@ __device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t r
     no_error(at);
   } else {
     bool failed = t.token >= p.vocab;
-    if (failed)
+    if (failed) {
       write_error(at, PB_TOKEN_ID, row, p.vocab, t.token, PB_FIELD_TOKEN, 0);
-    else
-      failed = row_failed<E>(p, row, r.bad, r.sum, at);
+    } else {
+      failed = bad_row(r.bad, r.sum);
+      if (failed) report_row<E>(p, row, r.bad, at);
+    }
     if (failed) {
       logprob = lse = entropy = nan32();
     } else {
       no_error(at);
-      const double log2_own = log2(r.sum), log2_sum = r.shift + log2_own;
-      logprob = (float)token_logprob(p, t.x, log2_sum);
-      lse = (float)(kLn2 * log2_sum);
+      const double log2_own = log2(r.sum);
+      logprob = (float)(kLn2 * (((double)t.x * (double)p.c - r.shift) - log2_own));
+      lse = (float)(kLn2 * (r.shift + log2_own));
       entropy = (float)(kLn2 * (log2_own - r.moment / r.sum));
     }
   }
@@ -523,31 +532,17 @@ __device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t r
   if (p.entropy) p.entropy[row] = entropy;
 }
 
-// The preference loss' rows: ln q[token] and log2_sum for the pair's pass, or
-// what is wrong with the row.
-template <typename E>
+// The preference loss' rows, for the pairs' pass.
 __device__ __forceinline__ void finish_pair_row(const ScoreParams& p, uint32_t row,
                                                 const RowSum& r, const TokenRow& t) {
   if (lane_id() != 0) return;
-  RowCoef coef{};
-  coef.state = kRowUntouched;
-  coef.token = r.bad;
-  coef.mass = r.sum;
-  if (r.bad == kNone && r.sum > 0.0) {
-    coef.log2_sum = r.shift + log2(r.sum);
-    coef.norm = token_logprob(p, t.x, coef.log2_sum);
-  }
-  p.coef[row] = coef;
+  PairRow* v = reinterpret_cast<PairRow*>(p.coef + row);
+  v->state = kRowUntouched;
+  v->shift = (float)r.shift;
+  v->bad = r.bad;
+  v->sum = r.sum;
+  v->logprob = bad_row(r.bad, r.sum) ? 0.0 : token_logprob(p, t.x, r);
 }
-
-// What the teacher's list says, the same in every lane: its log-sum-exp, its
-// mass sum p, sum p ln p, sum p u, and the student's weight of the listed ids,
-// sum 2^(u - top_u).
-struct ListSum {
-  double norm, mass, plogp, pu, listed, top_u;
-  uint32_t bad_id, bad_logit, bad_x;
-  uint32_t any;
-};
 
 // A row's list, two entries a lane (i = lane, lane + 64); kNone past its end.
 struct ListLanes {
@@ -568,9 +563,9 @@ __device__ __forceinline__ ListLanes load_list(const ScoreParams& p, uint32_t ro
   return l;
 }
 
-// The part of the sums that needs no student; pr: the lane's p.
-__device__ __forceinline__ ListSum sum_teacher(const ScoreParams& p, const ListLanes& l,
-                                               uint32_t lane, double (&pr)[2]) {
+// The first entry whose id another entry has too, or kNone.
+__device__ __forceinline__ uint32_t first_repeat(const ScoreParams& p, const ListLanes& l,
+                                                 uint32_t lane) {
   uint32_t seen[2] = {0, 0};  // entries of the same id, the entry itself included
 #pragma unroll
   for (uint32_t j = 0; j < 64; ++j) {
@@ -586,175 +581,217 @@ __device__ __forceinline__ ListSum sum_teacher(const ScoreParams& p, const ListL
       seen[1] += a == l.id[1] ? 1u : 0u;
     }
   }
+  const bool second = l.id[1] != kNone && seen[1] > 1u;
+  return wave_min_word(l.id[0] != kNone && seen[0] > 1u ? lane : second ? lane + 64u : kNone);
+}
+
+// What the teacher's list says by itself, the same in every lane: its
+// log-sum-exp, its mass sum p, sum p ln p, the first bad entries, and whether
+// anything in it weighs.
+struct ListSum {
+  double norm, mass, plogp;
+  uint32_t bad_id, bad_logit;
+  uint32_t any;
+};
+
+// pr: the lane's p.
+__device__ __forceinline__ ListSum sum_teacher(const ScoreParams& p, const ListLanes& l,
+                                               uint32_t lane, uint32_t repeat, double (&pr)[2]) {
   ListSum s{};
-  s.bad_id = s.bad_logit = s.bad_x = kNone;
-  float top_t = -__builtin_inff();
+  s.bad_id = s.bad_logit = kNone;
+  float top = -__builtin_inff();
   bool on[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint32_t i = lane + 64u * h;
-    on[h] = l.id[h] != kNone;
-    if (on[h] && (l.id[h] >= p.vocab || seen[h] > 1u)) {
-      s.bad_id = i < s.bad_id ? i : s.bad_id;
-      on[h] = false;
-    }
+    on[h] = l.id[h] < p.vocab;
+    if (l.id[h] != kNone && !on[h]) s.bad_id = i < s.bad_id ? i : s.bad_id;
     if (on[h] && !(l.logit[h] < __builtin_inff())) s.bad_logit = i < s.bad_logit ? i : s.bad_logit;
-    if (on[h]) top_t = fmaxf(top_t, l.logit[h]);
+    if (on[h]) top = fmaxf(top, l.logit[h]);
   }
   s.bad_id = wave_min_word(s.bad_id);
+  s.bad_id = repeat < s.bad_id ? repeat : s.bad_id;
   s.bad_logit = wave_min_word(s.bad_logit);
-  if (p.teacher_lse != nullptr && !__builtin_isfinite(l.lse))
-    s.bad_logit = p.k < s.bad_logit ? p.k : s.bad_logit;
-  top_t = wave_max_f32(top_t);
-  s.any = top_t > -__builtin_inff();
+  const bool lse_given = p.teacher_lse != nullptr;
+  if (lse_given && !__builtin_isfinite(l.lse)) s.bad_logit = p.k < s.bad_logit ? p.k : s.bad_logit;
+  top = wave_max_f32(top);
+  s.any = top > -__builtin_inff() && s.bad_logit == kNone;
   pr[0] = pr[1] = 0.0;
   if (!s.any) return s;
-  if (p.teacher_lse != nullptr) {
-    s.norm = (double)l.lse;
-  } else {
-    double sum = 0.0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      sum += on[h] ? exp(((double)l.logit[h] - (double)top_t) * p.inv_t) : 0.0;
-    s.norm = (double)top_t * p.inv_t + log(wave_sum_f64(sum));
-  }
+  // e = 2^.. of each entry by the teacher's lse, or by its largest logit
+  const double base = lse_given ? (double)l.lse : (double)top * p.inv_t;
+  double sum = 0.0, moment = 0.0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const double lp = (double)l.logit[h] * p.inv_t - s.norm;
-    pr[h] = on[h] ? exp(lp) : 0.0;
-    s.mass += pr[h];
-    if (pr[h] > 0.0) s.plogp += pr[h] * lp;
+    if (h == 1 && p.k <= 64) break;
+    const double d = (double)l.logit[h] * p.inv_t - base;
+    pr[h] = on[h] ? exp(d) : 0.0;
+    sum += pr[h];
+    if (pr[h] > 0.0) moment += pr[h] * d;
   }
-  s.mass = wave_sum_f64(s.mass);
-  s.plogp = wave_sum_f64(s.plogp);
+  sum = wave_sum_f64(sum);
+  moment = wave_sum_f64(moment);
+  if (lse_given) {
+    s.norm = base;
+    s.mass = sum;
+    s.plogp = moment;
+    return s;
+  }
+  const double own = log(sum), inv = 1.0 / sum;
+  s.norm = base + own;
+  s.mass = 1.0;
+  s.plogp = moment * inv - own;
+  pr[0] *= inv;
+  pr[1] *= inv;
   return s;
 }
 
-// The part that needs the student's logits x of the listed ids.
-__device__ __forceinline__ void sum_student(const ScoreParams& p, const uint32_t (&id)[2],
-                                            const float (&x)[2], const double (&pr)[2],
-                                            ListSum& s) {
-  float top_x = -__builtin_inff();
-  double pu = 0.0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (id[h] >= p.vocab) continue;
-    if (!(x[h] * p.c < kTooBig)) s.bad_x = id[h] < s.bad_x ? id[h] : s.bad_x;
-    top_x = fmaxf(top_x, x[h]);
-    if (pr[h] > 0.0) pu += pr[h] * ((double)x[h] * (double)p.c);
-  }
-  s.pu = wave_sum_f64(pu);
-  s.bad_x = wave_min_word(s.bad_x);
-  top_x = wave_max_f32(top_x);
-  s.top_u = top_x * p.c > -kTooBig ? (double)top_x * (double)p.c : -__builtin_inf();
-  if (p.teacher_lse == nullptr || !(s.top_u > -__builtin_inf())) return;
-  double listed = 0.0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (id[h] < p.vocab) listed += exp2((double)x[h] * (double)p.c - s.top_u);
-  s.listed = wave_sum_f64(listed);
-}
-
-// A listed id's gradient.
+// A listed id's gradient; pr: its p.
 __device__ __forceinline__ float listed_grad(const ScoreParams& p, const RowCoef& r, float x,
-                                             float logit) {
-  const double q = exp2((double)x * (double)p.c - r.log2_sum);
-  const double t = exp((double)logit * p.inv_t - r.norm);
-  return (float)(r.weight * (r.mass * q - t));
+                                             double pr) {
+  const double q = exp2((double)x * (double)p.c - (double)r.shift) * r.inv;
+  return (float)(r.weight * (r.mass * q - pr));
 }
 
+// One wave: the row's sums joined with those of its listed ids (x, the lane's
+// logits of them), and what its gradient needs.
+struct DistillRow {
+  RowCoef coef;
+  double shift, rest, whole;  // sums 2^(u - shift) off the list and of the row
+  double left;                // the teacher's mass in the rest bucket
+  bool skipped, failed;
+};
 template <typename E>
-__device__ __forceinline__ RowCoef finish_distill(const ScoreParams& p, uint32_t row,
-                                                  const RowSum& r, const ListSum& s) {
+__device__ __forceinline__ DistillRow distill_row(const ScoreParams& p, uint32_t row, float weight,
+                                                  const RowSum& r, const ListSum& s,
+                                                  const uint32_t (&id)[2], const float (&x)[2]) {
+  DistillRow o{};
+  o.coef.state = kRowZero;
   pb_inference_error* at = p.err ? p.err + row : nullptr;
-  const float w = p.weight ? p.weight[row] : 1.0f;
-  RowCoef coef{};
-  coef.state = kRowZero;
-  if (lane_id() != 0) return coef;
-  float loss = 0.0f, lse = 0.0f;
-  if (w == 0.0f) {
-    no_error(at);
-  } else {
-    const bool rest_bucket = p.teacher_lse != nullptr;
-    // the student's sum over the listed ids joins the rest's
-    double rest = r.sum, whole = r.sum, shift = r.shift;
-    if (rest_bucket && s.top_u > -__builtin_inf()) {
-      shift = r.sum > 0.0 && r.shift > s.top_u ? r.shift : s.top_u;
-      rest = r.sum > 0.0 ? r.sum * exp2(r.shift - shift) : 0.0;
-      whole = rest + s.listed * exp2(s.top_u - shift);
+  const bool writer = lane_id() == 0;
+  o.skipped = weight == 0.0f;
+  if (o.skipped) {
+    if (writer) no_error(at);
+    return o;
+  }
+  uint32_t bad = r.bad;
+  o.shift = r.shift;
+  o.rest = o.whole = r.sum;
+  if (p.teacher_lse != nullptr) {
+    // the listed ids were left out of the row's sums: their logits are looked at here
+    float top = -__builtin_inff();
+    uint32_t bad_x = kNone;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (id[h] >= p.vocab) continue;
+      if (!(x[h] * p.c < kTooBig)) bad_x = id[h] < bad_x ? id[h] : bad_x;
+      top = fmaxf(top, x[h]);
     }
-    const uint32_t bad = s.bad_x < r.bad ? s.bad_x : r.bad;
-    bool failed = true;
-    if (s.bad_id != kNone)
+    bad_x = wave_min_word(bad_x);
+    bad = bad_x < bad ? bad_x : bad;
+    top = wave_max_f32(top) * p.c;
+    if (top > -kTooBig) {
+      o.shift = r.sum > 0.0 && r.shift > (double)top ? r.shift : (double)top;
+      double listed = 0.0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && p.k <= 64) break;
+        if (id[h] < p.vocab) listed += exp2((double)x[h] * (double)p.c - o.shift);
+      }
+      o.rest = r.sum > 0.0 ? r.sum * exp2(r.shift - o.shift) : 0.0;
+      o.whole = o.rest + wave_sum_f64(listed);
+    }
+  }
+  o.failed = true;
+  if (s.bad_id != kNone) {
+    if (writer)
       write_error(at, PB_TOKEN_ID, row, p.vocab, p.teacher_id[(size_t)row * p.k + s.bad_id],
                   PB_FIELD_TOKEN, s.bad_id);
-    else if (s.bad_logit != kNone)
+  } else if (s.bad_logit != kNone) {
+    if (writer)
       write_error(at, PB_NONFINITE_INPUT, row, 0,
                   b_of(s.bad_logit == p.k ? p.teacher_lse[row]
                                           : p.teacher_logit[(size_t)row * p.k + s.bad_logit]),
                   PB_FIELD_FINITE, s.bad_logit);
-    else
-      failed = row_failed<E>(p, row, bad, whole, at);
-    if (failed) {
-      loss = lse = nan32();
-      coef.state = kRowNan;
-    } else {
-      no_error(at);
-      const double log2_sum = shift + log2(whole);
-      lse = (float)(kLn2 * log2_sum);
-      if (s.any) {
-        double l = s.plogp - kLn2 * (s.pu - s.mass * log2_sum), mass = s.mass;
-        double off = mass;  // what q is multiplied by off the list
-        if (rest_bucket) {
-          const double left = mass < 1.0 ? 1.0 - mass : 0.0;
-          if (left > 0.0 && rest > 0.0) {
-            l += left * log(left * whole / rest);
-            mass += left;
-            off = mass - left * (whole / rest);
-          }
-        }
-        loss = (float)l;
-        const double weight = (double)w * p.inv_t;
-        coef.state = weight == weight ? kRowNormal : kRowNan;
-        set_factors(coef, log2_sum, weight * off, 0.0);
-        coef.norm = s.norm;
-        coef.mass = mass;
-        coef.weight = weight;
-        coef.token = kNone;
-      }
+  } else if (bad_row(bad, o.whole)) {
+    if (writer) report_row<E>(p, row, bad, at);
+  } else {
+    o.failed = false;
+    if (writer) no_error(at);
+  }
+  if (o.failed) o.coef.state = kRowNan;
+  if (o.failed || !s.any) return o;
+  double mass = s.mass, off = mass;  // off: what q is multiplied by off the list
+  if (p.teacher_lse != nullptr && mass < 1.0 && o.rest > 0.0) {
+    o.left = 1.0 - mass;
+    mass += o.left;
+    off = mass - o.left * (o.whole / o.rest);
+  }
+  o.coef.weight = (double)weight * p.inv_t;
+  o.coef.state = weight == weight ? kRowNormal : kRowNan;
+  o.coef.inv = 1.0 / o.whole;
+  o.coef.shift = (float)o.shift;
+  o.coef.alpha = (float)(o.coef.weight * off * o.coef.inv);
+  o.coef.norm = s.norm;
+  o.coef.mass = mass;
+  o.coef.token = kNone;
+  return o;
+}
+__device__ __forceinline__ void write_distill(const ScoreParams& p, uint32_t row,
+                                              const DistillRow& o, const ListSum& s,
+                                              const float (&x)[2], const double (&pr)[2]) {
+  double loss = 0.0, lse = 0.0;
+  if (o.failed) {
+    loss = lse = (double)nan32();
+  } else if (!o.skipped) {
+    const double log2_sum = o.shift + log2(o.whole);
+    lse = kLn2 * log2_sum;
+    if (s.any) {
+      double pu = 0.0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (pr[h] > 0.0) pu += pr[h] * ((double)x[h] * (double)p.c);
+      loss = s.plogp - kLn2 * (wave_sum_f64(pu) - s.mass * log2_sum);
+      if (o.left > 0.0) loss += o.left * log(o.left * o.whole / o.rest);
     }
   }
-  p.loss[row] = loss;
-  if (p.lse) p.lse[row] = lse;
-  return coef;
+  if (lane_id() != 0) return;
+  p.loss[row] = (float)loss;
+  if (p.lse) p.lse[row] = (float)lse;
 }
 
-// A row's scalars from its sums; wave 0, every lane.
+// A row's scalars from its sums; one wave.
 template <typename E>
 __device__ __forceinline__ void finish_row(const ScoreParams& p, uint32_t row, const RowSum& r) {
   const uint32_t lane = lane_id();
   if (p.mode == kModeDistill) {
+    const float weight = p.weight ? p.weight[row] : 1.0f;
     ListSum s{};
-    if (!row_unread(p, row)) {
+    uint32_t id[2] = {kNone, kNone};
+    float x[2] = {0.0f, 0.0f};
+    double pr[2] = {0.0, 0.0};
+    if (weight != 0.0f) {
       const ListLanes l = load_list(p, row, lane);
-      float x[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        x[h] = l.id[h] < p.vocab ? E::one(row_ptr<E>(p, row)[l.id[h]]) : 0.0f;
-      double pr[2];
-      s = sum_teacher(p, l, lane, pr);
-      sum_student(p, l.id, x, pr, s);
+      for (int h = 0; h < 2; ++h) {
+        id[h] = l.id[h];
+        x[h] = id[h] < p.vocab ? E::one(row_ptr<E>(p, row)[id[h]]) : 0.0f;
+      }
+      s = sum_teacher(p, l, lane, first_repeat(p, l, lane), pr);
     }
-    const RowCoef c = finish_distill<E>(p, row, r, s);
-    if (lane == 0 && p.grad) p.coef[row] = c;
+    const DistillRow o = distill_row<E>(p, row, weight, r, s, id, x);
+    if (lane == 0 && p.grad) p.coef[row] = o.coef;
+    write_distill(p, row, o, s, x, pr);
     return;
   }
-  const TokenRow t = token_row<E>(p, row);
+  TokenRow t = token_row(p, row);
+  if (t.token < p.vocab) t.x = E::one(row_ptr<E>(p, row)[t.token]);
   if (p.mode == kModePolicy) {
-    const RowCoef c = finish_policy<E>(p, row, r, t);
-    if (lane == 0 && p.grad) p.coef[row] = c;
+    const PolicyRow o = policy_row<E>(p, row, r, t);
+    if (lane == 0 && p.grad) p.coef[row] = o.coef;
+    write_policy(p, row, o);
   } else if (p.mode == kModePreference) {
-    finish_pair_row<E>(p, row, r, t);
+    finish_pair_row(p, row, r, t);
   } else {
     finish_logprobs<E>(p, row, r, t);
   }
@@ -829,6 +866,10 @@ __global__ __launch_bounds__(kStatsThreads) void stats_kernel(const ScoreParams 
 
 // ---- preference loss: one workgroup a pair ----
 
+__device__ __forceinline__ PairRow pair_row(const ScoreParams& p, uint32_t row) {
+  return *reinterpret_cast<const PairRow*>(p.coef + row);
+}
+
 template <typename E>
 __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
   __shared__ double sums[2][4];
@@ -854,11 +895,11 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
     for (uint32_t row = a + threadIdx.x; row < e; row += 256u) {
       const uint32_t token = p.token[row];
       if (token == PB_NO_TOKEN) continue;
-      const RowCoef& v = p.coef[row];
-      if (token >= p.vocab || v.token != kNone || !(v.mass > 0.0))
+      const PairRow v = pair_row(p, row);
+      if (token >= p.vocab || bad_row(v.bad, v.sum))
         failed = row < failed ? row : failed;
       else
-        mine[row < b ? 0 : 1] += v.norm;
+        mine[row < b ? 0 : 1] += v.logprob;
     }
   }
   const double c = wave_sum_f64(mine[0]), d = wave_sum_f64(mine[1]);
@@ -883,7 +924,7 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
       if (token >= p.vocab) {
         write_error(at, PB_TOKEN_ID, first, p.vocab, token, PB_FIELD_TOKEN, 0);
       } else {
-        row_failed<E>(p, first, p.coef[first].token, p.coef[first].mass, at);
+        report_row<E>(p, first, pair_row(p, first).bad, at);
       }
       loss = slope = l[0] = l[1] = (double)nan32();
     } else {
@@ -918,8 +959,8 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
     if (slope != slope) {
       coef.state = kRowNan;
     } else if (token != PB_NO_TOKEN && w != 0.0f) {
-      const RowCoef& v = p.coef[row];
-      coef = token_coef(v.log2_sum, row < b ? slope : -slope, v.norm, token);
+      const PairRow v = pair_row(p, row);
+      coef = token_coef(v.shift, v.sum, row < b ? slope : -slope, v.logprob, token);
     }
     p.coef[row] = coef;
   }
@@ -943,8 +984,14 @@ __global__ __launch_bounds__(256) void logprobs_coef_kernel(const ScoreParams p)
     } else if (g != 0.0 || ge != 0.0) {
       r.state = kRowNormal;
       // g (delta - q) - ge q (ln q + H)
-      set_factors(r, log2_sum, (-g - ge * h) * p.inv_t, -ge * p.inv_t);
-      const double lp = token_logprob(p, E::one(row_ptr<E>(p, row)[token]), log2_sum), q = exp(lp);
+      // g (delta - q) - ge q (ln q + H), about the log-sum's nearest binary32;
+      // what that rounding leaves out goes into the factors
+      r.shift = (float)log2_sum;
+      const double d = (double)r.shift - log2_sum, f = exp2(d) * p.inv_t;
+      r.alpha = (float)(f * ((-g - ge * h) - ge * kLn2 * d));
+      r.beta = (float)(f * -ge * kLn2);
+      const double lp = kLn2 * ((double)E::one(row_ptr<E>(p, row)[token]) * (double)p.c - log2_sum),
+                   q = exp(lp);
       r.token = token;
       r.patch = (float)((g * -expm1(lp) - (q > 0.0 ? ge * q * (lp + h) : 0.0)) * p.inv_t);
     }
@@ -1004,7 +1051,8 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
       const uint32_t id = p.teacher_id[entry];
       if (id >= lo && id < hi) {
         at = id - lo;
-        patch = listed_grad(p, r, E::one(in[at]), p.teacher_logit[entry]);
+        const double pr = exp((double)p.teacher_logit[entry] * p.inv_t - r.norm);
+        patch = listed_grad(p, r, E::one(in[at]), pr);
       }
     }
     __syncthreads();
@@ -1027,14 +1075,17 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
 
 // ---- a row's loss and gradient in one launch ----
 // One workgroup takes a whole row and keeps its first kHeld chunks a thread in
-// registers between the statistics and the gradient: a row of 163,840 16-bit
-// logits is read from memory once.  What lies beyond (32-bit rows over 81,920
+// registers between the statistics and the gradient: a row of 155,648 16-bit
+// logits is read from memory once.  What lies beyond (32-bit rows over 77,824
 // ids) is read again.  The row's special elements (its token, or the teacher's
-// list) hang in a chain on the thread that holds them, which leaves their logits
-// for the row's scalars and writes their gradients, so that no store waits for
-// another.
+// list) hang in chains on the threads that hold them: the owner leaves their
+// logits for the row's scalars, takes them out of the sums where the list has a
+// rest bucket, and stores their gradients over its own chunks', so that no store
+// waits for another thread's.
 
-constexpr uint32_t kHeld = 20;
+constexpr uint32_t kHeld = 19;
+// With a rest bucket the row's scalars need more registers of their own.
+constexpr uint32_t kHeldTail = 16;
 
 struct FusedShared {
   BlockSum sums;
@@ -1044,44 +1095,28 @@ struct FusedShared {
   uint32_t id[PB_TOP_LOGITS_MAX];
   uint32_t next[PB_TOP_LOGITS_MAX];
   float x[PB_TOP_LOGITS_MAX];
-  float logit[PB_TOP_LOGITS_MAX];
 };
 
 template <typename E, uint32_t kThreads, bool kTail>
 struct FusedRow {
+  static constexpr uint32_t kHeld = kTail ? kHeldTail : pb::kHeld;
   static constexpr uint32_t kPer = E::kPer;
   using Raw = typename E::Raw;
   const ScoreParams& p;
   FusedShared& l;
   const Raw* in;
-  uint32_t whole, first_entry;
-  uint64_t mine;  // bit c: the thread's chunk c holds a special element
+  uint32_t whole;
+  uint32_t first_entry;
 
-  // Takes the special elements out of chunk c (i = its index in the row).
-  __device__ __forceinline__ void leave(float (&x)[E::kPer], uint32_t i) const {
+  // The special elements of the thread's chunk i out of x.
+  __device__ __forceinline__ void take_out(float (&x)[E::kPer], uint32_t i) const {
     for (uint32_t e = first_entry; e != kNone; e = l.next[e]) {
       const uint32_t j = l.id[e] - i * kPer;
 #pragma unroll
       for (uint32_t q = 0; q < kPer; ++q)
-        if (q == j) {
-          l.x[e] = x[q];
-          if (kTail) x[q] = -__builtin_inff();
-        }
+        if (q == j) x[q] = -__builtin_inff();
     }
   }
-  // Puts their gradients in.
-  __device__ __forceinline__ void patch(float (&g)[E::kPer], uint32_t i, const RowCoef& r) const {
-    for (uint32_t e = first_entry; e != kNone; e = l.next[e]) {
-      const uint32_t j = l.id[e] - i * kPer;
-      if (j >= kPer) continue;
-      const float f = p.mode == kModeDistill ? listed_grad(p, r, l.x[e], l.logit[e]) : r.patch;
-#pragma unroll
-      for (uint32_t q = 0; q < kPer; ++q)
-        if (q == j) g[q] = f;
-    }
-  }
-  __device__ __forceinline__ bool special(uint32_t c) const { return (mine >> c) & 1u; }
-
   // The partial chunk behind the whole ones, by the thread whose turn it is.
   __device__ __forceinline__ uint32_t rest() const { return p.vocab - whole * kPer; }
   __device__ __forceinline__ bool has_rest() const {
@@ -1092,70 +1127,68 @@ struct FusedRow {
     for (uint32_t q = 0; q < kPer; ++q)
       x[q] = q < rest() ? E::one(in[(size_t)whole * kPer + q]) : -__builtin_inff();
   }
-
-  // fn(x, i) for every chunk of the thread, the special elements left out.
+  // fn(x, i) for the thread's chunks from index `from` on, from memory.
   template <typename Fn>
-  __device__ __forceinline__ void each(const uint4 (&v)[kHeld], Fn fn) const {
+  __device__ __forceinline__ void each_read(uint32_t from, Fn fn) const {
     float x[E::kPer];
-#pragma unroll
-    for (uint32_t c = 0; c < kHeld; ++c) {
-      const uint32_t i = c * kThreads + threadIdx.x;
-      if (i < whole) {
-        unpack<E, false>(v[c], 0, x);
-        if (special(c)) leave(x, i);
-        fn(x, i);
-      }
-    }
-    for (uint32_t c = kHeld, i = kHeld * kThreads + threadIdx.x; i < whole; ++c, i += kThreads) {
+#pragma unroll 1
+    for (uint32_t i = from + threadIdx.x; i < whole; i += kThreads) {
       unpack<E, false>(load_chunk<E>(in + (size_t)i * kPer), 0, x);
-      if (special(c)) leave(x, i);
+      if (kTail) take_out(x, i);
       fn(x, i);
     }
     if (has_rest()) {
       load_rest(x);
-      leave(x, whole);
+      if (kTail) take_out(x, whole);
       fn(x, whole);
     }
   }
-
-  __device__ __forceinline__ Acc sums(const uint4 (&v)[kHeld], uint32_t* bad) const {
-    const float c = p.c;
-    Acc s;
-    bool first = true;
-    each(v, [&](const float (&x)[E::kPer], uint32_t) {
-      if (first) {
-        first = false;
-        float m = x[0];
+  __device__ __forceinline__ void start(Acc& s, const float (&x)[E::kPer]) const {
+    float m = x[0];
 #pragma unroll
-        for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
-        const float u = m * c;
-        s.shift = u > -kTooBig ? u : 0.0f;
-      }
-      add_chunk<E, false>(s, x, c);
-    });
-    *bad = kNone;
-    if (first || (s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) return s;
-    return sums_again(v, bad);
+    for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
+    const float u = m * p.c;
+    s.shift = u > -kTooBig ? u : 0.0f;
   }
 
-  // PartScan's second scan.
-  __device__ __forceinline__ Acc sums_again(const uint4 (&v)[kHeld], uint32_t* bad) const {
+  // special: bit c is set where the thread's chunk c holds a special element.
+  __device__ __forceinline__ Acc sums(const uint4 (&v)[kHeld], uint32_t special,
+                                      uint32_t* bad) const {
     const float c = p.c;
+    Acc s;
+    float x[E::kPer];
+#pragma unroll
+    for (uint32_t n = 0; n < kHeld; ++n) {
+      const uint32_t i = n * kThreads + threadIdx.x;
+      if (i < whole) {
+        unpack<E, false>(v[n], 0, x);
+        if (kTail && (special >> n & 1u)) take_out(x, i);
+        if (n == 0) start(s, x);
+        add_chunk<E, false>(s, x, c);
+      }
+    }
+    each_read(kHeld * kThreads, [&](const float (&y)[E::kPer], uint32_t i) {
+      if (i < kThreads) start(s, y);
+      add_chunk<E, false>(s, y, c);
+    });
+    *bad = kNone;
+    if (s.sum >= 0x1p-60f && s.sum <= 0x1p100f) return s;
+    // PartScan's second scan, from memory
     float top = -__builtin_inff();
     uint32_t at_bad = kNone;
-    each(v, [&](const float (&x)[E::kPer], uint32_t i) {
+    each_read(0, [&](const float (&y)[E::kPer], uint32_t i) {
 #pragma unroll
       for (int e = 0; e < E::kPer; ++e) {
-        const float u = x[e] * c;
+        const float u = y[e] * c;
         if (!(u < kTooBig) && at_bad == kNone) at_bad = i * kPer + e;
         top = fmaxf(top, u);
       }
     });
-    Acc s;
+    s = Acc();
     *bad = at_bad;
     if (at_bad != kNone || !(top > -kTooBig)) return s;
     s.shift = top;
-    each(v, [&](const float (&x)[E::kPer], uint32_t) { add_chunk<E, false>(s, x, c); });
+    each_read(0, [&](const float (&y)[E::kPer], uint32_t) { add_chunk<E, false>(s, y, c); });
     return s;
   }
 };
@@ -1163,118 +1196,131 @@ struct FusedRow {
 template <typename E, uint32_t kThreads, bool kTail>
 __global__ __launch_bounds__(kThreads) void fused_kernel(const ScoreParams p) {
   using Raw = typename E::Raw;
-  constexpr uint32_t kPer = E::kPer;
+  constexpr uint32_t kPer = E::kPer, kHeld = kTail ? kHeldTail : pb::kHeld;
   __shared__ FusedShared l;
   __shared__ uint32_t head[kThreads];
   const uint32_t row = blockIdx.x, lane = lane_id(), wave = threadIdx.x >> 6;
+  const uint32_t mine = threadIdx.x * kPer;  // the thread's place in a round of chunks
   const bool distill = p.mode == kModeDistill;
   const Raw* in = row_ptr<E>(p, row);
   Raw* out = static_cast<Raw*>(p.grad) + (size_t)row * p.grad_ld;
   const uint32_t whole = p.vocab / kPer;
-  if (row_unread(p, row)) {
+  FusedRow<E, kThreads, kTail> f{p, l, in, whole, kNone};
+  uint4 v[kHeld];
+  RowSum r{0.0, 0.0, 0.0, kNone};
+  TokenRow token{};
+  float weight = 1.0f;
+  if (distill)
+    weight = p.weight ? uniform_float(p.weight + row) : 1.0f;
+  else
+    token = token_row(p, row);
+  const bool unread = row_unread(p, row);
+  if (!unread) {
+    // the list first: its loads come back before the row's
+    ListLanes list{};
     if (wave == 0) {
-      const RowSum none{0.0, 0.0, 0.0, kNone};
-      const RowCoef c = distill ? finish_distill<E>(p, row, none, ListSum{})
-                                : finish_policy<E>(p, row, none, token_row<E>(p, row));
-      if (lane == 0) l.coef.state = c.state;
+      if (distill) {
+        list = load_list(p, row, lane);
+      } else {
+        list.id[0] = lane == 0 ? token.token : kNone;
+        list.id[1] = kNone;
+      }
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < kHeld; ++n)
+      if (n * kThreads + threadIdx.x < whole)
+        v[n] = stream_chunk<E>(in + (size_t)n * (kThreads * kPer) + mine);
+    head[threadIdx.x] = kNone;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t e = lane + 64u * h;
+        l.id[e] = list.id[h];
+        l.x[e] = 0.0f;
+        if (list.id[h] < p.vocab)
+          l.next[e] = atomicExch(&head[list.id[h] / kPer % kThreads], e);
+      }
     }
     __syncthreads();
-    fill_row<E, kThreads>(out, 0, p.vocab, l.coef.state);
-    return;
+    f.first_entry = head[threadIdx.x];
+    uint32_t special = 0;
+    for (uint32_t e = f.first_entry; e != kNone; e = l.next[e]) {
+      const uint32_t id = l.id[e];
+      l.x[e] = E::one(in[id]);
+      if (kTail && id / kPer < kHeld * kThreads) special |= 1u << (id / kPer / kThreads);
+    }
+    if (wave == 0 && distill) {
+      double pr[2];
+      const ListSum s = sum_teacher(p, list, lane, first_repeat(p, list, lane), pr);
+      l.pr[lane] = pr[0];
+      l.pr[lane + 64] = pr[1];
+      if (lane == 0) l.list = s;
+    }
+    uint32_t bad;
+    const Acc s = f.sums(v, special, &bad);
+    r = block_sum<kThreads>(s, bad, l.sums);
   }
-  // the list or the token first: its loads come back before the row's
-  ListLanes list{};
-  TokenRow token{};
+  DistillRow student;
+  PolicyRow policy;
+  ListSum list_sum{};
+  uint32_t id[2] = {kNone, kNone};
+  float x[2] = {0.0f, 0.0f};
+  double pr[2] = {0.0, 0.0};
   if (wave == 0) {
     if (distill) {
-      list = load_list(p, row, lane);
-    } else {
-      token = token_row<E>(p, row);
-      list.id[0] = lane == 0 ? token.token : kNone;
-      list.id[1] = kNone;
-    }
-  }
-  uint4 v[kHeld];
+      if (!unread) {
+        list_sum = l.list;
 #pragma unroll
-  for (uint32_t c = 0; c < kHeld; ++c) {
-    const uint32_t i = c * kThreads + threadIdx.x;
-    if (i < whole) v[c] = stream_chunk<E>(in + (size_t)i * kPer);
-  }
-  head[threadIdx.x] = kNone;
-  __syncthreads();
-  if (wave == 0) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t e = lane + 64u * h;
-      l.id[e] = list.id[h];
-      l.logit[e] = list.logit[h];
-      l.x[e] = 0.0f;
-      if (list.id[h] < p.vocab)
-        l.next[e] = atomicExch(&head[list.id[h] / kPer % kThreads], e);
-    }
-  }
-  __syncthreads();
-  FusedRow<E, kThreads, kTail> f{p, l, in, whole, head[threadIdx.x], 0};
-  for (uint32_t e = f.first_entry; e != kNone; e = l.next[e])
-    f.mine |= 1ull << (l.id[e] / kPer / kThreads);
-  if (wave == 0 && distill) {
-    double pr[2];
-    const ListSum s = sum_teacher(p, list, lane, pr);
-    l.pr[lane] = pr[0];
-    l.pr[lane + 64] = pr[1];
-    if (lane == 0) l.list = s;
-  }
-  uint32_t bad;
-  const Acc s = f.sums(v, &bad);
-  const RowSum r = block_sum<kThreads>(s, bad, l.sums);
-  if (wave == 0) {
-    RowCoef c;
-    if (distill) {
-      ListSum sums = l.list;
-      const uint32_t id[2] = {l.id[lane], l.id[lane + 64]};
-      const float x[2] = {l.x[lane], l.x[lane + 64]};
-      const double pr[2] = {l.pr[lane], l.pr[lane + 64]};
-      sum_student(p, id, x, pr, sums);
-      c = finish_distill<E>(p, row, r, sums);
+        for (int h = 0; h < 2; ++h) {
+          id[h] = l.id[lane + 64 * h];
+          x[h] = l.x[lane + 64 * h];
+          pr[h] = l.pr[lane + 64 * h];
+        }
+      }
+      student = distill_row<E>(p, row, weight, r, list_sum, id, x);
+      if (lane == 0) l.coef = student.coef;
+      write_distill(p, row, student, list_sum, x, pr);
     } else {
-      c = finish_policy<E>(p, row, r, token);
+      if (!unread) token.x = l.x[0];
+      policy = policy_row<E>(p, row, r, token);
+      if (lane == 0) l.coef = policy.coef;
+      write_policy(p, row, policy);
     }
-    if (lane == 0) l.coef = c;
   }
   __syncthreads();
-  const RowCoef k = l.coef;
+  const RowCoef& k = l.coef;
   if (k.state != kRowNormal) {
     fill_row<E, kThreads>(out, 0, p.vocab, k.state);
     return;
   }
+  const RowCoef near{k.shift, k.alpha};  // what most elements need
   float g[kPer];
 #pragma unroll
-  for (uint32_t c = 0; c < kHeld; ++c) {
-    const uint32_t i = c * kThreads + threadIdx.x;
-    if (i < whole) {
+  for (uint32_t n = 0; n < kHeld; ++n) {
+    if (n * kThreads + threadIdx.x < whole) {
 #pragma unroll
-      for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(E::get(v[c], e), p.c, k);
-      if (f.special(c)) f.patch(g, i, k);
-      store_chunk<E>(out + (size_t)i * kPer, E::pack(g));
+      for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(E::get(v[n], e), p.c, near);
+      store_chunk<E>(out + (size_t)n * (kThreads * kPer) + mine, E::pack(g));
     }
   }
-  for (uint32_t c = kHeld, i = kHeld * kThreads + threadIdx.x; i < whole; ++c, i += kThreads) {
+#pragma unroll 1
+  for (uint32_t i = kHeld * kThreads + threadIdx.x; i < whole; i += kThreads) {
     const uint4 w = load_chunk<E>(in + (size_t)i * kPer);
 #pragma unroll
-    for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(E::get(w, e), p.c, k);
-    if (f.special(c)) f.patch(g, i, k);
+    for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(E::get(w, e), p.c, near);
     store_chunk<E>(out + (size_t)i * kPer, E::pack(g));
   }
   if (f.has_rest()) {
     float x[kPer];
     f.load_rest(x);
 #pragma unroll
-    for (uint32_t e = 0; e < kPer; ++e) g[e] = grad_of<E, false>(x[e], p.c, k);
-    f.patch(g, whole, k);
-#pragma unroll
     for (uint32_t e = 0; e < kPer; ++e)
-      if (e < f.rest()) out[(size_t)whole * kPer + e] = E::raw(g[e]);
+      if (e < f.rest()) out[(size_t)whole * kPer + e] = E::raw(grad_of<E, false>(x[e], p.c, near));
   }
+  // the thread's own special elements, over what it has just stored
+  for (uint32_t e = f.first_entry; e != kNone; e = l.next[e])
+    out[l.id[e]] = E::raw(distill ? listed_grad(p, k, l.x[e], l.pr[e]) : k.patch);
 }
 
 // ---- top logits ----
@@ -1437,8 +1483,11 @@ __global__ __launch_bounds__(kSelectThreads) void top_select_kernel(const ScoreP
     const RowSum r = wave_join(v.shift, v.sum, v.moment, v.bad);
     if (threadIdx.x == 0) {
       pb_inference_error* at = p.err ? p.err + row : nullptr;
-      failed = row_failed<E>(p, row, r.bad, r.sum, at);
-      if (!failed) no_error(at);
+      failed = bad_row(r.bad, r.sum);
+      if (failed)
+        report_row<E>(p, row, r.bad, at);
+      else
+        no_error(at);
       if (p.lse) p.lse[row] = failed ? nan32() : (float)(kLn2 * (r.shift + log2(r.sum)));
     }
   }
@@ -1498,7 +1547,7 @@ void plan_scores(uint32_t dtype, ScoreParams* p) {
                              : chunks <= 256 * kHeld ? 256
                              : chunks <= 512 * kHeld ? 512
                                                      : 1024;
-    if (chunks <= 64u * threads && p->rows >= kFusedRows) p->fused = threads;
+    if (p->rows >= kFusedRows) p->fused = threads;
   }
   p->tile_shift = tile_shift_of(p->vocab);
   const uint32_t tile = 1u << p->tile_shift;
