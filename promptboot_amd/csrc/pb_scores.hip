@@ -26,7 +26,7 @@ constexpr uint32_t kStatsThreads = 512;
 constexpr uint32_t kStatsUnroll = 4;
 constexpr bool kStreamLoads = false;
 constexpr uint32_t kGradThreads = 256;
-constexpr uint32_t kSelectThreads = 512;
+constexpr uint32_t kTopThreads = 256;
 constexpr float kTooBig = 3.0e38f;  // |u| past this has left binary32's range
 
 // ---- element types: 16 bytes are one chunk ----
@@ -216,12 +216,12 @@ __device__ __forceinline__ void unpack(const uint4& v, uint32_t marks, float (&x
 }
 
 // A thread's sums over its chunks of [lo, hi), chunk i of thread t being
-// element lo + (i kStatsThreads + t) kPer.  The shift is the thread's first
+// element lo + (i kThreads + t) kPer.  The shift is the thread's first
 // chunk's largest u: nothing then underflows that weighs, and where a later u
 // passes it by over 100, or the first chunk is masked out, the sum shows it
 // (too large, or too small) and the thread goes over its chunks again with their
 // true maximum.  So the pass does no comparison per element.
-template <typename E, bool kEntropy, bool kTail>
+template <typename E, uint32_t kThreads, bool kEntropy, bool kTail>
 struct PartScan {
   const typename E::Raw* row;
   const uint32_t* marks;
@@ -233,15 +233,15 @@ struct PartScan {
     constexpr uint32_t kPer = E::kPer;
     const uint32_t whole = (hi - lo) / kPer;
     uint32_t i = threadIdx.x;
-    for (; i + (kStatsUnroll - 1) * kStatsThreads < whole; i += kStatsUnroll * kStatsThreads) {
+    for (; i + (kStatsUnroll - 1) * kThreads < whole; i += kStatsUnroll * kThreads) {
       uint4 v[kStatsUnroll];
 #pragma unroll
       for (uint32_t q = 0; q < kStatsUnroll; ++q)
-        v[q] = stream_chunk<E>(row + lo + (size_t)(i + q * kStatsThreads) * kPer);
+        v[q] = stream_chunk<E>(row + lo + (size_t)(i + q * kThreads) * kPer);
 #pragma unroll
-      for (uint32_t q = 0; q < kStatsUnroll; ++q) chunk(v[q], (i + q * kStatsThreads) * kPer, fn);
+      for (uint32_t q = 0; q < kStatsUnroll; ++q) chunk(v[q], (i + q * kThreads) * kPer, fn);
     }
-    for (; i < whole; i += kStatsThreads)
+    for (; i < whole; i += kThreads)
       chunk(stream_chunk<E>(row + lo + (size_t)i * kPer), i * kPer, fn);
     const uint32_t rest = (hi - lo) - whole * kPer;
     if (rest != 0 && i == whole) {
@@ -281,7 +281,11 @@ struct PartScan {
     });
     *bad = kNone;
     if (first || (s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) return s;
-    // again, with the largest u of all
+    return again(bad);
+  }
+
+  // The sums about the largest u of all.
+  __device__ __forceinline__ Acc again(uint32_t* bad) const {
     float top = -__builtin_inff();
     uint32_t at_bad = kNone;
     each([&](const float (&x)[E::kPer], uint32_t at) {
@@ -292,7 +296,7 @@ struct PartScan {
         top = fmaxf(top, u);
       }
     });
-    s = Acc();
+    Acc s;
     if (at_bad != kNone) {
       *bad = at_bad;
       return s;
@@ -850,7 +854,7 @@ __global__ __launch_bounds__(kStatsThreads) void stats_kernel(const ScoreParams 
   const uint32_t lo = split * p.span;
   const uint32_t hi = p.vocab - lo < p.span ? p.vocab : lo + p.span;
   if (kTail) mark_ids(p, row, lo, hi, marks);
-  const PartScan<E, kEntropy, kTail> scan{row_ptr<E>(p, row), marks, lo, hi, p.c};
+  const PartScan<E, kStatsThreads, kEntropy, kTail> scan{row_ptr<E>(p, row), marks, lo, hi, p.c};
   uint32_t bad;
   const Acc s = scan.run(&bad);
   RowSum r = block_sum<kStatsThreads>(s, bad, l);
@@ -1327,43 +1331,22 @@ __global__ __launch_bounds__(kThreads) void fused_kernel(const ScoreParams p) {
 // A row's tiles of 2^tile_shift consecutive logits: the k largest logits lie in
 // the k tiles of the largest maxima (the lower tile first among equal ones),
 // since each of those holds a logit that ranks before any logit of another tile.
+// So one pass over the row leaves its sums and a word a tile, and only k to
+// k + kSlack tiles are read again.
 
-template <typename E>
-__global__ __launch_bounds__(kStatsThreads) void top_tiles_kernel(const ScoreParams p) {
-  __shared__ BlockSum l;
-  __shared__ uint32_t words[kMaxTiles];
-  const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
-  const uint32_t lo = split * p.span;
-  const uint32_t hi = p.vocab - lo < p.span ? p.vocab : lo + p.span;
-  const uint32_t tiles = (hi - lo + (1u << p.tile_shift) - 1u) >> p.tile_shift;
-  for (uint32_t i = threadIdx.x; i < tiles; i += kStatsThreads) words[i] = 0;
-  __syncthreads();
-  const PartScan<E, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi, p.c};
-  uint32_t bad;
-  const Acc s = scan.run(&bad);
-  scan.each([&](const float (&x)[E::kPer], uint32_t at) {
-    float m = x[0];
-#pragma unroll
-    for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
-    atomicMax(&words[at >> p.tile_shift], ord_of(b_of(m)));
-  });
-  const RowSum r = block_sum<kStatsThreads>(s, bad, l);
-  if (threadIdx.x == 0)
-    p.part[(size_t)row * p.splits + split] = RowPart{(float)r.shift, r.bad, r.sum, r.moment};
-  const uint32_t all = (p.vocab + (1u << p.tile_shift) - 1u) >> p.tile_shift;
-  uint32_t* to = p.tiles + (size_t)row * all + (lo >> p.tile_shift);
-  for (uint32_t i = threadIdx.x; i < tiles; i += kStatsThreads) to[i] = words[i];
-}
+constexpr uint32_t kSlack = 64;            // tiles more than k that may be read
+constexpr uint32_t kMaxList = PB_TOP_LOGITS_MAX + kSlack;
+constexpr uint32_t kMaxCandidates = 512;
+constexpr uint32_t kRounds = 32;           // of the search for the k-th largest word
 
-constexpr uint32_t kMaxCandidates = 1024;
-
-struct SelectShared {
-  uint32_t words[kMaxTiles];
+struct TopShared {
+  BlockSum sums;
   uint64_t keys[kMaxCandidates];
-  uint32_t list[PB_TOP_LOGITS_MAX];
-  uint32_t counts[kSelectThreads / 64];
+  uint64_t best[kTopThreads / 64];
+  uint32_t list[kMaxList];
+  uint32_t counts[kRounds];
   uint32_t n_list, n_keys;
-  uint64_t best[kSelectThreads / 64];
+  uint32_t state;  // of the row: whether this workgroup selects, and whether it failed
 };
 
 // Larger key: larger value, then lower id.
@@ -1375,39 +1358,114 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return f_of((ord & 0x80000000u) ? (ord & 0x7fffffffu) : ~ord);
 }
 
+// The largest of a chunk over the lanes that share its 64 elements.
+template <typename E>
+__device__ __forceinline__ float tile_max(float m) {
+  const uint32_t lane = lane_id();
+  m = fmaxf(m, f_of(lane_xor(b_of(m), 1, lane)));
+  m = fmaxf(m, f_of(lane_xor(b_of(m), 2, lane)));
+  m = fmaxf(m, f_of(lane_xor(b_of(m), 4, lane)));
+  if (E::kPer == 4) m = fmaxf(m, f_of(lane_xor(b_of(m), 8, lane)));
+  return m;
+}
+
+// The part's sums, and its tiles' words; every lane of a wave takes part in
+// every round, with -inf where the part has ended.
+template <typename E>
+__device__ __forceinline__ Acc scan_tiles(const ScoreParams& p, const typename E::Raw* in,
+                                          uint32_t n, uint32_t* words) {
+  constexpr uint32_t kPer = E::kPer, kGroup = 64u / kPer;
+  const uint32_t whole = n / kPer, rest = n - whole * kPer;
+  Acc s;
+  bool first = true;
+  auto take = [&](const float (&x)[E::kPer], uint32_t i) {
+    float m = fmaxf(x[0], x[1]);
+#pragma unroll
+    for (int e = 2; e < E::kPer; e += 2) m = fmaxf(m, fmaxf(x[e], x[e + 1]));
+    if (first) {
+      first = false;
+      const float u = m * p.c;
+      s.shift = u > -kTooBig ? u : 0.0f;
+    }
+    add_chunk<E, false>(s, x, p.c);
+    const uint32_t word = ord_of(b_of(tile_max<E>(m)));
+    if (p.tile_shift == 6) {
+      if (threadIdx.x % kGroup == 0 && i * kPer < n) words[i / kGroup] = word;
+    } else if (threadIdx.x % kGroup == 0 && i * kPer < n) {
+      atomicMax(&words[(i * kPer) >> p.tile_shift], word);
+    }
+  };
+  float x[E::kPer];
+  uint32_t base = 0;
+  for (; base + 4u * kTopThreads <= whole; base += 4u * kTopThreads) {
+    uint4 v[4];
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q)
+      v[q] = stream_chunk<E>(in + (size_t)(base + q * kTopThreads + threadIdx.x) * kPer);
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q) {
+      unpack<E, false>(v[q], 0, x);
+      take(x, base + q * kTopThreads + threadIdx.x);
+    }
+  }
+  for (; base < whole + (rest ? 1u : 0u); base += kTopThreads) {
+    const uint32_t i = base + threadIdx.x;
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; ++e) x[e] = -__builtin_inff();
+    if (i < whole) {
+      unpack<E, false>(stream_chunk<E>(in + (size_t)i * kPer), 0, x);
+    } else if (i == whole) {
+#pragma unroll
+      for (uint32_t e = 0; e < kPer; ++e)
+        if (e < rest) x[e] = E::one(in[(size_t)whole * kPer + e]);
+    }
+    take(x, i);
+  }
+  return s;
+}
+
 // The k best of a row from its tiles' words in LDS; every thread.
 template <typename E>
-__device__ void select_top(const ScoreParams& p, uint32_t row, uint32_t tiles, SelectShared& l) {
+__device__ void select_top(const ScoreParams& p, uint32_t row, uint32_t tiles,
+                           const uint32_t* words, TopShared& l) {
+  constexpr uint32_t kPer = E::kPer, kWaves = kTopThreads / 64;
   const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
   const uint32_t want = p.k < tiles ? p.k : tiles;
-  constexpr uint32_t kWaves = kSelectThreads / 64;
-  // the want-th largest word, bit by bit
-  uint32_t level = 0;
-  for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-    const uint32_t trial = level | bit;
+  if (threadIdx.x < kRounds) l.counts[threadIdx.x] = 0;
+  if (threadIdx.x == 0) l.n_list = l.n_keys = 0;
+  __syncthreads();
+  // A word that `want` to `want` + kSlack words reach, by halving; failing that
+  // (many equal words) the want-th largest.
+  uint32_t low = 0, high = ~0u, reach = tiles;  // reach: words >= low
+  for (uint32_t round = 0; round < kRounds && reach > want + kSlack; ++round) {
+    const uint32_t middle = low + (high - low) / 2u + 1u;
     uint32_t n = 0;
-    for (uint32_t i = threadIdx.x; i < tiles; i += kSelectThreads) n += l.words[i] >= trial ? 1u : 0u;
-    const uint32_t sum = wave_sum_word(n);
-    if (lane == 0) l.counts[wave] = sum;
+    for (uint32_t i = threadIdx.x; i < ((tiles + 63u) & ~63u); i += kTopThreads)
+      n += (uint32_t)__popcll((unsigned long long)__ballot(i < tiles && words[i] >= middle));
+    if (lane == 0) atomicAdd(&l.counts[round], n);
     __syncthreads();
-    uint32_t total = 0;
-    for (uint32_t w = 0; w < kWaves; ++w) total += l.counts[w];
-    if (total >= want) level = trial;
-    __syncthreads();
+    n = l.counts[round];
+    if (n >= want) {
+      low = middle;
+      reach = n;
+    } else {
+      high = middle - 1u;
+    }
   }
-  // the tiles above it, and the first of those at it
-  if (threadIdx.x == 0) l.n_keys = 0;
-  if (wave == 0) {
+  if (reach <= want + kSlack) {
+    for (uint32_t i = threadIdx.x; i < tiles; i += kTopThreads)
+      if (words[i] >= low) l.list[atomicAdd(&l.n_list, 1u)] = i;
+  } else if (wave == 0) {
+    // the tiles above the word, and the first of those at it
     uint32_t above = 0;
-    for (uint32_t i = lane; i < tiles; i += 64u) above += l.words[i] > level ? 1u : 0u;
-    above = wave_sum_word(above);
-    uint32_t n = 0, equal = want - above;
+    for (uint32_t i = lane; i < tiles; i += 64u) above += words[i] > low ? 1u : 0u;
+    uint32_t n = 0, equal = want - wave_sum_word(above);
     for (uint32_t base = 0; base < tiles; base += 64u) {
       const uint32_t i = base + lane;
-      const uint32_t v = i < tiles ? l.words[i] : 0u;
-      const bool at = i < tiles && v == level;
+      const uint32_t v = i < tiles ? words[i] : 0u;
+      const bool at = i < tiles && v == low;
       const uint64_t same = __ballot(at);
-      const bool take = (i < tiles && v > level) || (at && lanes_below(same) < equal);
+      const bool take = (i < tiles && v > low) || (at && lanes_below(same) < equal);
       const uint64_t taken = __ballot(take);
       if (take) l.list[n + lanes_below(taken)] = i;
       n += (uint32_t)__popcll((unsigned long long)taken);
@@ -1417,27 +1475,38 @@ __device__ void select_top(const ScoreParams& p, uint32_t row, uint32_t tiles, S
     if (lane == 0) l.n_list = n;
   }
   __syncthreads();
-  const typename E::Raw* x = row_ptr<E>(p, row);
-  const uint32_t size = 1u << p.tile_shift, n_list = l.n_list;
-  const uint32_t total = n_list << p.tile_shift;
-  uint32_t* out_id = p.top_id + (size_t)row * p.k;
-  float* out_value = p.top_value + (size_t)row * p.k;
-  for (uint32_t i = threadIdx.x; i < total; i += kSelectThreads) {
-    const uint32_t id = (l.list[i >> p.tile_shift] << p.tile_shift) + (i & (size - 1u));
-    if (id >= p.vocab) continue;
-    const uint64_t key = value_key(E::one(x[id]), id);
-    if ((uint32_t)(key >> 32) >= level) {
+  // the listed tiles' logits that reach the word: all of the k largest, and few others
+  const typename E::Raw* in = row_ptr<E>(p, row);
+  const uint32_t per_tile = 1u << p.tile_shift, total = l.n_list << p.tile_shift;
+  auto offer = [&](float x, uint32_t id) {
+    const uint64_t key = value_key(x, id);
+    if ((uint32_t)(key >> 32) >= low) {
       const uint32_t at = atomicAdd(&l.n_keys, 1u);
       if (at < kMaxCandidates) l.keys[at] = key;
     }
+  };
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x * kPer; i < total; i += kTopThreads * kPer) {
+    const uint32_t id = (l.list[i >> p.tile_shift] << p.tile_shift) + (i & (per_tile - 1u));
+    if (id + kPer <= p.vocab) {
+      const uint4 v = load_chunk<E>(in + id);
+#pragma unroll
+      for (uint32_t e = 0; e < kPer; ++e) offer(E::get(v, e), id + e);
+    } else {
+      for (uint32_t e = 0; e < kPer; ++e)
+        if (id + e < p.vocab) offer(E::one(in[id + e]), id + e);
+    }
   }
   __syncthreads();
+  uint32_t* out_id = p.top_id + (size_t)row * p.k;
+  float* out_value = p.top_value + (size_t)row * p.k;
   const uint32_t n = l.n_keys;
-  if (tiles > p.k && n <= kMaxCandidates) {
+  if (n >= p.k && n <= kMaxCandidates) {
     // a key's rank is the number of keys above it (no two are equal)
-    for (uint32_t i = threadIdx.x; i < n; i += kSelectThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += kTopThreads) {
       const uint64_t key = l.keys[i];
       uint32_t rank = 0;
+#pragma unroll 8
       for (uint32_t j = 0; j < n; ++j) rank += l.keys[j] > key ? 1u : 0u;
       if (rank < p.k) {
         out_id[rank] = 0xffffffffu - (uint32_t)key;
@@ -1450,10 +1519,10 @@ __device__ void select_top(const ScoreParams& p, uint32_t row, uint32_t tiles, S
   uint64_t last = ~0ull;
   for (uint32_t rank = 0; rank < p.k; ++rank) {
     uint64_t best = 0;
-    for (uint32_t i = threadIdx.x; i < total; i += kSelectThreads) {
-      const uint32_t id = (l.list[i >> p.tile_shift] << p.tile_shift) + (i & (size - 1u));
+    for (uint32_t i = threadIdx.x; i < total; i += kTopThreads) {
+      const uint32_t id = (l.list[i >> p.tile_shift] << p.tile_shift) + (i & (per_tile - 1u));
       if (id >= p.vocab) continue;
-      const uint64_t key = value_key(E::one(x[id]), id);
+      const uint64_t key = value_key(E::one(in[id]), id);
       if (key < last && key > best) best = key;
     }
     best = wave_max64(best);
@@ -1469,37 +1538,77 @@ __device__ void select_top(const ScoreParams& p, uint32_t row, uint32_t tiles, S
   }
 }
 
+constexpr uint32_t kTopWaits = 0, kTopSelects = 1, kTopFailed = 2;
+
+// A part's pass, and by the row's last part its selection.  The words of a row
+// in parts go through the workspace at the device's scope, as RowPart does.
 template <typename E>
-__global__ __launch_bounds__(kSelectThreads) void top_select_kernel(const ScoreParams p) {
-  __shared__ SelectShared l;
-  __shared__ bool failed;
-  const uint32_t row = blockIdx.x;
-  const uint32_t tiles = (p.vocab + (1u << p.tile_shift) - 1u) >> p.tile_shift;
-  for (uint32_t i = threadIdx.x; i < tiles; i += kSelectThreads)
-    l.words[i] = p.tiles[(size_t)row * tiles + i];
+__global__ __launch_bounds__(kTopThreads) void top_kernel(const ScoreParams p) {
+  __shared__ TopShared l;
+  extern __shared__ uint32_t words[];  // the row's
+  const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
+  const uint32_t lo = split * p.span;
+  const uint32_t hi = p.vocab - lo < p.span ? p.vocab : lo + p.span;
+  const uint32_t round_up = (1u << p.tile_shift) - 1u;
+  const uint32_t own = (hi - lo + round_up) >> p.tile_shift;
+  const uint32_t tiles = (p.vocab + round_up) >> p.tile_shift;
+  if (p.tile_shift > 6) {
+    for (uint32_t i = threadIdx.x; i < own; i += kTopThreads) words[i] = 0;
+    __syncthreads();
+  }
+  Acc s = scan_tiles<E>(p, row_ptr<E>(p, row) + lo, hi - lo, words);
+  uint32_t bad = kNone;
+  if (!(s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) {
+    const PartScan<E, kTopThreads, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi, p.c};
+    s = scan.again(&bad);
+  }
+  RowSum r = block_sum<kTopThreads>(s, bad, l.sums);  // its barrier: the words are there
+  uint32_t* shared_words = p.tiles + (size_t)row * tiles;
+  if (p.splits > 1) {
+    for (uint32_t i = threadIdx.x; i < own; i += kTopThreads)
+      __hip_atomic_store(shared_words + (lo >> p.tile_shift) + i, words[i], __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
   if (threadIdx.x < 64) {
-    RowPart v{0.0f, kNone, 0.0, 0.0};
-    if (threadIdx.x < p.splits) v = p.part[(size_t)row * p.splits + threadIdx.x];
-    const RowSum r = wave_join(v.shift, v.sum, v.moment, v.bad);
+    bool last = true;
+    if (p.splits > 1) {
+      last = last_part(p, row, split, r);
+      if (last) {
+        RowPart v{0.0f, kNone, 0.0, 0.0};
+        if (lane_id() < p.splits) v = collect_part(p.part + (size_t)row * p.splits + lane_id());
+        r = wave_join(v.shift, v.sum, v.moment, v.bad);
+      }
+    }
     if (threadIdx.x == 0) {
-      pb_inference_error* at = p.err ? p.err + row : nullptr;
-      failed = bad_row(r.bad, r.sum);
-      if (failed)
-        report_row<E>(p, row, r.bad, at);
-      else
-        no_error(at);
-      if (p.lse) p.lse[row] = failed ? nan32() : (float)(kLn2 * (r.shift + log2(r.sum)));
+      l.state = kTopWaits;
+      if (last) {
+        pb_inference_error* at = p.err ? p.err + row : nullptr;
+        const bool failed = bad_row(r.bad, r.sum);
+        if (failed)
+          report_row<E>(p, row, r.bad, at);
+        else
+          no_error(at);
+        if (p.lse) p.lse[row] = failed ? nan32() : (float)(kLn2 * (r.shift + log2(r.sum)));
+        l.state = failed ? kTopFailed : kTopSelects;
+      }
     }
   }
   __syncthreads();
-  if (failed) {
-    for (uint32_t i = threadIdx.x; i < p.k; i += kSelectThreads) {
+  if (l.state == kTopWaits) return;
+  if (l.state == kTopFailed) {
+    for (uint32_t i = threadIdx.x; i < p.k; i += kTopThreads) {
       p.top_id[(size_t)row * p.k + i] = PB_NO_TOKEN;
       p.top_value[(size_t)row * p.k + i] = nan32();
     }
     return;
   }
-  select_top<E>(p, row, tiles, l);
+  if (p.splits > 1) {
+    for (uint32_t i = threadIdx.x; i < tiles; i += kTopThreads)
+      words[i] = __hip_atomic_load(shared_words + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  select_top<E>(p, row, tiles, words, l);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -1607,8 +1716,8 @@ struct Launch {
     grad(p, p.grad_entropy != nullptr, s);
   }
   static void top(const ScoreParams& p, hipStream_t s) {
-    top_tiles_kernel<E><<<p.rows * p.splits, kStatsThreads, 0, s>>>(p);
-    top_select_kernel<E><<<p.rows, kSelectThreads, 0, s>>>(p);
+    const size_t words = (size_t)ceil_div(p.vocab, 1u << p.tile_shift) * 4;
+    top_kernel<E><<<p.rows * p.splits, kTopThreads, words, s>>>(p);
   }
   template <uint32_t kThreads>
   static void fused(const ScoreParams& p, hipStream_t s) {
