@@ -107,6 +107,7 @@ struct ScoreParams {
   uint32_t grad_splits;  // workgroups per row of the gradient pass
   uint32_t grad_span;
   uint32_t fused;        // threads of a workgroup that takes a whole row, or 0
+  uint32_t keep;         // the statistics pass leaves the logits in the caches
   uint32_t tile_shift;   // log2 of the elements of a top-logits tile
   uint32_t* ticket;      // rows: parts of the row that are done, 0 between calls
   RowPart* part;         // rows x splits
