@@ -818,8 +818,8 @@ __device__ __forceinline__ void publish_part(RowPart* at, const RowSum& r) {
                      __HIP_MEMORY_SCOPE_AGENT);
   __hip_atomic_store(w + 2, __builtin_bit_cast(uint64_t, r.moment), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
+__device__ __forceinline__ void acknowledged() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ RowPart collect_part(const RowPart* at) {
   const uint64_t* w = reinterpret_cast<const uint64_t*>(at);
   const uint64_t head = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -828,18 +828,22 @@ __device__ __forceinline__ RowPart collect_part(const RowPart* at) {
   return RowPart{f_of((uint32_t)head), (uint32_t)(head >> 32), __builtin_bit_cast(double, sum),
                  __builtin_bit_cast(double, moment)};
 }
-// Publishes this part of a row; true in the wave whose part was the last.
-__device__ __forceinline__ bool last_part(const ScoreParams& p, uint32_t row, uint32_t split,
-                                          const RowSum& r) {
+// Takes the ticket of a part whose words are acknowledged; true in the wave whose
+// part was the row's last.
+__device__ __forceinline__ bool last_part(const ScoreParams& p, uint32_t row) {
   uint32_t before = 0;
-  if (lane_id() == 0) {
-    publish_part(p.part + (size_t)row * p.splits + split, r);
+  if (lane_id() == 0)
     before = __hip_atomic_fetch_add(&p.ticket[row], 1u, __ATOMIC_RELAXED,
                                     __HIP_MEMORY_SCOPE_AGENT);
-  }
   if (bcast32(before, 0) != p.splits - 1u) return false;
   if (lane_id() == 0) p.ticket[row] = 0;
   return true;
+}
+// The row's parts joined, by one wave.
+__device__ __forceinline__ RowSum join_parts(const ScoreParams& p, uint32_t row) {
+  RowPart v{0.0f, kNone, 0.0, 0.0};
+  if (lane_id() < p.splits) v = collect_part(p.part + (size_t)row * p.splits + lane_id());
+  return wave_join(v.shift, v.sum, v.moment, v.bad);
 }
 
 // The statistics pass.  A row's parts leave their sums in the workspace, and
@@ -865,10 +869,10 @@ __global__ __launch_bounds__(kStatsThreads) void stats_kernel(const ScoreParams 
   RowSum r = block_sum<kStatsThreads>(s, bad, l);
   if (threadIdx.x >= 64) return;
   if (p.splits > 1) {
-    if (!last_part(p, row, split, r)) return;
-    RowPart v{0.0f, kNone, 0.0, 0.0};
-    if (lane_id() < p.splits) v = collect_part(p.part + (size_t)row * p.splits + lane_id());
-    r = wave_join(v.shift, v.sum, v.moment, v.bad);
+    if (lane_id() == 0) publish_part(p.part + (size_t)row * p.splits + split, r);
+    acknowledged();
+    if (!last_part(p, row)) return;
+    r = join_parts(p, row);
   }
   finish_row<E>(p, row, r);
 }
@@ -1644,48 +1648,42 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
   RowSum r = block_sum<kTopThreads>(s, bad, l.sums);  // its barrier: the words are there
   uint32_t* shared_words = p.tiles + (size_t)row * tiles;
   if (p.splits > 1) {
+    if (threadIdx.x == 0) publish_part(p.part + (size_t)row * p.splits + split, r);
     for (uint32_t i = threadIdx.x; i < own; i += kTopThreads)
       __hip_atomic_store(shared_words + (lo >> p.tile_shift) + i, words[i], __ATOMIC_RELAXED,
                          __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    acknowledged();
     __syncthreads();
+    if (threadIdx.x < 64) {
+      const bool last = last_part(p, row);
+      if (threadIdx.x == 0) l.state = last ? kTopSelects : kTopWaits;
+    }
+    __syncthreads();
+    if (l.state == kTopWaits) return;
+    for (uint32_t i = threadIdx.x; i < tiles; i += kTopThreads)
+      words[i] = __hip_atomic_load(shared_words + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();  // l.state is written again
   }
   if (threadIdx.x < 64) {
-    bool last = true;
-    if (p.splits > 1) {
-      last = last_part(p, row, split, r);
-      if (last) {
-        RowPart v{0.0f, kNone, 0.0, 0.0};
-        if (lane_id() < p.splits) v = collect_part(p.part + (size_t)row * p.splits + lane_id());
-        r = wave_join(v.shift, v.sum, v.moment, v.bad);
-      }
-    }
+    if (p.splits > 1) r = join_parts(p, row);
     if (threadIdx.x == 0) {
-      l.state = kTopWaits;
-      if (last) {
-        pb_inference_error* at = p.err ? p.err + row : nullptr;
-        const bool failed = bad_row(r.bad, r.sum);
-        if (failed)
-          report_row<E>(p, row, r.bad, at);
-        else
-          no_error(at);
-        if (p.lse) p.lse[row] = failed ? nan32() : (float)(kLn2 * (r.shift + log2(r.sum)));
-        l.state = failed ? kTopFailed : kTopSelects;
-      }
+      pb_inference_error* at = p.err ? p.err + row : nullptr;
+      const bool failed = bad_row(r.bad, r.sum);
+      if (failed)
+        report_row<E>(p, row, r.bad, at);
+      else
+        no_error(at);
+      if (p.lse) p.lse[row] = failed ? nan32() : (float)(kLn2 * (r.shift + log2(r.sum)));
+      l.state = failed ? kTopFailed : kTopSelects;
     }
   }
   __syncthreads();
-  if (l.state == kTopWaits) return;
   if (l.state == kTopFailed) {
     for (uint32_t i = threadIdx.x; i < p.k; i += kTopThreads) {
       p.top_id[(size_t)row * p.k + i] = PB_NO_TOKEN;
       p.top_value[(size_t)row * p.k + i] = nan32();
     }
     return;
-  }
-  if (p.splits > 1) {
-    for (uint32_t i = threadIdx.x; i < tiles; i += kTopThreads)
-      words[i] = __hip_atomic_load(shared_words + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   select_top<E>(p, row, tiles, words, l);
 }
@@ -1695,6 +1693,7 @@ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 
 // Workgroups that a pass over few rows is cut into.
 constexpr uint32_t kTargetGroups = 1024;
+constexpr uint32_t kTopGroups = 512;
 constexpr uint64_t kCacheBytes = 256ull << 20;
 // Rows from which a loss and its gradient take one launch, a workgroup a row.
 constexpr uint32_t kFusedRows = 256;
@@ -1743,7 +1742,7 @@ void plan_scores(uint32_t dtype, ScoreParams* p) {
   p->tile_shift = tile_shift_of(p->vocab);
   const uint32_t tile = 1u << p->tile_shift;
   if (p->rows == 0) return;
-  uint32_t splits = kTargetGroups / p->rows;
+  uint32_t splits = (p->mode == kModeTop ? kTopGroups : kTargetGroups) / p->rows;
   const uint32_t most = ceil_div(p->vocab, 4096u);
   if (splits > most) splits = most;
   if (splits > kMaxSplits) splits = kMaxSplits;
