@@ -320,6 +320,7 @@ struct RowSum {
 
 // One RowSum per lane into one, the same in every lane.  The factors between
 // parts come from the 32-bit exp2: the part that holds the largest u has 1.
+template <bool kMoment>
 __device__ __forceinline__ RowSum wave_join(float shift, double sum, double moment, uint32_t bad) {
   const bool live = sum > 0.0;
   const float top = wave_max_f32(live ? shift : -__builtin_inff());
@@ -327,7 +328,7 @@ __device__ __forceinline__ RowSum wave_join(float shift, double sum, double mome
   const double f = live ? (double)exp2_hw(off) : 0.0;
   RowSum r;
   r.sum = wave_sum_f64(f * sum);
-  r.moment = wave_sum_f64(f * (moment + (double)off * sum));
+  r.moment = kMoment ? wave_sum_f64(f * (moment + (double)off * sum)) : 0.0;
   r.bad = wave_min_word(bad);
   r.shift = r.sum > 0.0 ? (double)top : 0.0;
   return r;
@@ -340,11 +341,11 @@ struct BlockSum {
   double sum[16];
   double moment[16];
 };
-template <uint32_t kThreads>
+template <uint32_t kThreads, bool kMoment>
 __device__ __forceinline__ RowSum block_sum(const Acc& s, uint32_t bad, BlockSum& l) {
   const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
-  const RowSum w = wave_join(s.shift, (double)s.sum, (double)s.moment, bad);
-  if (lane == 0) {
+  const RowSum w = wave_join<kMoment>(s.shift, (double)s.sum, (double)s.moment, bad);
+  if (lane == 0 && wave < kThreads / 64) {
     l.shift[wave] = (float)w.shift;
     l.sum[wave] = w.sum;
     l.moment[wave] = w.moment;
@@ -353,8 +354,8 @@ __device__ __forceinline__ RowSum block_sum(const Acc& s, uint32_t bad, BlockSum
   __syncthreads();
   if (wave != 0) return w;
   const bool on = lane < kThreads / 64;
-  return wave_join(on ? l.shift[lane] : 0.0f, on ? l.sum[lane] : 0.0, on ? l.moment[lane] : 0.0,
-                   on ? l.bad[lane] : kNone);
+  return wave_join<kMoment>(on ? l.shift[lane] : 0.0f, on ? l.sum[lane] : 0.0,
+                            on ? l.moment[lane] : 0.0, on ? l.bad[lane] : kNone);
 }
 
 // Marks the teacher's ids that lie in [lo, hi); every thread, then a barrier.
@@ -768,41 +769,65 @@ __device__ __forceinline__ void write_distill(const ScoreParams& p, uint32_t row
   if (p.lse) p.lse[row] = (float)lse;
 }
 
+// What a wave of its own has made of a row's list while the others scan the row.
+struct ListShared {
+  ListSum sum;
+  uint32_t id[PB_TOP_LOGITS_MAX];
+  float x[PB_TOP_LOGITS_MAX];
+  double pr[PB_TOP_LOGITS_MAX];
+};
+template <typename E>
+__device__ __forceinline__ void prepare_list(const ScoreParams& p, uint32_t row, ListShared& l) {
+  const uint32_t lane = lane_id();
+  const ListLanes list = load_list(p, row, lane);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l.id[lane + 64 * h] = list.id[h];
+    l.x[lane + 64 * h] = list.id[h] < p.vocab ? E::one(row_ptr<E>(p, row)[list.id[h]]) : 0.0f;
+  }
+  double pr[2];
+  const ListSum s = sum_teacher(p, list, lane, first_repeat(p, list, lane), pr);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) l.pr[lane + 64 * h] = pr[h];
+  if (lane == 0) l.sum = s;
+}
+
 // A row's scalars from its sums; one wave.
 template <typename E>
 __device__ __forceinline__ void finish_row(const ScoreParams& p, uint32_t row, const RowSum& r) {
-  const uint32_t lane = lane_id();
-  if (p.mode == kModeDistill) {
-    const float weight = p.weight ? p.weight[row] : 1.0f;
-    ListSum s{};
-    uint32_t id[2] = {kNone, kNone};
-    float x[2] = {0.0f, 0.0f};
-    double pr[2] = {0.0, 0.0};
-    if (weight != 0.0f) {
-      const ListLanes l = load_list(p, row, lane);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        id[h] = l.id[h];
-        x[h] = id[h] < p.vocab ? E::one(row_ptr<E>(p, row)[id[h]]) : 0.0f;
-      }
-      s = sum_teacher(p, l, lane, first_repeat(p, l, lane), pr);
-    }
-    const DistillRow o = distill_row<E>(p, row, weight, r, s, id, x);
-    if (lane == 0 && p.grad) p.coef[row] = o.coef;
-    write_distill(p, row, o, s, x, pr);
-    return;
-  }
   TokenRow t = token_row(p, row);
   if (t.token < p.vocab) t.x = E::one(row_ptr<E>(p, row)[t.token]);
   if (p.mode == kModePolicy) {
     const PolicyRow o = policy_row<E>(p, row, r, t);
-    if (lane == 0 && p.grad) p.coef[row] = o.coef;
+    if (lane_id() == 0 && p.grad) p.coef[row] = o.coef;
     write_policy(p, row, o);
   } else if (p.mode == kModePreference) {
     finish_pair_row(p, row, r, t);
   } else {
     finish_logprobs<E>(p, row, r, t);
   }
+}
+template <typename E>
+__device__ __forceinline__ void finish_list_row(const ScoreParams& p, uint32_t row,
+                                                const RowSum& r, const ListShared& l) {
+  const uint32_t lane = lane_id();
+  const float weight = p.weight ? uniform_float(p.weight + row) : 1.0f;
+  ListSum s{};
+  uint32_t id[2] = {kNone, kNone};
+  float x[2] = {0.0f, 0.0f};
+  double pr[2] = {0.0, 0.0};
+  if (weight != 0.0f) {
+    s = l.sum;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      id[h] = l.id[lane + 64 * h];
+      x[h] = l.x[lane + 64 * h];
+      pr[h] = l.pr[lane + 64 * h];
+    }
+  }
+  const DistillRow o = distill_row<E>(p, row, weight, r, s, id, x);
+  if (lane == 0 && p.grad) p.coef[row] = o.coef;
+  write_distill(p, row, o, s, x, pr);
 }
 
 // Parts of a row pass between workgroups of one launch, which may run on XCDs
@@ -840,10 +865,11 @@ __device__ __forceinline__ bool last_part(const ScoreParams& p, uint32_t row) {
   return true;
 }
 // The row's parts joined, by one wave.
+template <bool kMoment>
 __device__ __forceinline__ RowSum join_parts(const ScoreParams& p, uint32_t row) {
   RowPart v{0.0f, kNone, 0.0, 0.0};
   if (lane_id() < p.splits) v = collect_part(p.part + (size_t)row * p.splits + lane_id());
-  return wave_join(v.shift, v.sum, v.moment, v.bad);
+  return wave_join<kMoment>(v.shift, v.sum, v.moment, v.bad);
 }
 
 // The statistics pass.  A row's parts leave their sums in the workspace, and
@@ -851,30 +877,50 @@ __device__ __forceinline__ RowSum join_parts(const ScoreParams& p, uint32_t row)
 // joins them and works out the row's scalars, so that they need no launch of
 // their own.
 // kKeep: the row is read again soon, and what the call reads may stay in the caches.
-template <typename E, bool kEntropy, bool kTail, bool kKeep>
-__global__ __launch_bounds__(kStatsThreads) void stats_kernel(const ScoreParams p) {
+// kList: the distillation; a fifth wave takes the teacher's list (at the end of
+// the row's last part instead, 12 rows took 14.8 us, so 13.0).
+constexpr uint32_t kNoList = 0, kListOnly = 1, kListWithRest = 2;
+template <typename E, bool kEntropy, uint32_t kList, bool kKeep>
+__global__ __launch_bounds__(kStatsThreads + (kList ? 64 : 0)) void stats_kernel(
+    const ScoreParams p) {
+  constexpr bool kTail = kList == kListWithRest;
   __shared__ BlockSum l;
+  __shared__ ListShared list;
   extern __shared__ uint32_t marks[];
   const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
   if (row_unread(p, row)) {
-    if (split == 0 && threadIdx.x < 64) finish_row<E>(p, row, RowSum{0.0, 0.0, 0.0, kNone});
+    if (split != 0 || threadIdx.x >= 64) return;
+    const RowSum none{0.0, 0.0, 0.0, kNone};
+    if (kList)
+      finish_list_row<E>(p, row, none, list);
+    else
+      finish_row<E>(p, row, none);
     return;
   }
   const uint32_t lo = split * p.span;
   const uint32_t hi = p.vocab - lo < p.span ? p.vocab : lo + p.span;
   if (kTail) mark_ids(p, row, lo, hi, marks);
-  const PartScan<E, kStatsThreads, kEntropy, kTail, kKeep> scan{row_ptr<E>(p, row), marks, lo, hi, p.c};
-  uint32_t bad;
-  const Acc s = scan.run(&bad);
-  RowSum r = block_sum<kStatsThreads>(s, bad, l);
+  uint32_t bad = kNone;
+  Acc s;
+  if (!kList || threadIdx.x < kStatsThreads) {
+    const PartScan<E, kStatsThreads, kEntropy, kTail, kKeep> scan{row_ptr<E>(p, row), marks, lo,
+                                                                 hi, p.c};
+    s = scan.run(&bad);
+  } else {
+    prepare_list<E>(p, row, list);
+  }
+  RowSum r = block_sum<kStatsThreads, kEntropy>(s, bad, l);
   if (threadIdx.x >= 64) return;
   if (p.splits > 1) {
     if (lane_id() == 0) publish_part(p.part + (size_t)row * p.splits + split, r);
     acknowledged();
     if (!last_part(p, row)) return;
-    r = join_parts(p, row);
+    r = join_parts<kEntropy>(p, row);
   }
-  finish_row<E>(p, row, r);
+  if (kList)
+    finish_list_row<E>(p, row, r, list);
+  else
+    finish_row<E>(p, row, r);
 }
 
 // ---- preference loss: one workgroup a pair ----
@@ -1297,7 +1343,7 @@ __global__ __launch_bounds__(kThreads, 4) void fused_kernel(const ScoreParams p)
     }
     uint32_t bad;
     const Acc s = f.sums(v, special, &bad);
-    r = block_sum<kThreads>(s, bad, l.sums);
+    r = block_sum<kThreads, false>(s, bad, l.sums);
   }
   DistillRow student;
   PolicyRow policy;
@@ -1645,7 +1691,7 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
     const PartScan<E, kTopThreads, false, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi, p.c};
     s = scan.again(&bad);
   }
-  RowSum r = block_sum<kTopThreads>(s, bad, l.sums);  // its barrier: the words are there
+  RowSum r = block_sum<kTopThreads, false>(s, bad, l.sums);  // its barrier: the words are there
   uint32_t* shared_words = p.tiles + (size_t)row * tiles;
   if (p.splits > 1) {
     if (threadIdx.x == 0) publish_part(p.part + (size_t)row * p.splits + split, r);
@@ -1665,7 +1711,7 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
     __syncthreads();  // l.state is written again
   }
   if (threadIdx.x < 64) {
-    if (p.splits > 1) r = join_parts(p, row);
+    if (p.splits > 1) r = join_parts<false>(p, row);
     if (threadIdx.x == 0) {
       pb_inference_error* at = p.err ? p.err + row : nullptr;
       const bool failed = bad_row(r.bad, r.sum);
@@ -1771,23 +1817,23 @@ void place_scores(void* work, ScoreParams* p) {
 
 namespace {
 
-template <typename E, bool kEntropy, bool kTail>
+template <typename E, bool kEntropy, uint32_t kList>
 void launch_stats(const ScoreParams& p, hipStream_t stream) {
-  const size_t marks = kTail ? ((size_t)p.span / 32 + 2) * 4 : 0;
-  const uint32_t groups = p.rows * p.splits;
+  const size_t marks = kList == kListWithRest ? ((size_t)p.span / 32 + 2) * 4 : 0;
+  const uint32_t groups = p.rows * p.splits, threads = kStatsThreads + (kList ? 64u : 0u);
   if (p.keep)
-    stats_kernel<E, kEntropy, kTail, true><<<groups, kStatsThreads, marks, stream>>>(p);
+    stats_kernel<E, kEntropy, kList, true><<<groups, threads, marks, stream>>>(p);
   else
-    stats_kernel<E, kEntropy, kTail, false><<<groups, kStatsThreads, marks, stream>>>(p);
+    stats_kernel<E, kEntropy, kList, false><<<groups, threads, marks, stream>>>(p);
 }
 
 template <typename E>
 struct Launch {
   static void logprobs(const ScoreParams& p, hipStream_t s) {
     if (p.entropy)
-      launch_stats<E, true, false>(p, s);
+      launch_stats<E, true, kNoList>(p, s);
     else
-      launch_stats<E, false, false>(p, s);
+      launch_stats<E, false, kNoList>(p, s);
   }
   static void grad(const ScoreParams& p, bool beta, hipStream_t s) {
     const uint32_t groups = p.rows * p.grad_splits;
@@ -1817,10 +1863,12 @@ struct Launch {
       case 256: return fused<256, 0>(p, s);
       case 512: return fused<512, kShelved>(p, s);
     }
-    if (p.teacher_lse)
-      launch_stats<E, false, true>(p, s);
+    if (p.mode != kModeDistill)
+      launch_stats<E, false, kNoList>(p, s);
+    else if (p.teacher_lse)
+      launch_stats<E, false, kListWithRest>(p, s);
     else
-      launch_stats<E, false, false>(p, s);
+      launch_stats<E, false, kListOnly>(p, s);
     if (p.grad) grad(p, false, s);
   }
   static void preference(const ScoreParams& p, hipStream_t s) {
@@ -1828,7 +1876,7 @@ struct Launch {
       pair_kernel<E><<<p.pairs, 256, 0, s>>>(p);
       return;
     }
-    launch_stats<E, false, false>(p, s);
+    launch_stats<E, false, kNoList>(p, s);
     pair_kernel<E><<<p.pairs, 256, 0, s>>>(p);
     if (p.grad) grad(p, false, s);
   }
