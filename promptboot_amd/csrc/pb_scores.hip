@@ -1761,8 +1761,11 @@ constexpr uint32_t kTargetGroups = 1024;
 constexpr uint32_t kTopGroups = 512;
 constexpr uint32_t kGradGroups = 65536;
 constexpr uint64_t kCacheBytes = 256ull << 20;
-// Rows from which a loss and its gradient take one launch, a workgroup a row.
-constexpr uint32_t kFusedRows = 256;
+// A loss and its gradient take one launch, a workgroup a row, for rows of up to
+// kShortRow bytes and from kFusedRows longer ones on.
+constexpr uint32_t kShortRow = 160 * 1024;
+constexpr uint32_t kFusedRows = 64;
+constexpr uint32_t kFewChunks = 4;  // a thread, below which more threads share a row
 
 uint32_t tile_shift_of(uint32_t vocab) {
   uint32_t shift = 6;
@@ -1800,10 +1803,21 @@ void plan_scores(uint32_t dtype, ScoreParams* p) {
   p->keep = (uint64_t)p->rows * p->vocab * (dtype == PB_F32 ? 4u : 2u) <= kCacheBytes;
   if (p->grad != nullptr && (p->mode == kModeDistill || p->mode == kModePolicy)) {
     const uint32_t chunks = ceil_div(p->vocab, dtype == PB_F32 ? 4u : 8u);
-    const uint32_t threads = chunks <= 64 * kHeld    ? 64
-                             : chunks <= 256 * kHeld ? 256
-                                                     : 512;
-    if (p->rows >= kFusedRows) p->fused = threads;
+    // threads a row: as few as hold it, or more where rows do not fill the compute
+    // units (64 rows of 8,000 bf16 logits: 7.2 us by 256 threads, 7.8 by 64)
+    uint32_t threads = chunks <= 64 * kHeld ? 64 : chunks <= 256 * kHeld ? 256 : 512;
+    if (p->rows <= 1024 && threads < 256 && chunks > 64 * kFewChunks) threads = 256;
+    if (p->rows <= 512 && threads < 512 && chunks > 256 * kFewChunks) threads = 512;
+    if (p->rows <= 256 && threads < 1024 && chunks > 512 * kFewChunks) threads = 1024;
+    // One launch or two passes, us by rows (policy loss with gradient):
+    //   rows              1           12          64          256         1,000
+    //   1,000 bf16    4.7 / 7.7   5.8 / 10.8  5.9 / 11.2  6.1 / 10.3  6.6 / 8.4
+    //   32,000 f32    8.5 / 11.5  9.2 / 9.8  10.0 / 12.9   14 / 22     48 / 51
+    //   100,003 f16    15 / 10     18 / 13     20 / 20     24 / 32     87 / 95
+    //   151,936 f32    21 / 9.8    21 / 15     23 / 26     54 / 61    247 / 253
+    // A long row takes one workgroup longer than many.
+    const uint64_t row_bytes = (uint64_t)p->vocab * (dtype == PB_F32 ? 4u : 2u);
+    if (row_bytes <= kShortRow || p->rows >= kFusedRows) p->fused = threads;
   }
   p->tile_shift = tile_shift_of(p->vocab);
   const uint32_t tile = 1u << p->tile_shift;
@@ -1881,6 +1895,7 @@ struct Launch {
       case 64: return fused<64, 0>(p, s);
       case 256: return fused<256, 0>(p, s);
       case 512: return fused<512, kShelved>(p, s);
+      case 1024: return fused<1024, 0>(p, s);
     }
     if (p.mode != kModeDistill)
       launch_stats<E, false, kNoList>(p, s);
