@@ -449,7 +449,7 @@ void pb_context_set_segments(pb_context *ctx, uint32_t segments);
  *
  * A logit of -inf (or one whose y / ln 2 is below binary32's range) weighs
  * nothing.  A row whose token is PB_NO_TOKEN, or whose weight is 0, is
- * skipped: its logits are not read, its outputs are 0, its gradient row is 0.
+ * skipped: its logits do not matter, its outputs are 0, its gradient row is 0.
  * A row error gives NaN outputs, a NaN gradient row and, when d_err is given,
  * a record with `position` = the row: PB_TOKEN_ID (an id >= vocab; needed =
  * vocab, available = the id), PB_NONFINITE_OUTPUT (a NaN or +inf logit, or a y
@@ -505,8 +505,8 @@ uint32_t pb_token_logprobs_grad(pb_context *ctx, const void *d_logits, uint32_t 
                                 void *stream, pb_inference_error *err);
 
 /* The k largest logits of each row, largest first and the lowest id first
- * among equal ones (-0 equals 0): d_token rows x k ids, d_value rows x k raw
- * logits as binary32; d_lse (optional) as pb_token_logprobs.  k <= vocab and
+ * among equal ones: d_token rows x k ids, d_value rows x k raw logits as
+ * binary32 (-0 counts as 0 and comes back as 0); d_lse (optional) as pb_token_logprobs.  k <= vocab and
  * k <= PB_TOP_LOGITS_MAX.  -inf logits are taken last, like any other value.
  * No row is skipped; a row error gives PB_NO_TOKEN ids. */
 uint32_t pb_top_logits(pb_context *ctx, const void *d_logits, uint32_t dtype, size_t vocab,
@@ -556,7 +556,7 @@ uint32_t pb_policy_loss(pb_context *ctx, const void *d_logits, uint32_t dtype, s
  * - e ln sigma(-h) with e = label_smoothing (0 to 1).  d_ref_logprob (NULL: 0)
  * and d_logprob (optional, l_s) have 2 x pairs entries, d_weight `pairs`: a
  * pair of weight 0 has loss, log-probabilities and gradient 0.  Rows before the
- * first and behind the last sequence are not read, and their gradient rows are
+ * first and behind the last sequence do not matter, and their gradient rows are
  * left as they are.  d_err (optional): one record per pair, the first of its
  * rows that failed (the whole pair is then NaN); PB_CAPACITY (needed = rows,
  * available = the offset) for offsets that decrease or pass `rows`, whose pair

@@ -179,6 +179,12 @@ struct Acc {
   float moment = 0.0f;
 };
 
+// The shift of a thread whose first chunk's largest u is `u`: that, or 0 where the
+// chunk is masked out.  Past binary32's range it is one that fails the fast sums.
+__device__ __forceinline__ float first_shift(float u) {
+  return u < kTooBig ? (u > -kTooBig ? u : 0.0f) : -__builtin_inff();
+}
+
 // Bits of the marks of the elements j .. j + kPer - 1 of a part that starts at lo.
 template <typename E>
 __device__ __forceinline__ uint32_t chunk_marks(const uint32_t* marks, uint32_t at) {
@@ -279,7 +285,7 @@ struct PartScan {
 #pragma unroll
         for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
         const float u = m * c;
-        s.shift = u > -kTooBig ? u : 0.0f;
+        s.shift = first_shift(u);
       }
       add_chunk<E, kEntropy>(s, x, c);
     });
@@ -1244,7 +1250,7 @@ struct FusedRow {
 #pragma unroll
     for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
     const float u = m * p.c;
-    s.shift = u > -kTooBig ? u : 0.0f;
+    s.shift = first_shift(u);
   }
 
   // special: bit c is set where the thread's chunk c holds a special element.
@@ -1492,7 +1498,7 @@ __device__ __forceinline__ Acc scan_tiles(const ScoreParams& p, const typename E
     if (first) {
       first = false;
       const float u = m * p.c;
-      s.shift = u > -kTooBig ? u : 0.0f;
+      s.shift = first_shift(u);
     }
     add_chunk<E, false>(s, x, p.c);
     const uint32_t word = ord_of(b_of(tile_max<E>(m)));

@@ -592,6 +592,7 @@ class DecodeBatch:
             lib().pb_sampling_state_new(ctypes.byref(self.states[r]), int(seed) & (2**64 - 1))
         self._saved = (_State * self.rows)()
         self.err = hip.DeviceArray((self.rows, ERROR_DTYPE.itemsize // 4), np.uint32)
+        self._scores = None
 
     def close(self):
         if self._own and self.sampler is not None:
@@ -633,14 +634,27 @@ class DecodeBatch:
                 vp(self.r24.data_ptr()), vp(self.token.data_ptr()), None,
                 vp(self.err.data_ptr()))
 
-    def step(self, logits, stream=None) -> np.ndarray:
+    def step(self, logits, stream=None, logprobs=None,
+             logprob_temperature: float = 1.0) -> np.ndarray:
         """One step on logits [rows, ld] (rows that have ended are ignored).
         Returns the tokens (NO_TOKEN for rows not sampled).  A refused step
-        leaves every SamplingState as it was."""
+        leaves every SamplingState as it was.
+
+        `logprobs` (a device buffer of rows binary32 values) receives
+        ln softmax(logits / logprob_temperature)[token] of each sampled token,
+        0 for rows not sampled: a rollout's behaviour log-probabilities, of the
+        raw logits (no repetition penalty, no cutoff)."""
         rows, ld = _shape(logits)
         if rows != self.rows:
             raise ValueError(f"logits have {rows} rows, the batch has {self.rows}")
         lp = _dev(logits, "logits", ndim=2)
+        score = None
+        if logprobs is not None:  # checked before anything is drawn
+            score = self._scorer().bind_token_logprobs(
+                logits, self.token, logprob=logprobs, temperature=logprob_temperature,
+                vocab=VOCAB, stream=stream)
+            if not 0.01 <= logprob_temperature <= 100.0:
+                raise ValueError(f"a temperature of {logprob_temperature} is not supported")
         before = self._draw(stream)
         e = _Error()
         try:
@@ -650,7 +664,16 @@ class DecodeBatch:
         except Exception:
             self._undraw()
             raise
+        if score is not None:
+            score()
         return self._settle(before, stream)
+
+    def _scorer(self):
+        if self._scores is None:
+            from .scores import RowScorer
+
+            self._scores = RowScorer(sampler=self.sampler)
+        return self._scores
 
     def lmhead_step(self, packed, hidden, cols: int | None = None, stream=None,
                     q8: bool = False) -> np.ndarray:

@@ -109,7 +109,9 @@ class RowScorer:
             self.reserve(max(rows, have[0]), max(vocab, have[1]))
 
     def _rows(self, logits, vocab, dtype):
-        """The leading arguments of a call on `logits`: (argument tuple, rows, dtype)."""
+        """The leading arguments of a call on `logits`, its rows, vocabulary and type."""
+        if self.sampler is None:
+            raise ValueError("the scorer's context is closed")
         ptr, rows, columns, ld = _matrix(logits, "logits", self.device)
         vocab = columns if vocab is None else int(vocab)
         if not 0 < vocab <= columns:
@@ -128,11 +130,12 @@ class RowScorer:
             raise ValueError("grad must have the logits' type")
         return ptr, ld
 
-    @staticmethod
-    def _call(name: str, argv: tuple, keep: tuple):
+    def _call(self, name: str, argv: tuple, keep: tuple):
         fn = getattr(lib(), name)
 
         def call():
+            if self.sampler is None or not self.sampler._ctx:
+                raise ValueError("the scorer's context is closed")
             e = _Error()
             st = fn(*argv, ctypes.byref(e))
             if st != OK:

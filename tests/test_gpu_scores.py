@@ -687,3 +687,103 @@ def test_teacher_to_student_and_rollout_to_policy(scorer):
     near(loss, -adv.double(), 1.1 * half + ref.EPS32 * adv.double().abs(), "loss")
     assert (kl.abs() <= 1e-12).all() and torch.equal(lp, behaviour)
     batch.close()
+
+
+def test_decode_steps_return_log_probabilities(scorer):
+    """A decode batch's own log-probabilities: of the tokens it drew, 0 for rows that have ended."""
+    rows, T = 5, 0.7
+    batch = s.DecodeBatch([[1, 2, 3]] * rows, list(range(7, 7 + rows)), [1, 4, 4, 2, 4], device=0)
+    plain = s.DecodeBatch([[1, 2, 3]] * rows, list(range(7, 7 + rows)), [1, 4, 4, 2, 4], device=0)
+    for step in range(4):
+        x, g = make_logits(rows, s.VOCAB, "f32", seed=60 + step)
+        lp = out(rows)
+        tokens = batch.step(x, logprobs=lp, logprob_temperature=T)
+        assert (tokens == plain.step(x)).all()
+        token = torch.from_numpy(tokens.view(np.int32)).to(DEV).long()
+        want = ref.logprobs(x, token, T)["logprob"]
+        near(lp, want, ref.scalar_tolerance(want, 2 * ref.lse_tolerance(x, T)), "logprob")
+        assert ((token >= 0) == (lp != 0)).all()
+    assert (tokens[[0, 3]] == s.NO_TOKEN).all() and batch.active() == plain.active()
+    before = [st.state() for st in batch.sampling_states()]
+    for bad in (dict(logprobs=torch.zeros(rows)), dict(logprobs=out(rows - 1)), dict(logprobs=out(rows, dtype=torch.float64)),
+                dict(logprobs=out(rows), logprob_temperature=0.0)):
+        with pytest.raises(ValueError):
+            batch.step(x, **bad)
+    assert [st.state() for st in batch.sampling_states()] == before
+    batch.close()
+    plain.close()
+
+
+def test_a_closed_scorer_refuses_its_calls():
+    sc = RowScorer(0)
+    x, g = make_logits(2, 50, "f32")
+    call = sc.bind_token_logprobs(x, ids_of(x, g).int(), logprob=out(2))
+    call()
+    torch.cuda.synchronize()
+    sc.close()
+    with pytest.raises(ValueError):
+        call()
+    with pytest.raises(ValueError):
+        sc.token_logprobs(x, ids_of(x, g).int(), logprob=out(2))
+
+
+def test_logits_just_past_the_range_fail_wherever_they_stand(scorer):
+    """y / ln 2 out of binary32's range, in the first chunk of a thread and in a later one."""
+    vocab = 40_000
+    for at in (3, vocab - 5):
+        for rows in (2, 1100):
+            x, g = make_logits(rows, vocab, "f32", seed=1)
+            x[1, at] = 2.2e38  # x log2(e) = 3.17e38
+            lp, loss, grad, err = out(rows), out(rows), torch.full_like(x, 5.0), records(rows)
+            token = ids_of(x, g).int()
+            scorer.token_logprobs(x, token, logprob=lp, err=err)
+            e = read_errors(err)
+            assert e["status"][1] == s.NONFINITE_OUTPUT and int(e["detail"][1]) & 0xFFFFFFFF == at
+            one = torch.ones(rows, device=DEV)
+            scorer.policy_loss(x, token, one, one, loss=loss, grad=grad, err=err)
+            e = read_errors(err)
+            assert e["status"][1] == s.NONFINITE_OUTPUT and int(e["detail"][1]) & 0xFFFFFFFF == at
+            assert lp[1].isnan() and loss[1].isnan() and grad[1].isnan().all() and torch.isfinite(grad[0]).all()
+            x[1, at] = -2.2e38  # below the range: weighs nothing
+            scorer.token_logprobs(x, token, logprob=lp, err=err)
+            assert not read_errors(err)["status"].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,k,tail", [(70, 9001, 60, True), (70, 170_001, 90, True), (70, 170_001, 90, False),
+                                               (600, 45_001, 128, True), (300, 25_003, 30, True), (2, 600_001, 100, True)])
+def test_lists_that_reach_every_part_of_a_row(scorer, dtype, rows, vocab, k, tail):
+    """Listed ids in the chunks that are held, kept in LDS and read again, neighbours in one chunk, the row's last."""
+    x, g = make_logits(rows, vocab, dtype, seed=vocab + k)
+    ids = torch.linspace(0, vocab - 1, k, device=DEV).long().repeat(rows, 1)
+    ids[:, 1], ids[:, 2], ids[:, k - 2] = 1, 2, vocab - 2
+    logit = torch.randn((rows, k), generator=g, device=DEV)
+    lse = (torch.logsumexp(logit.double(), 1) + 0.2).float() if tail else None
+    w = torch.rand(rows, generator=g, device=DEV) + 0.5
+    loss, grad = out(rows), torch.full_like(x, 5.0)
+    scorer.distill_loss(x, ids.int(), logit, teacher_lse=lse, weight=w, loss=loss, grad=grad)
+    tol = 2 * ref.lse_tolerance(x, 1.0)
+    for lo in range(0, rows, 100):  # in 64 bits by parts
+        r = slice(lo, lo + 100)
+        part = None if lse is None else lse[r]
+        want = ref.distill(x[r], ids[r], logit[r], 1.0, part, w[r])
+        near(loss[r], want["loss"], ref.scalar_tolerance(want["loss"], tol[r]), "loss")
+        near_grad(grad[r], want["grad"], distill_scale(x[r], ids[r], logit[r], 1.0, part, w[r]), x[r], 1.0, tol[r])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,vocab", [(64, 155_650), (64, 33), (1030, 5003), (70, 80_003)])
+def test_policy_tokens_in_every_part_of_a_row(scorer, dtype, rows, vocab):
+    x, g = make_logits(rows, vocab, dtype, seed=vocab)
+    token = torch.linspace(0, vocab - 1, rows, device=DEV).long()
+    lp = ref.logprobs(x, token)["logprob"].float()
+    adv = torch.ones(rows, device=DEV)
+    loss, grad = out(rows), torch.full_like(x, 5.0)
+    scorer.policy_loss(x, token.int(), lp, adv, loss=loss, grad=grad)
+    want = ref.policy(x, token, lp, adv)
+    tol = 2 * ref.lse_tolerance(x, 1.0) + ref.EPS32 * lp.double().abs()
+    q = torch.softmax(x.double(), 1)
+    one = torch.zeros_like(q).scatter_(1, token[:, None], 1.0)
+    bound = ref.grad_tolerance(want["grad"], adv[:, None].double() * 1.1, q, tol[:, None], x.dtype)
+    bound = bound + tol[:, None] * (one - q).abs() + one * q * tol[:, None]
+    near(grad, want["grad"], bound, "grad")
