@@ -1639,7 +1639,7 @@ __device__ void select_top(const ScoreParams& p, uint32_t row, uint32_t tiles,
       if (at < kMaxCandidates) l.keys[at] = key;
     }
   };
-#pragma unroll 4
+#pragma unroll 1
   for (uint32_t i = threadIdx.x * kPer; i < total; i += kTopThreads * kPer) {
     const uint32_t id = (l.list[i >> p.tile_shift] << p.tile_shift) + (i & (per_tile - 1u));
     if (id + kPer <= p.vocab) {
@@ -1766,7 +1766,7 @@ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 constexpr uint32_t kTargetGroups = 1024;
 constexpr uint32_t kTopGroups = 512;
 constexpr uint32_t kGradGroups = 65536;
-constexpr uint64_t kCacheBytes = 256ull << 20;
+constexpr uint64_t kCacheBytes = 400000000;
 // A loss and its gradient take one launch, a workgroup a row, for rows of up to
 // kShortRow bytes and from kFusedRows longer ones on.
 constexpr uint32_t kShortRow = 160 * 1024;
@@ -1804,9 +1804,12 @@ ScoresLayout scores_layout(uint32_t rows, uint32_t vocab) {
 
 void plan_scores(uint32_t dtype, ScoreParams* p) {
   p->fused = 0;
-  // 1,000 rows of 304 KB, forward and gradient: 146 us with the first read kept,
-  // 151 without; past the caches' 256 MB it is 258 and 226 us for the forward.
-  p->keep = (uint64_t)p->rows * p->vocab * (dtype == PB_F32 ? 4u : 2u) <= kCacheBytes;
+  // Forward and gradient of rows of 304 KB, us with the first read kept in the
+  // caches and without: 900 rows 128 / 132, 1,300 rows 189 / 191, 2,000 rows 287 /
+  // 283, 3,000 rows 431 / 426.  Of a preference batch's rows many are prompts or
+  // padding, which are not read (2,563 rows, 1,023 of them read: 213 / 222).
+  const uint64_t logit_bytes = (uint64_t)p->rows * p->vocab * (dtype == PB_F32 ? 4u : 2u);
+  p->keep = logit_bytes <= (p->mode == kModePreference ? 2u : 1u) * kCacheBytes;
   if (p->grad != nullptr && (p->mode == kModeDistill || p->mode == kModePolicy)) {
     const uint32_t chunks = ceil_div(p->vocab, dtype == PB_F32 ? 4u : 8u);
     // threads a row: as few as hold it, or more where rows do not fill the compute
