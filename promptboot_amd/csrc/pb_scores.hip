@@ -878,7 +878,8 @@ __device__ __forceinline__ RowSum join_parts(const ScoreParams& p, uint32_t row)
   return wave_join<kMoment>(v.shift, v.sum, v.moment, v.bad);
 }
 
-// The statistics pass.  A row's parts leave their sums in the workspace, and
+// The statistics pass; large batches read at 6.9 TB/s (4,096 rows of 151,936 bf16
+// logits in 182 us, a plain read's 7.0).  A row's parts leave their sums in the workspace, and
 // the workgroup that comes last (by the row's ticket, which it sets back to 0)
 // joins them and works out the row's scalars, so that they need no launch of
 // their own.
@@ -1158,14 +1159,19 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
 }
 
 // ---- a row's loss and gradient in one launch ----
-// One workgroup takes a whole row and keeps its first kHeld chunks a thread in
-// registers between the statistics and the gradient: a row of 155,648 16-bit
-// logits is read from memory once.  What lies beyond (32-bit rows over 77,824
-// ids) is read again.  The row's special elements (its token, or the teacher's
-// list) hang in chains on the threads that hold them: the owner leaves their
-// logits for the row's scalars, takes them out of the sums where the list has a
-// rest bucket, and stores their gradients over its own chunks', so that no store
-// waits for another thread's.
+// One workgroup takes a whole row and holds on to it between the statistics and
+// the gradient: its first kHeld chunks a thread in registers, with 512 threads
+// kShelved more in LDS.  512 threads hold 114,688 16-bit logits and leave room for
+// a second workgroup, whose loads run under the first one's scalars and stores;
+// what lies beyond is read again.  Of 4,096 rows of 151,936 bf16 logits a quarter
+// is, and they take 490 us: 2.5 GB at 5.1 TB/s, where a large copy reaches 5.0
+// (1,024 threads that hold the whole row, alone on their compute unit, 566 us
+// before and 548 after the change to 512; taking the next row's loads into the
+// gradient's stores, 590; requesting the chunks read again ahead, 525).
+// The row's special elements (its token, or the teacher's list) hang in chains on
+// the threads that hold them: the owner leaves their logits for the row's scalars,
+// takes them out of the sums where the list has a rest bucket, and stores their
+// gradients over its own chunks', so that no store waits for another thread's.
 
 constexpr uint32_t kHeld = 19;
 // With a rest bucket the row's scalars need more registers of their own.
@@ -1444,7 +1450,9 @@ __global__ __launch_bounds__(kThreads, 4) void fused_kernel(const ScoreParams p)
 // the k tiles of the largest maxima (the lower tile first among equal ones),
 // since each of those holds a logit that ranks before any logit of another tile.
 // So one pass over the row leaves its sums and a word a tile, and only k to
-// k + kSlack tiles are read again.
+// k + kSlack tiles are read again: 2,048 rows of 151,936 bf16 logits in 101 us, 6.2
+// TB/s, with the vector units busy two thirds of the time (109 us with quieting
+// maxima and separate lane moves, 163 by halving the words' range for the k-th).
 
 constexpr uint32_t kSlack = 64;            // tiles more than k that may be read
 constexpr uint32_t kMaxList = PB_TOP_LOGITS_MAX + kSlack;
@@ -1471,20 +1479,42 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return f_of((ord & 0x80000000u) ? (ord & 0x7fffffffu) : ~ord);
 }
 
-// The largest of a chunk over the lanes that share its 64 elements.
+// The largest of three without the compiler's quieting of signalling NaNs (a row
+// that holds a NaN fails by its sum).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 template <typename E>
-__device__ __forceinline__ float tile_max(float m) {
-  const uint32_t lane = lane_id();
-  m = fmaxf(m, f_of(lane_xor(b_of(m), 1, lane)));
-  m = fmaxf(m, f_of(lane_xor(b_of(m), 2, lane)));
-  m = fmaxf(m, f_of(lane_xor(b_of(m), 4, lane)));
-  if (E::kPer == 4) m = fmaxf(m, f_of(lane_xor(b_of(m), 8, lane)));
-  return m;
+__device__ __forceinline__ float chunk_max(const float (&x)[E::kPer]) {
+  float m = max3(x[0], x[1], x[2]);
+  if constexpr (E::kPer == 8) {
+    m = max3(m, x[3], x[4]);
+    return max3(m, x[5], max3(x[6], x[7], x[7]));
+  } else {
+    return max3(m, x[3], x[3]);
+  }
+}
+// A chunk's largest value as an order word (-0 as 0), over the lanes that share
+// its 64 elements: the four of a quad, mirrored halves of 8 and, for 32-bit rows,
+// mirrored 16.
+template <typename E>
+__device__ __forceinline__ uint32_t tile_word(float m) {
+  const uint32_t bits = b_of(m + 0.0f);
+  uint32_t w = bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u);
+  w = max(w, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, true));
+  w = max(w, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x4E, 0xF, 0xF, true));
+  w = max(w, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x141, 0xF, 0xF, true));
+  if (E::kPer == 4)
+    w = max(w, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x140, 0xF, 0xF, true));
+  return w;
 }
 
 // The part's sums, and its tiles' words; every lane of a wave takes part in
-// every round, with -inf where the part has ended.
-template <typename E>
+// every round, with -inf where the part has ended.  `words` has room for the
+// last round's whole wave.  kWide: tiles of more than 64 elements.
+template <typename E, bool kWide>
 __device__ __forceinline__ Acc scan_tiles(const ScoreParams& p, const typename E::Raw* in,
                                           uint32_t n, uint32_t* words) {
   constexpr uint32_t kPer = E::kPer, kGroup = 64u / kPer;
@@ -1492,21 +1522,18 @@ __device__ __forceinline__ Acc scan_tiles(const ScoreParams& p, const typename E
   Acc s;
   bool first = true;
   auto take = [&](const float (&x)[E::kPer], uint32_t i) {
-    float m = fmaxf(x[0], x[1]);
-#pragma unroll
-    for (int e = 2; e < E::kPer; e += 2) m = fmaxf(m, fmaxf(x[e], x[e + 1]));
+    const float m = chunk_max<E>(x);
     if (first) {
       first = false;
-      const float u = m * p.c;
-      s.shift = first_shift(u);
+      s.shift = first_shift(m * p.c);
     }
     add_chunk<E, false>(s, x, p.c);
-    const uint32_t word = ord_of(b_of(tile_max<E>(m)));
-    if (p.tile_shift == 6) {
-      if (threadIdx.x % kGroup == 0 && i * kPer < n) words[i / kGroup] = word;
-    } else if (threadIdx.x % kGroup == 0 && i * kPer < n) {
+    const uint32_t word = tile_word<E>(m);
+    // the lanes of a tile write the same word
+    if (kWide)
       atomicMax(&words[(i * kPer) >> p.tile_shift], word);
-    }
+    else
+      words[i / kGroup] = word;
   };
   float x[E::kPer];
   uint32_t base = 0;
@@ -1710,7 +1737,9 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
     for (uint32_t i = threadIdx.x; i < own; i += kTopThreads) words[i] = 0;
     __syncthreads();
   }
-  Acc s = scan_tiles<E>(p, row_ptr<E>(p, row) + lo, hi - lo, words);
+  const typename E::Raw* in = row_ptr<E>(p, row) + lo;
+  Acc s = p.tile_shift > 6 ? scan_tiles<E, true>(p, in, hi - lo, words)
+                           : scan_tiles<E, false>(p, in, hi - lo, words);
   uint32_t bad = kNone;
   if (!(s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) {
     const PartScan<E, kTopThreads, false, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi, p.c};
@@ -1889,7 +1918,9 @@ struct Launch {
       grad<kFromForward, false>(p, s);
   }
   static void top(const ScoreParams& p, hipStream_t s) {
-    const size_t words = (size_t)ceil_div(p.vocab, 1u << p.tile_shift) * 4;
+    // and what the last round of threads writes past the row's end
+    const size_t words =
+        (size_t)(ceil_div(p.vocab, 1u << p.tile_shift) + kTopThreads * E::kPer / 64u) * 4;
     top_kernel<E><<<p.rows * p.splits, kTopThreads, words, s>>>(p);
   }
   template <uint32_t kThreads, uint32_t kShelf>
