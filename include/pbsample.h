@@ -560,7 +560,8 @@ uint32_t pb_policy_loss(pb_context *ctx, const void *d_logits, uint32_t dtype, s
  * left as they are.  d_err (optional): one record per pair, the first of its
  * rows that failed (the whole pair is then NaN); PB_CAPACITY (needed = rows,
  * available = the offset) for offsets that decrease or pass `rows`, whose pair
- * gets a NaN loss and no gradient. */
+ * gets a NaN loss and no gradient; so does a pair of which such offsets make a
+ * row another sequence's too, but the one whose sequence comes last. */
 uint32_t pb_preference_loss(pb_context *ctx, const void *d_logits, uint32_t dtype, size_t vocab,
                             size_t ld, uint32_t rows, double temperature, const uint32_t *d_token,
                             const uint32_t *d_seq_start, uint32_t pairs,

@@ -113,6 +113,7 @@ struct ScoreParams {
   RowPart* part;         // rows x splits
   RowCoef* coef;         // rows
   uint32_t* tiles;       // rows x tile count: a top-logits tile's largest value, ordered
+  uint32_t* sequence;    // rows: the preference loss' sequence of each, in the tiles' place
 };
 
 // Largest part of a row of one workgroup of the statistics pass: its marks of

@@ -127,7 +127,8 @@ __device__ __forceinline__ uint32_t wave_fold(uint32_t v, Step step) {
   return step(v, lane_xor(v, 1, lane));
 }
 __device__ __forceinline__ float wave_max_f32(float v) {
-  return f_of(wave_fold(b_of(v), [](uint32_t a, uint32_t b) { return b_of(fmaxf(f_of(a), f_of(b))); }));
+  return f_of(wave_fold(
+      b_of(v), [](uint32_t a, uint32_t b) { return b_of(fmaxf(f_of(a), f_of(b))); }));
 }
 __device__ __forceinline__ uint32_t wave_min_word(uint32_t v) {
   return wave_fold(v, [](uint32_t a, uint32_t b) { return b < a ? b : a; });
@@ -547,10 +548,27 @@ __device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t r
   if (p.entropy) p.entropy[row] = entropy;
 }
 
+// The last sequence that starts at or before a row, by one wave: one look at every
+// 64th part of what is left.  Where offsets decrease, sequences may share rows; the
+// row then still has one owner, and the pairs that find another's fail.
+__device__ __forceinline__ uint32_t sequence_of(const ScoreParams& p, uint32_t row) {
+  uint32_t at = 0, n = 2u * p.pairs + 1u;
+  while (n > 1u) {
+    const uint32_t step = (n + 63u) / 64u, i = lane_id() * step;
+    const uint64_t before = __ballot(i < n && p.seq_start[at + i] <= row);
+    const uint32_t k = before ? 63u - (uint32_t)__builtin_clzll(before) : 0u;
+    at += k * step;
+    n = n - k * step < step ? n - k * step : step;
+  }
+  return at;
+}
+
 // The preference loss' rows, for the pairs' pass.
 __device__ __forceinline__ void finish_pair_row(const ScoreParams& p, uint32_t row,
                                                 const RowSum& r, const TokenRow& t) {
+  const uint32_t sequence = sequence_of(p, row);
   if (lane_id() != 0) return;
+  p.sequence[row] = sequence;
   PairRow* v = reinterpret_cast<PairRow*>(p.coef + row);
   v->state = kRowUntouched;
   v->shift = (float)r.shift;
@@ -879,10 +897,10 @@ __device__ __forceinline__ RowSum join_parts(const ScoreParams& p, uint32_t row)
 }
 
 // The statistics pass; large batches read at 6.9 TB/s (4,096 rows of 151,936 bf16
-// logits in 182 us, a plain read's 7.0).  A row's parts leave their sums in the workspace, and
-// the workgroup that comes last (by the row's ticket, which it sets back to 0)
-// joins them and works out the row's scalars, so that they need no launch of
-// their own.
+// logits in 182 us; a plain read reaches 7.0).  A row's parts leave their sums in
+// the workspace, and the workgroup that comes last (by the row's ticket, which it
+// sets back to 0) joins them and works out the row's scalars, so that they need no
+// launch of their own.
 // kKeep: the row is read again soon, and what the call reads may stay in the caches.
 // kList: the distillation; a fifth wave takes the teacher's list (at the end of
 // the row's last part instead, 12 rows took 14.8 us, so 13.0).
@@ -939,43 +957,46 @@ __device__ __forceinline__ PairRow pair_row(const ScoreParams& p, uint32_t row) 
 template <typename E>
 __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
   __shared__ double sums[2][4];
-  __shared__ uint32_t worst[4];
+  __shared__ uint32_t worst[4], foreign[4];
   __shared__ double slope_at;
   const uint32_t pair = blockIdx.x, lane = lane_id(), wave = threadIdx.x >> 6;
   pb_inference_error* at = p.err ? p.err + pair : nullptr;
   const uint32_t a = p.seq_start[2 * pair], b = p.seq_start[2 * pair + 1],
                  e = p.seq_start[2 * pair + 2];
+  auto refuse = [&](uint32_t offset) {
+    if (threadIdx.x != 0) return;
+    write_error(at, PB_CAPACITY, pair, p.rows, offset, PB_FIELD_BYTES, 10);
+    p.loss[pair] = nan32();
+    if (p.logprob) p.logprob[2 * pair] = p.logprob[2 * pair + 1] = nan32();
+  };
   // rows outside the first and the last offset have no statistics
-  if (a > b || b > e || e > p.rows || a < p.seq_start[0] || e > p.seq_start[2 * p.pairs]) {
-    if (threadIdx.x == 0) {
-      write_error(at, PB_CAPACITY, pair, p.rows, e > p.rows ? e : b, PB_FIELD_BYTES, 10);
-      p.loss[pair] = nan32();
-      if (p.logprob) p.logprob[2 * pair] = p.logprob[2 * pair + 1] = nan32();
-    }
-    return;
-  }
+  if (a > b || b > e || e > p.rows || a < p.seq_start[0] || e > p.seq_start[2 * p.pairs])
+    return refuse(e > p.rows ? e : b);
   const float w = p.weight ? p.weight[pair] : 1.0f;
   double mine[2] = {0.0, 0.0};
-  uint32_t failed = kNone;
-  if (w != 0.0f) {
-    for (uint32_t row = a + threadIdx.x; row < e; row += 256u) {
-      const uint32_t token = p.token[row];
-      if (token == PB_NO_TOKEN) continue;
-      const PairRow v = pair_row(p, row);
-      if (token >= p.vocab || bad_row(v.bad, v.sum))
-        failed = row < failed ? row : failed;
-      else
-        mine[row < b ? 0 : 1] += v.logprob;
-    }
+  uint32_t failed = kNone, stray = 0;
+  for (uint32_t row = a + threadIdx.x; row < e; row += 256u) {
+    const uint32_t token = p.token[row];
+    const PairRow v = pair_row(p, row);
+    // every row has to be this pair's before any coefficient is written
+    stray |= p.sequence[row] ^ (2u * pair + (row < b ? 0u : 1u));
+    if (w == 0.0f || token == PB_NO_TOKEN) continue;
+    if (token >= p.vocab || bad_row(v.bad, v.sum))
+      failed = row < failed ? row : failed;
+    else
+      mine[row < b ? 0 : 1] += v.logprob;
   }
   const double c = wave_sum_f64(mine[0]), d = wave_sum_f64(mine[1]);
   const uint32_t f = wave_min_word(failed);
+  const bool strays = __ballot(stray != 0) != 0;
   if (lane == 0) {
+    foreign[wave] = strays ? 1u : 0u;
     sums[0][wave] = c;
     sums[1][wave] = d;
     worst[wave] = f;
   }
   __syncthreads();
+  if (foreign[0] | foreign[1] | foreign[2] | foreign[3]) return refuse(a);
   if (threadIdx.x == 0) {
     double l[2] = {0.0, 0.0};
     uint32_t first = kNone;
@@ -1164,10 +1185,11 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
 // kShelved more in LDS.  512 threads hold 114,688 16-bit logits and leave room for
 // a second workgroup, whose loads run under the first one's scalars and stores;
 // what lies beyond is read again.  Of 4,096 rows of 151,936 bf16 logits a quarter
-// is, and they take 490 us: 2.5 GB at 5.1 TB/s, where a large copy reaches 5.0
-// (1,024 threads that hold the whole row, alone on their compute unit, 566 us
-// before and 548 after the change to 512; taking the next row's loads into the
-// gradient's stores, 590; requesting the chunks read again ahead, 525).
+// is, and they take 490 us: 2.5 GB at 5.1 TB/s, where a large copy reaches 5.0.
+// While gradients still went through the caches the same rows took 548 us, 566 by
+// 1,024 threads that hold the whole row alone on their compute unit, and 590 with
+// the next row's loads run into the gradient's stores; requesting the chunks that
+// are read again ahead of their turn costs registers and took 525 instead of 495.
 // The row's special elements (its token, or the teacher's list) hang in chains on
 // the threads that hold them: the owner leaves their logits for the row's scalars,
 // takes them out of the sums where the list has a rest bucket, and stores their
@@ -1220,7 +1242,8 @@ struct FusedRow {
     for (uint32_t q = 0; q < kPer; ++q)
       x[q] = q < rest() ? E::one(in[(size_t)whole * kPer + q]) : -__builtin_inff();
   }
-  // fn(chunk, i) for the thread's whole chunks from index `from` on, from memory, four loads at once.
+  // fn(chunk, i) for the thread's whole chunks from index `from` on, from memory, four loads at
+  // once.
   template <typename Fn>
   __device__ __forceinline__ void each_chunk(uint32_t from, Fn fn) const {
     uint32_t i = from + threadIdx.x;
@@ -1235,7 +1258,8 @@ struct FusedRow {
 #pragma unroll 1
     for (; i < whole; i += kThreads) fn(load_chunk<E>(in + (size_t)i * kPer), i);
   }
-  // fn(x, i), the partial chunk included and the special elements left out; keep(chunk, i) before it.
+  // fn(x, i), the partial chunk included and the special elements left out; keep(chunk, i) before
+  // it.
   template <typename Keep, typename Fn>
   __device__ __forceinline__ void each_read(uint32_t from, Keep keep, Fn fn) const {
     float x[E::kPer];
@@ -1302,7 +1326,8 @@ struct FusedRow {
     *bad = at_bad;
     if (at_bad != kNone || !(top > -kTooBig)) return s;
     s.shift = top;
-    each_read(0, forget, [&](const float (&y)[E::kPer], uint32_t) { add_chunk<E, false>(s, y, c); });
+    each_read(0, forget,
+              [&](const float (&y)[E::kPer], uint32_t) { add_chunk<E, false>(s, y, c); });
     return s;
   }
 };
@@ -1428,7 +1453,8 @@ __global__ __launch_bounds__(kThreads, 4) void fused_kernel(const ScoreParams p)
 #pragma unroll 1
   for (uint32_t n = 0; n < kShelf; ++n) {
     const uint32_t i = (kHeld + n) * kThreads + threadIdx.x;
-    if (i < whole) store_chunk<E>(out + (size_t)i * kPer, gradient(shelf[n * kThreads + threadIdx.x]));
+    if (i < whole)
+      store_chunk<E>(out + (size_t)i * kPer, gradient(shelf[n * kThreads + threadIdx.x]));
   }
   f.each_chunk((kHeld + kShelf) * kThreads, [&](const uint4& w, uint32_t i) {
     store_chunk<E>(out + (size_t)i * kPer, gradient(w));
@@ -1742,7 +1768,8 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
                            : scan_tiles<E, false>(p, in, hi - lo, words);
   uint32_t bad = kNone;
   if (!(s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) {
-    const PartScan<E, kTopThreads, false, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi, p.c};
+    const PartScan<E, kTopThreads, false, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi,
+                                                              p.c};
     s = scan.again(&bad);
   }
   RowSum r = block_sum<kTopThreads, false>(s, bad, l.sums);  // its barrier: the words are there
@@ -1884,7 +1911,7 @@ void place_scores(void* work, ScoreParams* p) {
   char* base = static_cast<char*>(work);
   p->part = reinterpret_cast<RowPart*>(base + l.part);
   p->coef = reinterpret_cast<RowCoef*>(base + l.coef);
-  p->tiles = reinterpret_cast<uint32_t*>(base + l.tiles);
+  p->tiles = p->sequence = reinterpret_cast<uint32_t*>(base + l.tiles);
 }
 
 namespace {

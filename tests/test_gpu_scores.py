@@ -491,6 +491,34 @@ def test_failed_pairs_have_records(scorer):
     assert grad[:12].isnan().all() and (grad[12:] == 5.0).all()
 
 
+@pytest.mark.parametrize("more", [0, 40, 5000])
+def test_pairs_that_share_rows_fail(scorer, more):
+    """Offsets that fall back would give rows to two pairs: they are the last sequence's alone."""
+    vocab, tail = 70, torch.arange(41, 41 + 2 * more)  # `more` pairs of one-row sequences behind the others
+    start = torch.cat([torch.tensor([0, 2, 6, 6, 8, 20, 3, 5, 7, 21, 40]), tail]).to(torch.int32)
+    pairs, rows = start.numel() // 2, int(start[-1]) + 2
+    x, g = make_logits(rows, vocab, "f32", seed=60 + more)
+    token = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+    lp = torch.log_softmax(x.double(), 1).gather(1, token[:, None])[:, 0]
+
+    def per_sequence(v):
+        return torch.cat([v.new_zeros(1), v.cumsum(0)])[start.to(DEV).long()].diff()[6:]
+
+    tol = ref.scalar_tolerance(per_sequence(lp), per_sequence(2 * ref.lse_tolerance(x, 1.0)))
+    for _ in range(3):
+        loss, logprob, grad, err = out(pairs), out(2 * pairs), torch.full((rows, vocab), 5.0, device=DEV), records(pairs)
+        scorer.preference_loss(x, token.int(), start.to(DEV), beta=0.1, loss=loss, logprob=logprob, grad=grad, err=err)
+        # the sequences: 0-1, 2-5 | none, 6-7 | 8-19, back to 3 | 3-4, 5-6 | 7-20, 21-39 | ...
+        e = read_errors(err)
+        want_bad = [True, True, True, False, False] + [False] * (pairs - 5)
+        assert (e["status"] == s.CAPACITY).tolist() == want_bad and (e["status"] != 0).tolist() == want_bad
+        bad = torch.tensor(want_bad)
+        assert loss.cpu()[bad].isnan().all() and logprob.cpu().view(-1, 2)[bad].isnan().all()
+        near(logprob[6:], per_sequence(lp), tol, "logprob")
+        assert (grad[:3] == 5.0).all() and (grad[-2:] == 5.0).all()
+        assert torch.isfinite(grad[3:rows - 2]).all() and (grad[3:rows - 2] != 5.0).all()
+
+
 # ---- how calls are made ----
 
 def all_calls(sc, x, token, g, stream=None):
