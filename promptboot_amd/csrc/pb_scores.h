@@ -37,20 +37,20 @@ struct RowCoef {
   uint32_t state;
   uint32_t token;
   float patch;
-  double inv;     // 1 / sum 2^(x c - shift) over the whole row
+  double inv;     // q = inv 2^(x c - shift)
   double norm;    // the teacher's log-sum-exp
   double mass;    // the teacher's mass, its rest bucket included
   double weight;  // weight / T
 };
 // The same room between the preference loss' statistics and its pairs' pass: a
-// row's sums, what is wrong with it (bad as in RowPart) and ln q[token].  A row
+// row's log-sum, what is wrong with it (bad as in RowPart) and ln q[token].  A row
 // that no pair takes stays untouched.
 struct PairRow {
   float shift;
   uint32_t bad;
-  uint32_t unused;
-  uint32_t state;  // kRowUntouched, where RowCoef has it
-  double sum;
+  uint32_t failed;
+  uint32_t state;   // kRowUntouched, where RowCoef has it
+  double log2_own;  // log2 sum 2^(x c - shift)
   double logprob;
 };
 static_assert(offsetof(PairRow, state) == offsetof(RowCoef, state), "a row's state has one place");

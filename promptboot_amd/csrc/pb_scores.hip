@@ -213,6 +213,24 @@ __device__ __forceinline__ void add_chunk(Acc& s, const float (&x)[E::kPer], flo
   if (kEntropy) s.moment = s.moment + m;
 }
 
+// 32-bit rows move a thread's shift up where a chunk passes it by more than 8: a
+// then keeps 20 bits behind the point for whatever weighs.  A larger step is left to
+// the second scan, and a sum that has failed stays failed (inf 0 is NaN).  16-bit
+// rows keep the first shift: their chunks hold twice the elements to compare for the
+// same bytes.
+template <typename E, bool kEntropy>
+__device__ __forceinline__ void follow(Acc& s, const float (&x)[E::kPer], float c) {
+  if constexpr (E::kPer == 4) {
+    const float u = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * c, rise = u - s.shift;
+    if (__builtin_expect(rise > 8.0f && rise < 0x1p60f, 0)) {
+      const float f = exp2_hw(-rise);
+      if (kEntropy) s.moment = f * fmaf(-rise, s.sum, s.moment);
+      s.sum = f * s.sum;
+      s.shift = u;
+    }
+  }
+}
+
 template <typename E, bool kTail>
 __device__ __forceinline__ void unpack(const uint4& v, uint32_t marks, float (&x)[E::kPer]) {
 #pragma unroll
@@ -288,6 +306,7 @@ struct PartScan {
         const float u = m * c;
         s.shift = first_shift(u);
       }
+      follow<E, kEntropy>(s, x, c);
       add_chunk<E, kEntropy>(s, x, c);
     });
     *bad = kNone;
@@ -402,22 +421,37 @@ __device__ __forceinline__ void no_error(pb_inference_error* at) {
 
 __device__ __forceinline__ float nan32() { return f_of(0x7fc00000u); }
 
-// Gradient slope (delta - q) of a row with one token; shift and sum its sums,
-// lp = ln q[token].
-__device__ __forceinline__ RowCoef token_coef(float shift, double sum, double slope, double lp,
-                                              uint32_t token) {
+// A gradient's shift is the row's log-sum, to the nearest binary32: the elements
+// that weigh then have small a, where a's own rounding is small too.  (About the
+// sums' shift, 40 below an outlier, gradients of 32-bit logits were off by 1e-6.)
+// What that rounding leaves out goes into the factors.  log2_own: log2 of the sum
+// about `shift`; the two stay apart, since together they lose it under large logits.
+struct GradShift {
+  float at;
+  double factor;  // q = factor 2^(u - at)
+};
+__device__ __forceinline__ GradShift grad_shift(double shift, double log2_own) {
+  const float at = (float)(shift + log2_own);
+  return {at, exp2(((double)at - shift) - log2_own)};
+}
+
+// Gradient slope (delta - q) of a row with one token; rise = q[token] - 1.
+__device__ __forceinline__ RowCoef token_coef(double shift, double log2_own, double slope,
+                                              double rise, uint32_t token) {
   RowCoef r{};
   r.state = slope == 0.0 ? kRowZero : slope == slope ? kRowNormal : kRowNan;
-  r.shift = shift;
-  r.alpha = (float)(-slope / sum);
+  const GradShift g = grad_shift(shift, log2_own);
+  r.shift = g.at;
+  r.alpha = (float)(-slope * g.factor);
   r.token = token;
-  r.patch = (float)(slope * -expm1(lp));
+  r.patch = (float)(slope * -rise);
   return r;
 }
 
 // ln q[token] in 64 bits; x the token's logit.
-__device__ __forceinline__ double token_logprob(const ScoreParams& p, float x, const RowSum& r) {
-  return kLn2 * (((double)x * (double)p.c - r.shift) - log2(r.sum));
+__device__ __forceinline__ double token_logprob(const ScoreParams& p, float x, double shift,
+                                                double log2_own) {
+  return kLn2 * (((double)x * (double)p.c - shift) - log2_own);
 }
 
 // Whether a row that was read has failed, and the record of it.
@@ -482,7 +516,8 @@ __device__ __forceinline__ PolicyRow policy_row(const ScoreParams& p, uint32_t r
     return o;
   }
   if (lane_id() == 0) no_error(at);
-  const double lp = token_logprob(p, t.x, r), gap = (double)t.ref_logprob - lp;
+  const double log2_own = log2(r.sum);
+  const double lp = token_logprob(p, t.x, r.shift, log2_own), gap = (double)t.ref_logprob - lp;
   const uint32_t lane = lane_id();
   const double rise = expm1(lane == 0 ? lp - (double)t.old_logprob : lane == 1 ? gap : lp);
   const double ratio = 1.0 + bcast_f64(rise, 0), away = bcast_f64(rise, 1);
@@ -502,11 +537,7 @@ __device__ __forceinline__ PolicyRow policy_row(const ScoreParams& p, uint32_t r
     }
   }
   slope = slope * (double)t.weight * p.inv_t;
-  o.coef.state = slope == 0.0 ? kRowZero : slope == slope ? kRowNormal : kRowNan;
-  o.coef.shift = (float)r.shift;
-  o.coef.alpha = (float)(-slope / r.sum);
-  o.coef.token = t.token;
-  o.coef.patch = (float)(slope * -bcast_f64(rise, 2));
+  o.coef = token_coef(r.shift, log2_own, slope, bcast_f64(rise, 2), t.token);
   return o;
 }
 __device__ __forceinline__ void write_policy(const ScoreParams& p, uint32_t row,
@@ -538,7 +569,7 @@ __device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t r
     } else {
       no_error(at);
       const double log2_own = log2(r.sum);
-      logprob = (float)(kLn2 * (((double)t.x * (double)p.c - r.shift) - log2_own));
+      logprob = (float)token_logprob(p, t.x, r.shift, log2_own);
       lse = (float)(kLn2 * (r.shift + log2_own));
       entropy = (float)(kLn2 * (log2_own - r.moment / r.sum));
     }
@@ -570,11 +601,13 @@ __device__ __forceinline__ void finish_pair_row(const ScoreParams& p, uint32_t r
   if (lane_id() != 0) return;
   p.sequence[row] = sequence;
   PairRow* v = reinterpret_cast<PairRow*>(p.coef + row);
+  const bool failed = bad_row(r.bad, r.sum);
   v->state = kRowUntouched;
-  v->shift = (float)r.shift;
   v->bad = r.bad;
-  v->sum = r.sum;
-  v->logprob = bad_row(r.bad, r.sum) ? 0.0 : token_logprob(p, t.x, r);
+  v->failed = failed ? 1u : 0u;
+  v->shift = (float)r.shift;
+  v->log2_own = failed ? 0.0 : log2(r.sum);
+  v->logprob = failed ? 0.0 : token_logprob(p, t.x, r.shift, v->log2_own);
 }
 
 // A row's list, two entries a lane (i = lane, lane + 64); kNone past its end.
@@ -691,6 +724,7 @@ __device__ __forceinline__ float listed_grad(const ScoreParams& p, const RowCoef
 struct DistillRow {
   RowCoef coef;
   double shift, rest, whole;  // sums 2^(u - shift) off the list and of the row
+  double log2_own;            // log2(whole)
   double left;                // the teacher's mass in the rest bucket
   bool skipped, failed;
 };
@@ -753,6 +787,7 @@ __device__ __forceinline__ DistillRow distill_row(const ScoreParams& p, uint32_t
     if (writer) no_error(at);
   }
   if (o.failed) o.coef.state = kRowNan;
+  if (!o.failed) o.log2_own = log2(o.whole);
   if (o.failed || !s.any) return o;
   double mass = s.mass, off = mass;  // off: what q is multiplied by off the list
   if (p.teacher_lse != nullptr && mass < 1.0 && o.rest > 0.0) {
@@ -762,8 +797,9 @@ __device__ __forceinline__ DistillRow distill_row(const ScoreParams& p, uint32_t
   }
   o.coef.weight = (double)weight * p.inv_t;
   o.coef.state = weight == weight ? kRowNormal : kRowNan;
-  o.coef.inv = 1.0 / o.whole;
-  o.coef.shift = (float)o.shift;
+  const GradShift g = grad_shift(o.shift, o.log2_own);
+  o.coef.shift = g.at;
+  o.coef.inv = g.factor;
   o.coef.alpha = (float)(o.coef.weight * off * o.coef.inv);
   o.coef.norm = s.norm;
   o.coef.mass = mass;
@@ -777,7 +813,7 @@ __device__ __forceinline__ void write_distill(const ScoreParams& p, uint32_t row
   if (o.failed) {
     loss = lse = (double)nan32();
   } else if (!o.skipped) {
-    const double log2_sum = o.shift + log2(o.whole);
+    const double log2_sum = o.shift + o.log2_own;
     lse = kLn2 * log2_sum;
     if (s.any) {
       double pu = 0.0;
@@ -981,7 +1017,7 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
     // every row has to be this pair's before any coefficient is written
     stray |= p.sequence[row] ^ (2u * pair + (row < b ? 0u : 1u));
     if (w == 0.0f || token == PB_NO_TOKEN) continue;
-    if (token >= p.vocab || bad_row(v.bad, v.sum))
+    if (token >= p.vocab || v.failed)
       failed = row < failed ? row : failed;
     else
       mine[row < b ? 0 : 1] += v.logprob;
@@ -1047,7 +1083,7 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
       coef.state = kRowNan;
     } else if (token != PB_NO_TOKEN && w != 0.0f) {
       const PairRow v = pair_row(p, row);
-      coef = token_coef(v.shift, v.sum, row < b ? slope : -slope, v.logprob, token);
+      coef = token_coef(v.shift, v.log2_own, row < b ? slope : -slope, expm1(v.logprob), token);
     }
     p.coef[row] = coef;
   }
@@ -1080,9 +1116,8 @@ __device__ __forceinline__ void fill_row(typename E::Raw* out, uint32_t lo, uint
 }
 
 // token_logprobs_grad: what the gradient needs, from the forward pass' outputs:
-// g (delta - q) - ge q (ln q + H), about the log-sum's nearest binary32; what that
-// rounding leaves out (d, at most 2^-18) goes into the factors.  `patch` is left to
-// the thread that holds the token.
+// g (delta - q) - ge q (ln q + H), about the log-sum's nearest binary32 as above (d
+// is what that leaves out).  `patch` is left to the thread that holds the token.
 struct TokenGrad {
   double log2_sum, g, ge, entropy;
 };
@@ -1296,6 +1331,7 @@ struct FusedRow {
         unpack<E, false>(v[n], 0, x);
         if (kTail && (special >> n & 1u)) take_out(x, i);
         if (n == 0) start(s, x);
+        follow<E, false>(s, x, c);
         add_chunk<E, false>(s, x, c);
       }
     }
@@ -1306,6 +1342,7 @@ struct FusedRow {
         },
         [&](const float (&y)[E::kPer], uint32_t i) {
           if (i < kThreads) start(s, y);
+          follow<E, false>(s, y, c);
           add_chunk<E, false>(s, y, c);
         });
     *bad = kNone;
@@ -1553,6 +1590,7 @@ __device__ __forceinline__ Acc scan_tiles(const ScoreParams& p, const typename E
       first = false;
       s.shift = first_shift(m * p.c);
     }
+    follow<E, false>(s, x, p.c);
     add_chunk<E, false>(s, x, p.c);
     const uint32_t word = tile_word<E>(m);
     // the lanes of a tile write the same word

@@ -491,6 +491,75 @@ def test_failed_pairs_have_records(scorer):
     assert grad[:12].isnan().all() and (grad[12:] == 5.0).all()
 
 
+@pytest.mark.parametrize("vocab", [2000, 2003])
+@pytest.mark.parametrize("operator", ["policy", "distill", "preference"])
+def test_outliers_cost_no_precision(scorer, operator, vocab):
+    """Two outliers far above everything a thread has met before them hold a 32-bit row's mass.
+
+    The factor of 2^(x c - shift) that each sum and gradient rounds to is near 1 for them if the shift follows:
+    an element's gradient is then off, relatively, by 2 (2^-23 + 4 2^-24) from the sums (in q and in the slope),
+    2^-23 from its own exponential, 5 2^-24 from the products, the gradient's rounding and a, and 2^-25 of what
+    separates the two.  About a shift that stays 49 below, a alone may be off by 2^-19 / 2 ln 2 in each of the two."""
+    rows, T = 400, 0.7
+    x, g = make_logits(rows, vocab, "f32", seed=vocab)
+    x.clamp_(max=10.0)
+    each = torch.arange(rows, device=DEV)
+    one, two = 1100 + each % 300, 1500 + each % 350
+    x[each, one] = 26.0 + torch.rand(rows, generator=g, device=DEV)
+    x[each, two] = x[each, one] - 0.5 * torch.rand(rows, generator=g, device=DEV)
+    token, grad, loss = two, out(rows, vocab), out(rows)
+    q = torch.softmax(x.double() / T, 1)
+    lp = torch.log(q[each, token])
+    if operator == "policy":
+        old, adv = lp.float() + 0.05, torch.ones(rows, device=DEV)
+        scorer.policy_loss(x, token.int(), old, adv, loss=loss, grad=grad, temperature=T, clip_low=0.2, clip_high=0.2)
+        slope = -torch.exp(lp - old.double()) / T
+    elif operator == "distill":
+        scorer.distill_loss(x, token.int()[:, None], torch.zeros((rows, 1), device=DEV), loss=loss, grad=grad,
+                            temperature=T)
+        slope = torch.full_like(lp, -1.0 / T)
+    else:
+        start = torch.arange(rows + 1, dtype=torch.int32, device=DEV)
+        scorer.preference_loss(x, token.int(), start, beta=0.1, loss=out(rows // 2), grad=grad, temperature=T)
+        h = 0.1 * (lp[0::2] - lp[1::2])
+        slope = torch.stack([-torch.sigmoid(-h), torch.sigmoid(-h)], 1).flatten() * 0.1 / T
+    want = -slope * q[each, one]
+    tol = (2 * 6 * 2.0 ** -24 + 2 * 2.0 ** -24 + 5 * 2.0 ** -24 + 2 * 2.0 ** -25) * want.abs()
+    near(grad[each, one], want, tol, "gradient")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("rise", [12.0, 60.0, 400.0, 30_000.0])
+def test_bad_logits_fail_under_later_larger_ones(scorer, dtype, bad, rise):
+    """A thread that has met a NaN or an infinity reports it whatever its later chunks hold."""
+    vocab, rows, at = 20_011, 70, 9
+    x, g = make_logits(rows, vocab, dtype, seed=3)
+    token = ids_of(x, g).int()
+    x[1, at] = bad
+    x[:, at + 1024::1024] = rise
+    x[:, at + 5::2048] = rise + 1.0
+    lp, ent, loss, grad, err = out(rows), out(rows), out(rows), torch.zeros_like(x), records(rows)
+    ids, value = out(rows, 5, dtype=torch.int32, fill=0), out(rows, 5)
+
+    def check():
+        e = read_errors(err)
+        assert e["status"][1] == s.NONFINITE_OUTPUT and int(e["detail"][1]) & 0xFFFFFFFF == at
+        assert (e["status"] != 0).sum() == 1
+
+    scorer.token_logprobs(x, token, logprob=lp, entropy=ent, err=err)
+    check()
+    scorer.top_logits(x, 5, token=ids, value=value, err=err)
+    check()
+    for n in (2, rows):
+        few = records(n)
+        scorer.policy_loss(x[:n], token[:n], torch.zeros_like(loss[:n]), torch.ones_like(loss[:n]), loss=loss[:n],
+                           grad=grad[:n], err=few)
+        assert read_errors(few)["status"][1] == s.NONFINITE_OUTPUT and grad[1].isnan().all()
+    good = torch.arange(rows, device=DEV) != 1
+    assert lp[1].isnan() and torch.isfinite(lp[good]).all() and torch.isfinite(ent[good]).all()
+
+
 @pytest.mark.parametrize("more", [0, 40, 5000])
 def test_pairs_that_share_rows_fail(scorer, more):
     """Offsets that fall back would give rows to two pairs: they are the last sequence's alone."""
