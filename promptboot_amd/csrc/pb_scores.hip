@@ -213,17 +213,35 @@ __device__ __forceinline__ void add_chunk(Acc& s, const float (&x)[E::kPer], flo
   if (kEntropy) s.moment = s.moment + m;
 }
 
-// 32-bit rows move a thread's shift up where a chunk passes it by more than 8: a
-// then keeps 20 bits behind the point for whatever weighs.  A larger step is left to
-// the second scan, and a sum that has failed stays failed (inf 0 is NaN).  16-bit
-// rows keep the first shift: their chunks hold twice the elements to compare for the
-// same bytes.
-template <typename E, bool kEntropy>
-__device__ __forceinline__ void follow(Acc& s, const float (&x)[E::kPer], float c) {
-  if constexpr (E::kPer == 4) {
-    const float u = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * c, rise = u - s.shift;
-    if (__builtin_expect(rise > 8.0f && rise < 0x1p60f, 0)) {
-      const float f = exp2_hw(-rise);
+// The largest of three without the compiler's quieting of signalling NaNs (a row
+// that holds a NaN fails by its sum).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <typename E>
+__device__ __forceinline__ float chunk_max(const float (&x)[E::kPer]) {
+  float m = max3(x[0], x[1], x[2]);
+  if constexpr (E::kPer == 8) {
+    m = max3(m, x[3], x[4]);
+    return max3(m, x[5], max3(x[6], x[7], x[7]));
+  } else {
+    return max3(m, x[3], x[3]);
+  }
+}
+// 32-bit rows move a thread's shift up where a chunk's largest value m passes it by
+// more than 16: a then keeps 19 bits behind the point for whatever weighs.  (By steps
+// of more than 8, which ordinary rows take too, 240 rows' statistics took 19.9 us, so
+// 16.7, and 16.4 without any.)  A step past 2^60 is left to the second scan, and a sum
+// that has failed stays failed (inf 0 is NaN).  16-bit rows keep the first shift: they
+// have twice the elements to compare for the same bytes.
+template <bool kEntropy>
+__device__ __forceinline__ void follow(Acc& s, float m, float c) {
+  const float over = fmaf(m, c, -s.shift);
+  if (__builtin_expect(over > 16.0f, 0)) {
+    if (over < 0x1p60f) {
+      const float u = m * c, rise = u - s.shift, f = exp2_hw(-rise);
       if (kEntropy) s.moment = f * fmaf(-rise, s.sum, s.moment);
       s.sum = f * s.sum;
       s.shift = u;
@@ -300,13 +318,10 @@ struct PartScan {
     each([&](const float (&x)[E::kPer], uint32_t) {
       if (first) {
         first = false;
-        float m = x[0];
-#pragma unroll
-        for (int e = 1; e < E::kPer; ++e) m = fmaxf(m, x[e]);
-        const float u = m * c;
-        s.shift = first_shift(u);
+        s.shift = first_shift(chunk_max<E>(x) * c);
+      } else if (E::kPer == 4) {
+        follow<kEntropy>(s, chunk_max<E>(x), c);
       }
-      follow<E, kEntropy>(s, x, c);
       add_chunk<E, kEntropy>(s, x, c);
     });
     *bad = kNone;
@@ -581,8 +596,9 @@ __device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t r
 
 // The last sequence that starts at or before a row, by one wave: one look at every
 // 64th part of what is left.  Where offsets decrease, sequences may share rows; the
-// row then still has one owner, and the pairs that find another's fail.
-__device__ __forceinline__ uint32_t sequence_of(const ScoreParams& p, uint32_t row) {
+// row then still has one owner, and the pairs that find another's fail.  The second
+// wave of a row's first part does it beside the first's scalars.
+__device__ __forceinline__ void note_sequence(const ScoreParams& p, uint32_t row) {
   uint32_t at = 0, n = 2u * p.pairs + 1u;
   while (n > 1u) {
     const uint32_t step = (n + 63u) / 64u, i = lane_id() * step;
@@ -591,15 +607,13 @@ __device__ __forceinline__ uint32_t sequence_of(const ScoreParams& p, uint32_t r
     at += k * step;
     n = n - k * step < step ? n - k * step : step;
   }
-  return at;
+  if (lane_id() == 0) p.sequence[row] = at;
 }
 
 // The preference loss' rows, for the pairs' pass.
 __device__ __forceinline__ void finish_pair_row(const ScoreParams& p, uint32_t row,
                                                 const RowSum& r, const TokenRow& t) {
-  const uint32_t sequence = sequence_of(p, row);
   if (lane_id() != 0) return;
-  p.sequence[row] = sequence;
   PairRow* v = reinterpret_cast<PairRow*>(p.coef + row);
   const bool failed = bad_row(r.bad, r.sum);
   v->state = kRowUntouched;
@@ -949,7 +963,10 @@ __global__ __launch_bounds__(kStatsThreads + (kList ? 64 : 0)) void stats_kernel
   __shared__ ListShared list;
   extern __shared__ uint32_t marks[];
   const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
+  const bool notes =
+      !kList && p.mode == kModePreference && split == 0 && threadIdx.x / 64u == 1u;
   if (row_unread(p, row)) {
+    if (notes) note_sequence(p, row);
     if (split != 0 || threadIdx.x >= 64) return;
     const RowSum none{0.0, 0.0, 0.0, kNone};
     if (kList)
@@ -971,6 +988,7 @@ __global__ __launch_bounds__(kStatsThreads + (kList ? 64 : 0)) void stats_kernel
     prepare_list<E>(p, row, list);
   }
   RowSum r = block_sum<kStatsThreads, kEntropy>(s, bad, l);
+  if (notes) note_sequence(p, row);
   if (threadIdx.x >= 64) return;
   if (p.splits > 1) {
     if (lane_id() == 0) publish_part(p.part + (size_t)row * p.splits + split, r);
@@ -1331,7 +1349,7 @@ struct FusedRow {
         unpack<E, false>(v[n], 0, x);
         if (kTail && (special >> n & 1u)) take_out(x, i);
         if (n == 0) start(s, x);
-        follow<E, false>(s, x, c);
+        if (E::kPer == 4) follow<false>(s, chunk_max<E>(x), c);
         add_chunk<E, false>(s, x, c);
       }
     }
@@ -1342,7 +1360,7 @@ struct FusedRow {
         },
         [&](const float (&y)[E::kPer], uint32_t i) {
           if (i < kThreads) start(s, y);
-          follow<E, false>(s, y, c);
+          if (E::kPer == 4) follow<false>(s, chunk_max<E>(y), c);
           add_chunk<E, false>(s, y, c);
         });
     *bad = kNone;
@@ -1542,23 +1560,6 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return f_of((ord & 0x80000000u) ? (ord & 0x7fffffffu) : ~ord);
 }
 
-// The largest of three without the compiler's quieting of signalling NaNs (a row
-// that holds a NaN fails by its sum).
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-template <typename E>
-__device__ __forceinline__ float chunk_max(const float (&x)[E::kPer]) {
-  float m = max3(x[0], x[1], x[2]);
-  if constexpr (E::kPer == 8) {
-    m = max3(m, x[3], x[4]);
-    return max3(m, x[5], max3(x[6], x[7], x[7]));
-  } else {
-    return max3(m, x[3], x[3]);
-  }
-}
 // A chunk's largest value as an order word (-0 as 0), over the lanes that share
 // its 64 elements: the four of a quad, mirrored halves of 8 and, for 32-bit rows,
 // mirrored 16.
@@ -1590,7 +1591,7 @@ __device__ __forceinline__ Acc scan_tiles(const ScoreParams& p, const typename E
       first = false;
       s.shift = first_shift(m * p.c);
     }
-    follow<E, false>(s, x, p.c);
+    if (E::kPer == 4) follow<false>(s, m, p.c);
     add_chunk<E, false>(s, x, p.c);
     const uint32_t word = tile_word<E>(m);
     // the lanes of a tile write the same word
