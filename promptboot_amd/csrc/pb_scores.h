@@ -37,10 +37,11 @@ struct RowCoef {
   uint32_t state;
   uint32_t token;
   float patch;
-  double inv;     // q = inv 2^(x c - shift)
-  double norm;    // the teacher's log-sum-exp
-  double mass;    // the teacher's mass, its rest bucket included
-  double weight;  // weight / T
+  float own_shift;  // of a listed id's q; off the list `shift` is the rest's
+  double inv;       // q = inv 2^(x c - own_shift)
+  double norm;      // the teacher's log-sum-exp
+  double mass;      // the teacher's mass, its rest bucket included
+  double weight;    // weight / T
 };
 // The same room between the preference loss' statistics and its pairs' pass: a
 // row's log-sum, what is wrong with it (bad as in RowPart) and ln q[token].  A row

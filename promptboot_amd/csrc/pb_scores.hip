@@ -729,17 +729,19 @@ __device__ __forceinline__ ListSum sum_teacher(const ScoreParams& p, const ListL
 // A listed id's gradient; pr: its p.
 __device__ __forceinline__ float listed_grad(const ScoreParams& p, const RowCoef& r, float x,
                                              double pr) {
-  const double q = exp2((double)x * (double)p.c - (double)r.shift) * r.inv;
+  const double q = exp2((double)x * (double)p.c - (double)r.own_shift) * r.inv;
   return (float)(r.weight * (r.mass * q - pr));
 }
 
 // One wave: the row's sums joined with those of its listed ids (x, the lane's
-// logits of them), and what its gradient needs.
+// logits of them), and what its gradient needs.  The student's mass off the list,
+// qr, is kept by its log2: finite logits may lie thousands below the listed ones, and
+// what off-list elements get, q (mass - left / qr), adds up to about -left all the same.
 struct DistillRow {
   RowCoef coef;
-  double shift, rest, whole;  // sums 2^(u - shift) off the list and of the row
-  double log2_own;            // log2(whole)
-  double left;                // the teacher's mass in the rest bucket
+  double shift, log2_own;  // the row's log2 sum 2^u is their sum
+  double log2_rest;        // log2 qr
+  double left;             // the teacher's mass in the rest bucket
   bool skipped, failed;
 };
 template <typename E>
@@ -757,7 +759,7 @@ __device__ __forceinline__ DistillRow distill_row(const ScoreParams& p, uint32_t
   }
   uint32_t bad = r.bad;
   o.shift = r.shift;
-  o.rest = o.whole = r.sum;
+  double whole = r.sum;  // sum 2^(u - o.shift) of the row
   if (p.teacher_lse != nullptr) {
     // the listed ids were left out of the row's sums: their logits are looked at here
     float top = -__builtin_inff();
@@ -779,8 +781,7 @@ __device__ __forceinline__ DistillRow distill_row(const ScoreParams& p, uint32_t
         if (h == 1 && p.k <= 64) break;
         if (id[h] < p.vocab) listed += exp2((double)x[h] * (double)p.c - o.shift);
       }
-      o.rest = r.sum > 0.0 ? r.sum * exp2(r.shift - o.shift) : 0.0;
-      o.whole = o.rest + wave_sum_f64(listed);
+      whole = (r.sum > 0.0 ? r.sum * exp2(r.shift - o.shift) : 0.0) + wave_sum_f64(listed);
     }
   }
   o.failed = true;
@@ -794,27 +795,38 @@ __device__ __forceinline__ DistillRow distill_row(const ScoreParams& p, uint32_t
                   b_of(s.bad_logit == p.k ? p.teacher_lse[row]
                                           : p.teacher_logit[(size_t)row * p.k + s.bad_logit]),
                   PB_FIELD_FINITE, s.bad_logit);
-  } else if (bad_row(bad, o.whole)) {
+  } else if (bad_row(bad, whole)) {
     if (writer) report_row<E>(p, row, bad, at);
   } else {
     o.failed = false;
     if (writer) no_error(at);
   }
   if (o.failed) o.coef.state = kRowNan;
-  if (!o.failed) o.log2_own = log2(o.whole);
+  if (!o.failed) o.log2_own = log2(whole);
   if (o.failed || !s.any) return o;
-  double mass = s.mass, off = mass;  // off: what q is multiplied by off the list
-  if (p.teacher_lse != nullptr && mass < 1.0 && o.rest > 0.0) {
-    o.left = 1.0 - mass;
-    mass += o.left;
-    off = mass - o.left * (o.whole / o.rest);
-  }
+  double mass = s.mass;
   o.coef.weight = (double)weight * p.inv_t;
   o.coef.state = weight == weight ? kRowNormal : kRowNan;
-  const GradShift g = grad_shift(o.shift, o.log2_own);
-  o.coef.shift = g.at;
+  GradShift g = grad_shift(o.shift, o.log2_own);
+  o.coef.own_shift = g.at;
   o.coef.inv = g.factor;
-  o.coef.alpha = (float)(o.coef.weight * off * o.coef.inv);
+  double off = mass;  // what 2^(u - log-sum) is multiplied by off the list
+  if (p.teacher_lse != nullptr && r.sum > 0.0) {
+    // q (mass - left / qr) = (q / qr) (mass qr - left), and q / qr is taken about the
+    // rest's own log-sum: about the row's, 2^a underflows and 1 / qr leaves binary32
+    // from 87 below the listed ids on.  (A listed element may then be inf before its
+    // own gradient is stored over it.)
+    const double log2_sum = log2(r.sum);
+    o.log2_rest = (r.shift - o.shift) + (log2_sum - o.log2_own);
+    if (mass < 1.0) {
+      o.left = 1.0 - mass;
+      mass += o.left;
+    }
+    g = grad_shift(r.shift, log2_sum);
+    off = mass * exp2(o.log2_rest) - o.left;
+  }
+  o.coef.shift = g.at;
+  o.coef.alpha = (float)(o.coef.weight * off * g.factor);
   o.coef.norm = s.norm;
   o.coef.mass = mass;
   o.coef.token = kNone;
@@ -835,7 +847,7 @@ __device__ __forceinline__ void write_distill(const ScoreParams& p, uint32_t row
       for (int h = 0; h < 2; ++h)
         if (pr[h] > 0.0) pu += pr[h] * ((double)x[h] * (double)p.c);
       loss = s.plogp - kLn2 * (wave_sum_f64(pu) - s.mass * log2_sum);
-      if (o.left > 0.0) loss += o.left * log(o.left * o.whole / o.rest);
+      if (o.left > 0.0) loss += o.left * (log(o.left) - kLn2 * o.log2_rest);
     }
   }
   if (lane_id() != 0) return;
