@@ -1086,10 +1086,11 @@ __global__ __launch_bounds__(256) void pair_kernel(const ScoreParams p) {
         const double rc = p.ref_logprob ? (double)p.ref_logprob[2 * pair] : 0.0;
         const double rr = p.ref_logprob ? (double)p.ref_logprob[2 * pair + 1] : 0.0;
         const double h = p.beta * ((l[0] - rc) - (l[1] - rr));
-        // -ln sigma(h) = max(-h, 0) + ln(1 + e^-|h|)
+        // -ln sigma(h) = max(-h, 0) + ln(1 + e^-|h|); a token without weight makes h
+        // infinite, and a term whose factor is 0 then counts 0
         const double soft = log1p(exp(-fabs(h)));
-        loss = (1.0 - p.smoothing) * ((h < 0.0 ? -h : 0.0) + soft) +
-               p.smoothing * ((h > 0.0 ? h : 0.0) + soft);
+        if (p.smoothing < 1.0) loss += (1.0 - p.smoothing) * ((h < 0.0 ? -h : 0.0) + soft);
+        if (p.smoothing > 0.0) loss += p.smoothing * ((h > 0.0 ? h : 0.0) + soft);
         if (h != h) loss = h;
         const double up = 1.0 / (1.0 + exp(-h)), down = 1.0 / (1.0 + exp(h));
         slope = (p.smoothing * up - (1.0 - p.smoothing) * down) * p.beta * (double)w * p.inv_t;

@@ -82,3 +82,30 @@ def test_a_rest_of_little_mass_keeps_its_gradient(scorer, rows, vocab, dtype, T,
     # an exponential below 2^-126 (1.2e-38) counts 0, times a factor of at most 1.3 w / T
     lost = 2e-38 * (1.0 + w.double() / T)[:, None]
     near(grad, want_grad, half * want_grad.abs() + bound * (1 + half) + float(info.tiny) * info.eps + lost, "grad")
+
+
+@pytest.mark.parametrize("smooth", [0.0, 0.1, 1.0])
+@pytest.mark.parametrize("masked", ["chosen", "rejected"])
+def test_a_token_without_weight_in_a_pair(scorer, masked, smooth):
+    """A -inf logit at a token makes the margin infinite: sigma of it is 1 or 0, and a term of factor 0 counts 0."""
+    vocab, beta, T = 300, 0.2, 0.7
+    x, g = make_logits(8, vocab, "f32", seed=5)
+    token = torch.randint(0, vocab, (8,), generator=g, device=DEV)
+    row = 1 if masked == "chosen" else 3
+    x[row, token[row]] = -math.inf
+    start = torch.tensor([0, 2, 4, 6, 8], dtype=torch.int32, device=DEV)
+    loss, logprob, grad, err = out(2), out(4), out(8, vocab), records(2)
+    scorer.preference_loss(x, token.int(), start, beta=beta, label_smoothing=smooth, loss=loss, logprob=logprob,
+                           grad=grad, err=err, temperature=T)
+    assert not read_errors(err).view(np.uint8).any()
+    factor = 1.0 - smooth if masked == "chosen" else smooth  # of the term that is infinite
+    assert loss[0] == (math.inf if factor > 0.0 else 0.0) and torch.isfinite(loss[1])
+    assert logprob[row // 2] == -math.inf and torch.isfinite(logprob[[1 - row // 2, 2, 3]]).all()
+    slope = (smooth if masked == "rejected" else smooth - 1.0) * beta / T
+    q = torch.softmax(x[:4].double() / T, 1)
+    one = torch.zeros_like(q).scatter_(1, token[:4, None], 1.0)
+    side = torch.tensor([1.0, 1.0, -1.0, -1.0], dtype=torch.float64, device=DEV)[:, None]
+    want = slope * side * (one - q)
+    tol = 2.0 * ref.lse_tolerance(x[:4], T)[:, None]
+    near(grad[:4], want, ref.grad_tolerance(want, abs(slope), q, tol, x.dtype) + abs(slope) * one * q * tol, "grad")
+    assert torch.isfinite(grad[4:]).all() and (grad[4:] != 0).any()
