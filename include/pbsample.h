@@ -457,8 +457,8 @@ void pb_context_set_segments(pb_context *ctx, uint32_t segments);
  * in which nothing weighs anything, index 0; available = the logit's bits as
  * binary32).
  *
- * Sums and statistics are held in 32 bits over a few hundred terms and in 64
- * bits above that; a row's scalars are worked out in 64 bits and rounded once.
+ * Sums and statistics are held in 32 bits over at most 768 terms and in 64 bits
+ * above that; a row's scalars are worked out in 64 bits and rounded once.
  * The order of every sum depends on the sizes and the alignment alone, so
  * results repeat bit for bit.
  *

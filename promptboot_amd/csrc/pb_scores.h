@@ -117,9 +117,12 @@ struct ScoreParams {
   uint32_t* sequence;    // rows: the preference loss' sequence of each, in the tiles' place
 };
 
-// Largest part of a row of one workgroup of the statistics pass: its marks of
-// the teacher's ids (a bit each) take 32 KB of LDS.
-constexpr uint32_t kMaxSpan = 262144;
+// Terms of a sum in 32 bits: a thread takes no more logits of a row, and what the
+// threads of a row have is joined in 64 bits.
+constexpr uint32_t kMaxTerms = 768;
+// So the largest part of a row of one workgroup (256 threads) of the statistics
+// pass; its marks of the teacher's ids (a bit each) take 24 KB of LDS.
+constexpr uint32_t kMaxSpan = 256 * kMaxTerms;
 // Top-logits tiles of one row: their words take 16 KB of LDS.
 constexpr uint32_t kMaxTiles = 4096;
 constexpr uint32_t kMaxSplits = 64;

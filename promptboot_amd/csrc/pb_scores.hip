@@ -23,9 +23,11 @@ namespace {
 
 constexpr double kLn2 = 0.693147180559945309417232121458;
 constexpr uint32_t kStatsThreads = 256;
+static_assert(kMaxSpan == kStatsThreads * kMaxTerms, "a part's threads take kMaxTerms each");
 constexpr uint32_t kStatsUnroll = 4;
 constexpr uint32_t kGradThreads = 256;
 constexpr uint32_t kTopThreads = 256;
+static_assert(kTopThreads == kStatsThreads, "both passes have the same parts");
 constexpr float kTooBig = 3.0e38f;  // |u| past this has left binary32's range
 
 // ---- element types: 16 bytes are one chunk ----
@@ -1932,9 +1934,11 @@ void plan_scores(uint32_t dtype, ScoreParams* p) {
     //   32,000 f32    8.5 / 11.5  9.2 / 9.8  10.0 / 12.9   14 / 22     48 / 51
     //   100,003 f16    15 / 10     18 / 13     20 / 20     24 / 32     87 / 95
     //   151,936 f32    21 / 9.8    21 / 15     23 / 26     54 / 61    247 / 253
-    // A long row takes one workgroup longer than many.
+    // A long row takes one workgroup longer than many, and past kMaxTerms logits a
+    // thread its sums would need more bits.
     const uint64_t row_bytes = (uint64_t)p->vocab * (dtype == PB_F32 ? 4u : 2u);
-    if (row_bytes <= kShortRow || p->rows >= kFusedRows) p->fused = threads;
+    if ((row_bytes <= kShortRow || p->rows >= kFusedRows) && p->vocab <= kMaxTerms * threads)
+      p->fused = threads;
   }
   p->tile_shift = tile_shift_of(p->vocab);
   const uint32_t tile = 1u << p->tile_shift;

@@ -109,3 +109,55 @@ def test_a_token_without_weight_in_a_pair(scorer, masked, smooth):
     tol = 2.0 * ref.lse_tolerance(x[:4], T)[:, None]
     near(grad[:4], want, ref.grad_tolerance(want, abs(slope), q, tol, x.dtype) + abs(slope) * one * q * tol, "grad")
     assert torch.isfinite(grad[4:]).all() and (grad[4:] != 0).any()
+
+
+def long_tolerance(y, per):
+    """ref.lse_tolerance for a thread's 768 terms, the most that are added in 32 bits: 768 / `per` sums of a chunk."""
+    return ref.EPS32 * (3.0 * y + 8.0 + 768 / per)
+
+
+def test_long_rows_are_not_summed_in_32_bits(scorer):
+    """The longest rows: every thread rounds the same way where all of its terms are alike."""
+    rows, vocab, low = 64, 4_194_304, 0.6785145998001099
+    x = torch.full((rows, vocab), -low, device=DEV)
+    x[:, :4096] = 0.0
+    token = torch.arange(rows, dtype=torch.int32, device=DEV) * 60_000
+    weigh = 4096.0 + (vocab - 4096) * math.exp(-low)
+    lse = math.log(weigh)
+    lp, loss, kl = out(rows), out(rows), out(rows)
+    grad = torch.full_like(x, 5.0)
+    own = x.gather(1, token.long()[:, None])[:, 0].double() - lse
+    scorer.policy_loss(x, token, own.float(), torch.ones(rows, device=DEV), loss=loss, logprob=lp, kl=kl, grad=grad)
+    tol = long_tolerance(low, 4)
+    near(lp, own, ref.scalar_tolerance(own, torch.full((rows,), 2 * tol, device=DEV)), "logprob")
+    # 1 / T times the ratio, which is 1 up to the rounding of the old log-probability and the error of the new
+    ratio = torch.exp(own - own.float().double())
+    want = (ratio / weigh * math.exp(-low))[:, None]
+    grad.scatter_(1, token.long()[:, None], want.float())
+    near(grad[:, 4096:].amin(1, keepdim=True), want, want * (4 * tol + 8 * ref.EPS32), "least gradient")
+    near(grad[:, 4096:].amax(1, keepdim=True), want, want * (4 * tol + 8 * ref.EPS32), "largest gradient")
+    few = torch.full((rows, 1), 7.0, device=DEV)
+    scorer.distill_loss(x, token[:, None], few, loss=loss, lse=lp, grad=grad)
+    want_lse = torch.full((rows,), lse, dtype=torch.float64, device=DEV)
+    near(lp, want_lse, ref.scalar_tolerance(want_lse, torch.full((rows,), tol, device=DEV)), "lse")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(66, 393_216), (66, 393_219), (300, 393_217), (64, 786_433), (3, 1_048_579)])
+def test_rows_around_the_longest_of_one_workgroup(scorer, rows, vocab, dtype):
+    k, T, per = 40, 0.7, 4 if dtype == "f32" else 8
+    x, g = make_logits(rows, vocab, dtype, seed=vocab, pad=1)
+    ids = torch.linspace(0, vocab - 1, k, device=DEV).long().repeat(rows, 1)
+    logit = torch.randn((rows, k), generator=g, device=DEV)
+    lse = (torch.logsumexp(logit.double() / T, 1) + 0.2).float()
+    w = torch.rand(rows, generator=g, device=DEV) + 0.5
+    loss, grad = out(rows), torch.full_like(x, 5.0)
+    scorer.distill_loss(x, ids.int(), logit, teacher_lse=lse, weight=w, loss=loss, grad=grad, temperature=T)
+    half = torch.finfo(x.dtype).eps / 2
+    for lo in range(0, rows, 32):
+        r = slice(lo, lo + 32)
+        want, want_grad, bound, _ = distill_rest(x[r], ids[r], logit[r], T, lse[r], w[r])
+        tol = long_tolerance(x[r].double().abs().amax(1) / T, per)
+        near(loss[r], want, ref.scalar_tolerance(want, 2 * tol), "loss")
+        bound = bound / (2.0 * ref.EPS32 * (3.0 * x[r].double().abs().amax(1) / T + 104.0))[:, None] * 2.0 * tol[:, None]
+        near(grad[r], want_grad, half * want_grad.abs() + bound * (1 + half) + 1e-36, "grad")
