@@ -194,6 +194,41 @@ __device__ __forceinline__ uint32_t chunk_marks(const uint32_t* marks, uint32_t 
   return (marks[at >> 5] >> (at & 31u)) & ((1u << E::kPer) - 1u);
 }
 
+// The largest of three without the compiler's quieting of signalling NaNs (a row
+// that holds a NaN fails by its sum).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <typename E>
+__device__ __forceinline__ float chunk_max(const float (&x)[E::kPer]) {
+  float m = max3(x[0], x[1], x[2]);
+  if constexpr (E::kPer == 8) {
+    m = max3(m, x[3], x[4]);
+    return max3(m, x[5], max3(x[6], x[7], x[7]));
+  } else {
+    return max3(m, x[3], x[3]);
+  }
+}
+// A thread's shift moves up where a chunk's largest value m passes it by more than 16:
+// a then keeps 19 bits behind the point for whatever weighs.  (By steps of more than 8,
+// which ordinary rows take too, 240 rows' 32-bit statistics took 19.9 us, so 16.7, and
+// 16.4 without any.)  A step past 2^60 is left to the second scan, and a sum that has
+// failed stays failed (inf 0 is NaN).
+template <bool kEntropy>
+__device__ __forceinline__ void follow(Acc& s, float m, float c) {
+  const float over = fmaf(m, c, -s.shift);
+  if (__builtin_expect(over > 16.0f, 0)) {
+    if (over < 0x1p60f) {
+      const float u = m * c, rise = u - s.shift, f = exp2_hw(-rise);
+      if (kEntropy) s.moment = f * fmaf(-rise, s.sum, s.moment);
+      s.sum = f * s.sum;
+      s.shift = u;
+    }
+  }
+}
+
 template <typename E, bool kEntropy>
 __device__ __forceinline__ void add_chunk(Acc& s, const float (&x)[E::kPer], float c) {
   float e[E::kPer], m = 0.0f;
@@ -214,41 +249,35 @@ __device__ __forceinline__ void add_chunk(Acc& s, const float (&x)[E::kPer], flo
   s.sum = s.sum + sum;
   if (kEntropy) s.moment = s.moment + m;
 }
-
-// The largest of three without the compiler's quieting of signalling NaNs (a row
-// that holds a NaN fails by its sum).
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-template <typename E>
-__device__ __forceinline__ float chunk_max(const float (&x)[E::kPer]) {
-  float m = max3(x[0], x[1], x[2]);
-  if constexpr (E::kPer == 8) {
-    m = max3(m, x[3], x[4]);
-    return max3(m, x[5], max3(x[6], x[7], x[7]));
-  } else {
-    return max3(m, x[3], x[3]);
+// The same for kCount chunks that are at hand, take(q, x) giving chunk q: where one of
+// their logits passes the shift by more than 16 their own sum shows it, and they are
+// summed again about the shift that follows.
+template <typename E, bool kEntropy, uint32_t kCount, typename Take>
+__device__ __forceinline__ void add_group(Acc& s, float c, Take take) {
+  float x[E::kPer];
+  Acc t{s.shift};
+#pragma unroll
+  for (uint32_t q = 0; q < kCount; ++q) {
+    take(q, x);
+    add_chunk<E, kEntropy>(t, x, c);
   }
-}
-// 32-bit rows move a thread's shift up where a chunk's largest value m passes it by
-// more than 16: a then keeps 19 bits behind the point for whatever weighs.  (By steps
-// of more than 8, which ordinary rows take too, 240 rows' statistics took 19.9 us, so
-// 16.7, and 16.4 without any.)  A step past 2^60 is left to the second scan, and a sum
-// that has failed stays failed (inf 0 is NaN).  16-bit rows keep the first shift: they
-// have twice the elements to compare for the same bytes.
-template <bool kEntropy>
-__device__ __forceinline__ void follow(Acc& s, float m, float c) {
-  const float over = fmaf(m, c, -s.shift);
-  if (__builtin_expect(over > 16.0f, 0)) {
-    if (over < 0x1p60f) {
-      const float u = m * c, rise = u - s.shift, f = exp2_hw(-rise);
-      if (kEntropy) s.moment = f * fmaf(-rise, s.sum, s.moment);
-      s.sum = f * s.sum;
-      s.shift = u;
+  if (__builtin_expect(t.sum > 0x1p16f, 0)) {
+    float m = -__builtin_inff();
+#pragma unroll
+    for (uint32_t q = 0; q < kCount; ++q) {
+      take(q, x);
+      m = fmaxf(m, chunk_max<E>(x));
+    }
+    follow<kEntropy>(s, m, c);
+    t = Acc{s.shift};
+#pragma unroll
+    for (uint32_t q = 0; q < kCount; ++q) {
+      take(q, x);
+      add_chunk<E, kEntropy>(t, x, c);
     }
   }
+  s.sum = s.sum + t.sum;
+  if (kEntropy) s.moment = s.moment + t.moment;
 }
 
 template <typename E, bool kTail>
@@ -261,11 +290,11 @@ __device__ __forceinline__ void unpack(const uint4& v, uint32_t marks, float (&x
 }
 
 // A thread's sums over its chunks of [lo, hi), chunk i of thread t being
-// element lo + (i kThreads + t) kPer.  The shift is the thread's first
-// chunk's largest u: nothing then underflows that weighs, and where a later u
-// passes it by over 100, or the first chunk is masked out, the sum shows it
-// (too large, or too small) and the thread goes over its chunks again with their
-// true maximum.  So the pass does no comparison per element.
+// element lo + (i kThreads + t) kPer.  The shift starts as the thread's first
+// chunk's largest u and follows what passes it: nothing then underflows that weighs.
+// Where the first chunk is masked out, or something in the row is out of range, the
+// sum shows it (too large, too small or none) and the thread goes over its chunks
+// again with their true maximum.
 template <typename E, uint32_t kThreads, bool kEntropy, bool kTail, bool kKeep>
 struct PartScan {
   template <typename T>
@@ -279,6 +308,14 @@ struct PartScan {
 
   template <typename Fn>
   __device__ __forceinline__ void each(Fn fn) const {
+    each(fn, [&](const uint4 (&v)[kStatsUnroll], uint32_t i) {
+#pragma unroll
+      for (uint32_t q = 0; q < kStatsUnroll; ++q) chunk(v[q], (i + q * kThreads) * E::kPer, fn);
+    });
+  }
+  // many(chunks, index of the first) where there are kStatsUnroll of them.
+  template <typename Fn, typename Many>
+  __device__ __forceinline__ void each(Fn fn, Many many) const {
     constexpr uint32_t kPer = E::kPer;
     const uint32_t whole = (hi - lo) / kPer;
     uint32_t i = threadIdx.x;
@@ -287,8 +324,7 @@ struct PartScan {
 #pragma unroll
       for (uint32_t q = 0; q < kStatsUnroll; ++q)
         v[q] = load<E>(row + lo + (size_t)(i + q * kThreads) * kPer);
-#pragma unroll
-      for (uint32_t q = 0; q < kStatsUnroll; ++q) chunk(v[q], (i + q * kThreads) * kPer, fn);
+      many(v, i);
     }
     for (; i < whole; i += kThreads)
       chunk(load<E>(row + lo + (size_t)i * kPer), i * kPer, fn);
@@ -317,15 +353,34 @@ struct PartScan {
   __device__ __forceinline__ Acc run(uint32_t* bad) const {
     Acc s;
     bool first = true;
-    each([&](const float (&x)[E::kPer], uint32_t) {
+    auto one = [&](const float (&x)[E::kPer], uint32_t) {
       if (first) {
         first = false;
         s.shift = first_shift(chunk_max<E>(x) * c);
-      } else if (E::kPer == 4) {
+      } else {
         follow<kEntropy>(s, chunk_max<E>(x), c);
       }
       add_chunk<E, kEntropy>(s, x, c);
-    });
+    };
+    if constexpr (E::kPer == 4) {
+      each(one);
+    } else {
+      // twice the elements to compare for the same bytes: by groups (1,023 of 2,563 bf16
+      // rows 74 us, 79 with a comparison a chunk, 74 without any)
+      each(one, [&](const uint4 (&v)[kStatsUnroll], uint32_t i) {
+        auto take = [&](uint32_t q, float (&x)[E::kPer]) {
+          const uint32_t at = (i + q * kThreads) * E::kPer;
+          unpack<E, kTail>(v[q], kTail ? chunk_marks<E>(marks, at) : 0u, x);
+        };
+        if (first) {
+          float x[E::kPer];
+          take(0, x);
+          first = false;
+          s.shift = first_shift(chunk_max<E>(x) * c);
+        }
+        add_group<E, kEntropy, kStatsUnroll>(s, c, take);
+      });
+    }
     *bad = kNone;
     if (first || (s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) return s;
     return again(bad);
@@ -1364,7 +1419,7 @@ struct FusedRow {
         unpack<E, false>(v[n], 0, x);
         if (kTail && (special >> n & 1u)) take_out(x, i);
         if (n == 0) start(s, x);
-        if (E::kPer == 4) follow<false>(s, chunk_max<E>(x), c);
+        follow<false>(s, chunk_max<E>(x), c);
         add_chunk<E, false>(s, x, c);
       }
     }
@@ -1375,7 +1430,7 @@ struct FusedRow {
         },
         [&](const float (&y)[E::kPer], uint32_t i) {
           if (i < kThreads) start(s, y);
-          if (E::kPer == 4) follow<false>(s, chunk_max<E>(y), c);
+          follow<false>(s, chunk_max<E>(y), c);
           add_chunk<E, false>(s, y, c);
         });
     *bad = kNone;
@@ -1606,7 +1661,7 @@ __device__ __forceinline__ Acc scan_tiles(const ScoreParams& p, const typename E
       first = false;
       s.shift = first_shift(m * p.c);
     }
-    if (E::kPer == 4) follow<false>(s, m, p.c);
+    follow<false>(s, m, p.c);
     add_chunk<E, false>(s, x, p.c);
     const uint32_t word = tile_word<E>(m);
     // the lanes of a tile write the same word

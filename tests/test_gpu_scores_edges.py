@@ -161,3 +161,51 @@ def test_rows_around_the_longest_of_one_workgroup(scorer, rows, vocab, dtype):
         near(loss[r], want, ref.scalar_tolerance(want, 2 * tol), "loss")
         bound = bound / (2.0 * ref.EPS32 * (3.0 * x[r].double().abs().amax(1) / T + 104.0))[:, None] * 2.0 * tol[:, None]
         near(grad[r], want_grad, half * want_grad.abs() + bound * (1 + half) + 1e-36, "grad")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(2, 100_003), (40, 20_011), (1_100, 9_001)])
+@pytest.mark.parametrize("gap", [15.0, 24.0, 45.0, 64.0])
+def test_saturated_rows_have_no_probability_above_one(scorer, rows, vocab, dtype, gap):
+    """One token holds all of a row's mass, `gap` above everything that its thread has met before it.
+
+    Its exponent keeps the place of 16: it is off by 2^-21, 2^a by ln 2 times that and 3 roundings of its own, and
+    nothing else is in the sum.  The moment's product e a has two roundings more, of at most 16.  (About a shift that
+    stays 64 / T ln 2 = 132 below, a alone is off by 2^-17: 5e-6 in the log-probability, 8e-5 in the entropy.)"""
+    T = 0.7
+    x, g = make_logits(rows, vocab, dtype, seed=vocab, spread=0.5)
+    x.clamp_(max=1.0)
+    token = vocab - 1 - torch.randint(0, vocab // 5, (rows,), generator=g, device=DEV)
+    top = gap + 2.0 + torch.rand((rows, 1), generator=g, device=DEV) * 3.0
+    x.scatter_(1, token[:, None], top.to(x.dtype))
+    want = ref.logprobs(x, token, T)
+    tol = 2.0 ** -21 * math.log(2) + 3 * ref.EPS32
+    tol_entropy = tol + math.log(2) * (2.0 ** -21 + 2 * 16 * ref.EPS32)
+    lp, ent, lse, loss = out(rows), out(rows), out(rows), out(rows)
+    value, ids = out(rows, 1), out(rows, 1, dtype=torch.int32, fill=0)
+
+    def check(what):
+        near(lp, want["logprob"], ref.scalar_tolerance(want["logprob"], torch.full_like(want["lse"], tol)), what)
+
+    def check_lse(what):
+        near(lse, want["lse"], ref.scalar_tolerance(want["lse"], torch.full_like(want["lse"], tol)), what)
+
+    scorer.token_logprobs(x, token.int(), logprob=lp, lse=lse, temperature=T)
+    check("logprob"), check_lse("lse")
+    scorer.token_logprobs(x, token.int(), logprob=lp, lse=lse, entropy=ent, temperature=T)
+    check("logprob beside the entropy"), check_lse("lse beside the entropy")
+    near(ent, want["entropy"], ref.scalar_tolerance(want["entropy"], torch.full_like(want["lse"], tol_entropy)), "entropy")
+    scorer.top_logits(x, 1, token=ids, value=value, lse=lse, temperature=T)
+    check_lse("lse of the top logits")
+    zero, grad = torch.zeros(rows, device=DEV), torch.empty_like(x)
+    scorer.policy_loss(x, token.int(), zero, zero, loss=loss, logprob=lp, temperature=T)
+    check("policy")
+    scorer.policy_loss(x, token.int(), zero, zero, loss=loss, logprob=lp, grad=grad, temperature=T)
+    check("policy with its gradient")
+    one = torch.zeros((rows, 1), device=DEV)
+    for rest in (None, zero + 0.1):
+        scorer.distill_loss(x, token.int()[:, None], one, teacher_lse=rest, loss=loss, lse=lse, grad=grad, temperature=T)
+        check_lse("distillation")
+    start = torch.arange(rows + 1, dtype=torch.int32, device=DEV)
+    scorer.preference_loss(x, token.int(), start, beta=0.1, loss=loss, logprob=lp, temperature=T)
+    check("preference")
