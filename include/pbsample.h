@@ -33,8 +33,8 @@
  *     (src/model_repl.rs:928-1150): pb_decode_step, pb_lmhead_decode_step,
  *     with the host helpers pb_decode_draw and pb_decode_settle;
  *   - scores and losses of logits rows, with their gradients: pb_token_logprobs,
- *     pb_token_logprobs_grad, pb_top_logits, pb_distill_loss, pb_policy_loss,
- *     pb_preference_loss;
+ *     pb_token_logprobs_grad (and their _wide forms), pb_top_logits,
+ *     pb_distill_loss, pb_policy_loss, pb_preference_loss;
  *   - host PRNG helpers: pb_sampling_state_new, pb_next_24, pb_fill_random_24.
  */
 #ifndef PBSAMPLE_H
@@ -496,13 +496,32 @@ uint32_t pb_token_logprobs(pb_context *ctx, const void *d_logits, uint32_t dtype
  * logits, with d_lse and d_entropy as pb_token_logprobs left them for the same
  * logits, tokens and temperature.  Either of d_grad_logprob and d_grad_entropy
  * may be NULL (0); d_entropy is needed with d_grad_entropy.  A row whose token
- * is bad, or whose d_lse is NaN, gets a NaN gradient row. */
+ * is bad, or whose d_lse is NaN, gets a NaN gradient row.  d_lse comes rounded,
+ * so every q of a row is off by up to 2^-25 times the power of two above |lse|,
+ * relatively (5e-7 at 10, 6e-5 at 2,000): gradients of 32-bit logits that are to
+ * have their own precision need the two calls below. */
 uint32_t pb_token_logprobs_grad(pb_context *ctx, const void *d_logits, uint32_t dtype,
                                 size_t vocab, size_t ld, uint32_t rows, double temperature,
                                 const uint32_t *d_token, const float *d_lse,
                                 const float *d_entropy, const float *d_grad_logprob,
                                 const float *d_grad_entropy, void *d_grad, size_t grad_ld,
                                 void *stream, pb_inference_error *err);
+
+/* The same two with the log-sum-exp in two words: d_lse_low (one per row, NULL
+ * for none) is what binary32 leaves out of d_lse, so that their sum holds it to
+ * some 48 bits.  d_lse_low needs d_lse. */
+uint32_t pb_token_logprobs_wide(pb_context *ctx, const void *d_logits, uint32_t dtype,
+                                size_t vocab, size_t ld, uint32_t rows, double temperature,
+                                const uint32_t *d_token, float *d_logprob, float *d_lse,
+                                float *d_lse_low, float *d_entropy, pb_inference_error *d_err,
+                                void *stream, pb_inference_error *err);
+uint32_t pb_token_logprobs_wide_grad(pb_context *ctx, const void *d_logits, uint32_t dtype,
+                                     size_t vocab, size_t ld, uint32_t rows, double temperature,
+                                     const uint32_t *d_token, const float *d_lse,
+                                     const float *d_lse_low, const float *d_entropy,
+                                     const float *d_grad_logprob, const float *d_grad_entropy,
+                                     void *d_grad, size_t grad_ld, void *stream,
+                                     pb_inference_error *err);
 
 /* The k largest logits of each row, largest first and the lowest id first
  * among equal ones: d_token rows x k ids, d_value rows x k raw logits as

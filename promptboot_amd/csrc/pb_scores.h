@@ -70,6 +70,7 @@ struct ScoreParams {
   // outputs of a row (or pair)
   float* logprob;
   float* lse;
+  float* lse_low;  // what binary32 leaves out of lse
   float* entropy;
   float* loss;
   float* kl;
@@ -79,6 +80,7 @@ struct ScoreParams {
 
   // token_logprobs_grad
   const float* in_lse;
+  const float* in_lse_low;
   const float* in_entropy;
   const float* grad_logprob;
   const float* grad_entropy;

@@ -625,7 +625,7 @@ __device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t r
                                                 const RowSum& r, const TokenRow& t) {
   if (lane_id() != 0) return;
   pb_inference_error* at = p.err ? p.err + row : nullptr;
-  float logprob = 0.0f, lse = 0.0f, entropy = 0.0f;
+  float logprob = 0.0f, lse = 0.0f, low = 0.0f, entropy = 0.0f;
   if (t.token == PB_NO_TOKEN) {
     no_error(at);
   } else {
@@ -637,17 +637,20 @@ __device__ __forceinline__ void finish_logprobs(const ScoreParams& p, uint32_t r
       if (failed) report_row<E>(p, row, r.bad, at);
     }
     if (failed) {
-      logprob = lse = entropy = nan32();
+      logprob = lse = low = entropy = nan32();
     } else {
       no_error(at);
       const double log2_own = log2(r.sum);
       logprob = (float)token_logprob(p, t.x, r.shift, log2_own);
-      lse = (float)(kLn2 * (r.shift + log2_own));
+      const double whole = kLn2 * (r.shift + log2_own);
+      lse = (float)whole;
+      low = (float)(whole - (double)lse);
       entropy = (float)(kLn2 * (log2_own - r.moment / r.sum));
     }
   }
   p.logprob[row] = logprob;
   if (p.lse) p.lse[row] = lse;
+  if (p.lse_low) p.lse_low[row] = low;
   if (p.entropy) p.entropy[row] = entropy;
 }
 
@@ -1214,7 +1217,8 @@ __device__ __forceinline__ RowCoef token_grad(const ScoreParams& p, uint32_t row
   r.state = kRowZero;
   r.token = uniform_word(p.token + row);
   if (r.token == PB_NO_TOKEN) return r;
-  const double lse = (double)uniform_float(p.in_lse + row);
+  double lse = (double)uniform_float(p.in_lse + row);
+  if (p.in_lse_low) lse += (double)uniform_float(p.in_lse_low + row);
   o->g = p.grad_logprob ? (double)uniform_float(p.grad_logprob + row) : 0.0;
   o->ge = p.grad_entropy ? (double)uniform_float(p.grad_entropy + row) : 0.0;
   o->entropy = p.grad_entropy ? (double)uniform_float(p.in_entropy + row) : 0.0;
@@ -1226,7 +1230,8 @@ __device__ __forceinline__ RowCoef token_grad(const ScoreParams& p, uint32_t row
     r.state = kRowNormal;
     r.shift = (float)o->log2_sum;
     const double d = ((double)r.shift - o->log2_sum) * kLn2;
-    const double f = (1.0 + d) * p.inv_t;  // e^d, up to 2^-37
+    // e^d; d, half a step of the log-sum, is small unless the logits are very large
+    const double f = (fabs(d) < 0x1p-9 ? 1.0 + d * (1.0 + 0.5 * d) : exp(d)) * p.inv_t;
     r.alpha = (float)(f * ((-o->g - o->ge * o->entropy) - o->ge * d));
     r.beta = (float)(f * -o->ge * kLn2);
   }

@@ -137,22 +137,56 @@ uint32_t pb_context_reserve_scores(pb_context* ctx, uint32_t rows, size_t vocab,
   return e == hipSuccess ? PB_OK : device_error(err, e);
 }
 
-uint32_t pb_token_logprobs(pb_context* ctx, const void* d_logits, uint32_t dtype, size_t vocab,
-                           size_t ld, uint32_t rows, double temperature, const uint32_t* d_token,
-                           float* d_logprob, float* d_lse, float* d_entropy,
-                           pb_inference_error* d_err, void* stream, pb_inference_error* err) {
+uint32_t pb_token_logprobs_wide(pb_context* ctx, const void* d_logits, uint32_t dtype,
+                                size_t vocab, size_t ld, uint32_t rows, double temperature,
+                                const uint32_t* d_token, float* d_logprob, float* d_lse,
+                                float* d_lse_low, float* d_entropy, pb_inference_error* d_err,
+                                void* stream, pb_inference_error* err) {
   const Rows r{d_logits, dtype, vocab, ld, rows, temperature, nullptr, 0};
-  const uint32_t st = check_rows(r, !d_logits || !d_token || !d_logprob, err);
+  const uint32_t st =
+      check_rows(r, !d_logits || !d_token || !d_logprob || (d_lse_low && !d_lse), err);
   if (st != PB_OK || rows == 0) return st;
-  if (!words({d_token, d_logprob, d_lse, d_entropy}) || !aligned(d_err, 8))
+  if (!words({d_token, d_logprob, d_lse, d_lse_low, d_entropy}) || !aligned(d_err, 8))
     return refuse(err, PB_ALIGNMENT, 8, 0, PB_FIELD_ALIGNMENT, 1);
   ScoreParams p = params_of(r, pb::kModeLogprobs);
   p.token = d_token;
   p.logprob = d_logprob;
   p.lse = d_lse;
+  p.lse_low = d_lse_low;
   p.entropy = d_entropy;
   p.err = d_err;
   return enqueue(ctx, p, dtype, pb::launch_token_logprobs, stream, err);
+}
+
+uint32_t pb_token_logprobs(pb_context* ctx, const void* d_logits, uint32_t dtype, size_t vocab,
+                           size_t ld, uint32_t rows, double temperature, const uint32_t* d_token,
+                           float* d_logprob, float* d_lse, float* d_entropy,
+                           pb_inference_error* d_err, void* stream, pb_inference_error* err) {
+  return pb_token_logprobs_wide(ctx, d_logits, dtype, vocab, ld, rows, temperature, d_token,
+                                d_logprob, d_lse, nullptr, d_entropy, d_err, stream, err);
+}
+
+uint32_t pb_token_logprobs_wide_grad(pb_context* ctx, const void* d_logits, uint32_t dtype,
+                                     size_t vocab, size_t ld, uint32_t rows, double temperature,
+                                     const uint32_t* d_token, const float* d_lse,
+                                     const float* d_lse_low, const float* d_entropy,
+                                     const float* d_grad_logprob, const float* d_grad_entropy,
+                                     void* d_grad, size_t grad_ld, void* stream,
+                                     pb_inference_error* err) {
+  const Rows r{d_logits, dtype, vocab, ld, rows, temperature, d_grad, grad_ld};
+  const uint32_t st = check_rows(
+      r, !d_logits || !d_token || !d_lse || !d_grad || (d_grad_entropy && !d_entropy), err);
+  if (st != PB_OK || rows == 0) return st;
+  if (!words({d_token, d_lse, d_lse_low, d_entropy, d_grad_logprob, d_grad_entropy}))
+    return refuse(err, PB_ALIGNMENT, 4, 0, PB_FIELD_ALIGNMENT, 1);
+  ScoreParams p = params_of(r, pb::kModeLogprobs);
+  p.token = d_token;
+  p.in_lse = d_lse;
+  p.in_lse_low = d_lse_low;
+  p.in_entropy = d_entropy;
+  p.grad_logprob = d_grad_logprob;
+  p.grad_entropy = d_grad_entropy;
+  return enqueue(ctx, p, dtype, pb::launch_token_logprobs_grad, stream, err);
 }
 
 uint32_t pb_token_logprobs_grad(pb_context* ctx, const void* d_logits, uint32_t dtype,
@@ -161,19 +195,9 @@ uint32_t pb_token_logprobs_grad(pb_context* ctx, const void* d_logits, uint32_t 
                                 const float* d_entropy, const float* d_grad_logprob,
                                 const float* d_grad_entropy, void* d_grad, size_t grad_ld,
                                 void* stream, pb_inference_error* err) {
-  const Rows r{d_logits, dtype, vocab, ld, rows, temperature, d_grad, grad_ld};
-  const uint32_t st = check_rows(
-      r, !d_logits || !d_token || !d_lse || !d_grad || (d_grad_entropy && !d_entropy), err);
-  if (st != PB_OK || rows == 0) return st;
-  if (!words({d_token, d_lse, d_entropy, d_grad_logprob, d_grad_entropy}))
-    return refuse(err, PB_ALIGNMENT, 4, 0, PB_FIELD_ALIGNMENT, 1);
-  ScoreParams p = params_of(r, pb::kModeLogprobs);
-  p.token = d_token;
-  p.in_lse = d_lse;
-  p.in_entropy = d_entropy;
-  p.grad_logprob = d_grad_logprob;
-  p.grad_entropy = d_grad_entropy;
-  return enqueue(ctx, p, dtype, pb::launch_token_logprobs_grad, stream, err);
+  return pb_token_logprobs_wide_grad(ctx, d_logits, dtype, vocab, ld, rows, temperature, d_token,
+                                     d_lse, nullptr, d_entropy, d_grad_logprob, d_grad_entropy,
+                                     d_grad, grad_ld, stream, err);
 }
 
 uint32_t pb_top_logits(pb_context* ctx, const void* d_logits, uint32_t dtype, size_t vocab,

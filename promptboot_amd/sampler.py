@@ -152,6 +152,12 @@ EXPORTS = {
     "pb_token_logprobs_grad": (
         u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, vp, vp, vp, vp, size_t, vp,
               ctypes.POINTER(_Error)]),
+    "pb_token_logprobs_wide": (
+        u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, vp, vp, vp, vp, vp,
+              ctypes.POINTER(_Error)]),
+    "pb_token_logprobs_wide_grad": (
+        u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, vp, vp, vp, vp, vp, size_t, vp,
+              ctypes.POINTER(_Error)]),
     "pb_top_logits": (
         u32, [vp, vp, u32, size_t, size_t, u32, u32, f64, vp, vp, vp, vp, vp,
               ctypes.POINTER(_Error)]),

@@ -1,8 +1,8 @@
 """Scores and losses of logits rows, with their gradients, over libpbsample.so.
 
-`RowScorer` reaches pb_token_logprobs, pb_token_logprobs_grad, pb_top_logits,
-pb_distill_loss, pb_policy_loss and pb_preference_loss (include/pbsample.h has
-their formulas, their row errors and which rows they skip).
+`RowScorer` reaches pb_token_logprobs, pb_token_logprobs_grad (in their _wide
+forms), pb_top_logits, pb_distill_loss, pb_policy_loss and pb_preference_loss
+(include/pbsample.h has their formulas, their row errors and which rows they skip).
 
 Logits are device buffers [rows, columns] of binary32, binary16 or bfloat16:
 tensors of another framework that shares this process's HIP runtime (their
@@ -146,38 +146,45 @@ class RowScorer:
 
     # ---- the calls ----
 
-    def bind_token_logprobs(self, logits, token, *, logprob, lse=None, entropy=None, err=None,
-                            temperature: float = 1.0, vocab=None, dtype=None, stream=None):
+    def bind_token_logprobs(self, logits, token, *, logprob, lse=None, lse_low=None, entropy=None,
+                            err=None, temperature: float = 1.0, vocab=None, dtype=None,
+                            stream=None):
         head, rows, vocab, code = self._rows(logits, vocab, dtype)
         a = dict(rows=rows)
         argv = (*head, float(temperature), self._dev(token, "token", **a),
                 self._dev(logprob, "logprob", **a), self._dev(lse, "lse", **a),
+                self._dev(lse_low, "lse_low", **a),
                 self._dev(entropy, "entropy", **a), self._dev(err, "err", row_elems=12, **a),
                 vp(hip.stream_handle(stream)))
-        return self._call("pb_token_logprobs", argv,
-                          (self, logits, token, logprob, lse, entropy, err))
+        return self._call("pb_token_logprobs_wide", argv,
+                          (self, logits, token, logprob, lse, lse_low, entropy, err))
 
     def token_logprobs(self, logits, token, **kw) -> None:
         """ln softmax(logits / temperature)[token] of each row; optionally the
-        rows' log-sum-exp and entropy."""
+        rows' log-sum-exp, what binary32 leaves out of it (lse_low, for the
+        gradient) and entropy."""
         self.bind_token_logprobs(logits, token, **kw)()
 
-    def bind_token_logprobs_grad(self, logits, token, lse, *, grad, grad_logprob=None,
-                                 grad_entropy=None, entropy=None, temperature: float = 1.0,
-                                 vocab=None, dtype=None, stream=None):
+    def bind_token_logprobs_grad(self, logits, token, lse, *, grad, lse_low=None,
+                                 grad_logprob=None, grad_entropy=None, entropy=None,
+                                 temperature: float = 1.0, vocab=None, dtype=None, stream=None):
         head, rows, vocab, code = self._rows(logits, vocab, dtype)
         a = dict(rows=rows)
         argv = (*head, float(temperature), self._dev(token, "token", **a),
-                self._dev(lse, "lse", **a), self._dev(entropy, "entropy", **a),
+                self._dev(lse, "lse", **a), self._dev(lse_low, "lse_low", **a),
+                self._dev(entropy, "entropy", **a),
                 self._dev(grad_logprob, "grad_logprob", **a),
                 self._dev(grad_entropy, "grad_entropy", **a),
                 *self._grad(grad, rows, vocab, code, dtype), vp(hip.stream_handle(stream)))
-        return self._call("pb_token_logprobs_grad", argv,
-                          (self, logits, token, lse, entropy, grad_logprob, grad_entropy, grad))
+        return self._call("pb_token_logprobs_wide_grad", argv,
+                          (self, logits, token, lse, lse_low, entropy, grad_logprob, grad_entropy,
+                           grad))
 
     def token_logprobs_grad(self, logits, token, lse, **kw) -> None:
         """The gradient of sum(grad_logprob * logprob + grad_entropy * entropy)
-        by the logits, from the lse (and entropy) that token_logprobs left."""
+        by the logits, from the lse (and entropy) that token_logprobs left.  With
+        lse_low too, 32-bit gradients are as exact as their type: lse alone is
+        rounded, by up to 5e-7 of every q where it is 10."""
         self.bind_token_logprobs_grad(logits, token, lse, **kw)()
 
     def bind_top_logits(self, logits, k: int, *, token, value, lse=None, err=None,

@@ -209,3 +209,62 @@ def test_saturated_rows_have_no_probability_above_one(scorer, rows, vocab, dtype
     start = torch.arange(rows + 1, dtype=torch.int32, device=DEV)
     scorer.preference_loss(x, token.int(), start, beta=0.1, loss=loss, logprob=lp, temperature=T)
     check("preference")
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 33), (1_100, 40), (3, 9_001)])
+@pytest.mark.parametrize("offset", [0.0, 300.0, -2_000.0])
+def test_a_log_sum_in_two_words_gives_exact_gradients(scorer, rows, vocab, offset):
+    """q = 2^(x c - log-sum), T = 1: c is off by 1.3e-8 of itself, which leaves 1.3e-8 |ln q| (the log-sum is off with
+    it); the exponent is a fused multiply-add, off by 2^-24 of itself; the sums of at most 9,001 / 256 / 4 + 1 chunks
+    of four have 10 + 3 + 2 roundings; 2^a, alpha, beta, their sum and product 6.  Weights under 2^-24 of the row's
+    largest count by their share alone.  lse alone is off by half a step of itself, 1.5e-5 at 300."""
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.randn((rows, vocab), generator=g, device=DEV) * 2.5 + offset
+    token = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+    gl, ge = torch.randn(rows, generator=g, device=DEV), torch.randn(rows, generator=g, device=DEV) * 0.1
+    lp, lse, low, ent = out(rows), out(rows), out(rows), out(rows)
+    scorer.token_logprobs(x, token.int(), logprob=lp, lse=lse, lse_low=low, entropy=ent)
+    want = ref.logprobs(x, token)
+    tol = ref.EPS32 * (10 + 3 + 2 + 6 + 24) + 24 * 1.3e-8
+    both = lse.double() + low.double()
+    near(both, want["lse"], tol + 1.3e-8 * want["lse"].abs(), "the log-sum")
+    assert (low.abs() <= 1.01 * ref.EPS32 * lse.abs() + 1e-12).all()
+    q = torch.softmax(x.double(), 1)
+    log_q = (x.double() - want["lse"][:, None])
+    for a, b in ((gl, None), (gl, ge)):
+        grad = out(rows, vocab)
+        kw = {} if b is None else dict(grad_entropy=b, entropy=ent)
+        scorer.token_logprobs_grad(x, token.int(), lse, lse_low=low, grad=grad, grad_logprob=a, **kw)
+        zero = torch.zeros_like(a)
+        want_grad = ref.logprobs_grad(x, token, a, zero if b is None else b)
+        scale = a.double().abs()[:, None]
+        if b is not None:  # ln q + H is off by its own roundings beside those of q
+            scale = scale + b.double().abs()[:, None] * (log_q.abs() + want["entropy"][:, None].abs() + 3.0)
+        near(grad, want_grad, ref.EPS32 * want_grad.abs() + scale * q * tol + 1e-37, "gradient")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [5, 1_100])
+def test_gradients_of_very_large_logits(scorer, rows, dtype):
+    """Three equal logits of 60,000 at T = 0.01: their log-sum's nearest binary32 is up to a half away, and each has a
+    third of the mass all the same, up to a handful of roundings."""
+    vocab, T = 700, 0.01
+    x, g = make_logits(rows, vocab, dtype, seed=rows)
+    where = torch.topk(torch.rand((rows, vocab), generator=g, device=DEV), 3, dim=1).indices
+    level = 50_000.0 + torch.arange(rows, device=DEV) % 10 * 1_024.0
+    x.scatter_(1, where, level[:, None].expand(-1, 3).to(x.dtype))
+    token = where[:, 0]
+    want = torch.zeros((rows, vocab), dtype=torch.float64, device=DEV)
+    want.scatter_(1, where, torch.tensor([2.0, -1.0, -1.0], dtype=torch.float64, device=DEV).expand(rows, 3) / 3 / T)
+    tol = torch.finfo(x.dtype).eps / 2 * want.abs() + 12 * ref.EPS32 * want.abs() + 1e-30
+    lp, lse, low, one = out(rows), out(rows), out(rows), torch.ones(rows, device=DEV)
+    scorer.token_logprobs(x, token.int(), logprob=lp, lse=lse, lse_low=low, temperature=T)
+    third = torch.full((rows,), -math.log(3.0), dtype=torch.float64, device=DEV)
+    near(lp, third, ref.scalar_tolerance(third, torch.full((rows,), 6 * ref.EPS32, device=DEV)), "logprob")
+    grad = torch.full_like(x, 5.0)
+    scorer.token_logprobs_grad(x, token.int(), lse, lse_low=low, grad=grad, grad_logprob=one, temperature=T)
+    near(grad, want, tol, "log-probability")
+    scorer.policy_loss(x, token.int(), lp, one, loss=out(rows), grad=grad, temperature=T)
+    near(grad, -want, tol, "policy")
+    scorer.distill_loss(x, where.int()[:, :1].contiguous(), one[:, None], loss=out(rows), grad=grad, temperature=T)
+    near(grad, -want, tol, "distillation")
