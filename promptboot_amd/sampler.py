@@ -649,7 +649,9 @@ class DecodeBatch:
         `logprobs` (a device buffer of rows binary32 values) receives
         ln softmax(logits / logprob_temperature)[token] of each sampled token,
         0 for rows not sampled: a rollout's behaviour log-probabilities, of the
-        raw logits (no repetition penalty, no cutoff)."""
+        raw logits (no repetition penalty, no cutoff).  Should the device refuse
+        the scoring alone, the step stands (its tokens are in `contexts`) and the
+        error is raised behind it."""
         rows, ld = _shape(logits)
         if rows != self.rows:
             raise ValueError(f"logits have {rows} rows, the batch has {self.rows}")
@@ -670,9 +672,12 @@ class DecodeBatch:
         except Exception:
             self._undraw()
             raise
-        if score is not None:
-            score()
-        return self._settle(before, stream)
+        try:
+            if score is not None:
+                score()
+        finally:  # the step is on its way: its draws are settled whatever the scoring does
+            tokens = self._settle(before, stream)
+        return tokens
 
     def _scorer(self):
         if self._scores is None:
