@@ -438,7 +438,8 @@ class BatchSampler:
                     detail=None, err=None, stream=None):
         """A zero-argument callable that enqueues this exact pb_sample_batch
         call: the arguments are checked and converted once, so each call
-        costs one foreign call, as it does a C caller (for timing loops)."""
+        costs one foreign call, as it does a C caller (for timing loops).  It
+        keeps the sampler, the buffers and the stream alive."""
         rows, ld = _shape(logits)
         hist_ld = _shape(history)[1] if history is not None else 0
         self._ensure(rows)
@@ -456,6 +457,7 @@ class BatchSampler:
             if st != OK:
                 raise InferenceError(e)
 
+        call.buffers = (self, stream, logits, random_24, history, history_len, token, detail, err)
         return call
 
     def bind_lmhead(self, packed, hidden, random_24, history=None, history_len=None, *,
@@ -480,6 +482,8 @@ class BatchSampler:
             if st != OK:
                 raise InferenceError(e)
 
+        call.buffers = (self, stream, packed, hidden, random_24, history, history_len, token,
+                        detail, err, logits)
         return call
 
     def pack_lmhead(self, weights, vocab: int = VOCAB, cols: int = 896, stream=None,

@@ -15,7 +15,7 @@ type and may be the logits themselves.
 
 Every method checks its arguments, enqueues on `stream` and returns; each has a
 `bind_` form that checks them once and returns a callable enqueuing that exact
-call (the buffers are kept alive by it), for loops over fixed buffers.
+call (it keeps the buffers and the stream alive), for loops over fixed buffers.
 """
 from __future__ import annotations
 
@@ -157,7 +157,7 @@ class RowScorer:
                 self._dev(entropy, "entropy", **a), self._dev(err, "err", row_elems=12, **a),
                 vp(hip.stream_handle(stream)))
         return self._call("pb_token_logprobs_wide", argv,
-                          (self, logits, token, logprob, lse, lse_low, entropy, err))
+                          (self, stream, logits, token, logprob, lse, lse_low, entropy, err))
 
     def token_logprobs(self, logits, token, **kw) -> None:
         """ln softmax(logits / temperature)[token] of each row; optionally the
@@ -177,8 +177,8 @@ class RowScorer:
                 self._dev(grad_entropy, "grad_entropy", **a),
                 *self._grad(grad, rows, vocab, code, dtype), vp(hip.stream_handle(stream)))
         return self._call("pb_token_logprobs_wide_grad", argv,
-                          (self, logits, token, lse, lse_low, entropy, grad_logprob, grad_entropy,
-                           grad))
+                          (self, stream, logits, token, lse, lse_low, entropy, grad_logprob,
+                           grad_entropy, grad))
 
     def token_logprobs_grad(self, logits, token, lse, **kw) -> None:
         """The gradient of sum(grad_logprob * logprob + grad_entropy * entropy)
@@ -194,7 +194,7 @@ class RowScorer:
         argv = (*head, int(k), float(temperature), self._dev(token, "token", row_elems=k, **a),
                 self._dev(value, "value", row_elems=k, **a), self._dev(lse, "lse", **a),
                 self._dev(err, "err", row_elems=12, **a), vp(hip.stream_handle(stream)))
-        return self._call("pb_top_logits", argv, (self, logits, token, value, lse, err))
+        return self._call("pb_top_logits", argv, (self, stream, logits, token, value, lse, err))
 
     def top_logits(self, logits, k: int, **kw) -> None:
         """Each row's k largest logits (a teacher's record): ids and raw values
@@ -217,8 +217,9 @@ class RowScorer:
                 *self._grad(grad, rows, vocab, code, dtype),
                 self._dev(err, "err", row_elems=12, **a),
                 vp(hip.stream_handle(stream)))
-        return self._call("pb_distill_loss", argv, (self, logits, teacher_id, teacher_logit,
-                                                    teacher_lse, weight, loss, lse, grad, err))
+        return self._call("pb_distill_loss", argv,
+                          (self, stream, logits, teacher_id, teacher_logit, teacher_lse, weight,
+                           loss, lse, grad, err))
 
     def distill_loss(self, logits, teacher_id, teacher_logit, **kw) -> None:
         """Divergence of each row from a teacher's top logits, and weight times
@@ -241,8 +242,8 @@ class RowScorer:
                 self._dev(err, "err", row_elems=12, **a),
                 vp(hip.stream_handle(stream)))
         return self._call("pb_policy_loss", argv,
-                          (self, logits, token, old_logprob, advantage, ref_logprob, weight, loss,
-                           logprob, kl, grad, err))
+                          (self, stream, logits, token, old_logprob, advantage, ref_logprob,
+                           weight, loss, logprob, kl, grad, err))
 
     def policy_loss(self, logits, token, old_logprob, advantage, **kw) -> None:
         """Clipped policy loss with a KL term of each row, and weight times its
@@ -267,8 +268,9 @@ class RowScorer:
                 *self._grad(grad, rows, vocab, code, dtype),
                 self._dev(err, "err", row_elems=12, **one),
                 vp(hip.stream_handle(stream)))
-        return self._call("pb_preference_loss", argv, (self, logits, token, seq_start, ref_logprob,
-                                                       weight, loss, logprob, grad, err))
+        return self._call("pb_preference_loss", argv,
+                          (self, stream, logits, token, seq_start, ref_logprob, weight, loss,
+                           logprob, grad, err))
 
     def preference_loss(self, logits, token, seq_start, **kw) -> None:
         """Loss of pairs of sequences (rows seq_start[s] .. seq_start[s + 1];
