@@ -104,9 +104,15 @@ class RowScorer:
         self._reserved = tuple(max(a, b) for a, b in zip(self._reserved, (rows, vocab)))
 
     def _ensure(self, rows: int, vocab: int) -> None:
+        # An outgrown workspace stays allocated with the context (a captured graph may
+        # use it): growing by doubling, all of them together are less than twice the last.
+        def grown(need, have, most):
+            return have if need <= have else max(need, min(2 * have, most))
+
         have = self._reserved
         if rows > have[0] or vocab > have[1]:
-            self.reserve(max(rows, have[0]), max(vocab, have[1]))
+            self.reserve(grown(rows, have[0], SCORE_MAX_ROWS),
+                         grown(vocab, have[1], SCORE_MAX_VOCAB))
 
     def _rows(self, logits, vocab, dtype):
         """The leading arguments of a call on `logits`, its rows, vocabulary and type."""
