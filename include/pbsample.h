@@ -464,7 +464,8 @@ void pb_context_set_segments(pb_context *ctx, uint32_t segments);
  *
  * Gradients have the logits' type (rounded to nearest even) and may go in
  * place of the logits (d_grad = d_logits and grad_ld = ld); any other overlap
- * of the two is refused with PB_STATE.  Columns from vocab on are not written.
+ * of the two is refused with PB_STATE (of rows with two strides, that of the
+ * ranges they span).  Columns from vocab on are not written.
  * A weight is the row's upstream gradient: gradients are multiplied by it,
  * losses are not.  NULL weights are 1.
  *

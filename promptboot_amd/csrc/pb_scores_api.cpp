@@ -46,6 +46,24 @@ struct Rows {
 
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
+// Whether a gradient that is not in place of the logits shares an element with
+// them.  Rows of one stride may lie between each other (the columns of one buffer,
+// or every other row of it); of two strides the ranges they span are compared.
+bool overlap(const Rows& r, size_t size) {
+  const uintptr_t a = (uintptr_t)r.logits, b = (uintptr_t)r.grad;
+  const uintptr_t a_end = a + ((size_t)(r.rows - 1) * r.ld + r.vocab) * size;
+  const uintptr_t b_end = b + ((size_t)(r.rows - 1) * r.grad_ld + r.vocab) * size;
+  if (a >= b_end || b >= a_end) return false;
+  if (r.ld != r.grad_ld) return true;
+  // row i of the logits and row i - k of the gradient start `m` elements apart, row i
+  // and row i - k - 1 ld - m
+  const int64_t d = ((int64_t)b - (int64_t)a) / (int64_t)size, ld = (int64_t)r.ld;
+  const int64_t k = d >= 0 ? d / ld : -((-d + ld - 1) / ld), m = d - k * ld;
+  const int64_t rows = r.rows, vocab = (int64_t)r.vocab;
+  return (k < rows && -k < rows && m < vocab) ||
+         (k + 1 < rows && -(k + 1) < rows && ld - m < vocab);
+}
+
 // The checks that every call makes of its rows.  `missing`: a required
 // pointer is null.
 uint32_t check_rows(const Rows& r, bool missing, pb_inference_error* err) {
@@ -65,12 +83,9 @@ uint32_t check_rows(const Rows& r, bool missing, pb_inference_error* err) {
   if (r.ld >> 40 || r.grad_ld >> 40)
     return refuse(err, PB_CAPACITY, (uint64_t)1 << 40, r.ld, PB_FIELD_LOGITS, 4);
   if (r.rows != 0 && missing) return refuse(err, PB_CAPACITY, 1, 0, PB_FIELD_BYTES, 3);
-  if (r.rows != 0 && r.grad != nullptr && !(r.grad == r.logits && r.grad_ld == r.ld)) {
-    const uintptr_t a = (uintptr_t)r.logits, b = (uintptr_t)r.grad;
-    const uintptr_t a_end = a + ((size_t)(r.rows - 1) * r.ld + r.vocab) * size;
-    const uintptr_t b_end = b + ((size_t)(r.rows - 1) * r.grad_ld + r.vocab) * size;
-    if (a < b_end && b < a_end) return refuse(err, PB_STATE, 0, 0, PB_FIELD_BYTES, 9);
-  }
+  if (r.rows != 0 && r.grad != nullptr && !(r.grad == r.logits && r.grad_ld == r.ld) &&
+      overlap(r, size))
+    return refuse(err, PB_STATE, 0, 0, PB_FIELD_BYTES, 9);
   return PB_OK;
 }
 

@@ -268,3 +268,36 @@ def test_gradients_of_very_large_logits(scorer, rows, dtype):
     near(grad, -want, tol, "policy")
     scorer.distill_loss(x, where.int()[:, :1].contiguous(), one[:, None], loss=out(rows), grad=grad, temperature=T)
     near(grad, -want, tol, "distillation")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(3, 60_001), (70, 1_003), (1_100, 301)])
+def test_gradients_between_the_rows_of_the_logits(scorer, rows, vocab, dtype):
+    """Logits and gradient as columns of one buffer, and as its even and odd rows."""
+    x, g = make_logits(rows, vocab, dtype, seed=vocab)
+    token = torch.randint(0, vocab, (rows,), generator=g, device=DEV).int()
+    one, lse = torch.ones(rows, device=DEV), out(rows)
+    ids, logit = token[:, None].contiguous(), torch.zeros((rows, 1), device=DEV)
+    start = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device=DEV)
+    scorer.token_logprobs(x, token, logprob=out(rows), lse=lse)
+
+    def calls(y, grad):
+        scorer.policy_loss(y, token, -one, one, loss=out(rows), grad=grad)
+        yield
+        scorer.distill_loss(y, ids, logit, loss=out(rows), grad=grad)
+        yield
+        scorer.preference_loss(y, token, start, beta=0.1, loss=out(1), grad=grad)
+        yield
+        scorer.token_logprobs_grad(y, token, lse, grad=grad, grad_logprob=one)
+        yield
+
+    beside = torch.full((rows, 2 * vocab + 3), 5.0, dtype=x.dtype, device=DEV)
+    between = torch.full((2 * rows, vocab + 1), 5.0, dtype=x.dtype, device=DEV)
+    apart = torch.empty_like(x)
+    for y, grad, rest in ((beside[:, :vocab], beside[:, vocab + 1:2 * vocab + 1], beside),
+                          (between[::2, :vocab], between[1::2, :vocab], between)):
+        y.copy_(x)
+        for _ in zip(calls(x, apart), calls(y, grad)):
+            assert torch.equal(grad, apart) and torch.equal(y, x)
+        grad.fill_(5.0), y.fill_(5.0)
+        assert (rest == 5.0).all()
