@@ -602,7 +602,7 @@ __device__ __forceinline__ PolicyRow policy_row(const ScoreParams& p, uint32_t r
   o.loss = open <= shut ? -open : -shut;
   if (open != open) o.loss = slope = open;
   if (p.ref_logprob != nullptr) {
-    o.kl = away - gap;
+    o.kl = gap == __builtin_inf() ? gap : away - gap;  // e^d outgrows d
     if (p.kl_coef != 0.0) {
       o.loss += p.kl_coef * o.kl;
       slope -= p.kl_coef * away;

@@ -301,3 +301,27 @@ def test_gradients_between_the_rows_of_the_logits(scorer, rows, vocab, dtype):
             assert torch.equal(grad, apart) and torch.equal(y, x)
         grad.fill_(5.0), y.fill_(5.0)
         assert (rest == 5.0).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 500), (4, 151_936), (1_100, 300)])
+def test_a_policy_token_without_weight(scorer, rows, vocab):
+    """ln q = -inf: the ratio is 0, and exp(d) - d - 1 grows without bound with d."""
+    x, g = make_logits(rows, vocab, "f32", seed=vocab)
+    token = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+    x.scatter_(1, token[:, None], -math.inf)
+    adv = torch.where(torch.arange(rows, device=DEV) % 2 == 0, 2.0, -2.0)
+    old, r = torch.full((rows,), -3.0, device=DEV), torch.full((rows,), -2.0, device=DEV)
+    for coef in (0.0, 0.1):
+        for grad in (None, torch.full_like(x, 5.0)):
+            loss, lp, kl, err = out(rows), out(rows), out(rows), records(rows)
+            scorer.policy_loss(x, token.int(), old, adv, ref_logprob=r, kl_coef=coef, loss=loss, logprob=lp, kl=kl,
+                               grad=grad, err=err)
+            assert not read_errors(err).view(np.uint8).any()
+            assert (lp == -math.inf).all() and (kl == math.inf).all()
+            if coef != 0.0:
+                assert (loss == math.inf).all()
+                continue
+            want = torch.where(adv > 0, 0.0, 1.6)  # the surrogate alone
+            near(loss, want, torch.full_like(want, 1e-6), "loss")
+            if grad is not None:  # an open ratio of 0 has a slope of 0
+                assert (grad == 0).all()
