@@ -98,10 +98,12 @@ class RowScorer:
 
     def reserve(self, rows: int, vocab: int = _s.VOCAB) -> None:
         """Sizes the context for calls of up to `rows` rows of up to `vocab`
-        ids; a set-up call, it may allocate."""
+        ids, each at least as large as reserved before; a set-up call, it may
+        allocate."""
+        rows, vocab = max(rows, self._reserved[0]), max(vocab, self._reserved[1])
         e = _Error()
         _check(lib().pb_context_reserve_scores(self.sampler._ctx, rows, vocab, ctypes.byref(e)), e)
-        self._reserved = tuple(max(a, b) for a, b in zip(self._reserved, (rows, vocab)))
+        self._reserved = (rows, vocab)
 
     def _ensure(self, rows: int, vocab: int) -> None:
         # An outgrown workspace stays allocated with the context (a captured graph may

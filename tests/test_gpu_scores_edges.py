@@ -325,3 +325,16 @@ def test_a_policy_token_without_weight(scorer, rows, vocab):
             near(loss, want, torch.full_like(want, 1e-6), "loss")
             if grad is not None:  # an open ratio of 0 has a slope of 0
                 assert (grad == 0).all()
+
+
+def test_many_long_rows_behind_separate_reservations():
+    sc = RowScorer(0)
+    sc.reserve(2_000, 100)
+    sc.reserve(2, 5_000)
+    x, g = make_logits(2_000, 5_000, "bf16", seed=1)
+    token = torch.randint(0, 5_000, (2_000,), generator=g, device=DEV)
+    lp = out(2_000)
+    sc.token_logprobs(x, token.int(), logprob=lp)
+    want = ref.logprobs(x, token)["logprob"]
+    near(lp, want, ref.scalar_tolerance(want, 2 * ref.lse_tolerance(x, 1.0)), "logprob")
+    sc.close()

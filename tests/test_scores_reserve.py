@@ -36,3 +36,26 @@ def test_a_first_call_reserves_what_it_needs_and_limits_hold():
     assert sc._reserved == (scores.SCORE_MAX_ROWS, scores.SCORE_MAX_VOCAB)
     sc._ensure(scores.SCORE_MAX_ROWS + 1, 5)  # the reservation itself refuses it
     assert sc.calls[-1][0] == scores.SCORE_MAX_ROWS + 1
+
+
+def test_reservations_cover_every_pair_of_what_they_name(monkeypatch):
+    """Many short rows, then few long ones: a call of many long rows does not reserve again, so both must fit."""
+    asked = []
+
+    class Lib:
+        @staticmethod
+        def pb_context_reserve_scores(ctx, rows, vocab, err):
+            asked.append((rows, vocab))
+            return 0
+
+    class Context:
+        _ctx, device = 1, 0
+
+    monkeypatch.setattr(scores, "lib", lambda: Lib)
+    sc = scores.RowScorer(sampler=Context())
+    sc.reserve(1000, 100)
+    sc.reserve(10, 50_000)
+    sc._ensure(1000, 50_000)
+    assert any(rows >= 1000 and vocab >= 50_000 for rows, vocab in asked)
+    sc.reserve(5, 5)
+    assert sc._reserved == (1000, 50_000)
