@@ -1932,10 +1932,23 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 
-// Workgroups that a pass over few rows is cut into.
+// Workgroups that the statistics of few rows are cut into: four of the eight that a
+// compute unit takes.  More parts lengthen the join, and rows that then come in two
+// parts are read no faster; fewer leave units idle.  Log-probabilities of rows of
+// 151,936 bf16 logits, us with a target of 512 / 1,024 / 2,048 / 4,096:
+//   4 rows 7.2 / 7.1 / 6.9 / 7.0   33 rows 9.3 / 14.6 / 16.8 / 16.8   150 rows 12.7 / 13.7 / 16.7 / 26.7
+//   400 rows 34 / 27 / 30 / 34     1,000 rows 56 / 56 / 64 / 63       2,000 rows 106 / 107 / 106 / 101
 constexpr uint32_t kTargetGroups = 1024;
+// The same for the top logits, whose parts publish their tiles' words too; f32, k = 64,
+// us with 256 / 512 / 1,024:
+//   4 rows 17.8 / 17.8 / 18.4   33 rows 22.8 / 23.1 / 29.0   70 rows 29.0 / 25.6 / 29.0
+//   150 rows 45 / 33 / 34       300 rows 51 / 50 / 48
 constexpr uint32_t kTopGroups = 512;
+// Of the gradient pass, never in parts of less than 4,096 elements; us with 8,192 /
+// 65,536, bf16: 40 rows 7.2 / 7.2, 300 rows 32 / 31, 1,000 rows 110 / 95, 3,000 rows
+// 348 / 290.
 constexpr uint32_t kGradGroups = 65536;
+// Logits that may stay in the caches between the two passes (plan_scores).
 constexpr uint64_t kCacheBytes = 400000000;
 // A loss and its gradient take one launch, a workgroup a row, for rows of up to
 // kShortRow bytes and from kFusedRows longer ones on.
@@ -1976,8 +1989,10 @@ void plan_scores(uint32_t dtype, ScoreParams* p) {
   p->fused = 0;
   // Forward and gradient of rows of 304 KB, us with the first read kept in the
   // caches and without: 900 rows 128 / 132, 1,300 rows 189 / 191, 2,000 rows 287 /
-  // 283, 3,000 rows 431 / 426.  Of a preference batch's rows many are prompts or
-  // padding, which are not read (2,563 rows, 1,023 of them read: 213 / 222).
+  // 283, 3,000 rows 431 / 426.  The preference loss keeps twice that: many of a batch's
+  // rows are prompts or padding, which are not read.  With none, 30 % and 60 % of the
+  // rows left out: 1,400 rows 200 / 203, 164 / 176, 124 / 146; 2,000 rows 290 / 297,
+  // 229 / 245, 177 / 198; 2,600 rows 379 / 377, 312 / 331, 229 / 257.
   const uint64_t logit_bytes = (uint64_t)p->rows * p->vocab * (dtype == PB_F32 ? 4u : 2u);
   p->keep = logit_bytes <= (p->mode == kModePreference ? 2u : 1u) * kCacheBytes;
   if (p->grad != nullptr && (p->mode == kModeDistill || p->mode == kModePolicy)) {
