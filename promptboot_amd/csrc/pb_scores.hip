@@ -1018,14 +1018,14 @@ __device__ __forceinline__ RowSum join_parts(const ScoreParams& p, uint32_t row)
   return wave_join<kMoment>(v.shift, v.sum, v.moment, v.bad);
 }
 
-// The statistics pass; large batches read at 6.9 TB/s (4,096 rows of 151,936 bf16
-// logits in 182 us; a plain read reaches 7.0).  A row's parts leave their sums in
-// the workspace, and the workgroup that comes last (by the row's ticket, which it
-// sets back to 0) joins them and works out the row's scalars, so that they need no
-// launch of their own.
+// The statistics pass; large batches read at 6.3 TB/s (4,096 rows of 151,936 bf16
+// logits in 197 us, 188 without the check of each group; a plain read reaches 7.0).
+// A row's parts leave their sums in the workspace, and the workgroup that comes last
+// (by the row's ticket, which it sets back to 0) joins them and works out the row's
+// scalars, so that they need no launch of their own.
 // kKeep: the row is read again soon, and what the call reads may stay in the caches.
 // kList: the distillation; a fifth wave takes the teacher's list (at the end of
-// the row's last part instead, 12 rows took 14.8 us, so 13.0).
+// the row's last part instead, 12 rows took 1.8 us longer).
 constexpr uint32_t kNoList = 0, kListOnly = 1, kListWithRest = 2;
 template <typename E, bool kEntropy, uint32_t kList, bool kKeep>
 __global__ __launch_bounds__(kStatsThreads + (kList ? 64 : 0)) void stats_kernel(
@@ -1313,7 +1313,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(const ScoreParams p)
 // kShelved more in LDS.  512 threads hold 114,688 16-bit logits and leave room for
 // a second workgroup, whose loads run under the first one's scalars and stores;
 // what lies beyond is read again.  Of 4,096 rows of 151,936 bf16 logits a quarter
-// is, and they take 490 us: 2.5 GB at 5.1 TB/s, where a large copy reaches 5.0.
+// is, and they take 494 us: 2.5 GB at 5.0 TB/s, a large copy's rate.
 // While gradients still went through the caches the same rows took 548 us, 566 by
 // 1,024 threads that hold the whole row alone on their compute unit, and 590 with
 // the next row's loads run into the gradient's stores; requesting the chunks that
@@ -1606,7 +1606,7 @@ __global__ __launch_bounds__(kThreads, 4) void fused_kernel(const ScoreParams p)
 // the k tiles of the largest maxima (the lower tile first among equal ones),
 // since each of those holds a logit that ranks before any logit of another tile.
 // So one pass over the row leaves its sums and a word a tile, and only k to
-// k + kSlack tiles are read again: 2,048 rows of 151,936 bf16 logits in 101 us, 6.2
+// k + kSlack tiles are read again: 2,048 rows of 151,936 bf16 logits in 104 us, 6.0
 // TB/s, with the vector units busy two thirds of the time (109 us with quieting
 // maxima and separate lane moves, 163 by halving the words' range for the k-th).
 
@@ -2010,7 +2010,8 @@ void plan_scores(uint32_t dtype, ScoreParams* p) {
     //   100,003 f16    15 / 10     18 / 13     20 / 20     24 / 32     87 / 95
     //   151,936 f32    21 / 9.8    21 / 15     23 / 26     54 / 61    247 / 253
     // A long row takes one workgroup longer than many, and past kMaxTerms logits a
-    // thread its sums would need more bits.
+    // thread its sums would need more bits (64 rows of 1,048,576 took one launch 282 us
+    // in f32 and 144 in bf16, and two passes 138 and 75).
     const uint64_t row_bytes = (uint64_t)p->vocab * (dtype == PB_F32 ? 4u : 2u);
     if ((row_bytes <= kShortRow || p->rows >= kFusedRows) && p->vocab <= kMaxTerms * threads)
       p->fused = threads;
