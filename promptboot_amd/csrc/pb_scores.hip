@@ -229,6 +229,13 @@ __device__ __forceinline__ void follow(Acc& s, float m, float c) {
   }
 }
 
+// Whether a thread's sum stands.  It is 1 and more about a first chunk's largest u; a
+// shift of 0, under a masked first chunk, has to be as near to what weighs.  A sum of
+// NaN or out of range holds something that has failed.
+__device__ __forceinline__ bool sum_holds(float sum) {
+  return sum >= 0x1p-16f && sum <= 0x1p100f;
+}
+
 template <typename E, bool kEntropy>
 __device__ __forceinline__ void add_chunk(Acc& s, const float (&x)[E::kPer], float c) {
   float e[E::kPer], m = 0.0f;
@@ -382,7 +389,7 @@ struct PartScan {
       });
     }
     *bad = kNone;
-    if (first || (s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) return s;
+    if (first || sum_holds(s.sum)) return s;
     return again(bad);
   }
 
@@ -1439,7 +1446,7 @@ struct FusedRow {
           add_chunk<E, false>(s, y, c);
         });
     *bad = kNone;
-    if (s.sum >= 0x1p-60f && s.sum <= 0x1p100f) return s;
+    if (sum_holds(s.sum)) return s;
     // PartScan's second scan, from memory
     float top = -__builtin_inff();
     uint32_t at_bad = kNone;
@@ -1881,7 +1888,7 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
   Acc s = p.tile_shift > 6 ? scan_tiles<E, true>(p, in, hi - lo, words)
                            : scan_tiles<E, false>(p, in, hi - lo, words);
   uint32_t bad = kNone;
-  if (!(s.sum >= 0x1p-60f && s.sum <= 0x1p100f)) {
+  if (!sum_holds(s.sum)) {
     const PartScan<E, kTopThreads, false, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi,
                                                               p.c};
     s = scan.again(&bad);

@@ -338,3 +338,40 @@ def test_many_long_rows_behind_separate_reservations():
     want = ref.logprobs(x, token)["logprob"]
     near(lp, want, ref.scalar_tolerance(want, 2 * ref.lse_tolerance(x, 1.0)), "logprob")
     sc.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(2, 100_003), (40, 20_011), (1_100, 9_001)])
+@pytest.mark.parametrize("level", [-8.0, -15.0, -25.0, -40.0])
+def test_masked_first_chunks_cost_no_precision(scorer, rows, vocab, dtype, level):
+    """All of a row is masked but one token below 0: its thread has met nothing to take a shift from.
+
+    A sum of at least 2^-16 is kept about 0: the exponent has the place of 16 and is off by 2^-21, as in the test of
+    saturated rows.  (Kept down to 2^-60 it was off by 2^-19: 1.3e-6 in the log-probability.)"""
+    T = 0.7
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.full((rows, vocab), -math.inf, device=DEV).to(torch.float32)
+    token = vocab - 1 - torch.randint(0, vocab // 5, (rows,), generator=g, device=DEV)
+    x.scatter_(1, token[:, None], level - torch.rand((rows, 1), generator=g, device=DEV) * 4.0)
+    x = x.to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype])
+    want_lse = x.gather(1, token[:, None])[:, 0].double() / T
+    tol = 2.0 ** -21 * math.log(2) + 3 * ref.EPS32
+    tol_lse = torch.full_like(want_lse, tol) + 2 * ref.EPS32 * want_lse.abs()  # c is rounded
+    zero = torch.zeros(rows, device=DEV)
+    lp, ent, lse, loss, grad = out(rows), out(rows), out(rows), out(rows), torch.empty_like(x)
+
+    def check(what):
+        near(lp, zero, torch.full_like(want_lse, tol), what)
+
+    scorer.token_logprobs(x, token.int(), logprob=lp, lse=lse, entropy=ent, temperature=T)
+    check("logprob")
+    near(lse, want_lse, ref.scalar_tolerance(want_lse, tol_lse), "lse")
+    near(ent, zero, torch.full_like(want_lse, tol + math.log(2) * (2.0 ** -21 + 2 * 16 * ref.EPS32)), "entropy")
+    scorer.top_logits(x, 1, token=out(rows, 1, dtype=torch.int32, fill=0), value=out(rows, 1), lse=lse, temperature=T)
+    near(lse, want_lse, ref.scalar_tolerance(want_lse, tol_lse), "lse of the top logits")
+    for kw in ({}, dict(grad=grad)):
+        scorer.policy_loss(x, token.int(), zero, zero, loss=loss, logprob=lp, temperature=T, **kw)
+        check("policy")
+    start = torch.arange(rows + 1, dtype=torch.int32, device=DEV)
+    scorer.preference_loss(x, token.int(), start, beta=0.1, loss=loss, logprob=lp, temperature=T)
+    check("preference")
