@@ -447,13 +447,13 @@ void pb_context_set_segments(pb_context *ctx, uint32_t segments);
  *              a call's gradient goes in its place (below).
  *   temperature  T, 0.01 to 100: y = x / T, and q = softmax(y) over the row.
  *
- * A logit of -inf (or one whose y / ln 2 is below binary32's range) weighs
+ * A logit of -inf (or one whose y / ln 2 is -2^31 or less: a mask) weighs
  * nothing.  A row whose token is PB_NO_TOKEN, or whose weight is 0, is
  * skipped: its logits do not matter, its outputs are 0, its gradient row is 0.
  * A row error gives NaN outputs, a NaN gradient row and, when d_err is given,
  * a record with `position` = the row: PB_TOKEN_ID (an id >= vocab; needed =
  * vocab, available = the id), PB_NONFINITE_OUTPUT (a NaN or +inf logit, or a y
- * / ln 2 above binary32's range: detail holds the first such index; or a row
+ * / ln 2 of 2^31 or more: detail holds the first such index; or a row
  * in which nothing weighs anything, index 0; available = the logit's bits as
  * binary32).
  *

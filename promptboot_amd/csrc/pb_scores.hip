@@ -28,7 +28,11 @@ constexpr uint32_t kStatsUnroll = 4;
 constexpr uint32_t kGradThreads = 256;
 constexpr uint32_t kTopThreads = 256;
 static_assert(kTopThreads == kStatsThreads, "both passes have the same parts");
-constexpr float kTooBig = 3.0e38f;  // |u| past this has left binary32's range
+// Logits count while |u| is below 2^31.  A shift is a rounded u, and what that leaves out,
+// up to 64 there, is in every exponent about it; further on 2^128 would be.  (With a
+// limit of 3e38, a mask of the type's lowest value at T = 2 made its thread's sum infinite
+// or 0, as the rounding fell.)
+constexpr float kTooBig = 0x1p31f;
 
 // ---- element types: 16 bytes are one chunk ----
 
@@ -183,7 +187,7 @@ struct Acc {
 };
 
 // The shift of a thread whose first chunk's largest u is `u`: that, or 0 where the
-// chunk is masked out.  Past binary32's range it is one that fails the fast sums.
+// chunk is masked out.  Past kTooBig it is one that fails the fast sums.
 __device__ __forceinline__ float first_shift(float u) {
   return u < kTooBig ? (u > -kTooBig ? u : 0.0f) : -__builtin_inff();
 }
@@ -229,11 +233,12 @@ __device__ __forceinline__ void follow(Acc& s, float m, float c) {
   }
 }
 
-// Whether a thread's sum stands.  It is 1 and more about a first chunk's largest u; a
-// shift of 0, under a masked first chunk, has to be as near to what weighs.  A sum of
-// NaN or out of range holds something that has failed.
-__device__ __forceinline__ bool sum_holds(float sum) {
-  return sum >= 0x1p-16f && sum <= 0x1p100f;
+// Whether a thread's sum stands.  It is 1 and more about a first chunk's largest u (up
+// to the rounding of a large one); a shift of 0, under a masked first chunk, has to be
+// as near to what weighs.  A sum of NaN or out of range, or one about a shift that is,
+// holds something that has failed.
+__device__ __forceinline__ bool sum_holds(const Acc& s) {
+  return s.sum >= 0x1p-16f && s.sum <= 0x1p100f && s.shift < kTooBig;
 }
 
 template <typename E, bool kEntropy>
@@ -389,7 +394,7 @@ struct PartScan {
       });
     }
     *bad = kNone;
-    if (first || sum_holds(s.sum)) return s;
+    if (first || sum_holds(s)) return s;
     return again(bad);
   }
 
@@ -1446,7 +1451,7 @@ struct FusedRow {
           add_chunk<E, false>(s, y, c);
         });
     *bad = kNone;
-    if (sum_holds(s.sum)) return s;
+    if (sum_holds(s)) return s;
     // PartScan's second scan, from memory
     float top = -__builtin_inff();
     uint32_t at_bad = kNone;
@@ -1888,7 +1893,7 @@ __global__ __launch_bounds__(kTopThreads, 8) void top_kernel(const ScoreParams p
   Acc s = p.tile_shift > 6 ? scan_tiles<E, true>(p, in, hi - lo, words)
                            : scan_tiles<E, false>(p, in, hi - lo, words);
   uint32_t bad = kNone;
-  if (!sum_holds(s.sum)) {
+  if (!sum_holds(s)) {
     const PartScan<E, kTopThreads, false, false, false> scan{row_ptr<E>(p, row), nullptr, lo, hi,
                                                               p.c};
     s = scan.again(&bad);

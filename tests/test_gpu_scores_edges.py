@@ -6,9 +6,10 @@ import numpy as np
 import pytest
 import torch
 
+from promptboot_amd import sampler as s
 from promptboot_amd.scores import RowScorer
 from tests import scores_reference as ref
-from tests.test_gpu_scores import DEV, make_logits, near, out, read_errors, records
+from tests.test_gpu_scores import DEV, TYPES, make_logits, near, out, read_errors, records
 
 pytestmark = pytest.mark.gpu
 
@@ -375,3 +376,82 @@ def test_masked_first_chunks_cost_no_precision(scorer, rows, vocab, dtype, level
     start = torch.arange(rows + 1, dtype=torch.int32, device=DEV)
     scorer.preference_loss(x, token.int(), start, beta=0.1, loss=loss, logprob=lp, temperature=T)
     check("preference")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(2, 473), (3, 100_003), (70, 9_001), (1_100, 300)])
+@pytest.mark.parametrize("T", [0.5, 1.0, 1.5, 2.0, 10.0, 100.0])
+def test_finite_masks_weigh_nothing(scorer, rows, vocab, T, dtype):
+    """-1e9 and less down to the type's lowest value, over whole chunks, threads and parts, at temperatures that keep
+    them in binary32's range."""
+    lowest = torch.finfo(TYPES[dtype]).min
+    levels = torch.tensor([-1e9, -1e10, -3e15, -1e30, lowest], device=DEV)
+    x, g = make_logits(rows, vocab, dtype, seed=vocab)
+    r = torch.arange(rows, device=DEV)
+    col = torch.arange(vocab, device=DEV)[None, :]
+    keep = torch.randint(0, vocab, (rows, 1), generator=g, device=DEV)
+    scattered = torch.rand((rows, vocab), generator=g, device=DEV) < 0.7
+    masked = torch.where((r % 3 == 0)[:, None], col < vocab // 2, torch.where((r % 3 == 1)[:, None], scattered, col != keep))
+    masked &= col != keep
+    x.copy_(torch.where(masked, levels[r % 5][:, None], x.float()))
+    clean = torch.where(masked, -math.inf, x.double())  # what a mask of -inf would leave
+    token = keep[:, 0]
+    want = ref.logprobs(clean, token, T)
+    y = clean / T
+    tol = ref.EPS32 * (3 * torch.where(torch.isfinite(y), y.abs(), 0.0).amax(1) + 8 + 192)
+    lp, lse, low, ent, loss, err = out(rows), out(rows), out(rows), out(rows), out(rows), records(rows)
+    scorer.token_logprobs(x, token.int(), logprob=lp, lse=lse, lse_low=low, entropy=ent, err=err, temperature=T)
+    assert not read_errors(err).view(np.uint8).any()
+    near(lp, want["logprob"], ref.scalar_tolerance(want["logprob"], 2 * tol), "logprob")
+    near(lse, want["lse"], ref.scalar_tolerance(want["lse"], tol), "lse")
+    near(ent, want["entropy"], ref.scalar_tolerance(want["entropy"], 4 * tol), "entropy")
+    one, grad = torch.ones(rows, device=DEV), torch.full_like(x, 5.0)
+    q = torch.softmax(y, 1)
+    delta = torch.zeros_like(q).scatter_(1, token[:, None], 1.0)
+    half = torch.finfo(x.dtype).eps / 2
+
+    def check(sign, what):
+        bound = (half * (delta - q).abs() + 4 * tol[:, None] * (q + (delta - q).abs())) / T + 1e-36
+        near(grad, sign * (delta - q) / T, bound, what)
+        assert (grad[masked] == 0).all(), what
+
+    scorer.token_logprobs_grad(x, token.int(), lse, lse_low=low, grad=grad, grad_logprob=one, temperature=T)
+    check(1.0, "log-probability")
+    scorer.policy_loss(x, token.int(), lp, one, loss=loss, grad=grad, err=err, temperature=T)
+    assert not read_errors(err).view(np.uint8).any()
+    check(-1.0, "policy")
+    zero = torch.zeros((rows, 1), device=DEV)
+    scorer.distill_loss(x, token.int()[:, None], zero, loss=loss, lse=lse, grad=grad, err=err, temperature=T)
+    assert not read_errors(err).view(np.uint8).any()
+    check(-1.0, "distillation")
+    near(loss, -want["logprob"], ref.scalar_tolerance(want["logprob"], 2 * tol), "distillation")
+    scorer.top_logits(x, 1, token=out(rows, 1, dtype=torch.int32, fill=0), value=out(rows, 1), lse=lse, err=err,
+                      temperature=T)
+    assert not read_errors(err).view(np.uint8).any()
+    near(lse, want["lse"], ref.scalar_tolerance(want["lse"], tol), "lse of the top logits")
+
+
+def test_rows_of_one_finite_mask(scorer):
+    """Up to 2^31 in y / ln 2 a row of equal logits is the uniform distribution; past it nothing weighs, or the row
+    fails at its first such logit."""
+    vocab = 3_001
+    for level, ok in [(-1e9, True), (-1.4e9, True), (1.4e9, True), (-1.6e9, False), (1.6e9, False), (-1e12, False),
+                      (1e12, False), (3e15, False), (-1e30, False), (1e30, False)]:
+        for rows in (2, 70):
+            x = torch.full((rows, vocab), level, device=DEV)
+            token = torch.arange(rows, dtype=torch.int32, device=DEV) * 7
+            lp, ent, loss, err = out(rows), out(rows), out(rows), records(rows)
+            grad = torch.full_like(x, 5.0)
+            scorer.token_logprobs(x, token, logprob=lp, entropy=ent, err=err)
+            e = read_errors(err)
+            scorer.policy_loss(x, token, torch.full_like(lp, -math.log(vocab)), torch.ones_like(lp), loss=loss, grad=grad)
+            if ok:
+                assert not e.view(np.uint8).any(), level
+                want = torch.full((rows,), -math.log(vocab), dtype=torch.float64, device=DEV)
+                near(lp, want, torch.full_like(want, 4e-6), "logprob")  # 12 sums of a chunk and 3 roundings: 2e-6
+                near(ent, -want, torch.full_like(want, 1.2e-5), "entropy")  # and a moment about up to 2^6
+                other = grad[:, -1].double() * vocab
+                near(other, torch.ones_like(want), torch.full_like(want, 2e-5), "gradient")
+            else:
+                assert (e["status"] == s.NONFINITE_OUTPUT).all() and not e["detail"].astype(np.uint32).any(), level
+                assert lp.isnan().all() and loss.isnan().all() and grad.isnan().all()
