@@ -35,6 +35,8 @@
  *   - scores and losses of logits rows, with their gradients: pb_token_logprobs,
  *     pb_token_logprobs_grad (and their _wide forms), pb_top_logits,
  *     pb_distill_loss, pb_policy_loss, pb_preference_loss;
+ *   - hidden-state rows, around a head: pb_embed_rows, pb_embed_rows_grad,
+ *     pb_norm_rows, pb_norm_rows_grad, pb_quantize_rows, pb_int8_matmul;
  *   - host PRNG helpers: pb_sampling_state_new, pb_next_24, pb_fill_random_24.
  */
 #ifndef PBSAMPLE_H
@@ -589,6 +591,118 @@ uint32_t pb_preference_loss(pb_context *ctx, const void *d_logits, uint32_t dtyp
                             double label_smoothing, float *d_loss, float *d_logprob, void *d_grad,
                             size_t grad_ld, pb_inference_error *d_err, void *stream,
                             pb_inference_error *err);
+
+/* ---- hidden-state rows (no counterpart in the reference's sampler path) ----
+ *
+ * What stands around a head: the table rows of drawn tokens, the norm in front of
+ * a product, rows in 8 bits, and the product of 8-bit rows with 8-bit channels (a
+ * head of any vocabulary and width, or any other layer).  The first two come with
+ * their gradients; rounding to 8 bits has none.
+ *
+ * Rows are `cols` elements of a pb_dtype, `ld` elements apart (ld >= cols), and
+ * start at any element; the elements between rows are neither read nor written.
+ * 8-bit rows are signed bytes, -127 to 127, that start at any byte.  cols is 1 to
+ * PB_HIDDEN_MAX_COLS, rows up to PB_HIDDEN_MAX_ROWS, vocab (and the channels of a
+ * product) 1 to PB_SCORE_MAX_VOCAB.
+ *
+ * Outputs are rounded to their type once, to nearest even.  Sums are held in 32
+ * bits over at most 768 terms, in 64 bits above that and for the norms' statistics;
+ * their order depends on the sizes alone (and, in the table's gradient, on the
+ * tokens), so results repeat bit for bit.
+ *
+ * An output may lie in an input's place where its description says so: the same
+ * address, type and distance of rows.  Any other element that an output shares with
+ * an input or another output is refused with PB_STATE.
+ *
+ * All pointers are device pointers; calls enqueue on `stream`, never allocate and
+ * never wait.  The gradients need a context reserved with
+ * pb_context_reserve_hidden for at least their rows and columns (else
+ * PB_CAPACITY), and calls on one context share its workspace: the rule on threads
+ * and streams above holds.  Returns PB_OK when the work was enqueued, else a status
+ * with *err filled (err may be NULL) and nothing enqueued.  d_err: one record per
+ * row, all-zero on success, with `position` = the row. */
+#define PB_HIDDEN_MAX_ROWS 1048576u
+#define PB_HIDDEN_MAX_COLS 32768u
+
+/* Sizes the context's workspace for the gradients below on up to `rows` rows of up
+ * to `cols` columns (as pb_context_reserve: a set-up call; it never shrinks the
+ * workspace, and one it outgrows stays allocated until pb_context_destroy). */
+uint32_t pb_context_reserve_hidden(pb_context *ctx, uint32_t rows, size_t cols,
+                                   pb_inference_error *err);
+
+/* d_out[r] = scale * table[token[r]], the product rounded once to out_dtype.  A token
+ * of PB_NO_TOKEN gives a row of zeros; an id >= vocab a row of NaN and a record
+ * (PB_TOKEN_ID; needed = vocab, available = the id).  scale is finite. */
+uint32_t pb_embed_rows(pb_context *ctx, const void *d_table, uint32_t dtype, size_t vocab,
+                       size_t cols, size_t table_ld, uint32_t rows, const uint32_t *d_token,
+                       double scale, void *d_out, uint32_t out_dtype, size_t out_ld,
+                       pb_inference_error *d_err, void *stream, pb_inference_error *err);
+
+/* The table's gradient: d_table_grad[v] = scale * sum of d_grad[r] over the rows r
+ * whose token is v, in the order of the rows.  accumulate 0: every row of the table
+ * is written, zeros where no token is.  accumulate 1: that sum is added to what is
+ * there, and other rows are left as they are.  Rows whose token is PB_NO_TOKEN or >=
+ * vocab add nothing, and what they hold does not matter. */
+uint32_t pb_embed_rows_grad(pb_context *ctx, const void *d_grad, uint32_t dtype, size_t vocab,
+                            size_t cols, size_t grad_ld, uint32_t rows, const uint32_t *d_token,
+                            double scale, uint32_t accumulate, void *d_table_grad,
+                            uint32_t table_dtype, size_t table_ld, void *stream,
+                            pb_inference_error *err);
+
+/* Root-mean-square norm: h = x + residual rounded to the rows' type (x itself
+ * without d_residual), y = h * weight / sqrt(mean(h * h) + eps).
+ *   d_residual  optional, of the rows' type.
+ *   d_weight    `cols` elements of weight_dtype, next to each other; NULL is all ones.
+ *   d_sum       optional: receives h; may lie in the place of d_x or d_residual.
+ *   d_out       optional: y, of out_dtype; may lie in the place of d_x or d_residual
+ *               (where d_sum does not).
+ *   d_q         optional: y in 8 bits; with s = max |y| / 127 over the row, the whole
+ *               number nearest to y / s, ties to even (which is worked out as if in
+ *               exact arithmetic), and d_scale[r] = s.  A row of zeros has s = 0.
+ * One of d_out and d_q has to be there, and d_scale with d_q.  eps > 0.
+ * A row whose h holds NaN or an infinity (or, with d_q, one of whose products h *
+ * weight does, or whose s passes binary32) fails: y and s are NaN, the 8-bit row is
+ * zeros, the record PB_NONFINITE_INPUT (detail: the first such index, cols if it is s;
+ * available = that h's bits as binary32); h is written as it is. */
+uint32_t pb_norm_rows(pb_context *ctx, const void *d_x, uint32_t dtype, size_t cols, size_t x_ld,
+                      uint32_t rows, const void *d_residual, size_t residual_ld,
+                      const void *d_weight, uint32_t weight_dtype, double eps, void *d_sum,
+                      size_t sum_ld, void *d_out, uint32_t out_dtype, size_t out_ld, int8_t *d_q,
+                      size_t q_ld, float *d_scale, pb_inference_error *d_err, void *stream,
+                      pb_inference_error *err);
+
+/* The norm's gradients, from h (d_sum of pb_norm_rows, or its d_x without a residual)
+ * and d_grad, the gradient by y, of grad_dtype:
+ *   d_grad_h       optional: by h, so by x and by the residual alike, of the rows'
+ *                  type; may lie in the place of d_h, d_grad or d_grad_sum.
+ *   d_grad_sum     optional, of the rows' type: what reaches h elsewhere, added.
+ *   d_grad_weight  optional: `cols` binary32 words, by the weight (without d_weight:
+ *                  by the ones); accumulate 1 adds to what is there.
+ * One of d_grad_h and d_grad_weight has to be there.  Values that are not finite
+ * spread as the formulas have it. */
+uint32_t pb_norm_rows_grad(pb_context *ctx, const void *d_h, uint32_t dtype, size_t cols,
+                           size_t h_ld, uint32_t rows, const void *d_weight,
+                           uint32_t weight_dtype, double eps, const void *d_grad,
+                           uint32_t grad_dtype, size_t grad_ld, const void *d_grad_sum,
+                           size_t grad_sum_ld, void *d_grad_h, size_t grad_h_ld,
+                           float *d_grad_weight, uint32_t accumulate, void *stream,
+                           pb_inference_error *err);
+
+/* Rows in 8 bits without a norm (weights, a channel a row; or activations): as d_q and
+ * d_scale of pb_norm_rows with y = x. */
+uint32_t pb_quantize_rows(pb_context *ctx, const void *d_x, uint32_t dtype, size_t cols,
+                          size_t x_ld, uint32_t rows, int8_t *d_q, size_t q_ld, float *d_scale,
+                          pb_inference_error *d_err, void *stream, pb_inference_error *err);
+
+/* d_out[r][n] = scale[r] * weight_scale[n] * sum_k q[r][k] weight[n][k] (+ bias[n]): `rows` rows
+ * times `channels` channels of `cols` signed bytes each (-128 counts as such).  The sum is
+ * exact; it, its products and the bias' addition are rounded to binary32 each, then to
+ * out_dtype.  d_bias optional.  A NaN scale makes its row or channel NaN. */
+uint32_t pb_int8_matmul(pb_context *ctx, const int8_t *d_q, size_t q_ld, const float *d_scale,
+                        uint32_t rows, size_t cols, const int8_t *d_weight, size_t weight_ld,
+                        const float *d_weight_scale, size_t channels, const float *d_bias,
+                        void *d_out, uint32_t out_dtype, size_t out_ld, void *stream,
+                        pb_inference_error *err);
 
 /* ---- device arithmetic probes (verification hooks, no reference
  * counterpart): evaluate, on the GPU, the exact binary32 routines the sampler

@@ -39,6 +39,8 @@ struct pb_context {
   size_t scores_bytes = 0;
   void* d_ticket = nullptr;  // its tickets: a word per row, 0 between calls
   size_t ticket_bytes = 0;
+  void* d_hidden = nullptr;  // workspace of the hidden-state rows' gradients
+  size_t hidden_bytes = 0;
   // Workspaces that pb_context_reserve outgrew.  A HIP graph captured before
   // the growth still launches kernels on them, so they stay allocated until
   // pb_context_destroy.
@@ -219,7 +221,7 @@ static void release(pb_context* ctx) {
   DeviceGuard guard(ctx->device);
   if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
   free_staging(ctx);
-  void* dev[] = {ctx->d_work, ctx->d_lm, ctx->d_scores, ctx->d_ticket, ctx->d_seen};
+  void* dev[] = {ctx->d_work, ctx->d_lm, ctx->d_scores, ctx->d_ticket, ctx->d_hidden, ctx->d_seen};
   for (void* p : dev)
     if (p) (void)hipFree(p);
   for (void* p : ctx->retired) (void)hipFree(p);
@@ -560,6 +562,17 @@ hipError_t scores_reserve(pb_context* ctx, uint32_t rows, size_t bytes) {
   ctx->d_ticket = fresh;
   ctx->ticket_bytes = have;
   return hipSuccess;
+}
+
+HiddenAccess hidden_access(pb_context* ctx) {
+  std::unique_lock<std::mutex> lock(ctx->mu);
+  return HiddenAccess{std::move(lock), ctx->device, ctx->d_hidden, ctx->hidden_bytes};
+}
+
+hipError_t hidden_reserve(pb_context* ctx, size_t bytes) {
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  DeviceGuard guard(ctx->device);
+  return grow_device(&ctx->d_hidden, &ctx->hidden_bytes, bytes, &ctx->retired);
 }
 
 uint32_t enqueue_sample_with_workspace(pb_context* ctx, void* work, size_t work_bytes,

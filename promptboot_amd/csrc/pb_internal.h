@@ -153,6 +153,16 @@ ScoresAccess scores_access(pb_context* ctx);
 // Grows that workspace to `bytes` and the tickets to `rows`; takes the lock itself.
 hipError_t scores_reserve(pb_context* ctx, uint32_t rows, size_t bytes);
 
+// The same for the workspace of the hidden-state rows' gradients.
+struct HiddenAccess {
+  std::unique_lock<std::mutex> lock;
+  int device;
+  void* work;
+  size_t bytes;
+};
+HiddenAccess hidden_access(pb_context* ctx);
+hipError_t hidden_reserve(pb_context* ctx, size_t bytes);
+
 // The context's device (pb_api.cpp).
 int context_device(const pb_context* ctx);
 // pb_sample_batch with `work` (work_bytes) as the slice workspace in place of

@@ -170,6 +170,24 @@ EXPORTS = {
     "pb_preference_loss": (
         u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, u32, vp, vp, f64, f64, vp, vp, vp,
               size_t, vp, vp, ctypes.POINTER(_Error)]),
+    "pb_context_reserve_hidden": (u32, [vp, u32, size_t, ctypes.POINTER(_Error)]),
+    "pb_embed_rows": (
+        u32, [vp, vp, u32, size_t, size_t, size_t, u32, vp, f64, vp, u32, size_t, vp, vp,
+              ctypes.POINTER(_Error)]),
+    "pb_embed_rows_grad": (
+        u32, [vp, vp, u32, size_t, size_t, size_t, u32, vp, f64, u32, vp, u32, size_t, vp,
+              ctypes.POINTER(_Error)]),
+    "pb_norm_rows": (
+        u32, [vp, vp, u32, size_t, size_t, u32, vp, size_t, vp, u32, f64, vp, size_t, vp, u32,
+              size_t, vp, size_t, vp, vp, vp, ctypes.POINTER(_Error)]),
+    "pb_norm_rows_grad": (
+        u32, [vp, vp, u32, size_t, size_t, u32, vp, u32, f64, vp, u32, size_t, vp, size_t, vp,
+              size_t, vp, u32, vp, ctypes.POINTER(_Error)]),
+    "pb_quantize_rows": (
+        u32, [vp, vp, u32, size_t, size_t, u32, vp, size_t, vp, vp, vp, ctypes.POINTER(_Error)]),
+    "pb_int8_matmul": (
+        u32, [vp, vp, size_t, vp, u32, size_t, vp, size_t, vp, size_t, vp, vp, u32, size_t, vp,
+              ctypes.POINTER(_Error)]),
     "pb_decode_draw": (None, [vp, vp, u32, vp, vp]),
     "pb_decode_settle": (u32, [vp, vp, vp, vp, u32]),
     "pb_version": (ctypes.c_char_p, []),
@@ -597,12 +615,15 @@ class DecodeBatch:
         self.r24, self.token, self.row_state = (
             self._io.part(k * self.rows, self.rows) for k in range(3))
         self.row_state.upload(self.row_state_host)
+        self.token.upload(np.full(self.rows, NO_TOKEN, np.uint32))
         self.states = (_State * self.rows)()
         for r, seed in enumerate(seeds):
             lib().pb_sampling_state_new(ctypes.byref(self.states[r]), int(seed) & (2**64 - 1))
         self._saved = (_State * self.rows)()
         self.err = hip.DeviceArray((self.rows, ERROR_DTYPE.itemsize // 4), np.uint32)
         self._scores = None
+        self._hidden = None
+        self._head = None  # an 8-bit head's rows, their scales and the logits
 
     def close(self):
         if self._own and self.sampler is not None:
@@ -689,6 +710,50 @@ class DecodeBatch:
 
             self._scores = RowScorer(sampler=self.sampler)
         return self._scores
+
+    def _hidden_rows(self):
+        if self._hidden is None:
+            from .hidden import HiddenRows
+
+            self._hidden = HiddenRows(sampler=self.sampler)
+        return self._hidden
+
+    def int8_step(self, hidden, weight, weight_scale, *, norm_weight=None, residual=None, sum=None,
+                  eps: float = 1e-6, bias=None, dtype=None, weight_dtype=None, stream=None,
+                  logprobs=None, logprob_temperature: float = 1.0) -> np.ndarray:
+        """One step through an 8-bit head of any width: hidden [rows, cols] in 8 bits, times
+        weight [VOCAB, cols] with its channels' weight_scale (+ bias), then step() on these
+        logits.  With norm_weight the head takes the root-mean-square norm of hidden (+
+        residual, kept in `sum`); without it, hidden as it is."""
+        rows, cols = _shape(hidden)
+        if rows != self.rows:
+            raise ValueError(f"hidden has {rows} rows, the batch has {self.rows}")
+        if _shape(weight) != (VOCAB, cols):
+            raise ValueError(f"the head has shape {_shape(weight)}, not ({VOCAB}, {cols})")
+        if norm_weight is None and (residual is not None or sum is not None):
+            raise ValueError("residual and sum belong to a norm: norm_weight is missing")
+        ops = self._hidden_rows()
+        if self._head is None or self._head[0].shape[1] != cols:
+            self._head = (hip.DeviceArray((rows, cols), np.int8), hip.DeviceArray(rows, np.float32),
+                          hip.DeviceArray((rows, VOCAB), np.uint32))
+        q, scale, logits = self._head
+        if norm_weight is None:
+            ops.quantize(hidden, q=q, scale=scale, dtype=dtype, stream=stream)
+        else:
+            ops.norm(hidden, norm_weight, eps=eps, residual=residual, sum=sum, q=q, scale=scale,
+                     dtype=dtype, weight_dtype=weight_dtype, stream=stream)
+        ops.matmul(q, scale, weight, weight_scale, out=logits, bias=bias, stream=stream)
+        return self.step(logits, stream=stream, logprobs=logprobs,
+                         logprob_temperature=logprob_temperature)
+
+    def embed(self, table, *, out, scale: float = 1.0, dtype=None, out_dtype=None,
+              stream=None) -> None:
+        """The table rows of the tokens that the last step drew, the next step's input (zeros
+        for rows not sampled), enqueued on `stream`."""
+        if _shape(out)[0] != self.rows:
+            raise ValueError(f"out has {_shape(out)[0]} rows, the batch has {self.rows}")
+        self._hidden_rows().embed(table, self.token, out=out, scale=scale, dtype=dtype,
+                                  out_dtype=out_dtype, stream=stream)
 
     def lmhead_step(self, packed, hidden, cols: int | None = None, stream=None,
                     q8: bool = False) -> np.ndarray:
