@@ -86,5 +86,10 @@ __device__ __forceinline__ uint4 stream_chunk(const typename E::Raw* p) {
   const Words4 v = __builtin_nontemporal_load(reinterpret_cast<const Loose4*>(p));
   return make_uint4(v.x, v.y, v.z, v.w);
 }
+// A store of what the launch does not read again: past the caches.
+template <typename E>
+__device__ __forceinline__ void store_chunk(typename E::Raw* p, const uint4& v) {
+  __builtin_nontemporal_store(Words4{v.x, v.y, v.z, v.w}, reinterpret_cast<Loose4*>(p));
+}
 
 }  // namespace pb

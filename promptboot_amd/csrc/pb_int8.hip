@@ -20,19 +20,31 @@ namespace {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef v4i Loose16 __attribute__((aligned(1), may_alias));
-typedef uint32_t Loose32 __attribute__((aligned(2), may_alias));
 
 __device__ __forceinline__ v4i load_whole(const int8_t* p) {
   return *reinterpret_cast<const Loose16*>(p);
 }
-// 16 bytes of a row of which n are there; zeros behind them.
-__device__ __forceinline__ v4i load_bytes(const int8_t* p, uint32_t n) {
-  if (n >= 16u) return load_whole(p);
+// The 16 bytes at `at` of a row of `cols` bytes, zeros behind its end.  A row's last piece is
+// taken from the row's last 16 bytes and shifted: byte by byte it cost 333 rows of 1,001
+// bytes 11 of 59 us.
+__device__ __forceinline__ v4i load_piece(const int8_t* row, uint32_t at, uint32_t cols) {
+  if (at + 16u <= cols) return load_whole(row + at);
   v4i v = {0, 0, 0, 0};
-#pragma unroll
-  for (uint32_t e = 0; e < 16; ++e)
-    if (e < n) v[e / 4] |= (int)((uint32_t)(uint8_t)p[e] << (8u * (e % 4)));
-  return v;
+  if (at >= cols) return v;
+  if (cols < 16u) {
+    for (uint32_t e = 0; e < cols; ++e)
+      v[e / 4] |= (int)((uint32_t)(uint8_t)row[e] << (8u * (e % 4)));
+    return v;
+  }
+  const uint32_t out = at + 16u - cols;  // bytes that another piece has
+  v = load_whole(row + cols - 16u);
+  if (out & 8u) v = v4i{v[2], v[3], 0, 0};
+  if (out & 4u) v = v4i{v[1], v[2], v[3], 0};
+  const uint32_t shift = out & 3u;
+  return v4i{(int)__builtin_amdgcn_alignbyte((uint32_t)v[1], (uint32_t)v[0], shift),
+             (int)__builtin_amdgcn_alignbyte((uint32_t)v[2], (uint32_t)v[1], shift),
+             (int)__builtin_amdgcn_alignbyte((uint32_t)v[3], (uint32_t)v[2], shift),
+             (int)__builtin_amdgcn_alignbyte(0u, (uint32_t)v[3], shift)};
 }
 
 __device__ __forceinline__ float scaled(int sum, float s, float ws, const float* bias, float b) {
@@ -40,295 +52,516 @@ __device__ __forceinline__ float scaled(int sum, float s, float ws, const float*
   return bias != nullptr ? y + b : y;
 }
 
-// ---- few rows: bound by the weights' bytes ----
+// ---- few rows of short products ----
 //
 // v_mfma_i32_16x16x64_i8 on operands that come straight from memory: lane l holds row (A)
 // or channel (B) l % 16 and the 16 bytes at 16 (l / 16) of the step's 64, so that a load
 // takes 64 neighbouring bytes of each of 16 channels.  Result register i of the lane is
-// D[4 (l / 16) + i][l % 16].  A wave takes NT x 16 channels and all rows (MT x 16), or
-// the split-th part of the contraction of them; the waves of a workgroup that share their
-// channels add up through LDS.
-template <typename Out, int MT, int NT>
-__global__ __launch_bounds__(512) void int8_few_kernel(Int8Params p, uint32_t split) {
-  constexpr int U = MT <= 2 ? 4 : 2;  // steps in flight beside those in use
-  extern __shared__ int partial[];    // [waves][MT][NT][4][64]
+// D[4 (l / 16) + i][l % 16].  A wave takes 16 channels and all rows, or the split-th part
+// of the contraction of them; the waves of a workgroup that share their channels add up
+// through LDS.  No barrier stands between a load and its use, so that a short product is
+// little more than a launch and two round trips.
+constexpr uint32_t kFewWaves = 4;
+template <typename Out>
+__global__ __launch_bounds__(64 * kFewWaves) void int8_few_kernel(Int8Params p, uint32_t split) {
+  constexpr uint32_t U = 4;  // steps on their way beside those in use
+  __shared__ int sums[kFewWaves][4][64];
   const uint32_t lane = lane_id();
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t waves = blockDim.x >> 6, own = waves / split;
-  const uint32_t group = blockIdx.x * own + wave / split, part = wave % split;
-  const uint32_t n0 = group * (16u * NT);
+  const uint32_t part = wave % split;
+  const uint32_t n = (blockIdx.x * (kFewWaves / split) + wave / split) * 16u + lane % 16u;
+  const uint32_t m = lane % 16u, piece = lane / 16u * 16u;
+  const int8_t* pw = p.weight + (size_t)(n < p.channels ? n : p.channels - 1u) * p.weight_ld;
+  const int8_t* pq = p.q + (size_t)(m < p.rows ? m : p.rows - 1u) * p.q_ld;
   const uint32_t steps = (p.cols + 63u) / 64u, per = (steps + split - 1u) / split;
-  const uint32_t piece = lane / 16u * 16u;
-  const int8_t* pw[NT];
-  const int8_t* pq[MT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const uint32_t n = n0 + j * 16u + lane % 16u;
-    pw[j] = p.weight + (size_t)(n < p.channels ? n : p.channels - 1u) * p.weight_ld + piece;
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const uint32_t m = i * 16u + lane % 16u;
-    pq[i] = p.q + (size_t)(m < p.rows ? m : p.rows - 1u) * p.q_ld + piece;
-  }
-  v4i acc[MT][NT] = {};
   const uint32_t from = part * per, to = from + per < steps ? from + per : steps;
-  const uint32_t whole = p.cols / 64u;  // steps that no row ends in
-  const uint32_t stop = to < whole ? to : whole;
-  uint32_t step = from;
-  auto multiply = [&](const v4i (&q)[MT], const v4i (&w)[NT]) {
+  v4i acc = {};
+  v4i q[2][U], w[2][U];
+  auto fetch = [&](int set, uint32_t step) {
+    if (step + U <= to && (step + U) * 64u <= p.cols) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (uint32_t u = 0; u < U; ++u) {
+        w[set][u] = load_whole(pw + (step + u) * 64u + piece);
+        q[set][u] = load_whole(pq + (step + u) * 64u + piece);
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[i], w[j], acc[i][j], 0, 0, 0);
-  };
-  v4i q[2][U][MT], w[2][U][NT];
-  auto fetch = [&](int set, uint32_t at) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) w[set][u][j] = load_whole(pw[j] + (size_t)(at + u) * 64u);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) q[set][u][i] = load_whole(pq[i] + (size_t)(at + u) * 64u);
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t at = step + u < to ? (step + u) * 64u + piece : p.cols;
+        w[set][u] = load_piece(pw, at, p.cols);
+        q[set][u] = load_piece(pq, at, p.cols);
+      }
     }
   };
   auto use = [&](int set) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) multiply(q[set][u], w[set][u]);
+    for (uint32_t u = 0; u < U; ++u)
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[set][u], w[set][u], acc, 0, 0, 0);
   };
-  if (step + U <= stop) {
-    fetch(0, step);
-    while (true) {
-      const bool second = step + 2u * U <= stop;
-      if (second) fetch(1, step + U);
-      use(0);
-      step += U;
-      if (!second) break;
-      const bool third = step + 2u * U <= stop;
-      if (third) fetch(0, step + U);
+  if (from < to) fetch(0, from);
+  for (uint32_t step = from; step < to; step += 2u * U) {
+    if (step + U < to) fetch(1, step + U);
+    use(0);
+    if (step + U < to) {
+      if (step + 2u * U < to) fetch(0, step + 2u * U);
       use(1);
-      step += U;
-      if (!third) break;
     }
   }
-  for (; step < to; ++step) {
-    const uint32_t at = step * 64u, left = at + piece < p.cols ? p.cols - at - piece : 0u;
-    v4i a[MT], b[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) b[j] = load_bytes(pw[j] + at, left);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) a[i] = load_bytes(pq[i] + at, left);
-    multiply(a, b);
-  }
   if (split > 1) {
-    int* to_lds = partial + (size_t)wave * (MT * NT * 256);
     if (part != 0) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) to_lds[((i * NT + j) * 4 + e) * 64 + lane] = acc[i][j][e];
+      for (int e = 0; e < 4; ++e) sums[wave][e][lane] = acc[e];
     }
     __syncthreads();
     if (part != 0) return;
     for (uint32_t s = 1; s < split; ++s) {
-      to_lds += MT * NT * 256;
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] += to_lds[((i * NT + j) * 4 + e) * 64 + lane];
+      for (int e = 0; e < 4; ++e) acc[e] += sums[wave + s][e][lane];
     }
   }
-  typename Out::Raw* out = static_cast<typename Out::Raw*>(p.out);
+  if (n >= p.channels) return;
+  const float ws = p.weight_scale[n], bias = p.bias ? p.bias[n] : 0.0f;
+  typename Out::Raw* out = static_cast<typename Out::Raw*>(p.out) + n;
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const uint32_t n = n0 + j * 16u + lane % 16u;
-    if (n >= p.channels) continue;
-    const float ws = p.weight_scale[n], bias = p.bias ? p.bias[n] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-#pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) {
-        const uint32_t m = i * 16u + lane / 16u * 4u + e;
-        if (m < p.rows)
-          out[(size_t)m * p.out_ld + n] = Out::raw(scaled(acc[i][j][e], p.scale[m], ws, p.bias, bias));
-      }
-    }
+  for (uint32_t e = 0; e < 4; ++e) {
+    const uint32_t r = lane / 16u * 4u + e;
+    if (r < p.rows)
+      out[(size_t)r * p.out_ld] = Out::raw(scaled(acc[e], p.scale[r], ws, p.bias, bias));
   }
 }
 
 // ---- many rows: tiles through LDS ----
 //
-// Four waves, WM x WN of them, each with BM x BN blocks of v_mfma_i32_32x32x32_i8: lane
-// 32 h + j holds row or channel j and the 16 bytes at 16 h of 32, result register i is
-// D[8 (i / 4) + 4 h + i % 4][j].  64 bytes of every row and channel are in LDS at a time,
-// twice: while one set is multiplied, the next comes through registers (rows may start at
-// any byte).  A row's four pieces of 16 bytes lie swapped by the row's number, so that
-// eight neighbouring lanes reach all of 128 bytes.
-template <typename Out, int WM, int WN, int BM, int BN>
-__global__ __launch_bounds__(256, 2) void int8_tile_kernel(Int8Params p, uint32_t m_tiles,
-                                                           uint32_t n_tiles) {
-  static_assert(WM * WN == 4, "four waves");
-  constexpr uint32_t TM = WM * BM * 32, TN = WN * BN * 32;
-  constexpr uint32_t CM = TM / 64, CN = TN / 64;  // pieces a thread brings
-  __shared__ __align__(16) int8_t lds[2][(TM + TN) * 64];
-  __shared__ float row_scale[TM];
-  const uint32_t lane = lane_id();
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  // an XCD takes neighbouring tiles, and all row tiles of a channel tile one after the other
-  const uint32_t item = xcd_contiguous_item(blockIdx.x, m_tiles * n_tiles);
-  const uint32_t m0 = item % m_tiles * TM, n0 = item / m_tiles * TN;
-  for (uint32_t r = threadIdx.x; r < TM; r += 256u)
-    row_scale[r] = m0 + r < p.rows ? p.scale[m0 + r] : 0.0f;
+// v_mfma_i32_32x32x32_i8 with the channels as A and the rows as B: lane 32 h + j holds
+// channel or row j and the 16 bytes at 16 h of 32, and result register i is the sum of
+// channel 8 (i / 4) + 4 h + i % 4 and row j: four neighbouring channels of one row.
+// KB bytes of every row and channel of a tile are in LDS at a time, twice: while one set
+// is multiplied the next is on its way.  The pieces of 16 bytes of a row lie swapped by
+// the row's number, so that the 16 rows that 16 lanes read together lie in 16 different
+// places of 256 bytes (with one swap for two rows, half of the LDS cycles were conflicts).
+template <int WM, int WN, int BM, int BN>
+struct Tile {
+  static constexpr uint32_t kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr uint32_t kRows = WM * BM * 32, kChannels = WN * BN * 32;
+};
 
-  const uint32_t r0 = threadIdx.x >> 2, piece = (threadIdx.x & 3u) * 16u;
-  const uint32_t swapped = r0 * 64u + (piece ^ (r0 >> 1 & 3u) * 16u);
-  const int8_t* pq[CM];
-  const int8_t* pw[CN];
+// Where piece `piece` of row `row` lies in a set whose rows are KB bytes.
+template <uint32_t KB>
+__device__ __forceinline__ uint32_t piece_at(uint32_t row, uint32_t piece) {
+  static_assert(KB == 64 || KB == 128 || KB == 256, "four, eight or sixteen pieces");
+  constexpr uint32_t kPieces = KB / 16u;
+  return row * KB + (piece ^ (row / (16u / kPieces) & (kPieces - 1u))) * 16u;
+}
+
+// The tile of a workgroup.  An XCD takes neighbouring tiles, and the row tiles of a group
+// one after the other for each channel tile, so that a group's rows stay in its L2: about
+// 1 MB, or four tiles (4,096 x 151,936 x 896 by groups of 1, 2, 4, 8 and 16 tiles of 256
+// rows: 743, 727, 717, 717 and 731 us).
+struct TilePlan {
+  uint32_t m_tiles, n_tiles, group;
+};
+__device__ __forceinline__ void tile_of(const TilePlan& t, uint32_t* m, uint32_t* n) {
+  const uint32_t item = xcd_contiguous_item(blockIdx.x, t.m_tiles * t.n_tiles);
+  const uint32_t whole = t.group * t.n_tiles, g = item / whole, in_group = item - g * whole;
+  const uint32_t left = t.m_tiles - g * t.group, rows = left < t.group ? left : t.group;
+  *m = g * t.group + in_group % rows;
+  *n = in_group / rows;
+}
+
+// A wave's part of one set's products: blocks of its rows and channels, and the part `wk` of
+// WK of the set's bytes.
+template <uint32_t KB, uint32_t TM, int WK, int BM, int BN>
+__device__ __forceinline__ void multiply_set(const int8_t* set, uint32_t wm, uint32_t wn,
+                                             uint32_t wk, v16i (&acc)[BM][BN]) {
+  constexpr uint32_t kSteps = KB / 32u / WK;
+  const uint32_t j = lane_id() & 31u, h = lane_id() >> 5;
 #pragma unroll
-  for (uint32_t i = 0; i < CM; ++i) {
-    const uint32_t r = m0 + r0 + i * 64u;
-    pq[i] = p.q + (size_t)(r < p.rows ? r : p.rows - 1u) * p.q_ld + piece;
+  for (uint32_t s = 0; s < kSteps; ++s) {
+    const uint32_t at = piece_at<KB>(j, 2u * (wk * kSteps + s) + h);
+    v4i a[BM], b[BN];
+#pragma unroll
+    for (int i = 0; i < BM; ++i)
+      a[i] = *reinterpret_cast<const v4i*>(set + (wm + i * 32u) * KB + at);
+#pragma unroll
+    for (int k = 0; k < BN; ++k)
+      b[k] = *reinterpret_cast<const v4i*>(set + (TM + wn + k * 32u) * KB + at);
+#pragma unroll
+    for (int i = 0; i < BM; ++i)
+#pragma unroll
+      for (int k = 0; k < BN; ++k)
+        acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[k], a[i], acc[i][k], 0, 0, 0);
   }
+}
+
+// Scales and stores a wave's sums.  They go through LDS (kSliceBytes a wave), 128 bytes of
+// 32 rows at a time, so that eight lanes store 128 neighbouring bytes, past the caches:
+// with one element a lane (64 bytes of a row together) and through the caches 4,096 x
+// 151,936 bf16 logits alone took 594 us, through LDS 356, and past the caches 262.
+constexpr uint32_t kSlicePitch = 144, kSliceBytes = 32 * kSlicePitch;
+template <typename Out, int BM, int BN>
+__device__ __forceinline__ void store_sums(const Int8Params& p, int8_t* slice,
+                                           const float* chan_scale, const float* chan_bias,
+                                           uint32_t m0, uint32_t n0, uint32_t wn,
+                                           const float (&row_scale)[BM],
+                                           const v16i (&acc)[BM][BN]) {
+  constexpr uint32_t kSize = 16 / Out::kPer;           // bytes of an element
+  constexpr int kBlocks = 128 / (32 * (int)kSize);     // blocks of channels of a slice
+  static_assert(BN % kBlocks == 0, "whole slices");
+  const uint32_t lane = lane_id(), j = lane & 31u, h = lane >> 5;
+  typename Out::Raw* out = static_cast<typename Out::Raw*>(p.out);
 #pragma unroll
-  for (uint32_t i = 0; i < CN; ++i) {
-    const uint32_t r = n0 + r0 + i * 64u;
-    pw[i] = p.weight + (size_t)(r < p.channels ? r : p.channels - 1u) * p.weight_ld + piece;
-  }
-  v4i vq[CM], vw[CN];
-  auto fetch = [&](uint32_t k) {
-    if (k + 64u <= p.cols) {
+  for (int i = 0; i < BM; ++i) {
 #pragma unroll
-      for (uint32_t i = 0; i < CM; ++i) vq[i] = load_whole(pq[i] + k);
+    for (int k0 = 0; k0 < BN; k0 += kBlocks) {
 #pragma unroll
-      for (uint32_t i = 0; i < CN; ++i) vw[i] = load_whole(pw[i] + k);
-    } else {
-      const uint32_t left = k + piece < p.cols ? p.cols - k - piece : 0u;
+      for (int k = k0; k < k0 + kBlocks; ++k) {
 #pragma unroll
-      for (uint32_t i = 0; i < CM; ++i) vq[i] = load_bytes(pq[i] + k, left);
+        for (uint32_t e = 0; e < 16; e += 4) {
+          const uint32_t c = k * 32u + 2u * e + 4u * h;  // of the wave's channels
+          const float4 ws = *reinterpret_cast<const float4*>(chan_scale + wn + c);
+          const float4 bs = *reinterpret_cast<const float4*>(chan_bias + wn + c);
+          const float y0 = scaled(acc[i][k][e], row_scale[i], ws.x, p.bias, bs.x);
+          const float y1 = scaled(acc[i][k][e + 1], row_scale[i], ws.y, p.bias, bs.y);
+          const float y2 = scaled(acc[i][k][e + 2], row_scale[i], ws.z, p.bias, bs.z);
+          const float y3 = scaled(acc[i][k][e + 3], row_scale[i], ws.w, p.bias, bs.w);
+          int8_t* to = slice + j * kSlicePitch + (c - k0 * 32u) * kSize;
+          if constexpr (kSize == 4)
+            *reinterpret_cast<float4*>(to) = make_float4(y0, y1, y2, y3);
+          else
+            *reinterpret_cast<uint2*>(to) = make_uint2(Out::two(y0, y1), Out::two(y2, y3));
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (uint32_t i = 0; i < CN; ++i) vw[i] = load_bytes(pw[i] + k, left);
+      for (uint32_t s = 0; s < 4; ++s) {
+        const uint32_t r = s * 8u + lane / 8u, piece = lane % 8u;
+        const uint4 v = *reinterpret_cast<const uint4*>(slice + r * kSlicePitch + piece * 16u);
+        const uint32_t m = m0 + i * 32u + r, n = n0 + wn + k0 * 32u + piece * Out::kPer;
+        if (m < p.rows && n < p.channels) {
+          typename Out::Raw* to = out + (size_t)m * p.out_ld + n;
+          if (n + Out::kPer <= p.channels) {
+            store_chunk<Out>(to, v);
+          } else {
+#pragma unroll
+            for (uint32_t e = 0; e + 1u < (uint32_t)Out::kPer; ++e)
+              if (n + e < p.channels) to[e] = Out::raw(Out::get(v, e));
+          }
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
     }
-  };
-  auto keep = [&](int8_t* to) {
+  }
+}
+
+// The channels' scales and biases of a tile, in LDS.
+template <uint32_t kThreads, uint32_t TN>
+__device__ __forceinline__ void load_channels(const Int8Params& p, uint32_t n0, float* scale,
+                                              float* bias) {
+  for (uint32_t c = threadIdx.x; c < TN; c += kThreads) {
+    const bool real = n0 + c < p.channels;
+    scale[c] = real ? p.weight_scale[n0 + c] : 0.0f;
+    bias[c] = real && p.bias ? p.bias[n0 + c] : 0.0f;
+  }
+}
+
+// The sums of the WK parts of a tile's contraction, in its first kWaves waves.
+template <uint32_t kWaves, int WK, int BM, int BN>
+__device__ __forceinline__ void join_parts(int8_t* lds, uint32_t wave, v16i (&acc)[BM][BN]) {
+  constexpr uint32_t kSums = BM * BN * 16 * 64;  // of a wave
+  int* sums = reinterpret_cast<int*>(lds) + lane_id();
+  if (wave >= kWaves) {
 #pragma unroll
-    for (uint32_t i = 0; i < CM; ++i) *reinterpret_cast<v4i*>(to + i * 4096u + swapped) = vq[i];
+    for (int i = 0; i < BM; ++i)
 #pragma unroll
-    for (uint32_t i = 0; i < CN; ++i)
-      *reinterpret_cast<v4i*>(to + TM * 64u + i * 4096u + swapped) = vw[i];
-  };
-  const uint32_t wm = wave / WN * (BM * 32u), wn = wave % WN * (BN * 32u);
-  const uint32_t j = lane & 31u, h = lane >> 5;
-  v16i acc[BM][BN] = {};
-  auto multiply = [&](const int8_t* from) {
+      for (int k = 0; k < BN; ++k)
 #pragma unroll
-    for (uint32_t s = 0; s < 2; ++s) {
-      const uint32_t at = j * 64u + ((2u * s + h) ^ (j >> 1 & 3u)) * 16u;
-      v4i a[BM], b[BN];
+        for (int e = 0; e < 16; ++e)
+          sums[(wave - kWaves) * kSums + ((i * BN + k) * 16 + e) * 64] = acc[i][k][e];
+  }
+  __syncthreads();
+  if (wave < kWaves) {
 #pragma unroll
-      for (int i = 0; i < BM; ++i)
-        a[i] = *reinterpret_cast<const v4i*>(from + (wm + i * 32u) * 64u + at);
-#pragma unroll
-      for (int i = 0; i < BN; ++i)
-        b[i] = *reinterpret_cast<const v4i*>(from + (TM + wn + i * 32u) * 64u + at);
+    for (int g = 0; g < WK - 1; ++g)
 #pragma unroll
       for (int i = 0; i < BM; ++i)
 #pragma unroll
         for (int k = 0; k < BN; ++k)
-          acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[k], acc[i][k], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            acc[i][k][e] += sums[(g * kWaves + wave) * kSums + ((i * BN + k) * 16 + e) * 64];
+  }
+  __syncthreads();
+}
+
+// Rows that start at any byte and end anywhere: pieces come through registers.
+template <typename Out, int WM, int WN, int BM, int BN, uint32_t KB, int WK>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void int8_tile_kernel(Int8Params p,
+                                                                         TilePlan plan) {
+  using T = Tile<WM, WN, BM, BN>;
+  constexpr uint32_t TM = T::kRows, TN = T::kChannels, kThreads = T::kThreads * WK;
+  constexpr uint32_t kPieces = KB / 16u, kAtOnce = kThreads / kPieces;  // rows at a time
+  constexpr uint32_t CM = TM / kAtOnce, CN = TN / kAtOnce;  // pieces a thread brings
+  static_assert(TM % kAtOnce == 0 && TN % kAtOnce == 0 && kAtOnce % 16 == 0, "whole turns");
+  constexpr uint32_t kSet = (TM + TN) * KB, kSlices = T::kWaves * kSliceBytes;
+  static_assert(T::kWaves * (WK - 1) * BM * BN * 4096 <= 2 * kSet, "the sums fit");
+  __shared__ __align__(16) int8_t lds[2 * kSet > kSlices ? 2 * kSet : kSlices];
+  __shared__ __align__(16) float chan_scale[TN], chan_bias[TN];
+  const uint32_t lane = lane_id();
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  uint32_t m0, n0;
+  tile_of(plan, &m0, &n0);
+  m0 *= TM;
+  n0 *= TN;
+  load_channels<kThreads, TN>(p, n0, chan_scale, chan_bias);
+  const uint32_t r0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces * 16u;
+  const uint32_t at = piece_at<KB>(r0, threadIdx.x % kPieces);  // kAtOnce rows on, the same swap
+  const int8_t* pq[CM];
+  const int8_t* pw[CN];
+#pragma unroll
+  for (uint32_t i = 0; i < CM; ++i) {
+    const uint32_t r = m0 + r0 + i * kAtOnce;
+    pq[i] = p.q + (size_t)(r < p.rows ? r : p.rows - 1u) * p.q_ld;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < CN; ++i) {
+    const uint32_t r = n0 + r0 + i * kAtOnce;
+    pw[i] = p.weight + (size_t)(r < p.channels ? r : p.channels - 1u) * p.weight_ld;
+  }
+  v4i vq[CM], vw[CN];
+  auto fetch = [&](uint32_t k) {
+    if (k + KB <= p.cols) {
+#pragma unroll
+      for (uint32_t i = 0; i < CM; ++i) vq[i] = load_whole(pq[i] + k + piece);
+#pragma unroll
+      for (uint32_t i = 0; i < CN; ++i) vw[i] = load_whole(pw[i] + k + piece);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < CM; ++i) vq[i] = load_piece(pq[i], k + piece, p.cols);
+#pragma unroll
+      for (uint32_t i = 0; i < CN; ++i) vw[i] = load_piece(pw[i], k + piece, p.cols);
     }
   };
+  auto keep = [&](int8_t* to) {
+#pragma unroll
+    for (uint32_t i = 0; i < CM; ++i) *reinterpret_cast<v4i*>(to + i * kAtOnce * KB + at) = vq[i];
+#pragma unroll
+    for (uint32_t i = 0; i < CN; ++i)
+      *reinterpret_cast<v4i*>(to + (TM + i * kAtOnce) * KB + at) = vw[i];
+  };
+  const uint32_t wk = wave / T::kWaves, place = wave % T::kWaves;
+  const uint32_t wm = place / WN * (BM * 32u), wn = place % WN * (BN * 32u);
+  float row_scale[BM];
+#pragma unroll
+  for (int i = 0; i < BM; ++i) {
+    const uint32_t m = m0 + wm + i * 32u + (lane & 31u);
+    row_scale[i] = m < p.rows ? p.scale[m] : 0.0f;
+  }
+  v16i acc[BM][BN] = {};
   fetch(0);
-  keep(lds[0]);
+  keep(lds);
   __syncthreads();
   uint32_t set = 0;
-  for (uint32_t k = 64; k < p.cols; k += 64u) {
+  for (uint32_t k = KB; k < p.cols; k += KB) {
     fetch(k);
-    multiply(lds[set]);
-    set ^= 1u;
-    keep(lds[set]);
+    multiply_set<KB, TM, WK>(lds + set, wm, wn, wk, acc);
+    set ^= kSet;
+    keep(lds + set);
     __syncthreads();
   }
-  multiply(lds[set]);
+  multiply_set<KB, TM, WK>(lds + set, wm, wn, wk, acc);
+  __syncthreads();
+  if constexpr (WK > 1) {
+    join_parts<T::kWaves, WK>(lds, wave, acc);
+    if (wk != 0) return;
+  }
+  store_sums<Out>(p, lds + wave * kSliceBytes, chan_scale, chan_bias, m0 + wm, n0, wn, row_scale,
+                  acc);
+}
 
-  // A lane's results are of one channel, 32 lanes' of neighbouring ones: 128 bytes of a
-  // row in 32 bits.  In 16 bits, lanes of two neighbouring channels change a row's
-  // value for another's, so that each stores both channels of one row.
-  typename Out::Raw* out = static_cast<typename Out::Raw*>(p.out);
+// Rows of whole, aligned pieces: they go from memory to LDS by themselves, a wave 1 KB at a
+// time, lane l to the 16 bytes at 16 l.  Those loads are written in assembly, since the
+// compiler would wait for all of them before each read of LDS; every wait for them stands
+// here, before the barrier behind which their set is read.
+__device__ const v4i kZeroPiece = {0, 0, 0, 0};  // what stands behind a row's end
+
+template <typename Out, int WM, int WN, int BM, int BN, uint32_t KB, uint32_t kSets, int WK>
+__global__ __launch_bounds__(64 * WM * WN * WK) void int8_pieces_kernel(Int8Params p, TilePlan plan) {
+  using T = Tile<WM, WN, BM, BN>;
+  constexpr uint32_t TM = T::kRows, TN = T::kChannels, kWaves = T::kWaves * WK;
+  constexpr uint32_t kPieces = KB / 16u;  // of a row
+  constexpr uint32_t kLoads = (TM + TN) * KB / 1024u / kWaves;  // a wave's of a set
+  static_assert((TM + TN) * KB % (1024u * kWaves) == 0, "as many for every wave");
+  constexpr uint32_t kSet = (TM + TN) * KB;
+  static_assert(T::kWaves * kSliceBytes <= kSets * kSet, "the slices fit");
+  __shared__ __align__(16) int8_t lds[kSets * kSet];
+  __shared__ __align__(16) float chan_scale[TN], chan_bias[TN];
+  const uint32_t lane = lane_id();
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  uint32_t m0, n0;
+  tile_of(plan, &m0, &n0);
+  m0 *= TM;
+  n0 *= TN;
+  // load i of the wave brings 1 KB of rows, a lane the piece whose place it has
+  const int8_t* from[kLoads];
+  uint32_t offset[kLoads];
 #pragma unroll
-  for (int k = 0; k < BN; ++k) {
-    const uint32_t n = n0 + wn + k * 32u + j;
-    const bool real = n < p.channels;
-    const float ws = real ? p.weight_scale[n] : 0.0f;
-    const float bias = real && p.bias ? p.bias[n] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < BM; ++i) {
-#pragma unroll
-      for (uint32_t e = 0; e < 16; e += 4) {
-        const uint32_t r = wm + i * 32u + e * 2u + h * 4u;
-        float y[4];
-#pragma unroll
-        for (uint32_t f = 0; f < 4; ++f)
-          y[f] = scaled(acc[i][k][e + f], row_scale[r + f], ws, p.bias, bias);
-        if constexpr (Out::kPer == 4) {
-#pragma unroll
-          for (uint32_t f = 0; f < 4; ++f)
-            if (real && m0 + r + f < p.rows)
-              out[(size_t)(m0 + r + f) * p.out_ld + n] = Out::raw(y[f]);
-        } else {
-          const bool odd = (lane & 1u) != 0;
-#pragma unroll
-          for (uint32_t f = 0; f < 4; f += 2) {
-            const float give = odd ? y[f] : y[f + 1], mine = odd ? y[f + 1] : y[f];
-            const float got = f_of(lane_xor(b_of(give), 1, lane));
-            const uint32_t both = odd ? Out::two(got, mine) : Out::two(mine, got);
-            const uint32_t m = m0 + r + f + (odd ? 1u : 0u), first = n & ~1u;
-            if (m < p.rows && first < p.channels) {
-              typename Out::Raw* to = out + (size_t)m * p.out_ld + first;
-              if (first + 1u < p.channels) *reinterpret_cast<Loose32*>(to) = both;
-              else *to = (typename Out::Raw)both;
-            }
-          }
-        }
-      }
+  for (uint32_t i = 0; i < kLoads; ++i) {
+    const uint32_t row = (wave * kLoads + i) * (64u / kPieces) + lane / kPieces;  // of the tile's rows, then channels
+    offset[i] = piece_at<KB>(row, lane % kPieces) - row * KB;
+    if (row < TM) {
+      const uint32_t r = m0 + row;
+      from[i] = p.q + (size_t)(r < p.rows ? r : p.rows - 1u) * p.q_ld + offset[i];
+    } else {
+      const uint32_t r = n0 + row - TM;
+      from[i] = p.weight + (size_t)(r < p.channels ? r : p.channels - 1u) * p.weight_ld + offset[i];
     }
   }
-}
-
-template <typename Out, int MT, int NT>
-hipError_t few_as(const Int8Params& p, hipStream_t stream) {
-  const uint32_t groups = (p.channels + 16u * NT - 1u) / (16u * NT);
-  const uint32_t steps = (p.cols + 63u) / 64u;
-  uint32_t split = 1;
-  while (split < 8 && groups * split < 4096 && steps / (2 * split) >= 4) split *= 2;
-  const uint32_t waves = split > 4 ? split : 4, own = waves / split;
-  const size_t lds = split > 1 ? (size_t)waves * MT * NT * 1024 : 0;
-  int8_few_kernel<Out, MT, NT><<<(groups + own - 1u) / own, waves * 64u, lds, stream>>>(p, split);
-  return hipGetLastError();
-}
-
-template <typename Out, int WM, int WN, int BM, int BN>
-hipError_t tile_as(const Int8Params& p, hipStream_t stream) {
-  const uint32_t m_tiles = (p.rows + WM * BM * 32u - 1u) / (WM * BM * 32u);
-  const uint32_t n_tiles = (p.channels + WN * BN * 32u - 1u) / (WN * BN * 32u);
-  int8_tile_kernel<Out, WM, WN, BM, BN><<<m_tiles * n_tiles, 256, 0, stream>>>(p, m_tiles, n_tiles);
-  return hipGetLastError();
+  auto bring = [&](int8_t* set, uint32_t step) {
+    const uint32_t k = step * KB;
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const int8_t* at = from[i] + k;
+      if (k + KB > p.cols && k + offset[i] >= p.cols)
+        at = reinterpret_cast<const int8_t*>(&kZeroPiece);
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)(
+          set + (wave * kLoads + i) * 1024u);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to),
+                   "v"(at)
+                   : "memory", "m0");
+    }
+  };
+  const uint32_t steps = (p.cols + KB - 1u) / KB;
+#pragma unroll
+  for (uint32_t i = 0; i + 1u < kSets; ++i)
+    if (i < steps) bring(lds + i * kSet, i);
+  load_channels<64 * kWaves, TN>(p, n0, chan_scale, chan_bias);
+  const uint32_t wk = wave / T::kWaves, place = wave % T::kWaves;
+  const uint32_t wm = place / WN * (BM * 32u), wn = place % WN * (BN * 32u);
+  float row_scale[BM];
+#pragma unroll
+  for (int i = 0; i < BM; ++i) {
+    const uint32_t m = m0 + wm + i * 32u + (lane & 31u);
+    row_scale[i] = m < p.rows ? p.scale[m] : 0.0f;
+  }
+  v16i acc[BM][BN] = {};
+  uint32_t use = 0, next = (kSets - 1u) * kSet;
+  for (uint32_t step = 0; step < steps; ++step) {
+    // This wave's loads of the set are there and its reads of the one before are done; then
+    // everyone's are.  Loads end in their order: those of the kSets - 2 sets behind may go on.
+    if (step + kSets - 1u <= steps)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kSets - 2u) * kLoads)
+                   : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (step + kSets - 1u < steps) bring(lds + next, step + kSets - 1u);
+    multiply_set<KB, TM, WK>(lds + use, wm, wn, wk, acc);
+    next = use;
+    use = use + kSet == kSets * kSet ? 0u : use + kSet;
+  }
+  __syncthreads();
+  if constexpr (WK > 1) {
+    static_assert(T::kWaves * (WK - 1) * BM * BN * 4096 <= kSets * kSet, "the sums fit");
+    join_parts<T::kWaves, WK>(lds, wave, acc);
+    if (wk != 0) return;
+  }
+  store_sums<Out>(p, lds + wave * kSliceBytes, chan_scale, chan_bias, m0 + wm, n0, wn, row_scale,
+                  acc);
 }
 
 template <typename Out>
+hipError_t few_as(const Int8Params& p, hipStream_t stream) {
+  const uint32_t groups = (p.channels + 15u) / 16u, steps = (p.cols + 63u) / 64u;
+  uint32_t split = 1;
+  while (split < kFewWaves && groups * split < 4096 && steps / (2 * split) >= 4) split *= 2;
+  const uint32_t own = kFewWaves / split;
+  int8_few_kernel<Out><<<(groups + own - 1u) / own, 64u * kFewWaves, 0, stream>>>(p, split);
+  return hipGetLastError();
+}
+
+template <typename T>
+TilePlan plan_tiles(const Int8Params& p) {
+  TilePlan t;
+  t.m_tiles = (p.rows + T::kRows - 1u) / T::kRows;
+  t.n_tiles = (p.channels + T::kChannels - 1u) / T::kChannels;
+  const uint32_t fit = (1u << 20) / (T::kRows * p.cols);
+  t.group = fit > 4u ? fit : 4u;
+  if (t.group > t.m_tiles) t.group = t.m_tiles;
+  return t;
+}
+template <typename Out, int WM, int WN, int BM, int BN, uint32_t KB, int WK>
+hipError_t tile_as(const Int8Params& p, hipStream_t stream) {
+  using T = Tile<WM, WN, BM, BN>;
+  const TilePlan t = plan_tiles<T>(p);
+  int8_tile_kernel<Out, WM, WN, BM, BN, KB, WK>
+      <<<t.m_tiles * t.n_tiles, T::kThreads * WK, 0, stream>>>(p, t);
+  return hipGetLastError();
+}
+template <typename Out, int WM, int WN, int BM, int BN, uint32_t KB, uint32_t kSets, int WK>
+hipError_t pieces_as(const Int8Params& p, hipStream_t stream) {
+  using T = Tile<WM, WN, BM, BN>;
+  const TilePlan t = plan_tiles<T>(p);
+  int8_pieces_kernel<Out, WM, WN, BM, BN, KB, kSets, WK>
+      <<<t.m_tiles * t.n_tiles, T::kThreads * WK, 0, stream>>>(p, t);
+  return hipGetLastError();
+}
+
+// Whole pieces: 16 bytes divide the columns, the addresses and the distances of rows.
+bool whole_pieces(const Int8Params& p) {
+  return ((p.cols | p.q_ld | p.weight_ld | (uintptr_t)p.q | (uintptr_t)p.weight) & 15u) == 0;
+}
+
+uint32_t tiles(const Int8Params& p, uint32_t rows, uint32_t channels) {
+  return (p.rows + rows - 1u) / rows * ((p.channels + channels - 1u) / channels);
+}
+
+// Which kernel takes a product (us, both sides of each line; rows x channels x columns).
+//
+// Up to 16 rows of up to 16,384 channels go without LDS tiles, and one or two rows of whole
+// pieces of any channels; few / tiles:
+//   1 x 1,024 x 4,096  4.5 / 9.2     16 x 1,000 x 4,001  12.7 / 16.1     16 x 20,000 x 900   13.6 / 11.5
+//   8 x 4,000 x 2,000  4.1 / 6.5     16 x 8,192 x 8,192  17.2 / 17.5     1 x 50,257 x 1,001  16.5 / 13.8
+//   1 x 151,936 x 896  26 / 28       4 x 151,936 x 896   28.4 / 28.2     8 x 151,936 x 896   31.4 / 28.3
+//
+// Tiles by how many there are for 256 compute units: where tiles of 64 x 64 do not fill
+// them, eight waves a tile, the contraction cut by four; then 64 x 128 tiles, one and two a
+// unit; then 128 x 128, two a unit; and 256 x 256 where their rounds are few enough: a round
+// takes 1.25 to 1.6 times as long as one of 128 x 128 tiles.  Of whole pieces:
+//                            64 x 64, K by 4   64 x 128, K by 2   64 x 128   128 x 128   256 x 256
+//   96 x 8,192 x 8,192                  18.5               24.7       32.5        43.9        96.0
+//   1,000 x 1,000 x 8,192               19.0               25.2       32.9        44.1        98.3
+//   256 x 8,192 x 8,192                 37.8               29.3       35.5        45.1        97.3
+//   512 x 4,096 x 4,096                 22.2               16.6       19.1        25.1        53.1
+//   500 x 5,000 x 896                   14.9               12.3        8.8         9.9        17.6
+//   2,048 x 2,048 x 2,048               26.9               19.0       15.3        16.2        30.3
+//   48 x 151,936 x 896                  58.0                  -       31.0           -           -
+//   1,024 x 8,192 x 8,192              139.6              106.4       97.8        80.6       106.5
+//   333 x 50,257 x 1,008                84.9               58.1       46.8        44.6        50.3
+//   1,000 x 10,000 x 896                46.0               29.6       23.1        23.6        19.2
+// Through registers:
+//   100 x 8,000 x 8,001                 41.4               63.5       86.8       106.8           -
+//   1,000 x 1,000 x 7,001               37.2               56.2       76.9        95.7           -
+//   2,000 x 2,000 x 2,001               35.6               23.9       27.0        31.9           -
+//   8 x 151,936 x 896                   44.6               32.1       28.7           -           -
+//   333 x 50,257 x 1,001                85.3               56.4       56.6        49.1           -
+template <typename Out>
 hipError_t int8_as(const Int8Params& p, hipStream_t stream) {
-  if (p.rows <= 16) return few_as<Out, 1, 1>(p, stream);
-  if (p.rows <= 32) return few_as<Out, 2, 1>(p, stream);
-  if (p.rows <= 48) return few_as<Out, 3, 2>(p, stream);
-  if (p.rows <= 64) return few_as<Out, 4, 2>(p, stream);
-  const uint64_t outputs = (uint64_t)p.rows * p.channels;
-  if (outputs >= (uint64_t)512 * 256 * 128) return tile_as<Out, 2, 2, 4, 2>(p, stream);
-  if (outputs >= (uint64_t)512 * 128 * 128) return tile_as<Out, 2, 2, 2, 2>(p, stream);
-  return tile_as<Out, 2, 2, 1, 1>(p, stream);
+  const bool whole = whole_pieces(p);
+  if (p.rows <= 16 && (p.channels <= 16384 || (p.rows <= 2 && whole)))
+    return few_as<Out>(p, stream);
+  const uint32_t of64 = tiles(p, 64, 64), of128 = tiles(p, 64, 128);
+  const uint32_t rounds = (tiles(p, 128, 128) + 511u) / 512u;
+  if (!whole) {
+    if (of64 <= 256) return tile_as<Out, 2, 1, 1, 2, 256, 4>(p, stream);
+    if (of128 <= 512) return tile_as<Out, 2, 2, 1, 2, 128, 2>(p, stream);
+    if (p.rows <= 64) return tile_as<Out, 2, 2, 1, 2, 64, 1>(p, stream);
+    return tile_as<Out, 2, 2, 2, 2, 64, 1>(p, stream);
+  }
+  if (of64 <= 256) return pieces_as<Out, 2, 1, 1, 2, 256, 4, 4>(p, stream);
+  if (of128 <= 256) return pieces_as<Out, 2, 2, 1, 2, 256, 3, 2>(p, stream);
+  if (of128 <= 512 || p.rows <= 64) return pieces_as<Out, 2, 2, 1, 2, 128, 3, 1>(p, stream);
+  const uint32_t large = (tiles(p, 256, 256) + 255u) / 256u;
+  if (8u * large < 5u * rounds) return pieces_as<Out, 2, 4, 4, 2, 128, 2, 1>(p, stream);
+  return pieces_as<Out, 2, 2, 2, 2, 128, 2, 1>(p, stream);
 }
 
 }  // namespace

@@ -35,12 +35,8 @@ static_assert(kTopThreads == kStatsThreads, "both passes have the same parts");
 // or 0, as the rounding fell.)
 constexpr float kTooBig = 0x1p31f;
 
-// Gradients pass the caches by: kept there, they push out the logits that are
-// still to be read (4,096 x 151,936 bf16 distillation 548 us, so 504).
-template <typename E>
-__device__ __forceinline__ void store_chunk(typename E::Raw* p, const uint4& v) {
-  __builtin_nontemporal_store(Words4{v.x, v.y, v.z, v.w}, reinterpret_cast<Loose4*>(p));
-}
+// Gradients pass the caches by (store_chunk): kept there, they push out the logits that
+// are still to be read (4,096 x 151,936 bf16 distillation 548 us, so 504).
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
