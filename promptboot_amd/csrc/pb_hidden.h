@@ -20,10 +20,12 @@ struct EmbedParams {
   pb_inference_error* err;
 };
 
-// Rows of one workgroup of the sort by token, and rows of one part of a sum.
+// The sort by token: rows that one workgroup sorts, rows of a workgroup of more, bits of a
+// pass.  Rows of one part of a sum.
+constexpr uint32_t kSortRows = 16384;
 constexpr uint32_t kSortTile = 4096;
 constexpr uint32_t kSortBits = 9;
-constexpr uint32_t kSumRows = 32;
+constexpr uint32_t kSumRows = 16;
 
 struct EmbedGradParams {
   const void* grad;
@@ -35,8 +37,9 @@ struct EmbedGradParams {
   void* table;
   size_t table_ld;
   // workspace: two sets of (id, row) pairs that the passes of the sort go between, the
-  // passes' counts [digit][tile], the parts' sums [part][2][cols], and the parts whose
-  // last token goes on in the next one (their number first)
+  // passes' counts [tile][digit], the parts' sums [part][2][cols], and the parts whose last
+  // token goes on in the next one, in two lists: how many each has, then those of fewer parts
+  // from the front and the others from the back
   uint32_t* id[2];
   uint32_t* row[2];
   uint32_t* count;

@@ -158,70 +158,210 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p, uint32_t shif
 // ---- the table's gradient ----
 //
 // The rows are sorted by token (a stable radix sort of (id, row) pairs, kSortBits at a
-// time: counts of a tile's digits, their prefix over digits and tiles, and the pairs'
-// places), so a token's rows come next to each other and in order.  Then the sorted rows
-// are cut into parts of kSumRows: a wave adds up its part's rows token by token, and
-// what lies whole within a part is written at once.  What crosses parts is left in the
-// workspace and joined in 64 bits.  No atomics touch the sums, so they repeat.
+// time), so a token's rows come next to each other and in order.  Then the sorted rows are
+// cut into parts of kSumRows: a wave adds up its part's rows token by token, and what lies
+// whole within a part is written at once.  What crosses parts is left in the workspace and
+// joined in 64 bits.  No atomics touch the sums, so they repeat.
+//
+// Where the whole table is written, its zeros go out beside the sort, from the same
+// launches: the sort keeps one compute unit busy, or a few, and the zeros the others.
+
+constexpr uint32_t kDigits = 1u << kSortBits;
+constexpr uint32_t sum_parts(uint32_t rows) { return (rows + kSumRows - 1u) / kSumRows; }
+// Parts behind its first up to which a token's sum is joined by one wave.
+constexpr uint32_t kLongParts = 32;
 
 // Rows that add nothing sort behind every token.
-__device__ __forceinline__ uint32_t sort_key(const EmbedGradParams& p, uint32_t pass, uint32_t i) {
-  if (pass != 0) return p.id[pass & 1u][i];
+__device__ __forceinline__ uint32_t token_key(const EmbedGradParams& p, uint32_t i) {
   const uint32_t id = p.token[i];
   return id < p.vocab ? id : p.vocab;
 }
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, uint32_t pass) {
+  return key >> (pass * kSortBits) & (kDigits - 1u);
+}
 
+// The lanes of the wave whose digit is this lane's, among those that are `real`.
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, bool real) {
+  uint64_t same = __ballot(real);
+#pragma unroll
+  for (uint32_t b = 0; b < kSortBits; ++b) {
+    const uint64_t set = __ballot(d >> b & 1u);
+    same &= (d >> b & 1u) ? set : ~set;
+  }
+  return same;
+}
+
+// Zeros for the `part`-th of `parts` runs of a table, by kThreads threads.
+template <typename T, uint32_t kThreads>
+__device__ __forceinline__ void zero_part(const EmbedGradParams& p, uint32_t part,
+                                          uint32_t parts) {
+  typename T::Raw* table = static_cast<typename T::Raw*>(p.table);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  if (p.table_ld == p.cols) {  // one run of elements, from 16 aligned bytes on
+    const size_t all = (size_t)p.vocab * p.cols;
+    const size_t odd = (16u - ((uintptr_t)table & 15u)) % 16u / sizeof(typename T::Raw);
+    const size_t head = odd < all ? odd : all, chunks = (all - head) / T::kPer;
+    // workgroups next to each other write next to each other: one window that moves on
+    constexpr uint32_t kTurn = 4u * kThreads;
+    for (size_t c0 = (size_t)part * kTurn; c0 < chunks; c0 += (size_t)parts * kTurn) {
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        const size_t c = c0 + k * kThreads + threadIdx.x;
+        if (c < chunks)
+          *reinterpret_cast<Words4*>(table + head + c * T::kPer) = Words4{0, 0, 0, 0};
+      }
+    }
+    if (part == 0) {
+      const size_t tail = head + chunks * T::kPer;
+      if (threadIdx.x < head) table[threadIdx.x] = 0;
+      if (tail + threadIdx.x < all) table[tail + threadIdx.x] = 0;
+    }
+    return;
+  }
+  const uint32_t from = (uint32_t)((uint64_t)p.vocab * part / parts);
+  const uint32_t to = (uint32_t)((uint64_t)p.vocab * (part + 1u) / parts);
+  const uint32_t wave = threadIdx.x >> 6, lane = lane_id();
+  for (uint32_t v = from + wave; v < to; v += kThreads / 64u) {
+    typename T::Raw* row = table + (size_t)v * p.table_ld;
+    for (uint32_t j = lane * T::kPer; j < p.cols; j += 64u * T::kPer) {
+      if (j + T::kPer <= p.cols) {
+        store_chunk<T>(row + j, zero);
+      } else {
+        for (uint32_t e = j; e < p.cols; ++e) row[e] = 0;
+      }
+    }
+  }
+}
+
+// Up to kSortRows rows: one workgroup sorts them in LDS, the others write zeros.  A pass
+// gives every wave a run of the rows: a row's rank among its wave's rows of its digit, then
+// the prefix over digits and waves.  (16,384 rows by the three launches a pass below took 53
+// us, all of them behind the zeros.)
+constexpr uint32_t kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr uint32_t kSortSteps = kSortRows / kSortThreads;
+template <typename T>
+__global__ __launch_bounds__(kSortThreads) void sort_rows_kernel(EmbedGradParams p,
+                                                                 uint32_t passes) {
+  __shared__ uint32_t key[kSortRows];
+  __shared__ uint16_t order[2][kSortRows];
+  __shared__ uint16_t place[kSortWaves][kDigits];
+  __shared__ uint32_t run[kSortWaves];
+  if (blockIdx.x != 0) {
+    zero_part<T, kSortThreads>(p, blockIdx.x - 1u, gridDim.x - 1u);
+    return;
+  }
+  const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
+  if (threadIdx.x < 2) p.cross[threadIdx.x] = 0;
+  for (uint32_t i = threadIdx.x; i < p.rows; i += kSortThreads) {
+    key[i] = token_key(p, i);
+    order[0][i] = (uint16_t)i;
+  }
+  // the rows in kSortWaves runs of whole steps
+  const uint32_t steps = (p.rows + kSortThreads - 1u) / kSortThreads;
+  const uint32_t first = wave * steps * 64u;
+  for (uint32_t pass = 0; pass < passes; ++pass) {
+    const uint16_t* from = order[pass & 1u];
+    for (uint32_t d = lane; d < kDigits; d += 64u) place[wave][d] = 0;
+    __syncthreads();
+    uint32_t digit[kSortSteps], rank[kSortSteps];
+#pragma unroll
+    for (uint32_t k = 0; k < kSortSteps; ++k) {
+      if (k >= steps) break;
+      const uint32_t i = first + k * 64u + lane;
+      const bool real = i < p.rows;
+      digit[k] = real ? digit_of(key[from[i]], pass) : 0u;
+      const uint64_t same = same_digit(digit[k], real);
+      // a wave's reads and writes of LDS keep their order; other waves have other rows
+      volatile uint16_t* seen = &place[wave][digit[k]];
+      const uint32_t before = real ? *seen : 0u;
+      rank[k] = before + lanes_below(same);
+      if (real && lanes_below(same) == 0)
+        *seen = (uint16_t)(before + (uint32_t)__popcll((unsigned long long)same));
+    }
+    __syncthreads();
+    // exclusive prefix over digits, within a digit over waves
+    uint32_t sum = 0;
+    if (threadIdx.x < kDigits) {
+#pragma unroll
+      for (uint32_t w = 0; w < kSortWaves; ++w) sum += place[w][threadIdx.x];
+    }
+    uint32_t upto = sum;
+#pragma unroll
+    for (uint32_t m = 1; m < 64; m <<= 1) {
+      const uint32_t o = (uint32_t)__shfl_up((int)upto, m, 64);
+      if (lane >= m) upto += o;
+    }
+    if (lane == 63) run[wave] = upto;
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+      uint32_t base = upto - sum;
+      for (uint32_t w = 0; w < wave; ++w) base += run[w];
+#pragma unroll
+      for (uint32_t w = 0; w < kSortWaves; ++w) {
+        const uint32_t n = place[w][threadIdx.x];
+        place[w][threadIdx.x] = (uint16_t)base;
+        base += n;
+      }
+    }
+    __syncthreads();
+    uint16_t* to = order[(pass + 1u) & 1u];
+#pragma unroll
+    for (uint32_t k = 0; k < kSortSteps; ++k) {
+      if (k >= steps) break;
+      const uint32_t i = first + k * 64u + lane;
+      if (i < p.rows) to[place[wave][digit[k]] + rank[k]] = from[i];
+    }
+    __syncthreads();
+  }
+  for (uint32_t i = threadIdx.x; i < p.rows; i += kSortThreads) {
+    const uint32_t r = order[passes & 1u][i];
+    p.id[passes & 1u][i] = key[r];
+    p.row[passes & 1u][i] = r;
+  }
+}
+
+// More rows: two launches a pass, the rows in tiles of kSortTile: counts of a tile's digits,
+// then the pairs' places, for which every tile adds up all counts.  The workgroups behind the
+// tiles' write the launch's share of the zeros.
+__device__ __forceinline__ uint32_t sort_key(const EmbedGradParams& p, uint32_t pass, uint32_t i) {
+  return pass != 0 ? p.id[pass & 1u][i] : token_key(p, i);
+}
+struct ZeroShare {
+  uint32_t part, parts;  // of all launches' workgroups: this launch's first, and how many
+};
+
+template <typename T>
 __global__ __launch_bounds__(256) void sort_count_kernel(EmbedGradParams p, uint32_t pass,
-                                                         uint32_t tiles) {
-  __shared__ uint32_t hist[1u << kSortBits];
+                                                         uint32_t tiles, ZeroShare zero) {
+  __shared__ uint32_t hist[kDigits];
   const uint32_t tile = blockIdx.x;
-  for (uint32_t d = threadIdx.x; d < (1u << kSortBits); d += 256u) hist[d] = 0;
-  if (pass == 0 && tile == 0 && threadIdx.x == 0) p.cross[0] = 0;
+  if (tile >= tiles) {
+    zero_part<T, 256>(p, zero.part + tile - tiles, zero.parts);
+    return;
+  }
+  for (uint32_t d = threadIdx.x; d < kDigits; d += 256u) hist[d] = 0;
+  if (pass == 0 && tile == 0 && threadIdx.x < 2) p.cross[threadIdx.x] = 0;
   __syncthreads();
   for (uint32_t k = 0; k < kSortTile / 256u; ++k) {
     const uint32_t i = tile * kSortTile + k * 256u + threadIdx.x;
-    if (i < p.rows) {
-      const uint32_t d = sort_key(p, pass, i) >> (pass * kSortBits) & ((1u << kSortBits) - 1u);
-      atomicAdd(&hist[d], 1u);
-    }
+    if (i < p.rows) atomicAdd(&hist[digit_of(sort_key(p, pass, i), pass)], 1u);
   }
   __syncthreads();
-  for (uint32_t d = threadIdx.x; d < (1u << kSortBits); d += 256u)
-    p.count[(size_t)d * tiles + tile] = hist[d];
+  for (uint32_t d = threadIdx.x; d < kDigits; d += 256u)
+    p.count[(size_t)tile * kDigits + d] = hist[d];
 }
 
-// Exclusive prefix of the counts, digit by digit and tile by tile, by one workgroup.
-__global__ __launch_bounds__(1024) void sort_prefix_kernel(uint32_t* count, uint32_t n) {
-  __shared__ uint32_t waves[16];
-  const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
-  const uint32_t per = (n + 1023u) / 1024u;
-  const uint32_t lo = threadIdx.x * per < n ? threadIdx.x * per : n;
-  const uint32_t hi = lo + per < n ? lo + per : n;
-  uint32_t sum = 0;
-  for (uint32_t i = lo; i < hi; ++i) sum += count[i];
-  uint32_t upto = sum;  // inclusive over the wave's lanes
-#pragma unroll
-  for (uint32_t m = 1; m < 64; m <<= 1) {
-    const uint32_t o = (uint32_t)__shfl_up((int)upto, m, 64);
-    if (lane >= m) upto += o;
-  }
-  if (lane == 63) waves[wave] = upto;
-  __syncthreads();
-  uint32_t base = upto - sum;
-  for (uint32_t w = 0; w < wave; ++w) base += waves[w];
-  for (uint32_t i = lo; i < hi; ++i) {
-    const uint32_t c = count[i];
-    count[i] = base;
-    base += c;
-  }
-}
-
+template <typename T>
 __global__ __launch_bounds__(256) void sort_place_kernel(EmbedGradParams p, uint32_t pass,
-                                                         uint32_t tiles) {
+                                                         uint32_t tiles, ZeroShare zero) {
   constexpr uint32_t kSteps = kSortTile / 256u;
-  __shared__ uint32_t place[4][1u << kSortBits];
+  __shared__ uint32_t place[4][kDigits];
   const uint32_t tile = blockIdx.x, lane = lane_id(), wave = threadIdx.x >> 6;
-  for (uint32_t d = threadIdx.x; d < 4u << kSortBits; d += 256u) (&place[0][0])[d] = 0;
+  if (tile >= tiles) {
+    zero_part<T, 256>(p, zero.part + tile - tiles, zero.parts);
+    return;
+  }
+  for (uint32_t d = threadIdx.x; d < 4u * kDigits; d += 256u) (&place[0][0])[d] = 0;
   __syncthreads();
   // a wave's rows in order, 64 at a time; a row's rank among the wave's rows of its digit
   const uint32_t first = tile * kSortTile + wave * (kSortTile / 4u);
@@ -234,31 +374,54 @@ __global__ __launch_bounds__(256) void sort_place_kernel(EmbedGradParams p, uint
 #pragma unroll
   for (uint32_t k = 0; k < kSteps; ++k) {
     const bool real = first + k * 64u + lane < p.rows;
-    const uint32_t d = key[k] >> (pass * kSortBits) & ((1u << kSortBits) - 1u);
-    uint64_t same = __ballot(real);
-#pragma unroll
-    for (uint32_t b = 0; b < kSortBits; ++b) {
-      const uint64_t set = __ballot(d >> b & 1u);
-      same &= (d >> b & 1u) ? set : ~set;
-    }
-    rank[k] = 0;
-    if (real) {
-      const uint32_t below = lanes_below(same);
-      uint32_t before = 0;
-      if (below == 0)
-        before = atomicAdd(&place[wave][d], (uint32_t)__popcll((unsigned long long)same));
-      const int leader = __ffsll((unsigned long long)same) - 1;
-      rank[k] = (uint32_t)__shfl((int)before, leader, 64) + below;
-    }
+    const uint64_t same = same_digit(digit_of(key[k], pass), real);
+    // a wave's reads and writes of LDS keep their order; other waves have other rows
+    volatile uint32_t* seen = &place[wave][digit_of(key[k], pass)];
+    const uint32_t before = real ? *seen : 0u;
+    rank[k] = before + lanes_below(same);
+    if (real && lanes_below(same) == 0)
+      *seen = before + (uint32_t)__popcll((unsigned long long)same);
   }
   __syncthreads();
-  for (uint32_t d = threadIdx.x; d < (1u << kSortBits); d += 256u) {
-    uint32_t base = p.count[(size_t)d * tiles + tile];
+  // where the tile's rows of a digit go: behind all rows of lower digits and those of the
+  // digit in earlier tiles.  A thread has two neighbouring digits.
+  static_assert(kDigits == 512, "two digits a thread");
+  const uint32_t d0 = 2u * threadIdx.x;
+  uint2 all = make_uint2(0, 0), before = make_uint2(0, 0);
+#pragma unroll 8
+  for (uint32_t t = 0; t < tiles; ++t) {
+    const uint2 c = *reinterpret_cast<const uint2*>(p.count + (size_t)t * kDigits + d0);
+    all.x += c.x;
+    all.y += c.y;
+    if (t < tile) {
+      before.x += c.x;
+      before.y += c.y;
+    }
+  }
+  uint32_t upto = all.x + all.y;  // inclusive over the wave's lanes
+#pragma unroll
+  for (uint32_t m = 1; m < 64; m <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)upto, m, 64);
+    if (lane >= m) upto += o;
+  }
+  __shared__ uint32_t run[4];
+  if (lane == 63) run[wave] = upto;
+  __syncthreads();
+  uint32_t base[2] = {upto - all.x - all.y, upto - all.y};
+#pragma unroll
+  for (uint32_t w = 0; w < 3; ++w) {
+    base[0] += w < wave ? run[w] : 0u;
+    base[1] += w < wave ? run[w] : 0u;
+  }
+  base[0] += before.x;
+  base[1] += before.y;
+#pragma unroll
+  for (uint32_t k = 0; k < 2; ++k) {
 #pragma unroll
     for (uint32_t w = 0; w < 4; ++w) {
-      const uint32_t n = place[w][d];
-      place[w][d] = base;
-      base += n;
+      const uint32_t n = place[w][d0 + k];
+      place[w][d0 + k] = base[k];
+      base[k] += n;
     }
   }
   __syncthreads();
@@ -268,25 +431,17 @@ __global__ __launch_bounds__(256) void sort_place_kernel(EmbedGradParams p, uint
   for (uint32_t k = 0; k < kSteps; ++k) {
     const uint32_t i = first + k * 64u + lane;
     if (i < p.rows) {
-      const uint32_t d = key[k] >> (pass * kSortBits) & ((1u << kSortBits) - 1u);
-      const uint32_t at = place[wave][d] + rank[k];
+      const uint32_t at = place[wave][digit_of(key[k], pass)] + rank[k];
       id[at] = key[k];
       row[at] = pass == 0 ? i : p.row[pass & 1u][i];
     }
   }
 }
 
-// Zeros for a whole table, 2^shift threads a row.
+// Zeros alone: a gradient without rows.
 template <typename T>
-__global__ __launch_bounds__(256) void zero_rows_kernel(typename T::Raw* table, size_t ld,
-                                                        uint32_t rows, uint32_t cols,
-                                                        uint32_t shift) {
-  const uint32_t row = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
-  if (row >= rows) return;
-  typename T::Raw* to = table + (size_t)row * ld;
-  const float zero[kChunk] = {};
-  for (uint32_t j = (threadIdx.x & ((1u << shift) - 1u)) * kChunk; j < cols; j += kChunk << shift)
-    store_row<T>(to + j, cols - j, zero);
+__global__ __launch_bounds__(256) void zero_table_kernel(EmbedGradParams p) {
+  zero_part<T, 256>(p, blockIdx.x, gridDim.x);
 }
 
 template <typename T, int N>
@@ -305,27 +460,45 @@ __device__ __forceinline__ void put_table(const EmbedGradParams& p, uint32_t id,
   store_row<T>(to, n, y);
 }
 
-// One wave: the sorted rows [part kSumRows, + kSumRows) and 64 chunks of columns.
+// One wave: the sorted rows [part kSumRows, + kSumRows) and 64 chunks of columns.  All of the
+// part's rows are requested before the first is added.
 template <typename G, typename T>
 __global__ __launch_bounds__(256) void sum_rows_kernel(EmbedGradParams p, uint32_t last,
                                                        uint32_t col_tiles, uint32_t units) {
   constexpr int N = G::kPer;
-  constexpr uint32_t kAhead = 8;
-  static_assert(kSumRows % kAhead == 0, "whole groups");
   const uint32_t unit =
       (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4u + (threadIdx.x >> 6)));
   if (unit >= units) return;
-  const uint32_t part = unit / col_tiles, tile = unit - part * col_tiles;
-  const uint32_t j = (tile * 64u + lane_id()) * N;
-  const uint32_t n = chunk_left(p.cols, j);
-  const uint32_t* id = p.id[last];
-  const uint32_t* row = p.row[last];
-  const typename G::Raw* grad = static_cast<const typename G::Raw*>(p.grad) + j;
+  const uint32_t part = unit / col_tiles, tile = unit - part * col_tiles, lane = lane_id();
+  const uint32_t j = (tile * 64u + lane) * N, n = chunk_left(p.cols, j);
   const uint32_t lo = part * kSumRows;
   const uint32_t hi = lo + kSumRows < p.rows ? lo + kSumRows : p.rows;
-  uint32_t cur = id[lo];
+  // the part's ids, with the one before and the one behind it: lane k has sorted row lo - 1 + k
+  static_assert(kSumRows + 2 <= 64, "a lane each");
+  const uint32_t at = lo + lane;  // + 1
+  const bool inside = at >= 1u && at <= p.rows && lane < kSumRows + 2u;
+  const uint32_t my_id = inside ? p.id[last][at - 1u] : kNone;
+  const uint32_t my_row = inside ? p.row[last][at - 1u] : 0u;
+  const typename G::Raw* grad = static_cast<const typename G::Raw*>(p.grad) + j;
+  uint4 x[kSumRows];
+#pragma unroll
+  for (uint32_t k = 0; k < kSumRows; ++k) {
+    const uint32_t row = bcast32(my_row, k + 1u);
+    x[k] = make_uint4(0, 0, 0, 0);
+    if (lo + k < hi && bcast32(my_id, k + 1u) < p.vocab) {
+      const typename G::Raw* from = grad + (size_t)row * p.grad_ld;
+      if (n >= (uint32_t)N) {
+        x[k] = load_chunk<G>(from);
+      } else if (n != 0) {
+        float y[N];
+        load_row<G>(from, n, y);
+        x[k] = G::pack(y);
+      }
+    }
+  }
+  uint32_t cur = bcast32(my_id, 1u);
   if (cur >= p.vocab) return;
-  bool from_before = lo > 0 && id[lo - 1] == cur;  // the sum goes on from the part before
+  bool from_before = lo > 0 && bcast32(my_id, 0u) == cur;  // the sum goes on from the part before
   float sum[N] = {};
   auto leave = [&](bool goes_on) {
     if (!from_before && !goes_on) {
@@ -333,71 +506,102 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(EmbedGradParams p, uint32
     } else {
       float* to = p.part + ((size_t)part * 2u + (from_before ? 0u : 1u)) * p.cols + j;
       store_row<F32>(reinterpret_cast<uint32_t*>(to), n, sum);
-      if (!from_before && tile == 0 && lane_id() == 0) p.cross[1u + atomicAdd(p.cross, 1u)] = part;
+      if (!from_before && tile == 0 && lane == 0) {
+        // in whose place of which list does not matter: each is joined by itself
+        const uint32_t far = hi - 1u + kLongParts * kSumRows;
+        if (far < p.rows && p.id[last][far] == cur)
+          p.cross[1u + sum_parts(p.rows) - atomicAdd(p.cross + 1, 1u)] = part;
+        else
+          p.cross[2u + atomicAdd(p.cross, 1u)] = part;
+      }
     }
   };
-  for (uint32_t i = lo; i < hi; i += kAhead) {
-    uint32_t ids[kAhead], rows[kAhead];
-    float x[kAhead][N];
-#pragma unroll
-    for (uint32_t k = 0; k < kAhead; ++k) {
-      const uint32_t at = i + k < hi ? i + k : hi - 1u;
-      ids[k] = (uint32_t)__builtin_amdgcn_readfirstlane((int)id[at]);
-      rows[k] = (uint32_t)__builtin_amdgcn_readfirstlane((int)row[at]);
-    }
-#pragma unroll
-    for (uint32_t k = 0; k < kAhead; ++k) load_row<G>(grad + (size_t)rows[k] * p.grad_ld, n, x[k]);
-#pragma unroll
-    for (uint32_t k = 0; k < kAhead; ++k) {
-      if (i + k >= hi) break;
-      if (ids[k] != cur) {
+#pragma clang loop unroll(full)
+  for (uint32_t k = 0; k < kSumRows; ++k) {
+    const uint32_t id = bcast32(my_id, k + 1u);
+    if (lo + k < hi && cur < p.vocab) {
+      if (id != cur) {
         leave(false);
-        cur = ids[k];
+        cur = id;
         from_before = false;
-        if (cur >= p.vocab) return;
 #pragma unroll
         for (int e = 0; e < N; ++e) sum[e] = 0.0f;
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum[e] = sum[e] + x[k][e];
+      for (int e = 0; e < N; ++e) sum[e] = sum[e] + G::get(x[k], e);
     }
   }
-  leave(hi < p.rows && id[hi] == cur);
+  if (cur < p.vocab) leave(hi < p.rows && bcast32(my_id, kSumRows + 1u) == cur);
 }
 
-// The sums that cross parts, 64 columns a workgroup: its waves take a run of parts each.
+// The first sorted row from `lo` on whose token is another: 64 places at a time.
+__device__ __forceinline__ uint32_t token_end(const uint32_t* id, uint32_t own, uint32_t lo,
+                                              uint32_t hi) {
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 63u) / 64u, at = lo + lane_id() * step;
+    const uint64_t not_own = __ballot(at >= hi || id[at] != own);
+    const uint32_t k = not_own ? (uint32_t)__ffsll((unsigned long long)not_own) - 1u : 64u;
+    const uint32_t end = lo + k * step;  // its place is behind the token's rows, or at hi
+    lo = k == 0 ? lo : end - step + 1u;
+    hi = end < hi ? end : hi;
+  }
+  return lo;
+}
+
+// The sums that cross parts.  A wave takes 256 columns of a token of up to kLongParts more
+// parts; a workgroup 64 columns of a longer one, its waves a run of parts each.
+constexpr uint32_t kJoinWaves = 16;
 template <typename T>
-__global__ __launch_bounds__(256) void join_rows_kernel(EmbedGradParams p, uint32_t last,
-                                                        uint32_t col_tiles) {
-  __shared__ double waves[4][64];
-  const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(EmbedGradParams p,
+                                                                    uint32_t last) {
+  __shared__ double waves[kJoinWaves][64];
+  const uint32_t lane = lane_id();
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t* id = p.id[last];
-  const uint32_t crossing = p.cross[0];
-  for (size_t unit = blockIdx.x; unit < (size_t)crossing * col_tiles; unit += gridDim.x) {
-    const uint32_t part = p.cross[1u + unit / col_tiles];
-    const uint32_t j = (uint32_t)(unit % col_tiles) * 64u + lane;
-    const uint32_t own = id[(part + 1u) * kSumRows - 1u];
-    // the first sorted row behind the token's last
-    uint32_t lo = (part + 1u) * kSumRows, hi = p.rows;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2u;
-      if (id[mid] == own) lo = mid + 1u;
-      else hi = mid;
+  const uint32_t few = p.cross[0], many = p.cross[1];
+  const uint32_t wide = (p.cols + 255u) / 256u, narrow = (p.cols + 63u) / 64u;
+  for (size_t unit = (size_t)blockIdx.x * kJoinWaves + wave; unit < (size_t)few * wide;
+       unit += (size_t)gridDim.x * kJoinWaves) {
+    const uint32_t part = p.cross[2u + unit / wide];
+    const uint32_t j = ((uint32_t)(unit % wide) * 64u + lane) * 4u, n = chunk_left(p.cols, j);
+    const uint32_t next = (part + 1u) * kSumRows, own = id[next - 1u];
+    const uint32_t most = next + kLongParts * kSumRows;
+    const uint32_t to = (token_end(id, own, next, most < p.rows ? most : p.rows) - 1u) / kSumRows;
+    float x[4];
+    load_row<F32, 4>(reinterpret_cast<const uint32_t*>(p.part + ((size_t)part * 2u + 1u) * p.cols + j),
+                     n, x);
+    double sum[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll 8
+    for (uint32_t k = part + 1u; k <= to; ++k) {
+      load_row<F32, 4>(reinterpret_cast<const uint32_t*>(p.part + (size_t)k * 2u * p.cols + j), n,
+                       x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = sum[e] + (double)x[e];
     }
-    const uint32_t n = (lo - 1u) / kSumRows - part + 1u;  // parts, the first one's tail included
-    const uint32_t from = (uint32_t)((uint64_t)n * wave / 4u);
-    const uint32_t to = (uint32_t)((uint64_t)n * (wave + 1u) / 4u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (float)sum[e];
+    put_table<T>(p, own, j, n, x);
+  }
+  for (size_t unit = blockIdx.x; unit < (size_t)many * narrow; unit += gridDim.x) {
+    const uint32_t part = p.cross[1u + sum_parts(p.rows) - (uint32_t)(unit / narrow)];
+    const uint32_t j = (uint32_t)(unit % narrow) * 64u + lane;
+    const uint32_t next = (part + 1u) * kSumRows, own = id[next - 1u];
+    const uint32_t n = (token_end(id, own, next, p.rows) - 1u) / kSumRows - part + 1u;
+    const uint32_t from = (uint32_t)((uint64_t)n * wave / kJoinWaves);
+    const uint32_t to = (uint32_t)((uint64_t)n * (wave + 1u) / kJoinWaves);
     double sum = 0.0;
-    if (j < p.cols)
+    if (j < p.cols) {
+#pragma unroll 8
       for (uint32_t k = from; k < to; ++k)
         sum = sum + (double)p.part[((size_t)(part + k) * 2u + (k == 0 ? 1u : 0u)) * p.cols + j];
+    }
     waves[wave][lane] = sum;
     __syncthreads();
     if (wave == 0 && j < p.cols) {
-      const float all[1] = {
-          (float)(((waves[0][lane] + waves[1][lane]) + waves[2][lane]) + waves[3][lane])};
+#pragma unroll
+      for (uint32_t w = 1; w < kJoinWaves; ++w) sum = sum + waves[w][lane];
+      const float y = p.scale * (float)sum;
       typename T::Raw* at = static_cast<typename T::Raw*>(p.table) + (size_t)own * p.table_ld + j;
-      const float y = all[0] * p.scale;
       *at = T::raw(p.accumulate ? T::one(*at) + y : y);
     }
     __syncthreads();
@@ -707,7 +911,6 @@ uint32_t row_shift(uint32_t cols) {
 }
 
 uint32_t sort_tiles(uint32_t rows) { return (rows + kSortTile - 1u) / kSortTile; }
-uint32_t sum_parts(uint32_t rows) { return (rows + kSumRows - 1u) / kSumRows; }
 
 // Workgroups of the norm's gradient, each with at most kMaxTerms rows a thread.
 constexpr uint32_t kGradGroups = 512;
@@ -773,39 +976,45 @@ hipError_t embed_from(const EmbedParams& p, uint32_t out_dtype, hipStream_t stre
   return embed_as<In, BF16>(p, stream);
 }
 
-template <typename T>
-hipError_t zero_table(const EmbedGradParams& p, hipStream_t stream) {
-  const uint32_t shift = row_shift(p.cols), at_once = 256u >> shift;
-  zero_rows_kernel<T><<<(p.vocab + at_once - 1u) / at_once, 256, 0, stream>>>(
-      static_cast<typename T::Raw*>(p.table), p.table_ld, p.vocab, p.cols, shift);
-  return hipGetLastError();
-}
+// Workgroups that write zeros beside a sort: four a compute unit, of 256 threads.
+constexpr uint32_t kZeroGroups = 1024;
 
 template <typename G, typename T>
 hipError_t embed_grad_as(const EmbedGradParams& p, hipStream_t stream) {
   hipError_t e = hipSuccess;
-  if (!p.accumulate && (e = zero_table<T>(p, stream)) != hipSuccess) return e;
-  if (p.rows == 0) return e;
-  const uint32_t tiles = sort_tiles(p.rows);
+  if (p.rows == 0) {
+    if (!p.accumulate) {
+      zero_table_kernel<T><<<kZeroGroups, 256, 0, stream>>>(p);
+      e = hipGetLastError();
+    }
+    return e;
+  }
   uint32_t bits = 0;
   while (p.vocab >> bits) ++bits;
   const uint32_t passes = (bits + kSortBits - 1u) / kSortBits;
-  for (uint32_t pass = 0; pass < passes; ++pass) {
-    sort_count_kernel<<<tiles, 256, 0, stream>>>(p, pass, tiles);
+  if (p.rows <= kSortRows) {
+    sort_rows_kernel<T><<<p.accumulate ? 1 : 256, kSortThreads, 0, stream>>>(p, passes);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    sort_prefix_kernel<<<1, 1024, 0, stream>>>(p.count, tiles << kSortBits);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    sort_place_kernel<<<tiles, 256, 0, stream>>>(p, pass, tiles);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
+  } else {
+    const uint32_t tiles = sort_tiles(p.rows), groups = p.accumulate ? 0 : kZeroGroups;
+    ZeroShare zero{0, 2u * passes * groups};
+    for (uint32_t pass = 0; pass < passes; ++pass) {
+      sort_count_kernel<T><<<tiles + groups, 256, 0, stream>>>(p, pass, tiles, zero);
+      zero.part += groups;
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      sort_place_kernel<T><<<tiles + groups, 256, 0, stream>>>(p, pass, tiles, zero);
+      zero.part += groups;
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
   }
   const uint32_t last = passes & 1u;
   const uint32_t col_tiles = (p.cols + 64u * G::kPer - 1u) / (64u * G::kPer);
   const uint32_t units = sum_parts(p.rows) * col_tiles;
   sum_rows_kernel<G, T><<<(units + 3u) / 4u, 256, 0, stream>>>(p, last, col_tiles, units);
   if ((e = hipGetLastError()) != hipSuccess || p.rows <= kSumRows) return e;
-  const uint32_t join_tiles = (p.cols + 63u) / 64u;
-  const size_t most = (size_t)(sum_parts(p.rows) - 1u) * join_tiles;
-  join_rows_kernel<T><<<(uint32_t)(most < 1024 ? most : 1024), 256, 0, stream>>>(p, last, join_tiles);
+  const size_t most = (size_t)(sum_parts(p.rows) - 1u) * ((p.cols + 63u) / 64u);
+  join_rows_kernel<T>
+      <<<(uint32_t)(most < 512 ? most : 512), 64 * kJoinWaves, 0, stream>>>(p, last);
   return hipGetLastError();
 }
 template <typename G>
@@ -820,7 +1029,7 @@ hipError_t embed_grad_from(const EmbedGradParams& p, uint32_t table_dtype, hipSt
 size_t embed_grad_bytes(uint32_t rows, size_t cols) {
   const size_t tiles = sort_tiles(rows), parts = sum_parts(rows);
   return 4 * round_up((size_t)rows * 4) + round_up((tiles << kSortBits) * 4) +
-         round_up((parts + 1) * 4) + round_up(parts * 2 * cols * 4);
+         round_up((parts + 2) * 4) + round_up(parts * 2 * cols * 4);
 }
 
 size_t norm_grad_bytes(uint32_t rows, size_t cols) {
@@ -845,7 +1054,7 @@ void place_embed_grad(void* work, EmbedGradParams* p) {
     p->row[k] = reinterpret_cast<uint32_t*>(take(words));
   }
   p->count = reinterpret_cast<uint32_t*>(take(((size_t)sort_tiles(p->rows) << kSortBits) * 4));
-  p->cross = reinterpret_cast<uint32_t*>(take(((size_t)sum_parts(p->rows) + 1) * 4));
+  p->cross = reinterpret_cast<uint32_t*>(take(((size_t)sum_parts(p->rows) + 2) * 4));
   p->part = reinterpret_cast<float*>(at);
 }
 
