@@ -120,7 +120,6 @@ __device__ __forceinline__ double wave_add(double v) {
     v = v + __builtin_bit_cast(double, shfl_xor64(__builtin_bit_cast(uint64_t, v), m));
   return v;
 }
-__device__ __forceinline__ uint64_t wave_max_word(uint64_t v) { return wave_max64(v); }
 
 // ---- table rows of tokens ----
 
@@ -610,9 +609,51 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(EmbedGradPar
 
 // ---- norms ----
 //
-// A row is held in registers between its statistics and its outputs: T threads take C
-// chunks of eight elements each.  mean(h^2) is summed in 64 bits: no binary32 row
-// overflows there, and 64-bit multiply-adds issue as often as 32-bit ones here.
+// A row is held in registers between its statistics and its outputs, as it is in memory: T
+// threads take C chunks of eight elements each.  mean(h^2) is summed in 64 bits: no
+// binary32 row overflows there, and a 64-bit multiply-add issues as fast as a 32-bit
+// product and its addition would.
+
+// Eight elements as they are in memory.
+template <typename E>
+struct Chunk {
+  static constexpr int kWords = kChunk / E::kPer;
+  uint4 v[kWords];
+  __device__ __forceinline__ float get(uint32_t e) const {
+    return E::get(v[e / E::kPer], (int)(e % E::kPer));
+  }
+  __device__ __forceinline__ void set(const float (&x)[kChunk]) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      float y[E::kPer];
+#pragma unroll
+      for (int e = 0; e < E::kPer; ++e) y[e] = x[k * E::kPer + e];
+      v[k] = E::pack(y);
+    }
+  }
+  // The first n from `p`, zeros behind them.
+  __device__ __forceinline__ void load(const typename E::Raw* p, uint32_t n) {
+    if (n >= kChunk) {
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) v[k] = load_chunk<E>(p + k * E::kPer);
+    } else {
+      float x[kChunk];
+      load_row<E>(p, n, x);
+      set(x);
+    }
+  }
+  __device__ __forceinline__ void store(typename E::Raw* p, uint32_t n) const {
+    if (n >= kChunk) {
+#pragma unroll
+      for (int k = 0; k < kWords; ++k)
+        *reinterpret_cast<Loose4*>(p + k * E::kPer) = Words4{v[k].x, v[k].y, v[k].z, v[k].w};
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < kChunk; ++e)
+        if (e < n) p[e] = E::raw(get(e));
+    }
+  }
+};
 
 // w of a chunk, ones without a weight.
 __device__ __forceinline__ void load_weight(const void* weight, uint32_t dtype, uint32_t j,
@@ -624,29 +665,58 @@ __device__ __forceinline__ void load_weight(const void* weight, uint32_t dtype, 
     load_any(weight, dtype, j, n, w);
   }
 }
-
-// Sums of `a` and maxima of `m` over a row's T threads, in every one of them.
-template <int T>
-__device__ __forceinline__ void row_reduce(double& a, uint64_t& m) {
-  a = wave_add(a);
-  m = wave_max_word(m);
-  if constexpr (T > 64) {
-    __shared__ double as[T / 64];
-    __shared__ uint64_t ms[T / 64];
-    __syncthreads();
-    if (lane_id() == 0) {
-      as[threadIdx.x >> 6] = a;
-      ms[threadIdx.x >> 6] = m;
-    }
-    __syncthreads();
-    a = as[0];
-    m = ms[0];
-#pragma unroll
-    for (int w = 1; w < T / 64; ++w) {
-      a = a + as[w];
-      m = ms[w] > m ? ms[w] : m;
-    }
+template <typename E>
+__device__ __forceinline__ void load_weight(const void* weight, uint32_t j, uint32_t n,
+                                            Chunk<E>& w) {
+  if (weight == nullptr) {
+    const float ones[kChunk] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+    w.set(ones);
+  } else {
+    w.load(static_cast<const typename E::Raw*>(weight) + j, n);
   }
+}
+
+// What is reduced over a row's T threads, in every one of them.
+template <int T, typename V, typename Join>
+__device__ __forceinline__ V row_join(V v, Join join) {
+  if constexpr (T > 64) {
+    __shared__ V waves[T / 64];
+    __syncthreads();
+    if (lane_id() == 0) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = waves[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) v = join(v, waves[w]);
+  }
+  return v;
+}
+struct Stats {
+  double sum;
+  uint64_t top;
+};
+template <int T>
+__device__ __forceinline__ Stats row_stats(double sum, uint64_t top) {
+  return row_join<T>(Stats{wave_add(sum), wave_max64(top)}, [](const Stats& a, const Stats& b) {
+    return Stats{a.sum + b.sum, a.top > b.top ? a.top : b.top};
+  });
+}
+struct Stats32 {
+  double sum;
+  uint32_t top;
+};
+template <int T>
+__device__ __forceinline__ Stats32 row_stats(double sum, uint32_t top) {
+  const uint32_t lane = lane_id();
+  auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  top = larger(top, lane_xor(top, 32, lane));
+  top = larger(top, lane_xor(top, 16, lane));
+  top = larger(top, lane_xor(top, 8, lane));
+  top = larger(top, lane_xor(top, 4, lane));
+  top = larger(top, lane_xor(top, 2, lane));
+  top = larger(top, lane_xor(top, 1, lane));
+  return row_join<T>(Stats32{wave_add(sum), top}, [](const Stats32& a, const Stats32& b) {
+    return Stats32{a.sum + b.sum, a.top > b.top ? a.top : b.top};
+  });
 }
 
 __device__ __forceinline__ uint64_t abs_bits(double v) {
@@ -671,63 +741,112 @@ __device__ __forceinline__ int nearest_step(double p, double top, double step) {
   const int whole = (int)t;
   return p < 0.0 ? -whole : whole;
 }
+__device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t low = __builtin_amdgcn_perm(b, a, 0x0c0c0400u);
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), low, 0x05040100u);
+}
 
-template <typename E, int T, int C>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(NormParams p) {
-  constexpr uint32_t kRows = T < 256 ? 256 / T : 1;
+// kNarrow: rows and weight of one 16-bit type, or no weight.  Their products h w are exact in
+// binary32, so the largest is, and all but values near a half are rounded in 32 bits:
+// p (127 / top) is off by 2^-24 of 127 there, and those that come nearer than 2^-15 to a half
+// go the exact way.  Rows whose largest product binary32 does not hold well (2^-60 to 2^120)
+// go it as a whole, and so do all others, in 64 bits.  (16,384 rows of 4,096 bf16 in 64
+// bits alone: 131 us.)
+template <typename E, bool kNarrow, int T, int C>
+__global__ __launch_bounds__(T < 128 ? 256 : T) void norm_kernel(NormParams p) {
+  constexpr uint32_t kRows = T < 128 ? 256 / T : 1;
   const uint32_t t = threadIdx.x % T;
   const uint32_t row = blockIdx.x * kRows + threadIdx.x / T;
   if (row >= p.rows) return;  // whole waves, and with T > 64 never
   const typename E::Raw* x = static_cast<const typename E::Raw*>(p.x) + (size_t)row * p.x_ld;
-  float h[C][kChunk], w[C][kChunk];
+  Chunk<E> h[C], w[kNarrow ? C : 1];
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
-    load_row<E>(x + j, n, h[i]);
-    load_weight(p.weight, p.weight_dtype, j, n, w[i]);
+    h[i].load(x + j, n);
+    if constexpr (kNarrow) load_weight<E>(p.weight, j, n, w[i]);
   }
   if (p.residual != nullptr) {
     const typename E::Raw* r =
         static_cast<const typename E::Raw*>(p.residual) + (size_t)row * p.residual_ld;
+    Chunk<E> more[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
-      float y[kChunk];
-      load_row<E>(r + j, n, y);
+      const uint32_t j = (i * T + t) * kChunk;
+      more[i].load(r + j, chunk_left(p.cols, j));
+    }
 #pragma unroll
-      for (uint32_t e = 0; e < kChunk; ++e) h[i][e] = E::one(E::raw(h[i][e] + y[e]));
+    for (int i = 0; i < C; ++i) {
+      float y[kChunk];
+#pragma unroll
+      for (uint32_t e = 0; e < kChunk; ++e) y[e] = h[i].get(e) + more[i].get(e);
+      h[i].set(y);
     }
   }
   if (p.sum != nullptr) {
     typename E::Raw* to = static_cast<typename E::Raw*>(p.sum) + (size_t)row * p.sum_ld;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
-      store_row<E>(to + j, n, h[i]);
+      const uint32_t j = (i * T + t) * kChunk;
+      h[i].store(to + j, chunk_left(p.cols, j));
     }
   }
+  auto weights = [&](int i, float (&y)[kChunk]) {
+    if constexpr (kNarrow) {
+#pragma unroll
+      for (uint32_t e = 0; e < kChunk; ++e) y[e] = w[i].get(e);
+    } else {
+      const uint32_t j = (i * T + t) * kChunk;
+      load_weight(p.weight, p.weight_dtype, j, chunk_left(p.cols, j), y);
+    }
+  };
 
   // statistics: the squares' sum, and the bits of the largest |h w| (a NaN's are larger still)
-  double squares = 0.0;
-  uint64_t top = 0;
+  const bool eight = p.q != nullptr;
+  double squares = 0.0, most = 0.0;
+  bool narrow = false, bad = false;
+  if constexpr (kNarrow) {
+    uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
+    for (int i = 0; i < C; ++i) {
 #pragma unroll
-    for (uint32_t e = 0; e < kChunk; ++e) {
-      const double v = (double)h[i][e];
-      squares = fma(v, v, squares);
-      if (p.q != nullptr) {
-        const uint32_t j = (i * T + t) * kChunk + e;
-        const uint64_t b = j < p.cols ? abs_bits(v * (double)w[i][e]) : 0;
+      for (uint32_t e = 0; e < kChunk; ++e) {
+        const float v = h[i].get(e);
+        squares = fma((double)v, (double)v, squares);
+        const uint32_t b = b_of(v * w[i].get(e)) & 0x7fffffffu;  // 0 behind the row's end
         top = b > top ? b : top;
       }
     }
+    const Stats32 s = row_stats<T>(squares, top);
+    squares = s.sum;
+    most = (double)f_of(s.top);
+    narrow = s.top >= 0x21800000u && s.top <= 0x7b800000u;  // 2^-60 to 2^120
   }
-  row_reduce<T>(squares, top);
+  if (!kNarrow || (eight && !narrow)) {
+    squares = 0.0;
+    uint64_t top = 0;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      float y[kChunk];
+      if (eight) weights(i, y);
+#pragma unroll
+      for (uint32_t e = 0; e < kChunk; ++e) {
+        const double v = (double)h[i].get(e);
+        squares = fma(v, v, squares);
+        if (eight) {
+          const uint64_t b = abs_bits(v * (double)y[e]);
+          top = b > top ? b : top;
+        }
+      }
+    }
+    const Stats s = row_stats<T>(squares, top);
+    squares = s.sum;
+    most = __builtin_bit_cast(double, s.top);
+    bad = s.top >= kInfBits;
+  }
   const double rstd = p.norm ? 1.0 / sqrt(squares / (double)p.cols + p.eps) : 1.0;
-  const double most = __builtin_bit_cast(double, top);
   const float scale = (float)(rstd * (most / 127.0));
-  const bool bad = !isfinite(squares) || (p.q != nullptr && (top >= kInfBits || !isfinite(scale)));
+  bad = !isfinite(squares) || (eight && (bad || !isfinite(scale)));
 
   if (p.out != nullptr) {
     const float r = bad ? __builtin_nanf("") : (float)rstd;
@@ -735,29 +854,47 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(NormParams p) {
     for (int i = 0; i < C; ++i) {
       const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
       float y[kChunk];
+      weights(i, y);
 #pragma unroll
-      for (uint32_t e = 0; e < kChunk; ++e) y[e] = h[i][e] * r * w[i][e];
+      for (uint32_t e = 0; e < kChunk; ++e) y[e] = h[i].get(e) * r * y[e];
       store_any(p.out, p.out_dtype, (size_t)row * p.out_ld + j, n, y);
     }
   }
-  if (p.q != nullptr) {
+  if (eight) {
     const double step = most > 0.0 ? 127.0 / most : 0.0;
+    const float step32 = (float)step;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
-      uint32_t word[2] = {};
+      float y[kChunk];
+      weights(i, y);
+      uint32_t q[kChunk];
+      bool exact = true;
+      if (kNarrow && narrow) {
+        // added to 1.5 2^23, a number is rounded to a whole one, whose low byte is the byte
+        float off = 0.0f;
 #pragma unroll
-      for (uint32_t e = 0; e < kChunk; ++e) {
-        const int v = bad ? 0 : nearest_step((double)h[i][e] * (double)w[i][e], most, step);
-        word[e / 4] |= ((uint32_t)v & 0xffu) << (8u * (e % 4));
+        for (uint32_t e = 0; e < kChunk; ++e) {
+          const float v = h[i].get(e) * y[e], whole = fmaf(v, step32, 0x1.8p23f);
+          q[e] = b_of(whole);
+          off = fmaxf(off, fabsf(fmaf(v, step32, -(whole - 0x1.8p23f))));
+        }
+        exact = off > 0.5f - 0x1p-15f;
       }
+      if (__builtin_expect(exact, !kNarrow)) {
+#pragma unroll
+        for (uint32_t e = 0; e < kChunk; ++e)
+          q[e] = (uint32_t)nearest_step((double)h[i].get(e) * (double)y[e], most, step);
+      }
+      uint32_t lo = four_bytes(q[0], q[1], q[2], q[3]), hi = four_bytes(q[4], q[5], q[6], q[7]);
+      if (bad) lo = hi = 0;
       int8_t* to = p.q + (size_t)row * p.q_ld + j;
       if (n >= kChunk) {
-        *reinterpret_cast<Bytes8*>(to) = Words2{word[0], word[1]};
+        *reinterpret_cast<Bytes8*>(to) = Words2{lo, hi};
       } else {
 #pragma unroll
         for (uint32_t e = 0; e < kChunk; ++e)
-          if (e < n) to[e] = (int8_t)(word[e / 4] >> (8u * (e % 4)));
+          if (e < n) to[e] = (int8_t)((e < 4 ? lo : hi) >> (8u * (e % 4)));
       }
     }
     if (t == 0) p.scale[row] = bad ? __builtin_nanf("") : scale;
@@ -771,18 +908,18 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(NormParams p) {
     uint64_t at = ~0ull;
 #pragma unroll
     for (int i = C - 1; i >= 0; --i) {
+      float y[kChunk];
+      weights(i, y);
 #pragma unroll
       for (int e = (int)kChunk - 1; e >= 0; --e) {
         const uint32_t j = (i * T + t) * kChunk + e;
-        const bool failed = !isfinite(h[i][e]) ||
-                            (p.q != nullptr && !isfinite((double)h[i][e] * (double)w[i][e]));
-        if (j < p.cols && failed) at = (uint64_t)j << 32 | b_of(h[i][e]);
+        const float v = h[i].get(e);
+        const bool failed =
+            !isfinite(v) || (eight && !isfinite((double)v * (double)y[e]));
+        if (j < p.cols && failed) at = (uint64_t)j << 32 | b_of(v);
       }
     }
-    double none = 0.0;
-    at = ~at;
-    row_reduce<T>(none, at);
-    at = ~at;
+    at = ~row_stats<T>(0.0, ~at).top;
     if (t == 0) {
       if (at == ~0ull) at = (uint64_t)p.cols << 32;  // the scale
       put_record(p.err, row, PB_NONFINITE_INPUT, 0, at & 0xffffffffu,
@@ -793,56 +930,114 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(NormParams p) {
 
 // The gradient.  With m = rstd and c = mean(g w h): dh = gh + m (g w - h m^2 c), and
 // the weight's is the sum of g h m over the rows.  The statistics are taken anew from h,
-// which is read anyway.  A workgroup goes over rows and holds its sums of the weight's
-// gradient in registers; they are joined over the workgroups in 64 bits.
-template <typename E, int T, int C>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void norm_grad_kernel(NormGradParams p) {
-  constexpr uint32_t kRows = T < 256 ? 256 / T : 1;
+// which is read anyway.  A workgroup goes over rows, the next one requested before the one at
+// hand is worked out, and holds its sums of the weight's gradient in registers; they are
+// joined over the workgroups in 64 bits.  Rows of more than 8,192 columns do not fit the
+// registers: their second pass reads them again, and the sums are in LDS.  kSame: gradients, weight
+// and rows of one type, held as they are in memory.
+template <typename E, bool kSame, int T, int C>
+__global__ __launch_bounds__(T < 128 ? 256 : T) void norm_grad_kernel(NormGradParams p) {
+  constexpr uint32_t kRows = T < 128 ? 256 / T : 1;
+  constexpr bool kHold = T < 1024, kHoldAll = kHold && kSame;
   const uint32_t t = threadIdx.x % T;
-  float w[C][kChunk], dw[C][kChunk];
+  auto column = [&](int i) { return (i * T + t) * kChunk; };
+  constexpr int kUnroll = kHold ? C : 1;
+  Chunk<E> w[kHoldAll ? C : 1];
+  // the sums of the weight's gradient
+  float held[kHold ? C : 1][kChunk];
+  __shared__ float kept[kHold ? 1 : C * kChunk][kHold ? 1 : T];
+  auto dw = [&](int i, uint32_t e) -> float& {
+    if constexpr (kHold) return held[i][e];
+    else return kept[i * kChunk + e][t];
+  };
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
-    load_weight(p.weight, p.weight_dtype, j, n, w[i]);
+    if constexpr (kHoldAll) load_weight<E>(p.weight, column(i), chunk_left(p.cols, column(i)), w[i]);
 #pragma unroll
-    for (uint32_t e = 0; e < kChunk; ++e) dw[i][e] = 0.0f;
+    for (uint32_t e = 0; e < kChunk; ++e) dw(i, e) = 0.0f;
   }
-  for (uint32_t row = blockIdx.x * kRows + threadIdx.x / T; row < p.rows;
-       row += p.groups * kRows) {
-    float h[C][kChunk], g[C][kChunk];
-    const typename E::Raw* hp = static_cast<const typename E::Raw*>(p.h) + (size_t)row * p.h_ld;
+  struct Row {
+    Chunk<E> h[kHold ? C : 1], g[kHoldAll ? C : 1], more[kHold ? C : 1];
+  };
+  auto load_rows = [&](Chunk<E>& c, const void* base, size_t ld, uint32_t row, int i) {
+    c.load(static_cast<const typename E::Raw*>(base) + (size_t)row * ld + column(i),
+           chunk_left(p.cols, column(i)));
+  };
+  auto request = [&](Row& r, uint32_t row) {
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
-      load_row<E>(hp + j, n, h[i]);
-      load_any(p.grad, p.grad_dtype, (size_t)row * p.grad_ld + j, n, g[i]);
+      load_rows(r.h[i], p.h, p.h_ld, row, i);
+      if constexpr (kSame) load_rows(r.g[i], p.grad, p.grad_ld, row, i);
+      if (p.grad_sum != nullptr) load_rows(r.more[i], p.grad_sum, p.grad_sum_ld, row, i);
     }
-    double squares = 0.0, along = 0.0;
+  };
+  const uint32_t turn = p.groups * kRows;
+  uint32_t row = blockIdx.x * kRows + threadIdx.x / T;
+  Row next{};
+  if (kHold && row < p.rows) request(next, row);
+  for (; row < p.rows; row += turn) {
+    const Row r = next;
+    if (kHold && row + turn < p.rows) request(next, row + turn);
+    // h, g and g w of a chunk
+    auto take = [&](int i, float (&h)[kChunk], float (&g)[kChunk], float (&gw)[kChunk]) {
+      const uint32_t j = column(i), n = chunk_left(p.cols, j);
+      if constexpr (kHold) {
 #pragma unroll
+        for (uint32_t e = 0; e < kChunk; ++e) h[e] = r.h[i].get(e);
+      } else {
+        load_row<E>(static_cast<const typename E::Raw*>(p.h) + (size_t)row * p.h_ld + j, n, h);
+      }
+      if constexpr (kHoldAll) {
+#pragma unroll
+        for (uint32_t e = 0; e < kChunk; ++e) {
+          g[e] = r.g[i].get(e);
+          gw[e] = g[e] * w[i].get(e);
+        }
+      } else {
+        load_any(p.grad, p.grad_dtype, (size_t)row * p.grad_ld + j, n, g);
+        load_weight(p.weight, p.weight_dtype, j, n, gw);
+#pragma unroll
+        for (uint32_t e = 0; e < kChunk; ++e) gw[e] = g[e] * gw[e];
+      }
+    };
+    double squares = 0.0, along = 0.0;
+#pragma unroll kUnroll
     for (int i = 0; i < C; ++i) {
+      float h[kChunk], g[kChunk], gw[kChunk];
+      take(i, h, g, gw);
 #pragma unroll
       for (uint32_t e = 0; e < kChunk; ++e) {
-        const double v = (double)h[i][e];
+        const double v = (double)h[e];
         squares = fma(v, v, squares);
-        along = fma((double)(g[i][e] * w[i][e]), v, along);
+        along = fma((double)gw[e], v, along);
       }
     }
-    uint64_t none = 0;
-    row_reduce<T>(squares, none);
-    row_reduce<T>(along, none);
-    const double rstd = 1.0 / sqrt(squares / (double)p.cols + p.eps);
-    const float m = (float)rstd, k = (float)(rstd * rstd * (along / (double)p.cols));
-#pragma unroll
+    struct Two {
+      double a, b;
+    };
+    const Two s = row_join<T>(Two{wave_add(squares), wave_add(along)}, [](Two x, Two y) {
+      return Two{x.a + y.a, x.b + y.b};
+    });
+    const double rstd = 1.0 / sqrt(s.a / (double)p.cols + p.eps);
+    const float m = (float)rstd, k = (float)(rstd * rstd * (s.b / (double)p.cols));
+#pragma unroll kUnroll
     for (int i = 0; i < C; ++i) {
-      const uint32_t j = (i * T + t) * kChunk, n = chunk_left(p.cols, j);
-      float y[kChunk];
+      const uint32_t j = column(i), n = chunk_left(p.cols, j);
+      float h[kChunk], g[kChunk], gw[kChunk];
+      take(i, h, g, gw);
       if (p.grad_h != nullptr) {
+        float y[kChunk];
 #pragma unroll
-        for (uint32_t e = 0; e < kChunk; ++e) y[e] = m * (g[i][e] * w[i][e] - h[i][e] * k);
+        for (uint32_t e = 0; e < kChunk; ++e) y[e] = m * (gw[e] - h[e] * k);
         if (p.grad_sum != nullptr) {
           float more[kChunk];
-          load_row<E>(static_cast<const typename E::Raw*>(p.grad_sum) +
-                          (size_t)row * p.grad_sum_ld + j, n, more);
+          if constexpr (kHold) {
+#pragma unroll
+            for (uint32_t e = 0; e < kChunk; ++e) more[e] = r.more[i].get(e);
+          } else {
+            load_row<E>(static_cast<const typename E::Raw*>(p.grad_sum) +
+                            (size_t)row * p.grad_sum_ld + j, n, more);
+          }
 #pragma unroll
           for (uint32_t e = 0; e < kChunk; ++e) y[e] = y[e] + more[e];
         }
@@ -850,53 +1045,56 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_grad_kernel(NormGradPa
                      y);
       }
 #pragma unroll
-      for (uint32_t e = 0; e < kChunk; ++e) dw[i][e] = dw[i][e] + g[i][e] * (h[i][e] * m);
+      for (uint32_t e = 0; e < kChunk; ++e) dw(i, e) = dw(i, e) + g[e] * (h[e] * m);
     }
   }
   if (p.grad_weight == nullptr) return;
   float* part = p.part + (size_t)blockIdx.x * p.cols;
   if constexpr (T == 64) {
-    extern __shared__ float waves[];  // [3][cols]: of all waves but the first
+    __shared__ float waves[3][C * 64 * kChunk];  // of all waves but the first
     const uint32_t wave = threadIdx.x >> 6;
+    if (wave != 0) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
+      for (int i = 0; i < C; ++i)
 #pragma unroll
-      for (uint32_t e = 0; e < kChunk; ++e) {
-        const uint32_t j = (i * T + t) * kChunk + e;
-        if (wave != 0 && j < p.cols) waves[(wave - 1u) * p.cols + j] = dw[i][e];
-      }
+        for (uint32_t e = 0; e < kChunk; ++e) waves[wave - 1u][(i * kChunk + e) * 64u + t] = dw(i, e);
     }
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
+    for (int i = 0; i < C; ++i)
 #pragma unroll
       for (uint32_t e = 0; e < kChunk; ++e) {
-        const uint32_t j = (i * T + t) * kChunk + e;
-        if (j < p.cols)
-          dw[i][e] = ((dw[i][e] + waves[j]) + waves[p.cols + j]) + waves[2u * p.cols + j];
+        const uint32_t at = (i * kChunk + e) * 64u + t;
+        dw(i, e) = ((dw(i, e) + waves[0][at]) + waves[1][at]) + waves[2][at];
       }
-    }
   }
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const uint32_t j = (i * T + t) * kChunk;
-    store_row<F32>(reinterpret_cast<uint32_t*>(part + j), chunk_left(p.cols, j), dw[i]);
+    const uint32_t j = column(i);
+    float y[kChunk];
+#pragma unroll
+    for (uint32_t e = 0; e < kChunk; ++e) y[e] = dw(i, e);
+    store_row<F32>(reinterpret_cast<uint32_t*>(part + j), chunk_left(p.cols, j), y);
   }
 }
 
-// The workgroups' sums of the weight's gradient, 64 columns a workgroup.
+// The workgroups' sums of the weight's gradient: 16 columns a workgroup, 64 of the sums at a
+// time.
 __global__ __launch_bounds__(1024) void norm_weight_kernel(NormGradParams p) {
-  __shared__ double waves[16][64];
-  const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
-  const uint32_t j = blockIdx.x * 64u + lane;
+  __shared__ double parts[64][16];
+  const uint32_t c = threadIdx.x % 16u, k0 = threadIdx.x / 16u;
+  const uint32_t j = blockIdx.x * 16u + c;
   double sum = 0.0;
-  if (j < p.cols)
-    for (uint32_t k = wave; k < p.groups; k += 16u) sum = sum + (double)p.part[(size_t)k * p.cols + j];
-  waves[wave][lane] = sum;
+  if (j < p.cols) {
+#pragma unroll 8
+    for (uint32_t k = k0; k < p.groups; k += 64u) sum = sum + (double)p.part[(size_t)k * p.cols + j];
+  }
+  parts[k0][c] = sum;
   __syncthreads();
-  if (wave != 0 || j >= p.cols) return;
-  for (uint32_t w = 1; w < 16; ++w) sum = sum + waves[w][lane];
+  if (k0 != 0 || j >= p.cols) return;
+#pragma unroll
+  for (uint32_t k = 1; k < 64; ++k) sum = sum + parts[k][c];
   p.grad_weight[j] = p.accumulate ? (float)((double)p.grad_weight[j] + sum) : (float)sum;
 }
 
@@ -913,7 +1111,7 @@ uint32_t row_shift(uint32_t cols) {
 uint32_t sort_tiles(uint32_t rows) { return (rows + kSortTile - 1u) / kSortTile; }
 
 // Workgroups of the norm's gradient, each with at most kMaxTerms rows a thread.
-constexpr uint32_t kGradGroups = 512;
+constexpr uint32_t kGradGroups = 1024;
 constexpr uint32_t kGradTerms = 768;
 uint32_t grad_groups(uint32_t rows, uint32_t rows_at_once) {
   const uint32_t all = (rows + rows_at_once - 1u) / rows_at_once;
@@ -924,41 +1122,41 @@ uint32_t grad_groups(uint32_t rows, uint32_t rows_at_once) {
 
 size_t round_up(size_t bytes) { return (bytes + 255u) & ~(size_t)255u; }
 
-template <typename E, template <typename, int, int> class Launch, typename P>
+// A row's threads and their chunks: few of them, so that many rows are on their way at once.
+template <typename E, bool kOne, template <typename, bool, int, int> class Launch, typename P>
 hipError_t by_width(const P& p, hipStream_t stream) {
   const uint32_t chunks = (p.cols + kChunk - 1u) / kChunk;
-  if (chunks <= 64) return Launch<E, 64, 1>::run(p, stream);
-  if (chunks <= 128) return Launch<E, 64, 2>::run(p, stream);
-  if (chunks <= 256) return Launch<E, 64, 4>::run(p, stream);
-  if (chunks <= 512) return Launch<E, 256, 2>::run(p, stream);
-  if (chunks <= 1024) return Launch<E, 256, 4>::run(p, stream);
-  if (chunks <= 2048) return Launch<E, 1024, 2>::run(p, stream);
-  return Launch<E, 1024, 4>::run(p, stream);
+  if (chunks <= 64) return Launch<E, kOne, 64, 1>::run(p, stream);
+  if (chunks <= 128) return Launch<E, kOne, 128, 1>::run(p, stream);
+  if (chunks <= 256) return Launch<E, kOne, 256, 1>::run(p, stream);
+  if (chunks <= 512) return Launch<E, kOne, 256, 2>::run(p, stream);
+  if (chunks <= 1024) return Launch<E, kOne, 512, 2>::run(p, stream);
+  if (chunks <= 2048) return Launch<E, kOne, 1024, 2>::run(p, stream);
+  return Launch<E, kOne, 1024, 4>::run(p, stream);
 }
 
-template <typename E, int T, int C>
+template <typename E, bool kNarrow, int T, int C>
 struct NormLaunch {
   static hipError_t run(const NormParams& p, hipStream_t stream) {
-    constexpr uint32_t kRows = T < 256 ? 256 / T : 1;
-    norm_kernel<E, T, C><<<(p.rows + kRows - 1u) / kRows, T < 256 ? 256 : T, 0, stream>>>(p);
+    constexpr uint32_t kRows = T < 128 ? 256 / T : 1;
+    norm_kernel<E, kNarrow, T, C><<<(p.rows + kRows - 1u) / kRows, T * kRows, 0, stream>>>(p);
     return hipGetLastError();
   }
 };
 
-template <typename E, int T, int C>
+template <typename E, bool kSame, int T, int C>
 struct NormGradLaunch {
   static hipError_t run(const NormGradParams& in, hipStream_t stream) {
-    constexpr uint32_t kRows = T < 256 ? 256 / T : 1;
+    constexpr uint32_t kRows = T < 128 ? 256 / T : 1;
     NormGradParams p = in;
     p.groups = grad_groups(p.rows, kRows);
-    const size_t lds = T == 64 && p.grad_weight != nullptr ? (size_t)3 * p.cols * 4 : 0;
     hipError_t e = hipSuccess;
     if (p.groups != 0) {  // without rows the weight's gradient is zeros
-      norm_grad_kernel<E, T, C><<<p.groups, T < 256 ? 256 : T, lds, stream>>>(p);
+      norm_grad_kernel<E, kSame, T, C><<<p.groups, T * kRows, 0, stream>>>(p);
       e = hipGetLastError();
     }
     if (e != hipSuccess || p.grad_weight == nullptr) return e;
-    norm_weight_kernel<<<(p.cols + 63u) / 64u, 1024, 0, stream>>>(p);
+    norm_weight_kernel<<<(p.cols + 15u) / 16u, 1024, 0, stream>>>(p);
     return hipGetLastError();
   }
 };
@@ -1075,15 +1273,25 @@ hipError_t launch_embed_grad(const EmbedGradParams& p, uint32_t dtype, uint32_t 
 }
 
 hipError_t launch_norm(const NormParams& p, uint32_t dtype, hipStream_t stream) {
-  if (dtype == PB_F32) return by_width<F32, NormLaunch>(p, stream);
-  if (dtype == PB_F16) return by_width<F16, NormLaunch>(p, stream);
-  return by_width<BF16, NormLaunch>(p, stream);
+  const bool one = p.weight == nullptr || p.weight_dtype == dtype;
+  if (dtype == PB_F32) return by_width<F32, false, NormLaunch>(p, stream);
+  if (dtype == PB_F16)
+    return one ? by_width<F16, true, NormLaunch>(p, stream)
+               : by_width<F16, false, NormLaunch>(p, stream);
+  return one ? by_width<BF16, true, NormLaunch>(p, stream)
+             : by_width<BF16, false, NormLaunch>(p, stream);
 }
 
+template <typename E>
+hipError_t norm_grad_as(const NormGradParams& p, uint32_t dtype, hipStream_t stream) {
+  if (p.grad_dtype == dtype && (p.weight == nullptr || p.weight_dtype == dtype))
+    return by_width<E, true, NormGradLaunch>(p, stream);
+  return by_width<E, false, NormGradLaunch>(p, stream);
+}
 hipError_t launch_norm_grad(const NormGradParams& p, uint32_t dtype, hipStream_t stream) {
-  if (dtype == PB_F32) return by_width<F32, NormGradLaunch>(p, stream);
-  if (dtype == PB_F16) return by_width<F16, NormGradLaunch>(p, stream);
-  return by_width<BF16, NormGradLaunch>(p, stream);
+  if (dtype == PB_F32) return norm_grad_as<F32>(p, dtype, stream);
+  if (dtype == PB_F16) return norm_grad_as<F16>(p, dtype, stream);
+  return norm_grad_as<BF16>(p, dtype, stream);
 }
 
 }  // namespace pb
