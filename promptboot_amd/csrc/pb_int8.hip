@@ -160,8 +160,9 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t row, uint32_t piece) {
 struct TilePlan {
   uint32_t m_tiles, n_tiles, group;
 };
-__device__ __forceinline__ void tile_of(const TilePlan& t, uint32_t* m, uint32_t* n) {
-  const uint32_t item = xcd_contiguous_item(blockIdx.x, t.m_tiles * t.n_tiles);
+__device__ __forceinline__ void tile_of(const TilePlan& t, uint32_t linear, uint32_t* m,
+                                        uint32_t* n) {
+  const uint32_t item = xcd_contiguous_item(linear, t.m_tiles * t.n_tiles);
   const uint32_t whole = t.group * t.n_tiles, g = item / whole, in_group = item - g * whole;
   const uint32_t left = t.m_tiles - g * t.group, rows = left < t.group ? left : t.group;
   *m = g * t.group + in_group % rows;
@@ -194,16 +195,25 @@ __device__ __forceinline__ void multiply_set(const int8_t* set, uint32_t wm, uin
 }
 
 // Scales and stores a wave's sums.  They go through LDS (kSliceBytes a wave), 128 bytes of
-// 32 rows at a time, so that eight lanes store 128 neighbouring bytes, past the caches:
-// with one element a lane (64 bytes of a row together) and through the caches 4,096 x
-// 151,936 bf16 logits alone took 594 us, through LDS 356, and past the caches 262.
+// 32 rows at a time, so that eight lanes store 128 neighbouring bytes: with one element a
+// lane (64 bytes of a row together) 4,096 x 151,936 bf16 logits alone took 594 us, so 356.
+// They go past the caches (262 us) where those 128 bytes are whole lines of 64, and through
+// them where they are not: there a line is put together from two stores, and memory takes
+// half lines badly.  With the product, past and through the caches:
+//   4,096 x 512 by 100,032 channels, rows of lines    bf16  322 / 350 us   fp32  399 /  465
+//              by 100,016 (32 bytes left / lines)           347 / 378            433 /  535
+//              by 100,008 (16 bytes left / 32)              430 / 390            916 /  624
+//              by 100,001 (2 bytes left / 4)                516 / 394          1,390 /  667
+//   333 x 1,001 by 50,304                                  44.6 / 46.9          46.5 / 65.4
+//              by 50,257                                   54.4 / 46.5          76.4 / 65.7
+constexpr uint32_t kLine = 64;
 constexpr uint32_t kSlicePitch = 144, kSliceBytes = 32 * kSlicePitch;
-template <typename Out, int BM, int BN>
-__device__ __forceinline__ void store_sums(const Int8Params& p, int8_t* slice,
-                                           const float* chan_scale, const float* chan_bias,
-                                           uint32_t m0, uint32_t n0, uint32_t wn,
-                                           const float (&row_scale)[BM],
-                                           const v16i (&acc)[BM][BN]) {
+template <typename Out, bool kPast, int BM, int BN>
+__device__ __forceinline__ void store_by(const Int8Params& p, int8_t* slice,
+                                         const float* chan_scale, const float* chan_bias,
+                                         uint32_t m0, uint32_t n0, uint32_t wn,
+                                         const float (&row_scale)[BM],
+                                         const v16i (&acc)[BM][BN]) {
   constexpr uint32_t kSize = 16 / Out::kPer;           // bytes of an element
   constexpr int kBlocks = 128 / (32 * (int)kSize);     // blocks of channels of a slice
   static_assert(BN % kBlocks == 0, "whole slices");
@@ -240,7 +250,10 @@ __device__ __forceinline__ void store_sums(const Int8Params& p, int8_t* slice,
         if (m < p.rows && n < p.channels) {
           typename Out::Raw* to = out + (size_t)m * p.out_ld + n;
           if (n + Out::kPer <= p.channels) {
-            store_chunk<Out>(to, v);
+            if constexpr (kPast)
+              store_chunk<Out>(to, v);
+            else
+              *reinterpret_cast<Loose4*>(to) = Words4{v.x, v.y, v.z, v.w};
           } else {
 #pragma unroll
             for (uint32_t e = 0; e + 1u < (uint32_t)Out::kPer; ++e)
@@ -251,6 +264,18 @@ __device__ __forceinline__ void store_sums(const Int8Params& p, int8_t* slice,
       __builtin_amdgcn_wave_barrier();
     }
   }
+}
+
+template <typename Out, int BM, int BN>
+__device__ __forceinline__ void store_sums(const Int8Params& p, int8_t* slice,
+                                           const float* chan_scale, const float* chan_bias,
+                                           uint32_t m0, uint32_t n0, uint32_t wn,
+                                           const float (&row_scale)[BM],
+                                           const v16i (&acc)[BM][BN]) {
+  if (((uintptr_t)p.out | p.out_ld * (16 / Out::kPer)) % kLine == 0)
+    store_by<Out, true>(p, slice, chan_scale, chan_bias, m0, n0, wn, row_scale, acc);
+  else
+    store_by<Out, false>(p, slice, chan_scale, chan_bias, m0, n0, wn, row_scale, acc);
 }
 
 // The channels' scales and biases of a tile, in LDS.
@@ -309,7 +334,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void int8_tile_kernel(Int8Par
   const uint32_t lane = lane_id();
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   uint32_t m0, n0;
-  tile_of(plan, &m0, &n0);
+  tile_of(plan, blockIdx.x, &m0, &n0);
   m0 *= TM;
   n0 *= TN;
   load_channels<kThreads, TN>(p, n0, chan_scale, chan_bias);
@@ -383,6 +408,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void int8_tile_kernel(Int8Par
 // compiler would wait for all of them before each read of LDS; every wait for them stands
 // here, before the barrier behind which their set is read.
 __device__ const v4i kZeroPiece = {0, 0, 0, 0};  // what stands behind a row's end
+__device__ __forceinline__ void to_lds(const int8_t* from, int8_t* wave_to) {
+  const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)wave_to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to),
+               "v"(from)
+               : "memory", "m0");
+}
 
 template <typename Out, int WM, int WN, int BM, int BN, uint32_t KB, uint32_t kSets, int WK>
 __global__ __launch_bounds__(64 * WM * WN * WK) void int8_pieces_kernel(Int8Params p, TilePlan plan) {
@@ -398,7 +429,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void int8_pieces_kernel(Int8Para
   const uint32_t lane = lane_id();
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   uint32_t m0, n0;
-  tile_of(plan, &m0, &n0);
+  tile_of(plan, blockIdx.x, &m0, &n0);
   m0 *= TM;
   n0 *= TN;
   // load i of the wave brings 1 KB of rows, a lane the piece whose place it has
@@ -423,11 +454,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void int8_pieces_kernel(Int8Para
       const int8_t* at = from[i] + k;
       if (k + KB > p.cols && k + offset[i] >= p.cols)
         at = reinterpret_cast<const int8_t*>(&kZeroPiece);
-      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) int8_t*)(
-          set + (wave * kLoads + i) * 1024u);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to),
-                   "v"(at)
-                   : "memory", "m0");
+      to_lds(at, set + (wave * kLoads + i) * 1024u);
     }
   };
   const uint32_t steps = (p.cols + KB - 1u) / KB;
@@ -468,6 +495,123 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void int8_pieces_kernel(Int8Para
                   acc);
 }
 
+// The same for many large tiles: a workgroup takes one after the other, and the first set of
+// the next is on its way while the last of this one is multiplied and its sums are stored.
+// 4,096 x 151,936 x 896 to bf16: 716 us, 1,560 TOP/s (a workgroup a tile 742); 4,096 x 8,192 x
+// 8,192 245 us, 2,240 TOP/s (252).  Without the stores the first takes 631: they end before
+// the next tile's second set, for loads wait behind them.
+constexpr uint32_t kLargeGroups = 256;  // one a compute unit
+template <typename Out>
+__global__ __launch_bounds__(512) void int8_large_kernel(Int8Params p, TilePlan plan) {
+  constexpr int WM = 2, WN = 4, BM = 4, BN = 2;
+  using T = Tile<WM, WN, BM, BN>;
+  constexpr uint32_t TM = T::kRows, TN = T::kChannels, KB = 128, kPieces = KB / 16u;
+  constexpr uint32_t kLoads = (TM + TN) * KB / 1024u / T::kWaves;
+  constexpr uint32_t kSet = (TM + TN) * KB;
+  // stores of a wave of a whole tile, none of which is left out
+  constexpr uint32_t kStores = BM * BN * 32u * 32u / (64u * Out::kPer);
+  __shared__ __align__(16) int8_t lds[2 * kSet];
+  __shared__ __align__(16) float chan_scale[2][TN], chan_bias[2][TN];
+  const uint32_t lane = lane_id();
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t wm = wave / WN * (BM * 32u), wn = wave % WN * (BN * 32u);
+  const uint32_t tiles = plan.m_tiles * plan.n_tiles, steps = (p.cols + KB - 1u) / KB;
+  const int8_t* from[kLoads];
+  uint32_t offset[kLoads];
+#pragma unroll
+  for (uint32_t i = 0; i < kLoads; ++i) {
+    const uint32_t row = (wave * kLoads + i) * (64u / kPieces) + lane / kPieces;
+    offset[i] = piece_at<KB>(row, lane % kPieces) - row * KB;
+  }
+  uint32_t m0, n0;
+  auto go_to = [&](uint32_t linear) {
+    tile_of(plan, linear, &m0, &n0);
+    m0 *= TM;
+    n0 *= TN;
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const uint32_t row = (wave * kLoads + i) * (64u / kPieces) + lane / kPieces;
+      if (row < TM) {
+        const uint32_t r = m0 + row;
+        from[i] = p.q + (size_t)(r < p.rows ? r : p.rows - 1u) * p.q_ld + offset[i];
+      } else {
+        const uint32_t r = n0 + row - TM;
+        from[i] = p.weight + (size_t)(r < p.channels ? r : p.channels - 1u) * p.weight_ld + offset[i];
+      }
+    }
+  };
+  auto bring = [&](int8_t* set, uint32_t step) {
+    const uint32_t k = step * KB;
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const int8_t* at = from[i] + k;
+      if (k + KB > p.cols && k + offset[i] >= p.cols)
+        at = reinterpret_cast<const int8_t*>(&kZeroPiece);
+      to_lds(at, set + (wave * kLoads + i) * 1024u);
+    }
+  };
+  // a tile's scales and biases, in registers
+  struct Scales {
+    float row[BM], chan, bias;
+  };
+  auto scales_of = [&]() {
+    Scales s;
+#pragma unroll
+    for (int i = 0; i < BM; ++i) {
+      const uint32_t m = m0 + wm + i * 32u + (lane & 31u);
+      s.row[i] = m < p.rows ? p.scale[m] : 0.0f;
+    }
+    const uint32_t n = n0 + threadIdx.x;
+    const bool real = threadIdx.x < TN && n < p.channels;
+    s.chan = real ? p.weight_scale[n] : 0.0f;
+    s.bias = real && p.bias ? p.bias[n] : 0.0f;
+    return s;
+  };
+  uint32_t item = blockIdx.x, use = 0, turn = 0;
+  bool stored = false;  // kStores stores are behind the loads of the first set
+  go_to(item);
+  Scales scales = scales_of();
+  bring(lds, 0);
+  while (true) {
+    if (threadIdx.x < TN) {  // the other pair may still be read by waves that store
+      chan_scale[turn][threadIdx.x] = scales.chan;
+      chan_bias[turn][threadIdx.x] = scales.bias;
+    }
+    const uint32_t my_m0 = m0, my_n0 = n0, next = item + kLargeGroups;
+    float row_scale[BM];
+#pragma unroll
+    for (int i = 0; i < BM; ++i) row_scale[i] = scales.row[i];
+    v16i acc[BM][BN] = {};
+    // As above; loads and stores end in their order, so with the tile's stores behind the loads
+    // all but the newest of those may go on.
+    if (stored)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kStores - 4u) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    for (uint32_t step = 1; step < steps; ++step) {
+      bring(lds + (use ^ kSet), step);
+      multiply_set<KB, TM, 1>(lds + use, wm, wn, 0, acc);
+      use ^= kSet;
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    if (next < tiles) {
+      go_to(next);
+      scales = scales_of();
+      bring(lds + (use ^ kSet), 0);
+    }
+    multiply_set<KB, TM, 1>(lds + use, wm, wn, 0, acc);
+    use ^= kSet;
+    // the set that was multiplied last takes the slices
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    store_sums<Out>(p, lds + (use ^ kSet) + wave * kSliceBytes, chan_scale[turn], chan_bias[turn],
+                    my_m0 + wm, my_n0, wn, row_scale, acc);
+    if (next >= tiles) return;
+    stored = my_m0 + TM <= p.rows && my_n0 + TN <= p.channels;
+    item = next;
+    turn ^= 1u;
+  }
+}
+
 template <typename Out>
 hipError_t few_as(const Int8Params& p, hipStream_t stream) {
   const uint32_t groups = (p.channels + 15u) / 16u, steps = (p.cols + 63u) / 64u;
@@ -505,6 +649,14 @@ hipError_t pieces_as(const Int8Params& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename Out>
+hipError_t large_as(const Int8Params& p, hipStream_t stream) {
+  const TilePlan t = plan_tiles<Tile<2, 4, 4, 2>>(p);
+  const uint32_t all = t.m_tiles * t.n_tiles;
+  int8_large_kernel<Out><<<all < kLargeGroups ? all : kLargeGroups, 512, 0, stream>>>(p, t);
+  return hipGetLastError();
+}
+
 // Whole pieces: 16 bytes divide the columns, the addresses and the distances of rows.
 bool whole_pieces(const Int8Params& p) {
   return ((p.cols | p.q_ld | p.weight_ld | (uintptr_t)p.q | (uintptr_t)p.weight) & 15u) == 0;
@@ -525,7 +677,8 @@ uint32_t tiles(const Int8Params& p, uint32_t rows, uint32_t channels) {
 // Tiles by how many there are for 256 compute units: where tiles of 64 x 64 do not fill
 // them, eight waves a tile, the contraction cut by four; then 64 x 128 tiles, one and two a
 // unit; then 128 x 128, two a unit; and 256 x 256 where their rounds are few enough: a round
-// takes 1.25 to 1.6 times as long as one of 128 x 128 tiles.  Of whole pieces:
+// takes 1.25 to 1.6 times as long as one of 128 x 128 tiles (below a workgroup takes one of
+// them; one after the other, as it is done, they take 2 to 4 % less).  Of whole pieces:
 //                            64 x 64, K by 4   64 x 128, K by 2   64 x 128   128 x 128   256 x 256
 //   96 x 8,192 x 8,192                  18.5               24.7       32.5        43.9        96.0
 //   1,000 x 1,000 x 8,192               19.0               25.2       32.9        44.1        98.3
@@ -542,7 +695,7 @@ uint32_t tiles(const Int8Params& p, uint32_t rows, uint32_t channels) {
 //   1,000 x 1,000 x 7,001               37.2               56.2       76.9        95.7           -
 //   2,000 x 2,000 x 2,001               35.6               23.9       27.0        31.9           -
 //   8 x 151,936 x 896                   44.6               32.1       28.7           -           -
-//   333 x 50,257 x 1,001                85.3               56.4       56.6        49.1           -
+//   333 x 50,257 x 1,001                85.3               56.4       56.6        46.5           -
 template <typename Out>
 hipError_t int8_as(const Int8Params& p, hipStream_t stream) {
   const bool whole = whole_pieces(p);
@@ -560,7 +713,7 @@ hipError_t int8_as(const Int8Params& p, hipStream_t stream) {
   if (of128 <= 256) return pieces_as<Out, 2, 2, 1, 2, 256, 3, 2>(p, stream);
   if (of128 <= 512 || p.rows <= 64) return pieces_as<Out, 2, 2, 1, 2, 128, 3, 1>(p, stream);
   const uint32_t large = (tiles(p, 256, 256) + 255u) / 256u;
-  if (8u * large < 5u * rounds) return pieces_as<Out, 2, 4, 4, 2, 128, 2, 1>(p, stream);
+  if (8u * large < 5u * rounds) return large_as<Out>(p, stream);
   return pieces_as<Out, 2, 2, 2, 2, 128, 2, 1>(p, stream);
 }
 
