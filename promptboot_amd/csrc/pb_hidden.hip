@@ -234,8 +234,8 @@ __device__ __forceinline__ void zero_part(const EmbedGradParams& p, uint32_t par
 
 // Up to kSortRows rows: one workgroup sorts them in LDS, the others write zeros.  A pass
 // gives every wave a run of the rows: a row's rank among its wave's rows of its digit, then
-// the prefix over digits and waves.  (16,384 rows by the three launches a pass below took 53
-// us, all of them behind the zeros.)
+// the prefix over digits and waves.  (By launches over tiles, as more rows take, 16,384 rows
+// took 53 us, all of them behind the zeros.)
 constexpr uint32_t kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr uint32_t kSortSteps = kSortRows / kSortThreads;
 template <typename T>

@@ -79,6 +79,12 @@ uint32_t check_types(std::initializer_list<uint32_t> types, pb_inference_error* 
   return PB_OK;
 }
 
+// binary32 holds 1 / sqrt(eps), what a row of zeros is multiplied by.
+uint32_t check_eps(double eps, pb_inference_error* err) {
+  if (!(eps >= 1e-75 && isfinite(eps))) return refuse(err, PB_ARITHMETIC, 0, 0, PB_FIELD_FINITE, 0);
+  return PB_OK;
+}
+
 // Distances and addresses of the buffers that are there.  Addresses of a buffer's end stay
 // below 2^62 bytes: at most 2^22 rows of 2^38 elements of 4 bytes.
 uint32_t check_buffers(std::initializer_list<Rows> all, pb_inference_error* err) {
@@ -240,7 +246,7 @@ uint32_t pb_norm_rows(pb_context* ctx, const void* d_x, uint32_t dtype, size_t c
   clear_error(err);
   uint32_t st = check_sizes(rows, cols, err);
   if (st != PB_OK || (st = check_types({dtype, weight_dtype, out_dtype}, err)) != PB_OK) return st;
-  if (!(eps > 0.0 && isfinite(eps))) return refuse(err, PB_ARITHMETIC, 0, 0, PB_FIELD_FINITE, 0);
+  if ((st = check_eps(eps, err)) != PB_OK) return st;
   const pb::NormParams p{d_x,  x_ld,   rows,      (uint32_t)cols, d_residual, residual_ld,
                          d_weight, weight_dtype, true, eps,     d_sum,      sum_ld,
                          d_out, out_dtype, out_ld, d_q,          q_ld,       d_scale, d_err};
@@ -270,7 +276,7 @@ uint32_t pb_norm_rows_grad(pb_context* ctx, const void* d_h, uint32_t dtype, siz
   uint32_t st = check_sizes(rows, cols, err);
   if (st != PB_OK || (st = check_types({dtype, weight_dtype, grad_dtype}, err)) != PB_OK)
     return st;
-  if (!(eps > 0.0 && isfinite(eps))) return refuse(err, PB_ARITHMETIC, 0, 0, PB_FIELD_FINITE, 0);
+  if ((st = check_eps(eps, err)) != PB_OK) return st;
   const size_t size = size_of(dtype);
   const Rows h{d_h, rows, cols, h_ld, size}, grad{d_grad, rows, cols, grad_ld, size_of(grad_dtype)};
   const Rows grad_sum{d_grad_sum, rows, cols, grad_sum_ld, size};

@@ -91,7 +91,7 @@ class HiddenRows:
             return None, 0
         ptr, r, c, ld = _matrix(x, name, self.device)
         kind = str(x.dtype).replace("torch.", "")
-        if kind not in ("int8", "uint8"):
+        if kind != "int8":
             raise ValueError(f"{name} must hold signed bytes, not {kind}")
         if rows is not None and r != rows or cols is not None and c != cols:
             raise ValueError(f"{name} has shape {_shape(x)}, not ({rows}, {cols})")

@@ -46,7 +46,7 @@ def embed_grad(grad, token, vocab, scale):
 
 def embed_grad_tolerance(total, want, absolute, scale, dtype):
     """`total` is the sum, `want` what is written (the sum, or that added to what was there)."""
-    # 31 additions of 32 rows at most in 32 bits; the factor and its product; the join's rounding; the addition
+    # at most 32 rows (the kernel takes 16) are added up in 32 bits; the factor and its product; the join's rounding; the addition
     scale32 = abs(float(np.float32(scale)) / scale - 1.0) if scale else 0.0
     inner = (31 + 3) * E * absolute + scale32 * total.abs() + E * want.abs()
     return out_tolerance(want, dtype, inner + tiny(torch.float32))
@@ -109,7 +109,7 @@ def norm_grad_tolerances(h, weight, grad, eps, want, want_weight, dtype):
     inner = E * (m * (2 * wg + 4 * hk) + 2 * m * (wg + hk) + want.abs())
     inner = inner + tiny(torch.float32) * (2 + m * (2 + f.abs()))
     terms = (g * f * m).abs().sum(0)
-    # m, h m and g h m; a thread adds up a row in 512 at most (or 768 rows), four waves' sums are added
+    # m, h m and g h m; a thread adds up a row in 512 at most (the kernel: in 1,024, or up to 768), four waves' sums are added
     n = min(768, -(-h.shape[0] // 512)) + 4
     return out_tolerance(want, dtype, inner), E * ((3 + n) * terms + want_weight.abs()) + tiny(torch.float32) * h.shape[0]
 

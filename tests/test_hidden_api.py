@@ -175,6 +175,15 @@ def test_reservation_is_checked():
     assert fn(None, 1, 0, None) == s.CAPACITY  # err may be NULL
 
 
+@pytest.mark.parametrize("name", ["norm", "norm_grad"])
+def test_the_root_of_eps_has_a_reciprocal(name):
+    """A row of zeros is multiplied by 1 / sqrt(eps), which binary32 has to hold."""
+    for eps in (1e-300, 1e-78, 0.99e-75):
+        assert call(name, eps=eps)[0] == s.ARITHMETIC, eps
+    for eps in (1e-75, 1e-12, 1.0, 1e300):
+        assert no_context(*call(name, eps=eps)), eps
+
+
 def test_header_constants():
     text = (s.LIB_PATH.parents[1] / "include" / "pbsample.h").read_text()
     for name in ("HIDDEN_MAX_ROWS", "HIDDEN_MAX_COLS"):
@@ -250,6 +259,16 @@ def test_shapes_and_types_are_checked(rows):
         with pytest.raises(ValueError):
             bad()
     assert [name for name, _ in rows.made] == ["pb_int8_matmul"]
+
+
+def test_unsigned_bytes_are_no_8_bit_rows(rows):
+    b = torch.int8
+    for bad in (lambda: rows.matmul(f(3, 8, dtype=torch.uint8), f(3), f(5, 8, dtype=b), f(5), out=f(3, 5)),
+                lambda: rows.matmul(f(3, 8, dtype=b), f(3), f(5, 8, dtype=torch.uint8), f(5), out=f(3, 5)),
+                lambda: rows.quantize(f(3, 8), q=f(3, 8, dtype=torch.uint8), scale=f(3))):
+        with pytest.raises(ValueError, match="signed bytes"):
+            bad()
+    assert not rows.made
 
 
 def test_reservations_grow_by_doubling_and_cover_every_pair(rows):
