@@ -215,8 +215,10 @@ __device__ __forceinline__ void store_by(const Int8Params& p, int8_t* slice,
                                          const float (&row_scale)[BM],
                                          const v16i (&acc)[BM][BN]) {
   constexpr uint32_t kSize = 16 / Out::kPer;           // bytes of an element
-  constexpr int kBlocks = 128 / (32 * (int)kSize);     // blocks of channels of a slice
+  constexpr int kWhole = 128 / (32 * (int)kSize);
+  constexpr int kBlocks = BN < kWhole ? BN : kWhole;  // blocks of channels of a slice
   static_assert(BN % kBlocks == 0, "whole slices");
+  constexpr uint32_t kLanes = kBlocks * 2u * kSize, kAtOnce = 64u / kLanes;  // a row's, and rows
   const uint32_t lane = lane_id(), j = lane & 31u, h = lane >> 5;
   typename Out::Raw* out = static_cast<typename Out::Raw*>(p.out);
 #pragma unroll
@@ -243,8 +245,8 @@ __device__ __forceinline__ void store_by(const Int8Params& p, int8_t* slice,
       }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (uint32_t s = 0; s < 4; ++s) {
-        const uint32_t r = s * 8u + lane / 8u, piece = lane % 8u;
+      for (uint32_t s = 0; s < 32u / kAtOnce; ++s) {
+        const uint32_t r = s * kAtOnce + lane / kLanes, piece = lane % kLanes;
         const uint4 v = *reinterpret_cast<const uint4*>(slice + r * kSlicePitch + piece * 16u);
         const uint32_t m = m0 + i * 32u + r, n = n0 + wn + k0 * 32u + piece * Out::kPer;
         if (m < p.rows && n < p.channels) {
@@ -668,50 +670,70 @@ uint32_t tiles(const Int8Params& p, uint32_t rows, uint32_t channels) {
 
 // Which kernel takes a product (us, both sides of each line; rows x channels x columns).
 //
-// Up to 16 rows of up to 16,384 channels go without LDS tiles, and one or two rows of whole
-// pieces of any channels; few / tiles:
-//   1 x 1,024 x 4,096  4.5 / 9.2     16 x 1,000 x 4,001  12.7 / 16.1     16 x 20,000 x 900   13.6 / 11.5
-//   8 x 4,000 x 2,000  4.1 / 6.5     16 x 8,192 x 8,192  17.2 / 17.5     1 x 50,257 x 1,001  16.5 / 13.8
-//   1 x 151,936 x 896  26 / 28       4 x 151,936 x 896   28.4 / 28.2     8 x 151,936 x 896   31.4 / 28.3
+// Up to 16 rows of up to 4,096 channels go without LDS tiles, and one or two rows of whole
+// pieces of any channels; few / the tiles that take it otherwise:
+//   16 x 4,096 x 4,096  6.9 / 7.4     8 x 8,192 x 8,192  14.6 / 12.5     1 x 8,192 x 8,192  13.4 / 12.4
+//   8 x 1,024 x 8,192   8.8 / 10.1    16 x 8,192 x 896    4.4 / 4.0      1 x 32,000 x 4,096  24 / 32
+//   16 x 4,001 x 4,001  13.2 / 15.5   1 x 8,192 x 8,001  24.4 / 23.4     1 x 151,936 x 896   26 / 28
+//   16 x 2,048 x 2,048  4.4 / 4.8     16 x 32,000 x 2,001  34 / 16       4 x 151,936 x 896   28.4 / 28.3
 //
-// Tiles by how many there are for 256 compute units: where tiles of 64 x 64 do not fill
-// them, eight waves a tile, the contraction cut by four; then 64 x 128 tiles, one and two a
-// unit; then 128 x 128, two a unit; and 256 x 256 where their rounds are few enough: a round
-// takes 1.25 to 1.6 times as long as one of 128 x 128 tiles (below a workgroup takes one of
-// them; one after the other, as it is done, they take 2 to 4 % less).  Of whole pieces:
-//                            64 x 64, K by 4   64 x 128, K by 2   64 x 128   128 x 128   256 x 256
-//   96 x 8,192 x 8,192                  18.5               24.7       32.5        43.9        96.0
-//   1,000 x 1,000 x 8,192               19.0               25.2       32.9        44.1        98.3
-//   256 x 8,192 x 8,192                 37.8               29.3       35.5        45.1        97.3
-//   512 x 4,096 x 4,096                 22.2               16.6       19.1        25.1        53.1
-//   500 x 5,000 x 896                   14.9               12.3        8.8         9.9        17.6
-//   2,048 x 2,048 x 2,048               26.9               19.0       15.3        16.2        30.3
-//   48 x 151,936 x 896                  58.0                  -       31.0           -           -
-//   1,024 x 8,192 x 8,192              139.6              106.4       97.8        80.6       106.5
-//   333 x 50,257 x 1,008                84.9               58.1       46.8        44.6        50.3
-//   1,000 x 10,000 x 896                46.0               29.6       23.1        23.6        19.2
-// Through registers:
-//   100 x 8,000 x 8,001                 41.4               63.5       86.8       106.8           -
-//   1,000 x 1,000 x 7,001               37.2               56.2       76.9        95.7           -
-//   2,000 x 2,000 x 2,001               35.6               23.9       27.0        31.9           -
-//   8 x 151,936 x 896                   44.6               32.1       28.7           -           -
-//   333 x 50,257 x 1,001                85.3               56.4       56.6        46.5           -
+// Tiles by how many there are for 256 compute units: where the small ones do not fill them,
+// eight waves take one, the contraction cut by eight or four.  32 x 32; 32 x 64, which up
+// to 64 rows run two a unit (their weights are read once, and wait for memory); 64 x 64;
+// then 64 x 128 tiles, one and two a unit; 128 x 128, two a unit; and 256 x 256 where their
+// rounds are few enough: a round takes 1.25 to 1.6 times as long as one of 128 x 128 tiles
+// (below a workgroup takes one of them; one after the other, as it is done, they take 2 to 4
+// % less).  Of whole pieces:
+//                       32 x 32   32 x 64   64 x 64   64 x 128   64 x 128   128 x 128   256 x 256
+//                        K by 8    K by 4    K by 4     K by 2
+//   24 x 8,192 x 8,192     12.6      14.5      17.3          -          -           -           -
+//   64 x 1,000 x 8,192     11.6      14.1      17.2          -          -           -           -
+//   300 x 1,024 x 4,096     8.9       8.6      10.6       14.1       17.8           -           -
+//   48 x 8,192 x 8,192     16.0      14.2      17.9       24.7       32.5        43.9        96.0
+//   32 x 16,384 x 4,096    12.7      12.4      13.8       14.4       17.9           -           -
+//   32 x 32,000 x 4,096    33.9      31.6      35.2       32.5       33.3           -           -
+//   32 x 50,304 x 896      12.7      11.7      21.2       14.1       10.6           -           -
+//   64 x 16,384 x 4,096    17.6      13.5      15.2       15.0       18.0           -           -
+//   64 x 32,000 x 4,096    42.9      38.1      36.1       32.8       33.6           -           -
+//   96 x 8,192 x 8,192     21.1      20.2      18.3       24.0       31.8        43.9        96.0
+//   256 x 4,096 x 4,096    15.9      11.9      11.0       14.4       17.8           -           -
+//   200 x 5,000 x 2,048    11.8      10.9      13.7        9.5       10.8           -           -
+//   256 x 8,192 x 8,192       -         -      37.8       29.3       35.5        45.1        97.3
+//   500 x 5,000 x 896         -         -      14.9       12.3        8.8         9.9        17.6
+//   2,048 x 2,048 x 2,048     -         -      26.9       19.0       15.3        16.2        30.3
+//   64 x 151,936 x 896     60.1      50.2      59.9       42.1       31.8           -           -
+//   1,024 x 8,192 x 8,192     -         -     139.6      106.4       97.8        80.6       106.5
+//   333 x 50,257 x 1,008      -         -      84.9       58.1       46.8        44.6        50.3
+//   1,000 x 10,000 x 896      -         -      46.0       29.6       23.1        23.6        19.2
+// Through registers (64 x 128 with K by 2, then of 64 bytes a step):
+//   24 x 8,192 x 8,001     27.5      33.2      41.8       64.1       87.2           -
+//   128 x 4,096 x 4,001    16.9      18.7      23.1       33.8       45.3           -
+//   32 x 32,000 x 2,001    18.7      15.9      20.1       21.8       27.1           -
+//   256 x 4,096 x 4,001    30.1      22.7      23.4       33.7       44.9           -
+//   200 x 5,000 x 2,001    22.6      19.7      19.2       19.5       24.6           -
+//   32 x 50,257 x 1,001    18.2      18.1      24.1       16.1       17.6           -
+//   2,000 x 2,000 x 2,001     -         -      35.6       23.9       27.0        31.9
+//   8 x 151,936 x 896         -         -      44.6       32.1       28.7           -
+//   333 x 50,257 x 1,001      -         -      85.3       56.4       56.6        46.5
 template <typename Out>
 hipError_t int8_as(const Int8Params& p, hipStream_t stream) {
   const bool whole = whole_pieces(p);
-  if (p.rows <= 16 && (p.channels <= 16384 || (p.rows <= 2 && whole)))
+  if (p.rows <= 16 && (p.channels <= 4096 || (p.rows <= 2 && whole)))
     return few_as<Out>(p, stream);
-  const uint32_t of64 = tiles(p, 64, 64), of128 = tiles(p, 64, 128);
-  const uint32_t rounds = (tiles(p, 128, 128) + 511u) / 512u;
+  const uint32_t of32 = tiles(p, 32, 32), of64 = tiles(p, 32, 64), of128 = tiles(p, 64, 128);
   if (!whole) {
-    if (of64 <= 256) return tile_as<Out, 2, 1, 1, 2, 256, 4>(p, stream);
+    if (of32 <= 512) return tile_as<Out, 1, 1, 1, 1, 256, 8>(p, stream);
+    if (of64 <= 512) return tile_as<Out, 1, 2, 1, 1, 256, 4>(p, stream);
     if (of128 <= 512) return tile_as<Out, 2, 2, 1, 2, 128, 2>(p, stream);
     if (p.rows <= 64) return tile_as<Out, 2, 2, 1, 2, 64, 1>(p, stream);
     return tile_as<Out, 2, 2, 2, 2, 64, 1>(p, stream);
   }
-  if (of64 <= 256) return pieces_as<Out, 2, 1, 1, 2, 256, 4, 4>(p, stream);
+  if (of32 <= 256) return pieces_as<Out, 1, 1, 1, 1, 256, 3, 8>(p, stream);
+  if (of64 <= (p.rows <= 64 ? 512u : 256u)) return pieces_as<Out, 1, 2, 1, 1, 256, 3, 4>(p, stream);
+  if (tiles(p, 64, 64) <= 256) return pieces_as<Out, 2, 1, 1, 2, 256, 4, 4>(p, stream);
   if (of128 <= 256) return pieces_as<Out, 2, 2, 1, 2, 256, 3, 2>(p, stream);
   if (of128 <= 512 || p.rows <= 64) return pieces_as<Out, 2, 2, 1, 2, 128, 3, 1>(p, stream);
+  const uint32_t rounds = (tiles(p, 128, 128) + 511u) / 512u;
   const uint32_t large = (tiles(p, 256, 256) + 255u) / 256u;
   if (8u * large < 5u * rounds) return large_as<Out>(p, stream);
   return pieces_as<Out, 2, 2, 2, 2, 128, 2, 1>(p, stream);

@@ -25,10 +25,14 @@ def ops():
 # rows x channels x columns, the columns in whole pieces of 16 bytes; run as they are and in rows that start anywhere
 SIZES = [
     # few rows: both numbers of rows and of channels at which they end
-    (1, 16_384, 64), (1, 16_385, 64), (2, 20_000, 48), (3, 20_000, 48), (16, 16_384, 32), (16, 16_385, 32), (17, 300, 32),
-    (16, 1, 16), (7, 5, 4_096),
-    # tiles of 64 x 64 with the contraction in four, up to 256 of them
-    (64, 16_384, 16), (96, 8_192, 912), (1_000, 1_000, 272), (64, 64, 1_040), (33, 70, 2_064),
+    (1, 16_384, 64), (1, 16_385, 64), (2, 20_000, 48), (3, 20_000, 48), (16, 4_096, 32), (16, 4_097, 32), (17, 4_096, 48),
+    (16, 16_385, 32), (17, 300, 32), (16, 1, 16), (7, 5, 4_096),
+    # tiles of 32 x 32 with the contraction in eight, up to 256 and 512 of them
+    (32, 8_192, 272), (32, 8_224, 272), (100, 2_040, 2_064), (32, 16_384, 144), (32, 16_416, 144), (64, 64, 1_040),
+    # of 32 x 64 with the contraction in four, up to 256 and 512 of them
+    (64, 16_384, 528), (64, 16_400, 528), (65, 5_440, 400), (65, 5_504, 400), (33, 16_384, 80), (33, 16_448, 80),
+    # of 64 x 64 with the contraction in four, up to 256 of them
+    (96, 8_192, 912), (1_000, 1_000, 272), (128, 8_192, 16), (128, 8_200, 272),
     # of 64 x 128 with the contraction in two
     (256, 8_192, 528), (200, 6_000, 400), (65, 8_200, 16),
     # of 64 x 128
