@@ -499,13 +499,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void int8_pieces_kernel(Int8Para
 
 // The same for many large tiles: a workgroup takes one after the other, and the first set of
 // the next is on its way while the last of this one is multiplied and its sums are stored.
-// 4,096 x 151,936 x 896 to bf16: 716 us, 1,560 TOP/s (a workgroup a tile 742); 4,096 x 8,192 x
-// 8,192 245 us, 2,240 TOP/s (252).  Without the stores the first takes 631: they end before
-// the next tile's second set, for loads wait behind them.
+// Tiles of 256 x 256: 4,096 x 151,936 x 896 to bf16 716 us, 1,560 TOP/s (a workgroup a tile
+// 742); 4,096 x 8,192 x 8,192 245 us, 2,240 TOP/s (252).  Without the stores the first takes
+// 631: they end before the next tile's second set, for loads wait behind them.  Of 128 x 256:
+// 1,024 x 8,192 x 8,192 73 us (128 x 128, two workgroups a unit, a tile each: 86), 700 x 6,144
+// x 4,096 32.8 (36.3), 3,000 x 8,192 x 1,024 35.3 (39.3), 384 x 50,304 x 896 30.3 (30.7),
+// 1,500 x 12,000 x 2,048 55.1 (52.3).
 constexpr uint32_t kLargeGroups = 256;  // one a compute unit
-template <typename Out>
-__global__ __launch_bounds__(512) void int8_large_kernel(Int8Params p, TilePlan plan) {
-  constexpr int WM = 2, WN = 4, BM = 4, BN = 2;
+template <typename Out, int WM, int WN, int BM, int BN>
+__global__ __launch_bounds__(64 * WM * WN) void int8_large_kernel(Int8Params p, TilePlan plan) {
   using T = Tile<WM, WN, BM, BN>;
   constexpr uint32_t TM = T::kRows, TN = T::kChannels, KB = 128, kPieces = KB / 16u;
   constexpr uint32_t kLoads = (TM + TN) * KB / 1024u / T::kWaves;
@@ -651,11 +653,13 @@ hipError_t pieces_as(const Int8Params& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename Out>
+template <typename Out, int WM, int WN, int BM, int BN>
 hipError_t large_as(const Int8Params& p, hipStream_t stream) {
-  const TilePlan t = plan_tiles<Tile<2, 4, 4, 2>>(p);
+  using T = Tile<WM, WN, BM, BN>;
+  const TilePlan t = plan_tiles<T>(p);
   const uint32_t all = t.m_tiles * t.n_tiles;
-  int8_large_kernel<Out><<<all < kLargeGroups ? all : kLargeGroups, 512, 0, stream>>>(p, t);
+  int8_large_kernel<Out, WM, WN, BM, BN>
+      <<<all < kLargeGroups ? all : kLargeGroups, T::kThreads, 0, stream>>>(p, t);
   return hipGetLastError();
 }
 
@@ -680,32 +684,35 @@ uint32_t tiles(const Int8Params& p, uint32_t rows, uint32_t channels) {
 // Tiles by how many there are for 256 compute units: where the small ones do not fill them,
 // eight waves take one, the contraction cut by eight or four.  32 x 32; 32 x 64, which up
 // to 64 rows run two a unit (their weights are read once, and wait for memory); 64 x 64;
-// then 64 x 128 tiles, one and two a unit; 128 x 128, two a unit; and 256 x 256 where their
-// rounds are few enough: a round takes 1.25 to 1.6 times as long as one of 128 x 128 tiles
-// (below a workgroup takes one of them; one after the other, as it is done, they take 2 to 4
-// % less).  Of whole pieces:
-//                       32 x 32   32 x 64   64 x 64   64 x 128   64 x 128   128 x 128   256 x 256
+// then 64 x 128 tiles, one and two a unit; 128 x 256; and 256 x 256 where their rounds are
+// few enough: one takes 1.4 to 1.8 times as long.  Of whole pieces:
+//                       32 x 32   32 x 64   64 x 64   64 x 128   64 x 128   128 x 256   256 x 256
 //                        K by 8    K by 4    K by 4     K by 2
 //   24 x 8,192 x 8,192     12.6      14.5      17.3          -          -           -           -
 //   64 x 1,000 x 8,192     11.6      14.1      17.2          -          -           -           -
 //   300 x 1,024 x 4,096     8.9       8.6      10.6       14.1       17.8           -           -
-//   48 x 8,192 x 8,192     16.0      14.2      17.9       24.7       32.5        43.9        96.0
+//   48 x 8,192 x 8,192     16.0      14.2      17.9       24.7       32.5           -           -
 //   32 x 16,384 x 4,096    12.7      12.4      13.8       14.4       17.9           -           -
 //   32 x 32,000 x 4,096    33.9      31.6      35.2       32.5       33.3           -           -
 //   32 x 50,304 x 896      12.7      11.7      21.2       14.1       10.6           -           -
 //   64 x 16,384 x 4,096    17.6      13.5      15.2       15.0       18.0           -           -
 //   64 x 32,000 x 4,096    42.9      38.1      36.1       32.8       33.6           -           -
-//   96 x 8,192 x 8,192     21.1      20.2      18.3       24.0       31.8        43.9        96.0
+//   96 x 8,192 x 8,192     21.1      20.2      18.3       24.0       31.8           -           -
 //   256 x 4,096 x 4,096    15.9      11.9      11.0       14.4       17.8           -           -
 //   200 x 5,000 x 2,048    11.8      10.9      13.7        9.5       10.8           -           -
-//   256 x 8,192 x 8,192       -         -      37.8       29.3       35.5        45.1        97.3
-//   500 x 5,000 x 896         -         -      14.9       12.3        8.8         9.9        17.6
-//   2,048 x 2,048 x 2,048     -         -      26.9       19.0       15.3        16.2        30.3
+//   256 x 8,192 x 8,192       -         -      37.8       29.3       35.5           -        97.3
+//   500 x 5,000 x 896         -         -      14.9       12.3        8.8           -        17.6
+//   2,048 x 2,048 x 2,048     -         -      26.9       19.0       15.3        18.8        29.1
 //   64 x 151,936 x 896     60.1      50.2      59.9       42.1       31.8           -           -
-//   1,024 x 8,192 x 8,192     -         -     139.6      106.4       97.8        80.6       106.5
-//   333 x 50,257 x 1,008      -         -      84.9       58.1       46.8        44.6        50.3
-//   1,000 x 10,000 x 896      -         -      46.0       29.6       23.1        23.6        19.2
-// Through registers (64 x 128 with K by 2, then of 64 bytes a step):
+//   700 x 6,144 x 4,096       -         -         -          -       42.4        32.8        52.3
+//   1,024 x 8,192 x 8,192     -         -         -          -       97.8        72.9        98.5
+//   333 x 50,304 x 1,008      -         -         -          -       46.8        36.6        38.0
+//   1,000 x 10,000 x 896      -         -         -          -       23.1        20.8        19.2
+//   3,000 x 8,192 x 1,024     -         -         -          -       48.5        35.3        38.1
+//   256 x 151,936 x 896       -         -         -          -          -        68.9        59.4
+//   4,096 x 4,096 x 4,096     -         -         -          -          -        75.0        65.9
+//   8,192 x 8,192 x 512       -         -         -          -          -        58.9        63.5
+// Through registers, 64 x 128 with K by 2 and without, and 128 x 128:
 //   24 x 8,192 x 8,001     27.5      33.2      41.8       64.1       87.2           -
 //   128 x 4,096 x 4,001    16.9      18.7      23.1       33.8       45.3           -
 //   32 x 32,000 x 2,001    18.7      15.9      20.1       21.8       27.1           -
@@ -733,10 +740,10 @@ hipError_t int8_as(const Int8Params& p, hipStream_t stream) {
   if (tiles(p, 64, 64) <= 256) return pieces_as<Out, 2, 1, 1, 2, 256, 4, 4>(p, stream);
   if (of128 <= 256) return pieces_as<Out, 2, 2, 1, 2, 256, 3, 2>(p, stream);
   if (of128 <= 512 || p.rows <= 64) return pieces_as<Out, 2, 2, 1, 2, 128, 3, 1>(p, stream);
-  const uint32_t rounds = (tiles(p, 128, 128) + 511u) / 512u;
-  const uint32_t large = (tiles(p, 256, 256) + 255u) / 256u;
-  if (8u * large < 5u * rounds) return large_as<Out>(p, stream);
-  return pieces_as<Out, 2, 2, 2, 2, 128, 2, 1>(p, stream);
+  const uint32_t rounds = (tiles(p, 128, 256) + kLargeGroups - 1u) / kLargeGroups;
+  const uint32_t large = (tiles(p, 256, 256) + kLargeGroups - 1u) / kLargeGroups;
+  if (8u * large < 5u * rounds) return large_as<Out, 2, 4, 4, 2>(p, stream);
+  return large_as<Out, 2, 4, 2, 2>(p, stream);
 }
 
 }  // namespace

@@ -37,8 +37,8 @@ SIZES = [
     (256, 8_192, 528), (200, 6_000, 400), (65, 8_200, 16),
     # of 64 x 128
     (300, 8_200, 144), (500, 8_190, 384), (20, 70_001, 80), (64, 40_000, 16),
-    # of 128 x 128
-    (1_024, 8_192, 272), (333, 30_001, 208), (129, 70_000, 16),
+    # of 128 x 256: one a workgroup, two and three; one step of columns and a ragged last one
+    (1_024, 8_192, 272), (333, 30_001, 208), (129, 70_000, 16), (300, 50_001, 112), (3_000, 8_190, 128), (700, 6_150, 400),
     # of 256 x 256: one a workgroup, two and three; one step of columns, two and a ragged last one
     (1_000, 10_000, 896), (2_048, 16_384, 16), (2_000, 17_001, 112), (2_000, 17_001, 128), (1_990, 17_001, 208),
     (2_048, 16_400, 256),
