@@ -123,7 +123,8 @@ __device__ __forceinline__ double wave_add(double v) {
 
 // ---- table rows of tokens ----
 
-// 2^kShift threads take a row.
+// 2^shift threads take a row.  40 rows of 896 bf16: 2.4 us, a launch; 16,384 of them: 11.4 us
+// (5.1 TB/s read and written).
 template <typename In, typename Out>
 __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p, uint32_t shift) {
   const uint32_t row = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
@@ -465,7 +466,9 @@ __device__ __forceinline__ void put_table(const EmbedGradParams& p, uint32_t id,
 }
 
 // One wave: the sorted rows [part kSumRows, + kSumRows) and 64 chunks of columns.  All of the
-// part's rows are requested before the first is added.
+// part's rows are requested before the first is added, which bounds a part by the registers.
+// 16,384 rows of 896 bf16 14 us, 700 of 1,001 in 32 bits 8.5: one round trip for the ids, one
+// for the rows.
 template <typename G, typename T>
 __global__ __launch_bounds__(256) void sum_rows_kernel(EmbedGradParams p, uint32_t last,
                                                        uint32_t col_tiles, uint32_t units) {
@@ -552,7 +555,7 @@ __device__ __forceinline__ uint32_t token_end(const uint32_t* id, uint32_t own, 
   return lo;
 }
 
-// The sums that cross parts.  A wave takes 256 columns of a token of up to kLongParts more
+// The sums that cross parts, 5 to 11 us.  A wave takes 256 columns of a token of up to kLongParts more
 // parts; a workgroup 64 columns of a longer one, its waves a run of parts each.
 constexpr uint32_t kJoinWaves = 16;
 template <typename T>
@@ -751,6 +754,11 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t 
   return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), low, 0x05040100u);
 }
 
+// A row's norm and its 8-bit rounding, from one read of the row: 16,384 rows of 4,096 bf16 with
+// a residual, the sum kept, 88 us (470 MB, 5.3 TB/s: no byte more than the formulas need by
+// the counters).  A single row of 896: 3.5 us, a launch and its chain of read, join over the
+// waves, quotient, store.
+//
 // kNarrow: rows and weight of one 16-bit type, or no weight.  Their products h w are exact in
 // binary32, so the largest is, and all but values near a half are rounded in 32 bits:
 // p (127 / top) is off by 2^-24 of 127 there, and those that come nearer than 2^-15 to a half
@@ -933,7 +941,8 @@ __global__ __launch_bounds__(T < 128 ? 256 : T) void norm_kernel(NormParams p) {
   }
 }
 
-// The gradient.  With m = rstd and c = mean(g w h): dh = gh + m (g w - h m^2 c), and
+// The gradient, bound by its rows' bytes: 8,192 rows of 2,048 bf16 25.9 us (5.5 TB/s
+// with the parts' sums).  With m = rstd and c = mean(g w h): dh = gh + m (g w - h m^2 c), and
 // the weight's is the sum of g h m over the rows.  The statistics are taken anew from h,
 // which is read anyway.  A workgroup goes over rows, the next one requested before the one at
 // hand is worked out, and holds its sums of the weight's gradient in registers; they are
@@ -1085,7 +1094,8 @@ __global__ __launch_bounds__(T < 128 ? 256 : T) void norm_grad_kernel(NormGradPa
 }
 
 // The workgroups' sums of the weight's gradient: 16 columns a workgroup, 64 of the sums at a
-// time.
+// time.  A launch of its own, 4 to 5 us: joined by the last workgroup to come instead, one
+// compute unit would read them all (1,024 x 2,048 sums: 8 MB).
 __global__ __launch_bounds__(1024) void norm_weight_kernel(NormGradParams p) {
   __shared__ double parts[64][16];
   const uint32_t c = threadIdx.x % 16u, k0 = threadIdx.x / 16u;
@@ -1115,29 +1125,57 @@ uint32_t row_shift(uint32_t cols) {
 
 uint32_t sort_tiles(uint32_t rows) { return (rows + kSortTile - 1u) / kSortTile; }
 
-// Workgroups of the norm's gradient, each with at most kMaxTerms rows a thread.
-constexpr uint32_t kGradGroups = 1024;
+// Chunks of a row's plan below: its threads times theirs.
+uint32_t row_span(uint32_t cols) {
+  uint32_t span = 64;
+  while (span * kChunk < cols) span *= 2;
+  return span;
+}
+
+// Workgroups of the norm's gradient.  More have more rows on their way, fewer leave fewer sums
+// to join: as many as hold kGradChunks chunks at once, 512 or more, and none with more than
+// kGradTerms rows a thread.  512 / 1,024 / 2,048 of them, us:
+//   65,536 x 512 (256 chunks)     58 /  57 /  59     16,384 x 4,096 (512)  103 / 119 / 118
+//   65,536 x 896 (128)           215 / 126 / 100     8,192 x 8,192 (1,024) 109 / 117 / 134
+//   8,192 x 2,048 (256)         33.1 / 32.8 / 37.8
+constexpr uint32_t kGradChunks = 1u << 18;
 constexpr uint32_t kGradTerms = 768;
-uint32_t grad_groups(uint32_t rows, uint32_t rows_at_once) {
-  const uint32_t all = (rows + rows_at_once - 1u) / rows_at_once;
-  const uint32_t least = (all + kGradTerms - 1u) / kGradTerms;
-  const uint32_t most = least > kGradGroups ? least : kGradGroups;
+uint32_t grad_groups(uint32_t rows, uint32_t cols) {
+  const uint32_t span = row_span(cols), at_once = span < 128 ? 256 / span : 1;
+  const uint32_t all = (rows + at_once - 1u) / at_once;
+  const uint32_t held = kGradChunks / (span * at_once), least = (all + kGradTerms - 1u) / kGradTerms;
+  uint32_t most = held > 512 ? held : 512;
+  if (most < least) most = least;
   return all < most ? all : most;
 }
 
 size_t round_up(size_t bytes) { return (bytes + 255u) & ~(size_t)255u; }
 
-// A row's threads and their chunks: few of them, so that many rows are on their way at once.
+// A row's threads and their chunks.  One chunk a thread, and two where the statistics' join
+// over the waves then weighs more; but two as well where there are rows enough to keep the
+// memory busy, so that more of them are on their way.  Norms of bf16 rows to 8 bits, us (threads,
+// chunks):
+//                  1 row                                70 rows                65,536 to 8,192 rows
+//   512   (64, 1)  2.6 (128, 1) 2.9                      3.6 / 3.8               56 / 77
+//   896   (64, 2)  3.7 (128, 1) 3.1 (256, 1) 3.2         5.3 / 3.9 / 4.1         96 / 91 / 159
+//   2,048 (128, 2) 3.1 (256, 1) 3.0 (512, 1) 3.5         4.8 / 4.1 / 4.2         93 / 90 / 159
+//   4,096 (128, 4) 4.2 (256, 2) 3.6 (512, 1) 3.2         7.2 / 5.3 / 4.4        104 / 91 / 95
+//   8,192 (256, 4) 4.6 (512, 2) 3.8 (1024, 1) 4.2        8.0 / 6.0 / 5.9        109 / 99 / 136
+//   16,384 (512, 4) 5.3 (1024, 2) 5.4                    9.2 / 8.7              123 / 122
+constexpr uint32_t kManyRows = 1024;  // 512 rows of 4,096: (256, 2) 6.6, (512, 1) 6.3; 8,192: 48.8, 49.8
 template <typename E, bool kOne, template <typename, bool, int, int> class Launch, typename P>
 hipError_t by_width(const P& p, hipStream_t stream) {
-  const uint32_t chunks = (p.cols + kChunk - 1u) / kChunk;
-  if (chunks <= 64) return Launch<E, kOne, 64, 1>::run(p, stream);
-  if (chunks <= 128) return Launch<E, kOne, 128, 1>::run(p, stream);
-  if (chunks <= 256) return Launch<E, kOne, 256, 1>::run(p, stream);
-  if (chunks <= 512) return Launch<E, kOne, 256, 2>::run(p, stream);
-  if (chunks <= 1024) return Launch<E, kOne, 512, 2>::run(p, stream);
-  if (chunks <= 2048) return Launch<E, kOne, 1024, 2>::run(p, stream);
-  return Launch<E, kOne, 1024, 4>::run(p, stream);
+  switch (row_span(p.cols)) {
+    case 64: return Launch<E, kOne, 64, 1>::run(p, stream);
+    case 128: return Launch<E, kOne, 128, 1>::run(p, stream);
+    case 256: return Launch<E, kOne, 256, 1>::run(p, stream);
+    case 512:
+      return p.rows < kManyRows ? Launch<E, kOne, 512, 1>::run(p, stream)
+                                : Launch<E, kOne, 256, 2>::run(p, stream);
+    case 1024: return Launch<E, kOne, 512, 2>::run(p, stream);
+    case 2048: return Launch<E, kOne, 1024, 2>::run(p, stream);
+    default: return Launch<E, kOne, 1024, 4>::run(p, stream);
+  }
 }
 
 template <typename E, bool kNarrow, int T, int C>
@@ -1152,9 +1190,9 @@ struct NormLaunch {
 template <typename E, bool kSame, int T, int C>
 struct NormGradLaunch {
   static hipError_t run(const NormGradParams& in, hipStream_t stream) {
-    constexpr uint32_t kRows = T < 128 ? 256 / T : 1;
+    constexpr uint32_t kRows = T < 128 ? 256 / T : 1;  // as grad_groups has it
     NormGradParams p = in;
-    p.groups = grad_groups(p.rows, kRows);
+    p.groups = grad_groups(p.rows, p.cols);
     hipError_t e = hipSuccess;
     if (p.groups != 0) {  // without rows the weight's gradient is zeros
       norm_grad_kernel<E, kSame, T, C><<<p.groups, T * kRows, 0, stream>>>(p);
@@ -1243,7 +1281,7 @@ size_t embed_grad_bytes(uint32_t rows, size_t cols) {
 }
 
 size_t norm_grad_bytes(uint32_t rows, size_t cols) {
-  return (size_t)grad_groups(rows, 1) * cols * 4;
+  return (size_t)grad_groups(rows, (uint32_t)cols) * cols * 4;
 }
 
 size_t hidden_workspace_bytes(uint32_t rows, size_t cols) {

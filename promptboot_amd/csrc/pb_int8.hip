@@ -60,7 +60,8 @@ __device__ __forceinline__ float scaled(int sum, float s, float ws, const float*
 // D[4 (l / 16) + i][l % 16].  A wave takes 16 channels and all rows, or the split-th part
 // of the contraction of them; the waves of a workgroup that share their channels add up
 // through LDS.  No barrier stands between a load and its use, so that a short product is
-// little more than a launch and two round trips.
+// little more than a launch and two round trips.  1 x 151,936 x 896: 25.7 us, 5.3 TB/s of
+// weights; 1 x 4,096 x 4,096: 5.5 us; 16 x 1,000 x 4,096: 6.2.
 constexpr uint32_t kFewWaves = 4;
 template <typename Out>
 __global__ __launch_bounds__(64 * kFewWaves) void int8_few_kernel(Int8Params p, uint32_t split) {
