@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from promptboot_amd import hip
-from promptboot_amd.hidden import HiddenRows
+from promptboot_amd.hidden import HIDDEN_MAX_ROWS, HiddenRows
+from promptboot_amd.scores import SCORE_MAX_VOCAB
 from tests import hidden_reference as ref
 from tests.test_gpu_hidden import DEV, EPS, TYPES, gen, in_8_bits, make, make_bytes, near, space, untouched
 
@@ -199,6 +200,66 @@ def test_rows_of_zeros_with_any_eps(ops, dtype, eps):
     else:
         near(dh, want, ref.out_tolerance(want, TYPES[dtype], 2.01 * ref.E * want.abs()), "grad_h")
     assert (dw == 0).all()
+
+
+# ---- the largest numbers of rows, ids and channels ----
+
+def test_the_most_rows_and_channels(ops):
+    g = gen(1)
+    most = HIDDEN_MAX_ROWS
+    q, scale = make_bytes(g, most, 16), torch.rand(most, generator=g, device=DEV)
+    weight, weight_scale = make_bytes(g, 3, 16), torch.rand(3, generator=g, device=DEV)
+    for cols in (16, 15):  # whole pieces and not
+        out = torch.empty((most, 3), device=DEV)
+        ops.matmul(q[:, :cols], scale, weight[:, :cols], weight_scale, out=out)
+        want, product = ref.matmul(q[:, :cols], scale, weight[:, :cols], weight_scale)
+        near(out, want, ref.matmul_tolerance(want, product, torch.float32), "rows")
+    channels = SCORE_MAX_VOCAB
+    weight, weight_scale = make_bytes(g, channels, 16), torch.rand(channels, generator=g, device=DEV)
+    for rows in (1, 5, 20):
+        for cols in (16, 15):
+            out = torch.empty((rows, channels), dtype=torch.bfloat16, device=DEV)
+            ops.matmul(q[:rows, :cols], scale[:rows], weight[:, :cols], weight_scale, out=out)
+            for at in range(0, channels, 1 << 21):
+                w, ws, o = weight[at:at + (1 << 21), :cols], weight_scale[at:at + (1 << 21)], out[:, at:at + (1 << 21)]
+                want, product = ref.matmul(q[:rows, :cols], scale[:rows], w, ws)
+                near(o, want, ref.matmul_tolerance(want, product, torch.bfloat16), (rows, cols, at))
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_the_most_rows_and_ids_of_a_table(ops, accumulate):
+    g = gen(2)
+    rows, vocab, cols = HIDDEN_MAX_ROWS, SCORE_MAX_VOCAB, 3
+    table = torch.randn((vocab, cols), generator=g, device=DEV)
+    token = torch.randint(-1, vocab, (rows,), generator=g, device=DEV)
+    token[:40_000] = vocab - 1
+    out = torch.empty((rows, cols), device=DEV)
+    ops.embed(table, token.int(), out=out)
+    assert torch.equal(out, torch.where((token >= 0)[:, None], table[token.clamp(min=0)], torch.zeros_like(out)))
+    grad = torch.randn((rows, cols), generator=g, device=DEV)
+    total, absolute = ref.embed_grad(grad, token, vocab, 1.0)
+    got = table.clone()
+    ops.embed_grad(grad, token.int(), table_grad=got, accumulate=accumulate)
+    want = total + table.double() if accumulate else total
+    near(got, want, ref.embed_grad_tolerance(total, want, absolute, 1.0, torch.float32), "table")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_most_rows_of_a_norm(ops, dtype):
+    g = gen(3)
+    rows, cols = HIDDEN_MAX_ROWS, 9
+    x, w = make(g, rows, cols, dtype), (1 + 0.3 * torch.randn(cols, generator=g, device=DEV)).to(TYPES[dtype])
+    out, q, scale = torch.empty_like(x), torch.empty((rows, cols), dtype=torch.int8, device=DEV), torch.empty(rows, device=DEV)
+    ops.norm(x, w, eps=EPS, out=out, q=q, scale=scale)
+    want = ref.norm(x, w, EPS)
+    near(out, want, ref.norm_tolerance(want, TYPES[dtype], w), "out")
+    in_8_bits(q, scale, x, w, EPS, cols)
+    grad, dh, dw = make(g, rows, cols, dtype), torch.empty_like(x), torch.empty(cols, device=DEV)
+    ops.norm_grad(x, w, grad, eps=EPS, grad_h=dh, grad_weight=dw)
+    want, want_weight = ref.norm_grad(x, w, grad, EPS)
+    tol, tol_weight = ref.norm_grad_tolerances(x, w, grad, EPS, want, want_weight, TYPES[dtype])
+    near(dh, want, tol, "grad_h")
+    near(dw, want_weight, tol_weight, "grad_weight")
 
 
 # ---- captured ----
