@@ -47,9 +47,10 @@ __device__ __forceinline__ v4i load_piece(const int8_t* row, uint32_t at, uint32
              (int)__builtin_amdgcn_alignbyte(0u, (uint32_t)v[3], shift)};
 }
 
-__device__ __forceinline__ float scaled(int sum, float s, float ws, const float* bias, float b) {
-  const float y = (float)sum * s * ws;
-  return bias != nullptr ? y + b : y;
+// A channel without a bias has -0, which leaves every number as it is.
+constexpr float kNoBias = -0.0f;
+__device__ __forceinline__ float scaled(int sum, float s, float ws, float bias) {
+  return (float)sum * s * ws + bias;
 }
 
 // ---- few rows of short products ----
@@ -121,13 +122,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void int8_few_kernel(Int8Params p, 
     }
   }
   if (n >= p.channels) return;
-  const float ws = p.weight_scale[n], bias = p.bias ? p.bias[n] : 0.0f;
+  const float ws = p.weight_scale[n], bias = p.bias ? p.bias[n] : kNoBias;
   typename Out::Raw* out = static_cast<typename Out::Raw*>(p.out) + n;
 #pragma unroll
   for (uint32_t e = 0; e < 4; ++e) {
     const uint32_t r = lane / 16u * 4u + e;
     if (r < p.rows)
-      out[(size_t)r * p.out_ld] = Out::raw(scaled(acc[e], p.scale[r], ws, p.bias, bias));
+      out[(size_t)r * p.out_ld] = Out::raw(scaled(acc[e], p.scale[r], ws, bias));
   }
 }
 
@@ -222,6 +223,19 @@ __device__ __forceinline__ void store_by(const Int8Params& p, int8_t* slice,
   constexpr uint32_t kLanes = kBlocks * 2u * kSize, kAtOnce = 64u / kLanes;  // a row's, and rows
   const uint32_t lane = lane_id(), j = lane & 31u, h = lane >> 5;
   typename Out::Raw* out = static_cast<typename Out::Raw*>(p.out);
+  // the lane's channels: 32 k + 2 e + 4 h and the three next to it, from register e on (with
+  // four blocks of rows the registers hold no biases too)
+  constexpr bool kHold = BM < 4;
+  float4 ws[BN][4], bs[kHold ? BN : 1][4];
+#pragma unroll
+  for (int k = 0; k < BN; ++k) {
+#pragma unroll
+    for (uint32_t e = 0; e < 16; e += 4) {
+      const uint32_t c = wn + k * 32u + 2u * e + 4u * h;
+      ws[k][e / 4] = *reinterpret_cast<const float4*>(chan_scale + c);
+      if constexpr (kHold) bs[k][e / 4] = *reinterpret_cast<const float4*>(chan_bias + c);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < BM; ++i) {
 #pragma unroll
@@ -230,14 +244,17 @@ __device__ __forceinline__ void store_by(const Int8Params& p, int8_t* slice,
       for (int k = k0; k < k0 + kBlocks; ++k) {
 #pragma unroll
         for (uint32_t e = 0; e < 16; e += 4) {
-          const uint32_t c = k * 32u + 2u * e + 4u * h;  // of the wave's channels
-          const float4 ws = *reinterpret_cast<const float4*>(chan_scale + wn + c);
-          const float4 bs = *reinterpret_cast<const float4*>(chan_bias + wn + c);
-          const float y0 = scaled(acc[i][k][e], row_scale[i], ws.x, p.bias, bs.x);
-          const float y1 = scaled(acc[i][k][e + 1], row_scale[i], ws.y, p.bias, bs.y);
-          const float y2 = scaled(acc[i][k][e + 2], row_scale[i], ws.z, p.bias, bs.z);
-          const float y3 = scaled(acc[i][k][e + 3], row_scale[i], ws.w, p.bias, bs.w);
-          int8_t* to = slice + j * kSlicePitch + (c - k0 * 32u) * kSize;
+          const float4 w = ws[k][e / 4];
+          float4 b;
+          if constexpr (kHold)
+            b = bs[k][e / 4];
+          else
+            b = *reinterpret_cast<const float4*>(chan_bias + wn + k * 32u + 2u * e + 4u * h);
+          const float y0 = scaled(acc[i][k][e], row_scale[i], w.x, b.x);
+          const float y1 = scaled(acc[i][k][e + 1], row_scale[i], w.y, b.y);
+          const float y2 = scaled(acc[i][k][e + 2], row_scale[i], w.z, b.z);
+          const float y3 = scaled(acc[i][k][e + 3], row_scale[i], w.w, b.w);
+          int8_t* to = slice + j * kSlicePitch + ((k - k0) * 32u + 2u * e + 4u * h) * kSize;
           if constexpr (kSize == 4)
             *reinterpret_cast<float4*>(to) = make_float4(y0, y1, y2, y3);
           else
@@ -288,7 +305,7 @@ __device__ __forceinline__ void load_channels(const Int8Params& p, uint32_t n0, 
   for (uint32_t c = threadIdx.x; c < TN; c += kThreads) {
     const bool real = n0 + c < p.channels;
     scale[c] = real ? p.weight_scale[n0 + c] : 0.0f;
-    bias[c] = real && p.bias ? p.bias[n0 + c] : 0.0f;
+    bias[c] = real && p.bias ? p.bias[n0 + c] : kNoBias;
   }
 }
 
@@ -569,7 +586,7 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_large_kernel(Int8Params p, 
     const uint32_t n = n0 + threadIdx.x;
     const bool real = threadIdx.x < TN && n < p.channels;
     s.chan = real ? p.weight_scale[n] : 0.0f;
-    s.bias = real && p.bias ? p.bias[n] : 0.0f;
+    s.bias = real && p.bias ? p.bias[n] : kNoBias;
     return s;
   };
   uint32_t item = blockIdx.x, use = 0, turn = 0;

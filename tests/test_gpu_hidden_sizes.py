@@ -79,6 +79,21 @@ def test_matmul_of_few_rows(ops, rows):
             assert untouched(full, 37, 5.0)
 
 
+@pytest.mark.parametrize("rows,channels,cols", [(3, 50, 64), (20, 200, 48), (20, 200, 47), (70, 9_000, 64), (700, 6_150, 400),
+                                                (2_000, 17_001, 112), (333, 30_001, 201)])
+def test_zeros_keep_their_sign_without_a_bias(ops, rows, channels, cols):
+    q, weight = torch.zeros((rows, cols), dtype=torch.int8, device=DEV), make_bytes(gen(1), channels, cols)
+    scale, weight_scale = torch.full((rows,), -2.0, device=DEV), torch.ones(channels, device=DEV)
+    weight_scale[1::2] = -1.0
+    out = torch.full((rows, channels), 5.0, device=DEV)
+    ops.matmul(q, scale, weight, weight_scale, out=out)
+    want = torch.zeros(channels, device=DEV)
+    want[0::2] = -0.0
+    assert torch.equal(out.view(torch.int32), want.view(torch.int32).expand(rows, -1))
+    ops.matmul(q, scale, weight, weight_scale, out=out, bias=torch.zeros(channels, device=DEV))
+    assert not out.view(torch.int32).any()  # -0 + 0
+
+
 # ---- the table's gradient ----
 
 def table_gradient(ops, g, rows, vocab, cols, dtype, table_dtype, token, pad, shift=0):
