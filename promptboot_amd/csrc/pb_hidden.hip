@@ -1285,8 +1285,15 @@ size_t norm_grad_bytes(uint32_t rows, size_t cols) {
 }
 
 size_t hidden_workspace_bytes(uint32_t rows, size_t cols) {
-  const size_t a = embed_grad_bytes(rows, cols), b = norm_grad_bytes(rows, cols);
-  return a > b ? a : b;
+  size_t most = embed_grad_bytes(rows, cols);
+  auto hold = [&](size_t c) {
+    const size_t b = norm_grad_bytes(rows, c);
+    if (b > most) most = b;
+  };
+  hold(cols);
+  // narrower rows may have more workgroups: the widest of each plan
+  for (size_t c = 64 * kChunk; c < cols; c *= 2) hold(c);
+  return most;
 }
 
 void place_embed_grad(void* work, EmbedGradParams* p) {

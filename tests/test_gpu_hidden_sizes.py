@@ -277,6 +277,26 @@ def test_the_most_rows_of_a_norm(ops, dtype):
     near(dw, want_weight, tol_weight, "grad_weight")
 
 
+@pytest.mark.parametrize("rows,cols", [(5_000, 1_500), (3_000, 520), (2_000, 1_025), (900, 5_000)])
+def test_a_reservation_holds_for_every_smaller_call(rows, cols):
+    """Narrower rows may be split over more workgroups than wider ones."""
+    o = HiddenRows(0)
+    try:
+        o.reserve(rows, cols)
+        for c in [c for c in (8, 511, 512, 513, 1_000, 1_024, 1_025, 1_500, 2_048, 4_096, cols) if c <= cols]:
+            for r in (1, rows // 2, rows):
+                x, dw = torch.ones((r, c), device=DEV), torch.empty(c, device=DEV)
+                o.norm_grad(x, None, x, eps=EPS, grad_weight=dw)
+                table, token = torch.empty((9, c), device=DEV), torch.full((r,), 3, dtype=torch.int32, device=DEV)
+                o.embed_grad(x, token, table_grad=table)
+                assert (table[3] == r).all() and (table[4] == 0).all()
+                near(dw, torch.full((c,), r / math.sqrt(1 + EPS), dtype=torch.float64, device=DEV),
+                     torch.full((c,), ref.E * 30.0 * r, device=DEV), "grad_weight")
+        assert o._reserved == (rows, cols)
+    finally:
+        o.close()
+
+
 # ---- captured ----
 
 @pytest.mark.parametrize("rows", [700, 16_384, 16_385])
