@@ -343,3 +343,36 @@ def test_gradients_in_a_captured_graph(rows, accumulate):
         graph.close()
     finally:
         ops.close()
+
+
+@pytest.mark.parametrize("rows,channels,cols", [(2, 5_000, 896), (30, 2_000, 512), (60, 9_000, 256), (100, 9_000, 256),
+                                                (300, 9_000, 256), (700, 6_150, 400), (2_000, 17_001, 112), (50, 3_000, 201),
+                                                (333, 30_001, 201)])
+def test_products_in_a_captured_graph_and_on_two_streams(ops, rows, channels, cols):
+    """A product of each kernel, replayed on new rows, and two of them at once."""
+    g = gen(rows)
+    q, weight = make_bytes(g, rows, cols), make_bytes(g, channels, cols)
+    scale, weight_scale = torch.rand(rows, generator=g, device=DEV), torch.rand(channels, generator=g, device=DEV)
+    out, other = torch.empty((rows, channels), device=DEV), torch.empty((rows, channels), device=DEV)
+    streams = hip.Stream(), hip.Stream()
+    calls = [ops.bind_matmul(q, scale, weight, weight_scale, out=o, stream=s) for o, s in zip((out, other), streams)]
+    torch.cuda.synchronize()
+    graph = hip.Graph(streams[0])
+    graph.begin()
+    calls[0]()
+    calls[0]()
+    graph.end()
+    for _ in range(3):
+        q.copy_(torch.randint(-127, 128, (rows, cols), generator=g, device=DEV))
+        want, product = ref.matmul(q, scale, weight, weight_scale)
+        out.fill_(5.0)
+        other.fill_(5.0)
+        torch.cuda.synchronize()
+        graph.launch()
+        for _ in range(3):
+            calls[1]()
+        for s in streams:
+            s.synchronize()
+        near(out, want, ref.matmul_tolerance(want, product, torch.float32), "replayed")
+        assert torch.equal(out, other)
+    graph.close()
