@@ -730,27 +730,36 @@ uint32_t tiles(const Int8Params& p, uint32_t rows, uint32_t channels) {
 //   256 x 151,936 x 896       -         -         -          -          -        68.9        59.4
 //   4,096 x 4,096 x 4,096     -         -         -          -          -        75.0        65.9
 //   8,192 x 8,192 x 512       -         -         -          -          -        58.9        63.5
-// Through registers, 64 x 128 with K by 2 and without, and 128 x 128:
-//   24 x 8,192 x 8,001     27.5      33.2      41.8       64.1       87.2           -
-//   128 x 4,096 x 4,001    16.9      18.7      23.1       33.8       45.3           -
-//   32 x 32,000 x 2,001    18.7      15.9      20.1       21.8       27.1           -
-//   256 x 4,096 x 4,001    30.1      22.7      23.4       33.7       44.9           -
-//   200 x 5,000 x 2,001    22.6      19.7      19.2       19.5       24.6           -
-//   32 x 50,257 x 1,001    18.2      18.1      24.1       16.1       17.6           -
-//   2,000 x 2,000 x 2,001     -         -      35.6       23.9       27.0        31.9
-//   8 x 151,936 x 896         -         -      44.6       32.1       28.7           -
-//   333 x 50,257 x 1,001      -         -      85.3       56.4       56.6        46.5
+// Through registers, 64 x 128 with K by 2 and without, 128 x 128 two a unit, and 256 x 256 by
+// the same rule (for a round of 128 x 128, 1.2 to 1.9):
+//   24 x 8,192 x 8,001     27.5      33.2      41.8       64.1       87.2           -           -
+//   128 x 4,096 x 4,001    16.9      18.7      23.1       33.8       45.3           -           -
+//   32 x 32,000 x 2,001    18.7      15.9      20.1       21.8       27.1           -           -
+//   256 x 4,096 x 4,001    30.1      22.7      23.4       33.7       44.9           -           -
+//   200 x 5,000 x 2,001    22.6      19.7      19.2       19.5       24.6           -           -
+//   32 x 50,257 x 1,001    18.2      18.1      24.1       16.1       17.6           -           -
+//   2,000 x 2,000 x 2,001     -         -      35.6       23.9       27.0        31.9           -
+//   8 x 151,936 x 896         -         -      44.6       32.1       28.7           -           -
+//   300 x 20,001 x 2,001      -         -         -          -          -        34.6        44.1
+//   1,500 x 12,000 x 1,001    -         -         -          -          -        44.0        53.4
+//   333 x 50,257 x 1,001      -         -      85.3       56.4       56.6        54.9        53.4
+//   2,000 x 20,000 x 2,001    -         -         -          -          -       165.5       137.0
+//   4,096 x 4,096 x 4,001     -         -         -          -          -       140.4        83.3
+//   4,096 x 30,001 x 897      -         -         -          -          -       262.3       239.2
 template <typename Out>
 hipError_t int8_as(const Int8Params& p, hipStream_t stream) {
   const bool whole = whole_pieces(p);
   if (p.rows <= 16 && (p.channels <= 4096 || (p.rows <= 2 && whole)))
     return few_as<Out>(p, stream);
   const uint32_t of32 = tiles(p, 32, 32), of64 = tiles(p, 32, 64), of128 = tiles(p, 64, 128);
+  const uint32_t large = (tiles(p, 256, 256) + kLargeGroups - 1u) / kLargeGroups;
   if (!whole) {
     if (of32 <= 512) return tile_as<Out, 1, 1, 1, 1, 256, 8>(p, stream);
     if (of64 <= 512) return tile_as<Out, 1, 2, 1, 1, 256, 4>(p, stream);
     if (of128 <= 512) return tile_as<Out, 2, 2, 1, 2, 128, 2>(p, stream);
     if (p.rows <= 64) return tile_as<Out, 2, 2, 1, 2, 64, 1>(p, stream);
+    const uint32_t rounds = (tiles(p, 128, 128) + 511u) / 512u;
+    if (8u * large < 5u * rounds) return tile_as<Out, 2, 4, 4, 2, 128, 1>(p, stream);
     return tile_as<Out, 2, 2, 2, 2, 64, 1>(p, stream);
   }
   if (of32 <= 256) return pieces_as<Out, 1, 1, 1, 1, 256, 3, 8>(p, stream);
@@ -759,7 +768,6 @@ hipError_t int8_as(const Int8Params& p, hipStream_t stream) {
   if (of128 <= 256) return pieces_as<Out, 2, 2, 1, 2, 256, 3, 2>(p, stream);
   if (of128 <= 512 || p.rows <= 64) return pieces_as<Out, 2, 2, 1, 2, 128, 3, 1>(p, stream);
   const uint32_t rounds = (tiles(p, 128, 256) + kLargeGroups - 1u) / kLargeGroups;
-  const uint32_t large = (tiles(p, 256, 256) + kLargeGroups - 1u) / kLargeGroups;
   if (8u * large < 5u * rounds) return large_as<Out, 2, 4, 4, 2>(p, stream);
   return large_as<Out, 2, 4, 2, 2>(p, stream);
 }

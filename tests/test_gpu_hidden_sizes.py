@@ -42,7 +42,7 @@ SIZES = [
     (1_024, 8_192, 272), (333, 30_001, 208), (129, 70_000, 16), (300, 50_001, 112), (3_000, 8_190, 128), (700, 6_150, 400),
     # of 256 x 256: one a workgroup, two and three; one step of columns, two and a ragged last one
     (1_000, 10_000, 896), (2_048, 16_384, 16), (2_000, 17_001, 112), (2_000, 17_001, 128), (1_990, 17_001, 208),
-    (2_048, 16_400, 256),
+    (2_048, 16_400, 256), (1_024, 16_384, 288), (2_000, 20_000, 400),
 ]
 
 
