@@ -15,7 +15,9 @@ buffer) for a row without one; scales, biases and the weight's gradient are bina
 
 Every method checks its arguments, enqueues on `stream` and returns; each has a `bind_`
 form that checks them once and returns a callable enqueuing that exact call (it keeps the
-buffers and the stream alive), for loops over fixed buffers.
+buffers and the stream alive), for loops over fixed buffers.  The callable's `check()`
+raises what the library would refuse of the call, but for a missing reservation, and
+enqueues nothing.
 """
 from __future__ import annotations
 
@@ -23,7 +25,7 @@ import ctypes
 
 from . import hip
 from . import sampler as _s
-from .sampler import OK, InferenceError, _check, _Error, _shape, lib, vp
+from .sampler import OK, STATE, InferenceError, _check, _Error, _shape, lib, vp
 from .scores import _dtype_of, _matrix, _on_device
 
 HIDDEN_MAX_ROWS = 1_048_576
@@ -116,7 +118,15 @@ class HiddenRows:
             if st != OK:
                 raise InferenceError(e)
 
-        call.buffers = keep
+        def check():
+            # without a context the library checks everything else, and enqueues nothing
+            self._context()
+            e = _Error()
+            st = fn(None, *argv[1:], ctypes.byref(e))
+            if st != OK and not (st == STATE and e.needed == 1):
+                raise InferenceError(e)
+
+        call.buffers, call.check = keep, check
         return call
 
     # ---- the calls ----

@@ -681,13 +681,21 @@ class DecodeBatch:
         if rows != self.rows:
             raise ValueError(f"logits have {rows} rows, the batch has {self.rows}")
         lp = _dev(logits, "logits", ndim=2)
-        score = None
-        if logprobs is not None:  # checked before anything is drawn
-            score = self._scorer().bind_token_logprobs(
-                logits, self.token, logprob=logprobs, temperature=logprob_temperature,
-                vocab=VOCAB, stream=stream)
-            if not 0.01 <= logprob_temperature <= 100.0:
-                raise ValueError(f"a temperature of {logprob_temperature} is not supported")
+        score = self._bind_scores(logits, logprobs, logprob_temperature, stream)
+        return self._step(lp, ld, score, stream)
+
+    def _bind_scores(self, logits, logprobs, temperature, stream):
+        """The scoring of the next step's tokens, checked before anything is drawn."""
+        if logprobs is None:
+            return None
+        score = self._scorer().bind_token_logprobs(
+            logits, self.token, logprob=logprobs, temperature=temperature, vocab=VOCAB,
+            stream=stream)
+        if not 0.01 <= temperature <= 100.0:
+            raise ValueError(f"a temperature of {temperature} is not supported")
+        return score
+
+    def _step(self, lp, ld, score, stream):
         before = self._draw(stream)
         e = _Error()
         try:
@@ -724,7 +732,9 @@ class DecodeBatch:
         """One step through an 8-bit head of any width: hidden [rows, cols] in 8 bits, times
         weight [VOCAB, cols] with its channels' weight_scale (+ bias), then step() on these
         logits.  With norm_weight the head takes the root-mean-square norm of hidden (+
-        residual, kept in `sum`); without it, hidden as it is."""
+        residual, kept in `sum`); without it, hidden as it is.  A refused step leaves `sum`
+        and the samplings' states as they were: all arguments, the product's and the step's
+        too, are checked before the norm is enqueued."""
         rows, cols = _shape(hidden)
         if rows != self.rows:
             raise ValueError(f"hidden has {rows} rows, the batch has {self.rows}")
@@ -738,13 +748,19 @@ class DecodeBatch:
                           hip.DeviceArray((rows, VOCAB), np.uint32))
         q, scale, logits = self._head
         if norm_weight is None:
-            ops.quantize(hidden, q=q, scale=scale, dtype=dtype, stream=stream)
+            rounding = ops.bind_quantize(hidden, q=q, scale=scale, dtype=dtype, stream=stream)
         else:
-            ops.norm(hidden, norm_weight, eps=eps, residual=residual, sum=sum, q=q, scale=scale,
-                     dtype=dtype, weight_dtype=weight_dtype, stream=stream)
-        ops.matmul(q, scale, weight, weight_scale, out=logits, bias=bias, stream=stream)
-        return self.step(logits, stream=stream, logprobs=logprobs,
-                         logprob_temperature=logprob_temperature)
+            rounding = ops.bind_norm(hidden, norm_weight, eps=eps, residual=residual, sum=sum, q=q,
+                                     scale=scale, dtype=dtype, weight_dtype=weight_dtype,
+                                     stream=stream)
+        product = ops.bind_matmul(q, scale, weight, weight_scale, out=logits, bias=bias,
+                                  stream=stream)
+        product.check()
+        score = self._bind_scores(logits, logprobs, logprob_temperature, stream)
+        self.sampler._ensure(rows)
+        rounding()
+        product()
+        return self._step(vp(logits.data_ptr()), VOCAB, score, stream)
 
     def embed(self, table, *, out, scale: float = 1.0, dtype=None, out_dtype=None,
               stream=None) -> None:
