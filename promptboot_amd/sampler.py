@@ -630,6 +630,10 @@ class DecodeBatch:
             self.sampler.close()
         self.sampler = None
 
+    def _open(self) -> None:
+        if self.sampler is None or not self.sampler._ctx:
+            raise ValueError("the batch's context is closed")
+
     def active(self) -> bool:
         return bool((self.row_state_host == ROW_ACTIVE).any())
 
@@ -677,6 +681,7 @@ class DecodeBatch:
         raw logits (no repetition penalty, no cutoff).  Should the device refuse
         the scoring alone, the step stands (its tokens are in `contexts`) and the
         error is raised behind it."""
+        self._open()
         rows, ld = _shape(logits)
         if rows != self.rows:
             raise ValueError(f"logits have {rows} rows, the batch has {self.rows}")
@@ -735,6 +740,7 @@ class DecodeBatch:
         residual, kept in `sum`); without it, hidden as it is.  A refused step leaves `sum`
         and the samplings' states as they were: all arguments, the product's and the step's
         too, are checked before the norm is enqueued."""
+        self._open()
         rows, cols = _shape(hidden)
         if rows != self.rows:
             raise ValueError(f"hidden has {rows} rows, the batch has {self.rows}")
@@ -766,6 +772,7 @@ class DecodeBatch:
               stream=None) -> None:
         """The table rows of the tokens that the last step drew, the next step's input (zeros
         for rows not sampled), enqueued on `stream`."""
+        self._open()
         if _shape(out)[0] != self.rows:
             raise ValueError(f"out has {_shape(out)[0]} rows, the batch has {self.rows}")
         self._hidden_rows().embed(table, self.token, out=out, scale=scale, dtype=dtype,
@@ -775,6 +782,7 @@ class DecodeBatch:
                     q8: bool = False) -> np.ndarray:
         """One step through the fused Q4_0 (or, with q8, Q8_0) LM head on
         hidden [rows, cols]."""
+        self._open()
         rows, width, nbytes = BatchSampler._head_args(packed, hidden, cols, q8)
         if rows != self.rows:
             raise ValueError(f"hidden has {rows} rows, the batch has {self.rows}")

@@ -79,3 +79,29 @@ def test_a_forced_slice_plan_has_its_workspace(head):
     assert torch.equal(residual, want) and (tokens == expect).all()
     for b in (batch, plain, sampler):
         b.close()
+
+
+@pytest.mark.parametrize("closed", ["batch", "sampler"])
+def test_a_closed_batch_refuses(head, closed):
+    weight, weight_scale = head
+    sampler = s.BatchSampler(0) if closed == "sampler" else None
+    batch = new_batch(sampler=sampler)
+    hidden, table = make(gen(1), ROWS, COLS, "bf16"), make(gen(2), s.VOCAB, COLS, "bf16")
+    residual, out = make(gen(3), ROWS, COLS, "bf16"), torch.full((ROWS, COLS), 5.0, dtype=torch.bfloat16, device=DEV)
+    logits, logprobs = torch.zeros((ROWS, s.VOCAB), device=DEV), torch.full((ROWS,), 5.0, device=DEV)
+    packed, rows_32 = torch.zeros(1, dtype=torch.uint8, device=DEV), torch.zeros((ROWS, COLS), device=DEV)
+    before = residual.clone()
+    states = batch.sampling_states()
+    (batch if closed == "batch" else sampler).close()
+    torch.cuda.synchronize()
+    for bad in (lambda: batch.embed(table, out=out),
+                lambda: batch.int8_step(hidden, weight, weight_scale),
+                lambda: batch.int8_step(hidden, weight, weight_scale, norm_weight=torch.ones(COLS, device=DEV),
+                                        residual=residual, sum=residual),
+                lambda: batch.step(logits), lambda: batch.step(logits, logprobs=logprobs),
+                lambda: batch.lmhead_step(packed, rows_32), lambda: batch.lmhead_step(packed, rows_32, q8=True)):
+        with pytest.raises(ValueError, match="closed"):
+            bad()
+    torch.cuda.synchronize()
+    assert torch.equal(residual, before) and (out == 5.0).all() and (logprobs == 5.0).all()
+    assert batch.sampling_states() == states
