@@ -268,6 +268,7 @@ uint32_t pb_segments_for_rows(uint32_t rows) {
 }
 
 void pb_context_set_segments(pb_context* ctx, uint32_t segments) {
+  if (!ctx) return;
   ctx->forced_segments = segments > 32 ? 32 : segments;
 }
 
@@ -348,6 +349,10 @@ uint32_t pb_context_reserve(pb_context* ctx, uint32_t rows, size_t cols, pb_infe
   if (cols != 0 && rows > PB_LMHEAD_MAX_ROWS) {
     set_error(err, PB_CAPACITY, PB_DOMAIN_NONE, PB_LMHEAD_MAX_ROWS, rows, PB_FIELD_BYTES, 8);
     return PB_CAPACITY;
+  }
+  if (ctx == nullptr) {
+    set_error(err, PB_STATE, PB_DOMAIN_NONE, 1, 0, PB_FIELD_NONE, 0);
+    return PB_STATE;
   }
   std::lock_guard<std::mutex> lock(ctx->mu);
   DeviceGuard guard(ctx->device);
@@ -729,6 +734,10 @@ static uint32_t enqueue_lmhead(pb_context* ctx, const uint8_t* d_packed, size_t 
       d_token == nullptr || (d_hist_len != nullptr && d_hist == nullptr)) {
     set_error(err, PB_CAPACITY, PB_DOMAIN_ARGMAX, 1, 0, PB_FIELD_BYTES, 3);
     return PB_CAPACITY;
+  }
+  if (ctx == nullptr) {
+    set_error(err, PB_STATE, PB_DOMAIN_NONE, 1, 0, PB_FIELD_NONE, 0);
+    return PB_STATE;
   }
   const uint32_t rows_pad = (rows + 63u) & ~63u;
   std::lock_guard<std::mutex> lock(ctx->mu);
