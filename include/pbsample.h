@@ -605,10 +605,12 @@ uint32_t pb_preference_loss(pb_context *ctx, const void *d_logits, uint32_t dtyp
  * PB_HIDDEN_MAX_COLS, rows up to PB_HIDDEN_MAX_ROWS, vocab (and the channels of a
  * product) 1 to PB_SCORE_MAX_VOCAB.
  *
- * Outputs are rounded to their type once, to nearest even.  Sums are held in 32
- * bits over at most 768 terms, in 64 bits above that and for the norms' statistics;
- * their order depends on the sizes alone (and, in the table's gradient, on the
- * tokens), so results repeat bit for bit.
+ * Outputs are rounded to binary32 and from there to their type, both to nearest even
+ * (a number that binary32 takes to the middle of two 16-bit ones goes to the even one,
+ * on whichever side of the middle it was).  Sums are held in 32 bits over at most 768
+ * terms, in 64 bits above that and for the norms' statistics; their order depends on
+ * the sizes alone (and, in the table's gradient, on the tokens), so results repeat bit
+ * for bit.
  *
  * An output may lie in an input's place where its description says so: the same
  * address, type and distance of rows.  Any other element that an output shares with
@@ -630,8 +632,9 @@ uint32_t pb_preference_loss(pb_context *ctx, const void *d_logits, uint32_t dtyp
 uint32_t pb_context_reserve_hidden(pb_context *ctx, uint32_t rows, size_t cols,
                                    pb_inference_error *err);
 
-/* d_out[r] = scale * table[token[r]], the product rounded once to out_dtype.  A token
- * of PB_NO_TOKEN gives a row of zeros; an id >= vocab a row of NaN and a record
+/* d_out[r] = scale * table[token[r]]: the product in binary64, rounded to binary32 and
+ * then to out_dtype.  A token of PB_NO_TOKEN gives a row of zeros; an id >= vocab a row
+ * of NaN and a record
  * (PB_TOKEN_ID; needed = vocab, available = the id).  scale is finite. */
 uint32_t pb_embed_rows(pb_context *ctx, const void *d_table, uint32_t dtype, size_t vocab,
                        size_t cols, size_t table_ld, uint32_t rows, const uint32_t *d_token,

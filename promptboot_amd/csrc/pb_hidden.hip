@@ -125,6 +125,9 @@ __device__ __forceinline__ double wave_add(double v) {
 
 // 2^shift threads take a row.  40 rows of 896 bf16: 2.4 us, a launch; 16,384 of them: 11.4 us
 // (5.1 TB/s read and written).
+// A product goes to its type by way of binary32: in one rounding 16,384 rows of 896 bf16 by
+// 31.6 took 17.4 us in place of 10.2.  (31.6 is 158 / 5 but for 4e-17, so many of its products
+// with 8 bits are next to the middle of two numbers, and what decides is behind the 53rd digit.)
 template <typename In, typename Out>
 __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p, uint32_t shift) {
   const uint32_t row = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
