@@ -645,7 +645,8 @@ uint32_t pb_embed_rows(pb_context *ctx, const void *d_table, uint32_t dtype, siz
  * whose token is v, in the order of the rows.  accumulate 0: every row of the table
  * is written, zeros where no token is.  accumulate 1: that sum is added to what is
  * there, and other rows are left as they are.  Rows whose token is PB_NO_TOKEN or >=
- * vocab add nothing, and what they hold does not matter. */
+ * vocab add nothing, and what they hold does not matter.  scale is rounded to binary32
+ * (and refused past its range); so are its product and the addition to the table. */
 uint32_t pb_embed_rows_grad(pb_context *ctx, const void *d_grad, uint32_t dtype, size_t vocab,
                             size_t cols, size_t grad_ld, uint32_t rows, const uint32_t *d_token,
                             double scale, uint32_t accumulate, void *d_table_grad,

@@ -454,13 +454,11 @@ __global__ __launch_bounds__(256) void zero_table_kernel(EmbedGradParams p) {
   zero_part<T, 256>(p, blockIdx.x, gridDim.x);
 }
 
+// A token's sum times the factor, as the table holds it.
 template <typename T, int N>
-__device__ __forceinline__ void put_table(const EmbedGradParams& p, uint32_t id, uint32_t j,
-                                          uint32_t n, const float (&sum)[N]) {
+__device__ __forceinline__ void put_product(const EmbedGradParams& p, uint32_t id, uint32_t j,
+                                            uint32_t n, float (&y)[N]) {
   typename T::Raw* to = static_cast<typename T::Raw*>(p.table) + (size_t)id * p.table_ld + j;
-  float y[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) y[e] = sum[e] * p.scale;
   if (p.accumulate) {
     float old[N];
     load_row<T>(to, n, old);
@@ -514,7 +512,12 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(EmbedGradParams p, uint32
   float sum[N] = {};
   auto leave = [&](bool goes_on) {
     if (!from_before && !goes_on) {
-      put_table<T>(p, cur, j, n, sum);
+      // the factor is a binary32 number: one of 64 bits, in two words or in binary64, took 16,384 rows
+      // added to a table from 68.5 to 70 us (this stands here sixteen times)
+      float y[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[e] = sum[e] * p.scale;
+      put_product<T>(p, cur, j, n, y);
     } else {
       float* to = p.part + ((size_t)part * 2u + (from_before ? 0u : 1u)) * p.cols + j;
       store_row<F32>(reinterpret_cast<uint32_t*>(to), n, sum);
@@ -591,8 +594,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(EmbedGradPar
       for (int e = 0; e < 4; ++e) sum[e] = sum[e] + (double)x[e];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = (float)sum[e];
-    put_table<T>(p, own, j, n, x);
+    for (int e = 0; e < 4; ++e) x[e] = (float)(sum[e] * (double)p.scale);
+    put_product<T>(p, own, j, n, x);
   }
   for (size_t unit = blockIdx.x; unit < (size_t)many * narrow; unit += gridDim.x) {
     const uint32_t part = p.cross[1u + sum_parts(p.rows) - (uint32_t)(unit / narrow)];
@@ -612,7 +615,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(EmbedGradPar
     if (wave == 0 && j < p.cols) {
 #pragma unroll
       for (uint32_t w = 1; w < kJoinWaves; ++w) sum = sum + waves[w][lane];
-      const float y = p.scale * (float)sum;
+      const float y = (float)(sum * (double)p.scale);
       typename T::Raw* at = static_cast<typename T::Raw*>(p.table) + (size_t)own * p.table_ld + j;
       *at = T::raw(p.accumulate ? T::one(*at) + y : y);
     }
