@@ -617,20 +617,31 @@ uint32_t pb_preference_loss(pb_context *ctx, const void *d_logits, uint32_t dtyp
  * an input or another output is refused with PB_STATE.
  *
  * All pointers are device pointers; calls enqueue on `stream`, never allocate and
- * never wait.  The gradients need a context reserved with
- * pb_context_reserve_hidden for at least their rows and columns (else
- * PB_CAPACITY), and calls on one context share its workspace: the rule on threads
- * and streams above holds.  Returns PB_OK when the work was enqueued, else a status
- * with *err filled (err may be NULL) and nothing enqueued.  d_err: one record per
- * row, all-zero on success, with `position` = the row. */
+ * never wait.  The gradients need a context reserved for their rows and columns by one
+ * of the reservations below (else PB_CAPACITY), and calls on one context share its
+ * workspace: the rule on threads and streams above holds.  Returns PB_OK when the work
+ * was enqueued, else a status with *err filled (err may be NULL) and nothing enqueued.
+ * d_err: one record per row, all-zero on success, with `position` = the row. */
 #define PB_HIDDEN_MAX_ROWS 1048576u
 #define PB_HIDDEN_MAX_COLS 32768u
 
 /* Sizes the context's workspace for the gradients below on up to `rows` rows of up
- * to `cols` columns (as pb_context_reserve: a set-up call; it never shrinks the
- * workspace, and one it outgrows stays allocated until pb_context_destroy). */
+ * to `cols` columns, in every pair of these (as pb_context_reserve: a set-up call; it
+ * never shrinks the workspace, and one it outgrows stays allocated until
+ * pb_context_destroy). */
 uint32_t pb_context_reserve_hidden(pb_context *ctx, uint32_t rows, size_t cols,
                                    pb_inference_error *err);
+
+/* The same for a call of that size of one gradient alone, which needs much less than
+ * both in every pair.  Where memory allows, an outgrown workspace is followed by one of
+ * twice its size or more, so that all of them together are less than twice the last. */
+uint32_t pb_context_reserve_embed_grad(pb_context *ctx, uint32_t rows, size_t cols,
+                                       pb_inference_error *err);
+uint32_t pb_context_reserve_norm_grad(pb_context *ctx, uint32_t rows, size_t cols,
+                                      pb_inference_error *err);
+
+/* The bytes of that workspace; 0 without a context. */
+size_t pb_context_hidden_bytes(pb_context *ctx);
 
 /* d_out[r] = scale * table[token[r]]: the product in binary64, rounded to binary32 and
  * then to out_dtype.  A token of PB_NO_TOKEN gives a row of zeros; an id >= vocab a row

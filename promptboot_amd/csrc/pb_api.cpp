@@ -574,9 +574,14 @@ HiddenAccess hidden_access(pb_context* ctx) {
   return HiddenAccess{std::move(lock), ctx->device, ctx->d_hidden, ctx->hidden_bytes};
 }
 
-hipError_t hidden_reserve(pb_context* ctx, size_t bytes) {
+hipError_t hidden_reserve(pb_context* ctx, size_t bytes, size_t most) {
   std::lock_guard<std::mutex> lock(ctx->mu);
   DeviceGuard guard(ctx->device);
+  if (bytes <= ctx->hidden_bytes) return hipSuccess;
+  const size_t twice = 2 * ctx->hidden_bytes < most ? 2 * ctx->hidden_bytes : most;
+  if (twice > bytes &&
+      grow_device(&ctx->d_hidden, &ctx->hidden_bytes, twice, &ctx->retired) == hipSuccess)
+    return hipSuccess;
   return grow_device(&ctx->d_hidden, &ctx->hidden_bytes, bytes, &ctx->retired);
 }
 

@@ -1,6 +1,6 @@
 // pb_hidden_api.cpp -- C ABI of the operators on hidden-state rows
 // (include/pbsample.h): argument checks and the calls' workspace.
-// Nothing here allocates but pb_context_reserve_hidden.
+// Nothing here allocates but the reservations.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -133,6 +133,25 @@ uint32_t finish(hipError_t e, pb_inference_error* err) {
   return e == hipSuccess ? PB_OK : device_error(err, e);
 }
 
+// A workspace of what `bytes_of` says, or where it grows by doubling of twice the one it
+// outgrows, up to what the largest call of either gradient needs.
+uint32_t reserve(pb_context* ctx, uint32_t rows, size_t cols,
+                 size_t (*bytes_of)(uint32_t rows, size_t cols), bool doubling,
+                 pb_inference_error* err) {
+  clear_error(err);
+  const uint32_t st = check_sizes(rows, cols, err);
+  if (st != PB_OK) return st;
+  if (ctx == nullptr) return no_context(err);
+  const size_t bytes = rows != 0 ? bytes_of(rows, cols) : 0;
+  const size_t most =
+      doubling ? pb::hidden_workspace_bytes(PB_HIDDEN_MAX_ROWS, PB_HIDDEN_MAX_COLS) : 0;
+  try {  // the list of outgrown workspaces grows
+    return finish(pb::hidden_reserve(ctx, bytes, most), err);
+  } catch (const std::exception&) {
+    return device_error(err, hipErrorOutOfMemory);
+  }
+}
+
 // What pb_norm_rows and pb_quantize_rows have in common, behind their own checks.
 uint32_t norm_rows(pb_context* ctx, const pb::NormParams& p, uint32_t dtype, bool required,
                    void* stream, pb_inference_error* err) {
@@ -164,15 +183,21 @@ extern "C" {
 
 uint32_t pb_context_reserve_hidden(pb_context* ctx, uint32_t rows, size_t cols,
                                    pb_inference_error* err) {
-  clear_error(err);
-  const uint32_t st = check_sizes(rows, cols, err);
-  if (st != PB_OK) return st;
-  if (ctx == nullptr) return no_context(err);
-  try {  // the list of outgrown workspaces grows
-    return finish(pb::hidden_reserve(ctx, pb::hidden_workspace_bytes(rows, cols)), err);
-  } catch (const std::exception&) {
-    return device_error(err, hipErrorOutOfMemory);
-  }
+  return reserve(ctx, rows, cols, pb::hidden_workspace_bytes, false, err);
+}
+
+uint32_t pb_context_reserve_embed_grad(pb_context* ctx, uint32_t rows, size_t cols,
+                                       pb_inference_error* err) {
+  return reserve(ctx, rows, cols, pb::embed_grad_bytes, true, err);
+}
+
+uint32_t pb_context_reserve_norm_grad(pb_context* ctx, uint32_t rows, size_t cols,
+                                      pb_inference_error* err) {
+  return reserve(ctx, rows, cols, pb::norm_grad_bytes, true, err);
+}
+
+size_t pb_context_hidden_bytes(pb_context* ctx) {
+  return ctx ? pb::hidden_access(ctx).bytes : 0;
 }
 
 uint32_t pb_embed_rows(pb_context* ctx, const void* d_table, uint32_t dtype, size_t vocab,

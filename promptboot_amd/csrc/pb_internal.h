@@ -161,7 +161,9 @@ struct HiddenAccess {
   size_t bytes;
 };
 HiddenAccess hidden_access(pb_context* ctx);
-hipError_t hidden_reserve(pb_context* ctx, size_t bytes);
+// Grows that workspace to `bytes`, or by doubling up to `most` bytes if those are more (0:
+// exactly); takes the lock itself.
+hipError_t hidden_reserve(pb_context* ctx, size_t bytes, size_t most);
 
 // The context's device (pb_api.cpp).
 int context_device(const pb_context* ctx);

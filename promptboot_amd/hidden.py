@@ -36,9 +36,10 @@ class HiddenRows:
     """Operators on hidden-state rows on one GPU.
 
     Uses the context of `sampler` (a BatchSampler) when given, else one of its own on
-    `device`.  The context's workspace is reserved before any gradient that needs more,
-    so the enqueued calls never allocate; gradients on one context must be ordered (one
-    stream, or streams that the caller orders)."""
+    `device`.  The context's workspace is reserved before any gradient that needs more
+    (as much as that one needs; reserve() does it beforehand), so the enqueued calls never
+    allocate; gradients on one context must be ordered (one stream, or streams that the
+    caller orders)."""
 
     def __init__(self, device: int = -1, sampler: "_s.BatchSampler | None" = None):
         self._own = sampler is None
@@ -52,12 +53,11 @@ class HiddenRows:
         self.sampler = None
 
     def reserve(self, rows: int, cols: int) -> None:
-        """Sizes the context for gradients of up to `rows` rows of up to `cols` columns,
-        each at least as large as reserved before; a set-up call, it may allocate."""
-        rows, cols = max(rows, self._reserved[0]), max(cols, self._reserved[1])
-        e = _Error()
-        _check(lib().pb_context_reserve_hidden(self._context(), rows, cols, ctypes.byref(e)), e)
-        self._reserved = (rows, cols)
+        """Sizes the context for gradients of up to `rows` rows of up to `cols` columns, in
+        every pair of these and of what was reserved before (a number that grows again at
+        least doubles); a set-up call, it may allocate."""
+        self._context()
+        self._ensure(rows, cols)
 
     def _ensure(self, rows: int, cols: int) -> None:
         # An outgrown workspace stays allocated with the context (a captured graph may
@@ -67,7 +67,17 @@ class HiddenRows:
 
         have = self._reserved
         if rows > have[0] or cols > have[1]:
-            self.reserve(grown(rows, have[0], HIDDEN_MAX_ROWS), grown(cols, have[1], HIDDEN_MAX_COLS))
+            both = grown(rows, have[0], HIDDEN_MAX_ROWS), grown(cols, have[1], HIDDEN_MAX_COLS)
+            self._reserve("pb_context_reserve_hidden", *both)
+            self._reserved = both
+
+    def _reserve(self, name: str, rows: int, cols: int) -> None:
+        e = _Error()
+        _check(getattr(lib(), name)(self._context(), rows, cols, ctypes.byref(e)), e)
+
+    def workspace_bytes(self) -> int:
+        """What the context holds for gradients."""
+        return lib().pb_context_hidden_bytes(self._context())
 
     def _context(self):
         if self.sampler is None or not self.sampler._ctx:
@@ -155,7 +165,7 @@ class HiddenRows:
         pt, table_code, table_ld = self._rows(table_grad, "table_grad", table_dtype, vocab, cols)
         argv = (ctx, ptr, code, vocab, cols, ld, rows, self._dev(token, "token", rows=rows), float(scale),
                 int(accumulate), pt, table_code, table_ld, vp(hip.stream_handle(stream)))
-        self._ensure(rows, cols)
+        self._reserve("pb_context_reserve_embed_grad", rows, cols)
         return self._call("pb_embed_rows_grad", argv, (self, stream, grad, token, table_grad))
 
     def embed_grad(self, grad, token, **kw) -> None:
@@ -200,7 +210,7 @@ class HiddenRows:
                 h_ld, self._dev(grad_weight, "grad_weight", rows=cols), int(accumulate),
                 vp(hip.stream_handle(stream)))
         if grad_weight is not None:
-            self._ensure(rows, cols)
+            self._reserve("pb_context_reserve_norm_grad", rows, cols)
         return self._call("pb_norm_rows_grad", argv,
                           (self, stream, h, weight, grad, grad_sum, grad_h, grad_weight))
 

@@ -171,6 +171,9 @@ EXPORTS = {
         u32, [vp, vp, u32, size_t, size_t, u32, f64, vp, vp, u32, vp, vp, f64, f64, vp, vp, vp,
               size_t, vp, vp, ctypes.POINTER(_Error)]),
     "pb_context_reserve_hidden": (u32, [vp, u32, size_t, ctypes.POINTER(_Error)]),
+    "pb_context_reserve_embed_grad": (u32, [vp, u32, size_t, ctypes.POINTER(_Error)]),
+    "pb_context_reserve_norm_grad": (u32, [vp, u32, size_t, ctypes.POINTER(_Error)]),
+    "pb_context_hidden_bytes": (size_t, [vp]),
     "pb_embed_rows": (
         u32, [vp, vp, u32, size_t, size_t, size_t, u32, vp, f64, vp, u32, size_t, vp, vp,
               ctypes.POINTER(_Error)]),
