@@ -97,7 +97,10 @@ static hipError_t grow_device(void** buf, size_t* have, size_t bytes,
   if (bytes <= *have) return hipSuccess;
   void* fresh = nullptr;
   hipError_t e = hipMalloc(&fresh, bytes);
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess) {
+    (void)hipGetLastError();  // it is returned: not for the next call to find
+    return e;
+  }
   if (*buf) retired->push_back(*buf);
   *buf = fresh;
   *have = bytes;
@@ -332,6 +335,7 @@ uint32_t pb_context_create(int device, pb_context** out) {
   if (e == hipSuccess) e = pb::resident_rows(device, &resident);
   if (e != hipSuccess) {
     release(ctx);
+    (void)hipGetLastError();
     return PB_DEVICE;
   }
   *out = ctx;

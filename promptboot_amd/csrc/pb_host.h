@@ -26,7 +26,10 @@ inline void clear_error(pb_inference_error* e) {
   if (e) memset(e, 0, sizeof *e);
 }
 
+// The error is returned, so the runtime's note of it is taken back: the next launch, of any
+// library in the process, would be taken for the failure.
 inline uint32_t device_error(pb_inference_error* e, hipError_t code) {
+  (void)hipGetLastError();
   set_error(e, PB_DEVICE, PB_DOMAIN_NONE, 0, (uint64_t)code, PB_FIELD_NONE, 0);
   return PB_DEVICE;
 }

@@ -28,6 +28,7 @@ _CAPTURE_MODE_THREAD_LOCAL = 1  # hipStreamCaptureModeThreadLocal
 
 _SIGS = {
     "hipGetErrorString": (ctypes.c_char_p, [_int]),
+    "hipGetLastError": (_int, []),
     "hipGetDeviceCount": (_int, [ctypes.POINTER(_int)]),
     "hipSetDevice": (_int, [_int]),
     "hipGetDevice": (_int, [ctypes.POINTER(_int)]),
@@ -78,6 +79,7 @@ def runtime() -> ctypes.CDLL:
 
 def _ok(call: str, code: int) -> None:
     if code != 0:
+        runtime().hipGetLastError()  # it is raised: not for the next call to find
         raise HipError(call, code)
 
 
