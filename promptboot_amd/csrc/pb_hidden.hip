@@ -1142,7 +1142,7 @@ uint32_t row_span(uint32_t cols) {
 
 // Workgroups of the norm's gradient.  More have more rows on their way, fewer leave fewer sums
 // to join: as many as hold kGradChunks chunks at once, 512 or more, and none with more than
-// kGradTerms rows a thread.  512 / 1,024 / 2,048 of them, us:
+// kGradTerms rows, whose sum it has in 32 bits.  512 / 1,024 / 2,048 of them, us:
 //   65,536 x 512 (256 chunks)     58 /  57 /  59     16,384 x 4,096 (512)  103 / 119 / 118
 //   65,536 x 896 (128)           215 / 126 / 100     8,192 x 8,192 (1,024) 109 / 117 / 134
 //   8,192 x 2,048 (256)         33.1 / 32.8 / 37.8
@@ -1151,7 +1151,8 @@ constexpr uint32_t kGradTerms = 768;
 uint32_t grad_groups(uint32_t rows, uint32_t cols) {
   const uint32_t span = row_span(cols), at_once = span < 128 ? 256 / span : 1;
   const uint32_t all = (rows + at_once - 1u) / at_once;
-  const uint32_t held = kGradChunks / (span * at_once), least = (all + kGradTerms - 1u) / kGradTerms;
+  const uint32_t held = kGradChunks / (span * at_once), turns = kGradTerms / at_once;
+  const uint32_t least = (all + turns - 1u) / turns;
   uint32_t most = held > 512 ? held : 512;
   if (most < least) most = least;
   return all < most ? all : most;

@@ -108,3 +108,14 @@ def test_without_a_context_there_is_no_workspace():
     closed.close()
     with pytest.raises(ValueError, match="closed"):
         closed.workspace_bytes()
+
+
+@pytest.mark.parametrize("rows,cols", [(HIDDEN_MAX_ROWS, 9), (HIDDEN_MAX_ROWS, 512), (786_433, 100), (786_432, 100),
+                                       (HIDDEN_MAX_ROWS, 513), (786_433, 1_025), (393_217, 2_049), (HIDDEN_MAX_ROWS, 32_768),
+                                       (100_000, 20), (3, 9)])
+def test_a_workgroup_adds_up_768_rows_at_most(rows, cols):
+    """Each workgroup's sums of the weight's gradient are in 32 bits, so they hold 768 terms at most."""
+    groups, left = divmod(need("norm_grad", rows, cols), cols * 4)
+    at_once = 4 if cols <= 512 else 1  # rows that a workgroup takes at a time
+    turns = -(-rows // at_once)
+    assert left == 0 and -(-turns // groups) * at_once <= 768
