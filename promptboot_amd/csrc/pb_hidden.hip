@@ -628,7 +628,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(EmbedGradPar
 // A row is held in registers between its statistics and its outputs, as it is in memory: T
 // threads take C chunks of eight elements each.  mean(h^2) is summed in 64 bits: no
 // binary32 row overflows there, and a 64-bit multiply-add issues as fast as a 32-bit
-// product and its addition would.
+// product and its addition would.  1 / sqrt(mean + eps) is used as binary32: for rows next to the
+// largest numbers (a root mean square past 2^126) that is below the normal range and has 21
+// digits or more.  All 24, by a power of two, cost every gradient of a norm 1 to 2 %.
 
 // Eight elements as they are in memory.
 template <typename E>
