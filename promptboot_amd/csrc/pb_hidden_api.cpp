@@ -33,24 +33,13 @@ struct Rows {
   size_t rows, cols, ld, size;
 };
 
-// Whether two buffers share a byte.  Rows at one distance may lie between each other
-// (the columns of one buffer, or every other row of it); at two distances the ranges that
-// they span are compared.
 bool overlap(const Rows& a, const Rows& b) {
   if (a.at == nullptr || b.at == nullptr || a.rows == 0 || b.rows == 0) return false;
-  const int64_t a0 = (int64_t)(uintptr_t)a.at, b0 = (int64_t)(uintptr_t)b.at;
-  const int64_t len_a = (int64_t)(a.cols * a.size), len_b = (int64_t)(b.cols * b.size);
-  const int64_t step_a = (int64_t)(a.ld * a.size), step_b = (int64_t)(b.ld * b.size);
-  const int64_t last_a = (int64_t)a.rows - 1, last_b = (int64_t)b.rows - 1;
-  if (a0 >= b0 + last_b * step_b + len_b || b0 >= a0 + last_a * step_a + len_a) return false;
-  if (step_a != step_b) return true;
-  // row i of a and row i + k of b share a byte where -len_b < d + k step < len_a
-  const int64_t d = b0 - a0, step = step_a;
-  auto floor_div = [](int64_t x, int64_t y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };
-  int64_t lo = floor_div(-len_b - d, step) + 1, hi = floor_div(len_a - 1 - d, step);
-  if (lo < -last_a) lo = -last_a;
-  if (hi > last_b) hi = last_b;
-  return lo <= hi;
+  auto bytes = [](const Rows& r) {
+    return pb::ByteRows{r.at, (int64_t)r.rows, (int64_t)(r.cols * r.size),
+                        (int64_t)(r.ld * r.size)};
+  };
+  return pb::share_a_byte(bytes(a), bytes(b));
 }
 
 bool same_place(const Rows& a, const Rows& b) {

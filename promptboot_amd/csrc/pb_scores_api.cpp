@@ -46,22 +46,11 @@ struct Rows {
 
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-// Whether a gradient that is not in place of the logits shares an element with
-// them.  Rows of one stride may lie between each other (the columns of one buffer,
-// or every other row of it); of two strides the ranges they span are compared.
+// Whether a gradient that is not in place of the logits shares an element with them.
 bool overlap(const Rows& r, size_t size) {
-  const uintptr_t a = (uintptr_t)r.logits, b = (uintptr_t)r.grad;
-  const uintptr_t a_end = a + ((size_t)(r.rows - 1) * r.ld + r.vocab) * size;
-  const uintptr_t b_end = b + ((size_t)(r.rows - 1) * r.grad_ld + r.vocab) * size;
-  if (a >= b_end || b >= a_end) return false;
-  if (r.ld != r.grad_ld) return true;
-  // row i of the logits and row i - k of the gradient start `m` elements apart, row i
-  // and row i - k - 1 ld - m
-  const int64_t d = ((int64_t)b - (int64_t)a) / (int64_t)size, ld = (int64_t)r.ld;
-  const int64_t k = d >= 0 ? d / ld : -((-d + ld - 1) / ld), m = d - k * ld;
-  const int64_t rows = r.rows, vocab = (int64_t)r.vocab;
-  return (k < rows && -k < rows && m < vocab) ||
-         (k + 1 < rows && -(k + 1) < rows && ld - m < vocab);
+  const int64_t rows = r.rows, bytes = (int64_t)(r.vocab * size);
+  return pb::share_a_byte({r.logits, rows, bytes, (int64_t)(r.ld * size)},
+                          {r.grad, rows, bytes, (int64_t)(r.grad_ld * size)});
 }
 
 // The checks that every call makes of its rows.  `missing`: a required
