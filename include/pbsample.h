@@ -675,8 +675,8 @@ uint32_t pb_embed_rows_grad(pb_context *ctx, const void *d_grad, uint32_t dtype,
  *               number nearest to y / s, ties to even (which is worked out as if in
  *               exact arithmetic), and d_scale[r] = s.  A row of zeros has s = 0.
  * One of d_out and d_q has to be there, and d_scale with d_q.  eps is finite and 1e-75 or
- * more (binary32 holds 1 / sqrt(eps)).  d_out has 1 / sqrt(mean(h * h) + eps) in binary32,
- * and so with 21 digits where the root mean square passes 2^126.
+ * more (binary32 holds 1 / sqrt(eps)).  d_out has 1 / sqrt(mean(h * h) + eps) in
+ * binary32, and so with fewer than 24 digits where that is below 2^-126.
  * A row whose h holds NaN or an infinity (or, with d_q, one of whose products h *
  * weight does, or whose s passes binary32) fails: y and s are NaN, the 8-bit row is
  * zeros, the record PB_NONFINITE_INPUT (detail: the first such index, cols if it is s;
@@ -695,9 +695,9 @@ uint32_t pb_norm_rows(pb_context *ctx, const void *d_x, uint32_t dtype, size_t c
  *   d_grad_sum     optional, of the rows' type: what reaches h elsewhere, added.
  *   d_grad_weight  optional: `cols` binary32 words, by the weight (without d_weight:
  *                  by the ones); accumulate 1 adds to what is there.
- * One of d_grad_h and d_grad_weight has to be there.  grad * weight, the row's factor (as
- * above) and h / sqrt(mean(h * h) + eps) are held in binary32.  Values that are not finite, and products past
- * binary32, spread as the formulas have it. */
+ * One of d_grad_h and d_grad_weight has to be there.  grad * weight, 1 / sqrt(mean(h * h) +
+ * eps) (as above) and its product with h are held in binary32.  Values that are not
+ * finite, and products past binary32, spread as the formulas have it. */
 uint32_t pb_norm_rows_grad(pb_context *ctx, const void *d_h, uint32_t dtype, size_t cols,
                            size_t h_ld, uint32_t rows, const void *d_weight,
                            uint32_t weight_dtype, double eps, const void *d_grad,

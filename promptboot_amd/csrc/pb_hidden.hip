@@ -629,8 +629,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_rows_kernel(EmbedGradPar
 // threads take C chunks of eight elements each.  mean(h^2) is summed in 64 bits: no
 // binary32 row overflows there, and a 64-bit multiply-add issues as fast as a 32-bit
 // product and its addition would.  1 / sqrt(mean + eps) is used as binary32: for rows next to the
-// largest numbers (a root mean square past 2^126) that is below the normal range and has 21
-// digits or more.  All 24, by a power of two, cost every gradient of a norm 1 to 2 %.
+// largest numbers (a root mean square past 2^126) that is below the normal range, where it has
+// 22 digits or more.  All 24, by a power of two, cost every gradient of a norm 1 to 2 %.
 
 // Eight elements as they are in memory.
 template <typename E>
@@ -773,8 +773,8 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t 
 // binary32, so the largest is, and all but values near a half are rounded in 32 bits:
 // p (127 / top) is off by 2^-24 of 127 there, and those that come nearer than 2^-15 to a half
 // go the exact way.  Rows whose largest product binary32 does not hold well (2^-60 to 2^120)
-// go it as a whole, and so do all others, in 64 bits.  (16,384 rows of 4,096 bf16 in 64
-// bits alone: 131 us.)
+// go it as a whole, and so do all others, in 64 bits: 16,384 rows of 4,096 bf16 under an f32
+// weight 110 us.
 template <typename E, bool kNarrow, int T, int C>
 __global__ __launch_bounds__(T < 128 ? 256 : T) void norm_kernel(NormParams p) {
   constexpr uint32_t kRows = T < 128 ? 256 / T : 1;

@@ -1,4 +1,5 @@
-// pb_host.h -- error records, overlaps of buffers and the device guard shared by the host side of the C ABI.
+// pb_host.h -- error records, overlaps of buffers and the device guard shared by the host
+// side of the C ABI.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -54,8 +54,8 @@ class HiddenRows:
 
     def reserve(self, rows: int, cols: int) -> None:
         """Sizes the context for gradients of up to `rows` rows of up to `cols` columns, in
-        every pair of these and of what was reserved before (a number that grows again at
-        least doubles); a set-up call, it may allocate."""
+        every pair of these and of what was reserved before (a number that grows again
+        doubles at least); a set-up call, it may allocate."""
         self._context()
         self._ensure(rows, cols)
 
